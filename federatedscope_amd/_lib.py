@@ -203,6 +203,54 @@ SIGNATURES['fsagg_peer_barrier'] = (
     _c_i, [ctypes.POINTER(_c_p), _c_i, _c_i, _c_u32, ctypes.c_uint64, _c_p,
            _c_p])
 
+
+
+class NsMat(ctypes.Structure):
+    """struct fsagg_ns_mat (include/fsagg.h)."""
+    _fields_ = [('g', _c_p), ('out', _c_p), ('rows', _c_i64),
+                ('cols', _c_i64), ('batch', _c_i64),
+                ('batch_stride', _c_i64), ('row_stride', _c_i64),
+                ('col_stride', _c_i64), ('dtype', ctypes.c_int32),
+                ('out_dtype', ctypes.c_int32)]
+
+
+class MuonMat(ctypes.Structure):
+    """struct fsagg_muon_mat (include/fsagg.h)."""
+    _fields_ = [('param', _c_p), ('avg', _c_p), ('momentum', _c_p),
+                ('rows', _c_i64), ('cols', _c_i64)]
+
+
+class MuonParams(ctypes.Structure):
+    """struct fsagg_muon_params (include/fsagg.h)."""
+    _fields_ = [('lr', _c_d), ('momentum', _c_d), ('weight_decay', _c_d),
+                ('a', _c_d), ('b', _c_d), ('c', _c_d), ('eps', _c_d),
+                ('steps', ctypes.c_int32), ('nesterov', ctypes.c_int32),
+                ('maximize', ctypes.c_int32), ('adjust', ctypes.c_int32)]
+
+
+class EmbedPart(ctypes.Structure):
+    """struct fsagg_embed_part (include/fsagg.h)."""
+    _fields_ = [('ids', _c_p), ('rows', _c_p), ('tokens', _c_i64),
+                ('row_stride', _c_i64), ('coef', _c_f),
+                ('ids64', ctypes.c_int32)]
+
+
+FSAGG_MUON_ORIGINAL, FSAGG_MUON_MATCH_RMS = 0, 1
+SIGNATURES['fsagg_newton_schulz_workspace_bytes'] = (
+    _c_sz, [_c_i64, _c_i64, _c_i64])
+SIGNATURES['fsagg_newton_schulz'] = (
+    _c_i, [_c_p, _c_i, _c_i, _c_p, _c_d, _c_p, _c_sz, _c_p])
+SIGNATURES['fsagg_muon_step_f32'] = (
+    _c_i, [_c_p, _c_i, _c_p, _c_p, _c_sz, _c_p])
+SIGNATURES['fsagg_embed_lookup'] = (
+    _c_i, [_c_p, _c_i64, _c_i64, _c_i64, _c_i, _c_p, _c_i, _c_i64, _c_f,
+           _c_p, _c_p])
+SIGNATURES['fsagg_embed_grad_workspace_bytes'] = (
+    _c_sz, [_c_i64, _c_i64, _c_i64])
+SIGNATURES['fsagg_embed_grad'] = (
+    _c_i, [_c_p, _c_i, _c_i, _c_i64, _c_i64, _c_p, _c_i, _c_i64, _c_i, _c_p,
+           _c_sz, _c_p])
+
 _lib = None
 _host = None
 HOST_PATH = os.path.join(_HERE, 'lib', '_fsagg_host.so')

@@ -1,0 +1,740 @@
+// Embedding rows: the lookup with a scale, and its gradient — the weighted
+// sum of many clients' rows by token (gfx950).
+//
+//   lookup:   out[t] = round(scale * E[ids[t]])
+//   gradient: out[v] = [out[v] +] sum over the tokens t with ids[t] = v, in
+//             token order, of coef(part of t) * rows[t], in fp32, rounded
+//             once.
+//
+// A token number outside [0, V) is padding: the lookup gives a zero row, the
+// gradient does not read its row at all.
+//
+// The gradient sorts the tokens by row (a stable radix sort, so a row's
+// tokens stay in token order and the result does not depend on timing), then
+// walks the sorted list in chunks of at most 64 tokens.  A wave owns a chunk
+// and 64 vectors of columns: it loads the rows of its chunk and keeps one
+// running sum in registers, written out where the token number changes.  A
+// row whose tokens cross chunks leaves one partial sum per chunk, added up
+// in order by a last pass; the split is fixed by the sizes alone.  Both
+// operators are bound by memory: they read each token's row once and write
+// each result row once.
+#include "common.h"
+
+#include <hip/hip_fp16.h>
+
+namespace fsagg {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / kWave;
+constexpr int kMaxParts = 64;     // parts per key launch (kernel arguments)
+constexpr int kTile = 4096;       // tokens per sorting workgroup
+constexpr int kSortBlock = 1024;
+constexpr int kSortWaves = kSortBlock / kWave;
+constexpr int kRounds = kTile / kSortBlock;  // 64-token rounds of a wave
+constexpr int kMaxDigit = 10;     // bits per radix pass
+// a launch counts its work items in 32 bits
+constexpr int64_t kMaxGrid = (int64_t(1) << 32) / kBlock - 1;
+
+// -- element types -----------------------------------------------------------
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<FSAGG_F32> {
+  using type = float;
+  static constexpr int kVec = 4;
+  __device__ static float get(float x) { return x; }
+  __device__ static float put(float x) { return x; }
+};
+template <>
+struct Elem<FSAGG_F16> {
+  using type = _Float16;
+  static constexpr int kVec = 8;
+  __device__ static float get(_Float16 x) { return float(x); }
+  __device__ static _Float16 put(float x) { return _Float16(x); }
+};
+template <>
+struct Elem<FSAGG_BF16> {
+  using type = uint16_t;
+  static constexpr int kVec = 8;
+  __device__ static float get(uint16_t x) {
+    return __uint_as_float(uint32_t(x) << 16);
+  }
+  // round to nearest even, NaN kept (quieted)
+  __device__ static uint16_t put(float v) {
+    const uint32_t u = __float_as_uint(v);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return uint16_t((u >> 16) | 0x40u);
+    return uint16_t((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+  }
+};
+
+// VEC elements as fp32: one 16-byte load (or less), or single elements
+template <int DT, int VEC>
+__device__ __forceinline__ void load_vec(const void *p, float (&v)[VEC]) {
+  using T = typename Elem<DT>::type;
+  if constexpr (VEC == 1) {
+    v[0] = Elem<DT>::get(*static_cast<const T *>(p));
+  } else {
+    typedef T tv __attribute__((ext_vector_type(VEC)));
+    const tv x = *static_cast<const tv *>(p);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = Elem<DT>::get(x[e]);
+  }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void store_vec(void *p, const float (&v)[VEC]) {
+  using T = typename Elem<DT>::type;
+  if constexpr (VEC == 1) {
+    *static_cast<T *>(p) = Elem<DT>::put(v[0]);
+  } else {
+    typedef T tv __attribute__((ext_vector_type(VEC)));
+    tv x;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[e] = Elem<DT>::put(v[e]);
+    *static_cast<tv *>(p) = x;
+  }
+}
+
+__device__ __forceinline__ int64_t load_id(const void *ids, int64_t t,
+                                           int ids64) {
+  return ids64 ? static_cast<const int64_t *>(ids)[t]
+               : int64_t(static_cast<const int32_t *>(ids)[t]);
+}
+
+// -- lookup ------------------------------------------------------------------
+constexpr int kLookVecs = 4;  // vectors of a row per lane
+
+// One wave per token and stretch of 64 * kLookVecs vectors of its row.
+template <int DT, int VEC>
+__global__ __launch_bounds__(kBlock) void embed_lookup_kernel(
+    const char *__restrict__ table, int64_t row_bytes, int64_t vocab,
+    const void *__restrict__ ids, int ids64, int64_t tokens, int64_t dim,
+    int stretches, float scale, char *__restrict__ out) {
+  constexpr int kE = sizeof(typename Elem<DT>::type);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave =
+      __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int64_t unit = int64_t(blockIdx.x) * kWaves + wave;
+  if (unit >= tokens * stretches) return;
+  const int64_t t = unit / stretches;
+  const int64_t c0 = (unit % stretches) * (kWave * kLookVecs * VEC);
+  const int64_t id = load_id(ids, t, ids64);
+  const bool ok = id >= 0 && id < vocab;
+  const char *src = table + (ok ? id : 0) * row_bytes;
+  char *dst = out + t * dim * kE;
+  float v[kLookVecs][VEC];
+#pragma unroll
+  for (int k = 0; k < kLookVecs; ++k) {
+    const int64_t c = c0 + (k * kWave + lane) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[k][e] = 0.0f;
+    if (ok && c < dim) load_vec<DT, VEC>(src + c * kE, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kLookVecs; ++k) {
+    const int64_t c = c0 + (k * kWave + lane) * VEC;
+    if (c < dim) {
+      if (ok) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[k][e] = __fmul_rn(v[k][e], scale);
+      }
+      store_vec<DT, VEC>(dst + c * kE, v[k]);
+    }
+  }
+}
+
+// -- gradient: keys and sort ---------------------------------------------------
+struct Part {
+  const void *ids;
+  const char *rows;
+  int64_t row_bytes;
+  int64_t start;  // first token of the part
+  float coef;
+  int32_t ids64;
+};
+struct Parts {
+  int n;
+  int64_t end;  // tokens up to the end of the last part here
+  Part part[kMaxParts];
+};
+
+// Arrays of a call, in its workspace.
+struct Sort {
+  uint32_t *key[2];
+  uint32_t *tok[2];
+  const char **row;  // by token
+  float *coef;       // by token
+  uint32_t *hist;    // [digits][blocks]
+  float *partial;    // [chunk][head, tail][dim]
+};
+
+// Key of every token of these parts: its row, or V for padding.
+__global__ __launch_bounds__(kBlock) void embed_key_kernel(Parts P, Sort W,
+                                                           uint32_t vocab) {
+  for (int64_t t = P.part[0].start + int64_t(blockIdx.x) * kBlock +
+                   threadIdx.x;
+       t < P.end; t += int64_t(gridDim.x) * kBlock) {
+    int lo = 0, hi = P.n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (P.part[mid].start <= t) lo = mid;
+      else hi = mid;
+    }
+    const Part &p = P.part[lo];
+    const int64_t i = t - p.start;
+    const int64_t id = load_id(p.ids, i, p.ids64);
+    W.key[0][t] = id >= 0 && id < int64_t(vocab) ? uint32_t(id) : vocab;
+    W.tok[0][t] = uint32_t(t);
+    W.row[t] = p.rows + i * p.row_bytes;
+    W.coef[t] = p.coef;
+  }
+}
+
+// Rank of every token of a workgroup's tile among the tile's tokens of the
+// same digit, in order: wave w owns tokens [256 w, 256 w + 256) in rounds of
+// 64; cnt[digit][wave] ends as the wave's count of the digit.
+__device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
+                                           const bool (&in)[kRounds],
+                                           int shift, int bits,
+                                           uint16_t *cnt,
+                                           uint32_t (&rank)[kRounds]) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const uint32_t mask = (1u << bits) - 1u;
+  for (int i = threadIdx.x; i < (kSortWaves << bits); i += kSortBlock)
+    cnt[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const uint32_t d = (key[k] >> shift) & mask;
+    uint64_t same = __ballot(in[k]);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t m = __ballot((d >> b) & 1u);
+      same &= ((d >> b) & 1u) ? m : ~m;
+    }
+    uint16_t *c = cnt + d * kSortWaves + wave;
+    const uint32_t before = in[k] ? *c : 0u;
+    rank[k] = before + __popcll(same & ((1ull << lane) - 1ull));
+    // the whole wave has read its counters (one instruction stream); the
+    // digit's last lane leaves the new count
+    __builtin_amdgcn_wave_barrier();
+    if (in[k] && (same >> lane) == 1ull)
+      *c = uint16_t(before + __popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void load_tile(const Sort &W, int src,
+                                          int64_t tokens, uint32_t (&key)[4],
+                                          uint32_t (&tok)[4], bool (&in)[4],
+                                          int64_t base) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t t = base + wave * (kRounds * kWave) + k * kWave + lane;
+    in[k] = t < tokens;
+    key[k] = in[k] ? W.key[src][t] : 0u;
+    tok[k] = in[k] ? W.tok[src][t] : 0u;
+  }
+}
+
+// hist[digit][block]
+__global__ __launch_bounds__(kSortBlock) void embed_hist_kernel(
+    Sort W, int src, int64_t tokens, int shift, int bits, int blocks) {
+  __shared__ uint32_t h[1 << kMaxDigit];
+  const int digits = 1 << bits;
+  for (int i = threadIdx.x; i < digits; i += kSortBlock) h[i] = 0;
+  __syncthreads();
+  const int64_t base = int64_t(blockIdx.x) * kTile;
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t t = base + k * kSortBlock + threadIdx.x;
+    if (t < tokens)
+      atomicAdd(&h[(W.key[src][t] >> shift) & (digits - 1)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < digits; i += kSortBlock)
+    W.hist[int64_t(i) * blocks + blockIdx.x] = h[i];
+}
+
+// Exclusive sum over the workgroup's kSortBlock values, in thread order.
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v,
+                                                    uint32_t *scratch) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  uint32_t s = v;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t u = __shfl_up(s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == kWave - 1) scratch[wave] = s;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w) before += scratch[w];
+  __syncthreads();
+  return before + s - v;
+}
+
+// One stable pass: every token of tile b goes to the digit's start plus the
+// digit's tokens in earlier tiles and waves plus its rank.
+__global__ __launch_bounds__(kSortBlock) void embed_scatter_kernel(
+    Sort W, int src, int64_t tokens, int shift, int bits, int blocks) {
+  __shared__ uint16_t cnt[kSortWaves << kMaxDigit];
+  __shared__ uint32_t at[1 << kMaxDigit];
+  __shared__ uint32_t scratch[kSortWaves];
+  uint32_t key[kRounds], tok[kRounds], rank[kRounds];
+  bool in[kRounds];
+  load_tile(W, src, tokens, key, tok, in, int64_t(blockIdx.x) * kTile);
+  const int digits = 1 << bits;
+  // thread d: digit d's total and its tokens in earlier tiles
+  uint32_t total = 0, mine = 0;
+  if (int(threadIdx.x) < digits) {
+    const uint32_t *h = W.hist + int64_t(threadIdx.x) * blocks;
+    for (int b = 0; b < blocks; ++b) {
+      if (b == int(blockIdx.x)) mine = total;
+      total += h[b];
+    }
+  }
+  const uint32_t first = block_exclusive(total, scratch);
+  if (int(threadIdx.x) < digits) at[threadIdx.x] = first + mine;
+  tile_ranks(key, in, shift, bits, cnt, rank);
+  const int wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    if (!in[k]) continue;
+    const uint32_t d = (key[k] >> shift) & (digits - 1);
+    uint32_t o = at[d] + rank[k];
+    for (int w = 0; w < wave; ++w) o += cnt[d * kSortWaves + w];
+    W.key[src ^ 1][o] = key[k];
+    W.tok[src ^ 1][o] = tok[k];
+  }
+}
+
+// -- gradient: sums ------------------------------------------------------------
+struct Out {
+  char *out;
+  int64_t row_bytes, dim, vocab, tokens;
+  int chunk, slices, accumulate;
+  int64_t chunks;
+  const uint32_t *key, *tok;
+};
+
+// first position in key[lo, hi) with key >= x, by the whole wave: 64 probes
+// a round
+__device__ __forceinline__ int64_t wave_lower_bound(const uint32_t *key,
+                                                    int64_t lo, int64_t hi,
+                                                    uint32_t x) {
+  const int lane = threadIdx.x & (kWave - 1);
+  while (hi > lo) {
+    const int64_t step = (hi - lo + kWave - 1) / kWave;
+    const int64_t p = lo + lane * step;
+    // probes whose key is below x: all before the answer
+    const uint64_t below = __ballot(p < hi && key[p < hi ? p : hi - 1] < x);
+    const int c = __popcll(below);
+    if (c == 0) return lo;
+    const int64_t nlo = lo + (c - 1) * step + 1;
+    const int64_t nhi = lo + c * step;
+    hi = nhi < hi ? nhi : hi;
+    lo = nlo;
+  }
+  return lo;
+}
+
+// Row sums of one chunk of sorted tokens and one slice of columns per wave;
+// workgroups past those write the zero rows that no token names.
+template <int GT, int OT, int VEC>
+__global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
+                                                           int sum_blocks,
+                                                           int zero_rows) {
+  constexpr int kGE = sizeof(typename Elem<GT>::type);
+  constexpr int kOE = sizeof(typename Elem<OT>::type);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave =
+      __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  if (int(blockIdx.x) >= sum_blocks) {
+    const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * zero_rows;
+    const int64_t r1 = r0 + zero_rows < O.vocab ? r0 + zero_rows : O.vocab;
+    const int64_t a = wave_lower_bound(O.key, 0, O.tokens, uint32_t(r0));
+    const int64_t b = wave_lower_bound(O.key, a, O.tokens, uint32_t(r1));
+    for (int64_t r = r0 + wave; r < r1; r += kWaves) {
+      const int64_t p = wave_lower_bound(O.key, a, b, uint32_t(r));
+      if (p < b && O.key[p] == uint32_t(r)) continue;
+      char *dst = O.out + r * O.row_bytes;
+      const float z[VEC] = {};
+      for (int64_t c = int64_t(lane) * VEC; c < O.dim; c += kWave * VEC)
+        store_vec<OT, VEC>(dst + c * kOE, z);
+    }
+    return;
+  }
+  const int64_t unit = int64_t(blockIdx.x) * kWaves + wave;
+  if (unit >= O.chunks * O.slices) return;
+  const int64_t chunk = unit / O.slices;
+  const int64_t c = ((unit % O.slices) * kWave + lane) * VEC;
+  const bool mine = c < O.dim;
+  const int64_t p0 = chunk * O.chunk;
+  const int64_t left = O.tokens - p0;
+  const int cnt = int(left < O.chunk ? left : O.chunk);
+  // lane i holds token i of the chunk
+  const uint32_t none = uint32_t(O.vocab);
+  uint32_t k = none;
+  const char *row = nullptr;
+  float coef = 0.0f;
+  if (lane < cnt) {
+    k = O.key[p0 + lane];
+    if (k != none) {
+      const uint32_t t = O.tok[p0 + lane];
+      row = W.row[t];
+      coef = W.coef[t];
+    }
+  }
+  // padding sorts last
+  const int valid = __popcll(__ballot(k != none));
+  if (valid == 0) return;
+  const uint32_t prev = p0 > 0 ? O.key[p0 - 1] : none;
+  const uint32_t next =
+      valid == cnt && p0 + cnt < O.tokens ? O.key[p0 + cnt] : none;
+  float acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+  bool head = __builtin_amdgcn_readlane(k, 0) == prev;
+  constexpr int kAhead = 8;
+  for (int i0 = 0; i0 < valid; i0 += kAhead) {
+    float v[kAhead][VEC];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u < valid ? i0 + u : valid - 1;
+      const uint64_t a = reinterpret_cast<uint64_t>(row);
+      const uint32_t alo = __builtin_amdgcn_readlane(uint32_t(a), i);
+      const uint32_t ahi = __builtin_amdgcn_readlane(uint32_t(a >> 32), i);
+      const char *src =
+          reinterpret_cast<const char *>((uint64_t(ahi) << 32) | alo);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[u][e] = 0.0f;
+      if (mine) load_vec<GT, VEC>(src + c * kGE, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u;
+      if (i >= valid) break;
+      const float w =
+          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(coef), i));
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] = __builtin_fmaf(v[u][e], w, acc[e]);
+      const uint32_t key = __builtin_amdgcn_readlane(k, i);
+      const uint32_t after =
+          i + 1 < valid ? __builtin_amdgcn_readlane(k, i + 1) : next;
+      const bool open = i + 1 == valid && after == key;  // goes on
+      if (after == key && !open) continue;
+      if (mine) {
+        if (head || open) {
+          float *dst = W.partial + (chunk * 2 + (head ? 0 : 1)) * O.dim + c;
+          store_vec<FSAGG_F32, VEC>(dst, acc);
+        } else {
+          char *dst = O.out + int64_t(key) * O.row_bytes + c * kOE;
+          if (O.accumulate) {
+            float o[VEC];
+            load_vec<OT, VEC>(dst, o);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] = __fadd_rn(o[e], acc[e]);
+          }
+          store_vec<OT, VEC>(dst, acc);
+        }
+      }
+      head = false;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+    }
+  }
+}
+
+// Rows whose tokens cross chunks: the wave of the chunk in which the row
+// begins adds the later chunks' partial sums in order.
+template <int OT, int VEC>
+__global__ __launch_bounds__(kBlock) void embed_join_kernel(Out O, Sort W) {
+  constexpr int kOE = sizeof(typename Elem<OT>::type);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave =
+      __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int64_t unit = int64_t(blockIdx.x) * kWaves + wave;
+  if (unit >= (O.chunks - 1) * O.slices) return;
+  const int64_t chunk = unit / O.slices;
+  const int64_t c = ((unit % O.slices) * kWave + lane) * VEC;
+  const int64_t end = (chunk + 1) * O.chunk;  // < tokens: not the last chunk
+  const uint32_t key = O.key[end - 1];
+  if (key == uint32_t(O.vocab) || O.key[end] != key) return;
+  // the row began here unless it fills the chunk and began before
+  if (O.key[chunk * O.chunk] == key && chunk > 0 &&
+      O.key[chunk * O.chunk - 1] == key)
+    return;
+  // chunks after this one that the row reaches
+  int64_t last = chunk + 1;
+  while (last + 1 < O.chunks && O.key[(last + 1) * O.chunk] == key) ++last;
+  if (c >= O.dim) return;
+  float acc[VEC];
+  load_vec<FSAGG_F32, VEC>(W.partial + (chunk * 2 + 1) * O.dim + c, acc);
+  for (int64_t q = chunk + 1; q <= last; ++q) {
+    float v[VEC];
+    load_vec<FSAGG_F32, VEC>(W.partial + q * 2 * O.dim + c, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = __fadd_rn(acc[e], v[e]);
+  }
+  char *dst = O.out + int64_t(key) * O.row_bytes + c * kOE;
+  if (O.accumulate) {
+    float o[VEC];
+    load_vec<OT, VEC>(dst, o);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = __fadd_rn(o[e], acc[e]);
+  }
+  store_vec<OT, VEC>(dst, acc);
+}
+
+// -- host ----------------------------------------------------------------------
+int elem_bytes(int dt) { return dt == FSAGG_F32 ? 4 : 2; }
+bool float_dtype(int dt) {
+  return dt == FSAGG_F32 || dt == FSAGG_F16 || dt == FSAGG_BF16;
+}
+
+// f(integral constant): the element type as a template argument
+template <typename F>
+void with_dtype(int dt, F f) {
+  if (dt == FSAGG_F32) f(std::integral_constant<int, FSAGG_F32>());
+  else if (dt == FSAGG_F16) f(std::integral_constant<int, FSAGG_F16>());
+  else f(std::integral_constant<int, FSAGG_BF16>());
+}
+
+int64_t chunk_tokens(int64_t tokens) {
+  (void)tokens;
+  return 32;
+}
+
+struct Sizes {
+  int64_t tokens, dim, chunk, chunks, blocks;
+  int bits, passes, digit;
+  size_t key, row, coef, hist, partial, total;
+};
+
+Sizes sizes_of(int64_t tokens, int64_t dim, int64_t vocab) {
+  Sizes Z;
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  Z.tokens = tokens;
+  Z.dim = dim;
+  Z.chunk = chunk_tokens(tokens);
+  Z.chunks = (tokens + Z.chunk - 1) / Z.chunk;
+  Z.blocks = (tokens + kTile - 1) / kTile;
+  Z.bits = 1;
+  while (Z.bits < 32 && (vocab >> Z.bits)) ++Z.bits;  // keys 0 .. vocab
+  Z.passes = (Z.bits + kMaxDigit - 1) / kMaxDigit;
+  Z.digit = (Z.bits + Z.passes - 1) / Z.passes;
+  Z.key = up(4 * tokens);
+  Z.row = up(8 * tokens);
+  Z.coef = up(4 * tokens);
+  Z.hist = up(size_t(4) * Z.blocks << Z.digit);
+  Z.partial = Z.chunks > 1 ? up(size_t(8) * Z.chunks * dim) : 0;
+  Z.total = 4 * Z.key + Z.row + Z.coef + Z.hist + Z.partial;
+  return Z;
+}
+
+}  // namespace
+}  // namespace fsagg
+
+using namespace fsagg;
+
+extern "C" int fsagg_embed_lookup(const void *table, int64_t vocab,
+                                  int64_t dim, int64_t row_stride, int dtype,
+                                  const void *ids, int ids64, int64_t tokens,
+                                  float scale, void *out,
+                                  fsagg_stream_t stream) {
+  const char *what = "fsagg_embed_lookup";
+  if (vocab < 0 || dim < 0 || tokens < 0 || !float_dtype(dtype) ||
+      (tokens > 0 && dim > 0 && (!ids || !out || (vocab > 0 && !table)))) {
+    set_error("%s: invalid argument", what);
+    return FSAGG_EINVAL;
+  }
+  if (tokens == 0 || dim == 0) return FSAGG_OK;
+  const int e = elem_bytes(dtype);
+  const bool vec = (dim * e) % 16 == 0 && (row_stride * e) % 16 == 0 &&
+                   aligned16(table) && aligned16(out);
+  const int v = vec ? 16 / e : 1;
+  const int64_t per = int64_t(kWave) * kLookVecs * v;
+  const int64_t stretches = (dim + per - 1) / per;
+  const int64_t grid = (tokens * stretches + kWaves - 1) / kWaves;
+  if (stretches > INT32_MAX || grid > kMaxGrid) {
+    set_error("%s: %lld tokens of %lld columns are too many for one call",
+              what, (long long)tokens, (long long)dim);
+    return FSAGG_EINVAL;
+  }
+  with_dtype(dtype, [&](auto dt) {
+    constexpr int D = decltype(dt)::value;
+    if (vec)
+      hipLaunchKernelGGL((embed_lookup_kernel<D, Elem<D>::kVec>), dim3(grid),
+                         dim3(kBlock), 0, as_stream(stream),
+                         static_cast<const char *>(table), row_stride * e,
+                         vocab, ids, ids64, tokens, dim, int(stretches),
+                         scale, static_cast<char *>(out));
+    else
+      hipLaunchKernelGGL((embed_lookup_kernel<D, 1>), dim3(grid),
+                         dim3(kBlock), 0, as_stream(stream),
+                         static_cast<const char *>(table), row_stride * e,
+                         vocab, ids, ids64, tokens, dim, int(stretches),
+                         scale, static_cast<char *>(out));
+  });
+  return check_launch(what);
+}
+
+extern "C" size_t fsagg_embed_grad_workspace_bytes(int64_t tokens,
+                                                   int64_t dim,
+                                                   int64_t vocab) {
+  if (tokens <= 0 || dim <= 0 || vocab < 0) return 0;
+  return sizes_of(tokens, dim, vocab).total;
+}
+
+extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
+                                int dtype, int64_t vocab, int64_t dim,
+                                void *out, int out_dtype, int64_t out_stride,
+                                int accumulate, void *workspace,
+                                size_t workspace_bytes,
+                                fsagg_stream_t stream) {
+  const char *what = "fsagg_embed_grad";
+  if (nparts < 0 || (nparts > 0 && !parts) || vocab < 0 || dim < 0 ||
+      !float_dtype(dtype) || !float_dtype(out_dtype) ||
+      (vocab > 0 && dim > 0 && !out)) {
+    set_error("%s: invalid argument", what);
+    return FSAGG_EINVAL;
+  }
+  if (vocab > FSAGG_EMBED_MAX_ROWS) {
+    set_error("%s: %lld rows, at most %d", what, (long long)vocab,
+              FSAGG_EMBED_MAX_ROWS);
+    return FSAGG_EINVAL;
+  }
+  const int e = elem_bytes(dtype), oe = elem_bytes(out_dtype);
+  // the vector width is the narrower type's: 16 bytes of gradients, and the
+  // same number of result elements
+  const int vec_elems = dtype == FSAGG_F32 ? 4 : 8;
+  bool vec = dim % vec_elems == 0 && (out_stride * oe) % 16 == 0 &&
+             aligned16(out);
+  int64_t tokens = 0;
+  for (int i = 0; i < nparts; ++i) {
+    const fsagg_embed_part &p = parts[i];
+    if (p.tokens < 0 || (p.tokens > 0 && dim > 0 && (!p.ids || !p.rows))) {
+      set_error("%s: part %d: invalid argument", what, i);
+      return FSAGG_EINVAL;
+    }
+    if (p.tokens > 0)
+      vec = vec && (p.row_stride * e) % 16 == 0 && aligned16(p.rows);
+    tokens += p.tokens;
+    if (tokens > FSAGG_EMBED_MAX_TOKENS) {
+      set_error("%s: more than %d tokens", what, FSAGG_EMBED_MAX_TOKENS);
+      return FSAGG_EINVAL;
+    }
+  }
+  if (vocab == 0 || dim == 0 || (tokens == 0 && accumulate)) return FSAGG_OK;
+  hipStream_t s = as_stream(stream);
+  const Sizes Z = sizes_of(tokens, dim, vocab);
+  if (tokens > 0 && (!workspace || workspace_bytes < Z.total)) {
+    set_error("%s: workspace of %zu bytes, %zu needed", what,
+              workspace ? workspace_bytes : size_t(0), Z.total);
+    return FSAGG_ESPACE;
+  }
+  if (!aligned16(workspace)) {
+    set_error("%s: workspace must be 16-byte aligned", what);
+    return FSAGG_EINVAL;
+  }
+  Sort W = {};
+  char *at = static_cast<char *>(workspace);
+  auto take = [&](size_t b) {
+    char *p = at;
+    at += b;
+    return p;
+  };
+  if (tokens > 0) {
+    for (int i = 0; i < 2; ++i) {
+      W.key[i] = reinterpret_cast<uint32_t *>(take(Z.key));
+      W.tok[i] = reinterpret_cast<uint32_t *>(take(Z.key));
+    }
+    W.row = reinterpret_cast<const char **>(take(Z.row));
+    W.coef = reinterpret_cast<float *>(take(Z.coef));
+    W.hist = reinterpret_cast<uint32_t *>(take(Z.hist));
+    W.partial = reinterpret_cast<float *>(take(Z.partial));
+  }
+  int64_t start = 0;
+  for (int i = 0; i < nparts;) {
+    Parts P;
+    P.n = 0;
+    const int64_t first = start;
+    for (; i < nparts && P.n < kMaxParts; ++i) {
+      const fsagg_embed_part &p = parts[i];
+      if (p.tokens == 0) continue;
+      Part &q = P.part[P.n++];
+      q.ids = p.ids;
+      q.rows = static_cast<const char *>(p.rows);
+      q.row_bytes = p.row_stride * e;
+      q.start = start;
+      q.coef = p.coef;
+      q.ids64 = p.ids64;
+      start += p.tokens;
+    }
+    P.end = start;
+    if (P.n == 0) continue;
+    hipLaunchKernelGGL(embed_key_kernel,
+                       dim3(stream_grid(start - first, kBlock, 2048)),
+                       dim3(kBlock), 0, s, P, W, uint32_t(vocab));
+  }
+  int src = 0;
+  if (tokens > 0)
+    for (int p = 0; p < Z.passes; ++p, src ^= 1) {
+      hipLaunchKernelGGL(embed_hist_kernel, dim3(Z.blocks), dim3(kSortBlock),
+                         0, s, W, src, tokens, p * Z.digit, Z.digit,
+                         int(Z.blocks));
+      hipLaunchKernelGGL(embed_scatter_kernel, dim3(Z.blocks),
+                         dim3(kSortBlock), 0, s, W, src, tokens, p * Z.digit,
+                         Z.digit, int(Z.blocks));
+    }
+  Out O;
+  O.out = static_cast<char *>(out);
+  O.row_bytes = out_stride * oe;
+  O.dim = dim;
+  O.vocab = vocab;
+  O.tokens = tokens;
+  O.chunk = int(Z.chunk);
+  O.chunks = Z.chunks;
+  O.accumulate = accumulate;
+  O.key = W.key[src];
+  O.tok = W.tok[src];
+  const int v = vec ? vec_elems : 1;
+  O.slices = int((dim + int64_t(kWave) * v - 1) / (int64_t(kWave) * v));
+  const int64_t sum_blocks = (Z.chunks * O.slices + kWaves - 1) / kWaves;
+  // rows per zero workgroup: about 64 KiB
+  int64_t zero_rows = 65536 / (dim * oe);
+  if (zero_rows < kWaves) zero_rows = kWaves;
+  if (zero_rows > 1024) zero_rows = 1024;
+  const int64_t zero_blocks =
+      accumulate ? 0 : (vocab + zero_rows - 1) / zero_rows;
+  const int64_t join_blocks =
+      Z.chunks > 1 ? ((Z.chunks - 1) * O.slices + kWaves - 1) / kWaves : 0;
+  if (sum_blocks + zero_blocks > kMaxGrid) {
+    set_error("%s: %lld tokens of %lld columns are too many for one call",
+              what, (long long)tokens, (long long)dim);
+    return FSAGG_EINVAL;
+  }
+  with_dtype(dtype, [&](auto gt) {
+    with_dtype(out_dtype, [&](auto ot) {
+      constexpr int D = decltype(gt)::value, Q = decltype(ot)::value;
+      constexpr int V = Elem<D>::kVec;
+      const dim3 grid(unsigned(sum_blocks + zero_blocks)), block(kBlock);
+      if (vec)
+        hipLaunchKernelGGL((embed_sum_kernel<D, Q, V>), grid, block, 0, s, O,
+                           W, int(sum_blocks), int(zero_rows));
+      else
+        hipLaunchKernelGGL((embed_sum_kernel<D, Q, 1>), grid, block, 0, s, O,
+                           W, int(sum_blocks), int(zero_rows));
+      if (join_blocks == 0) return;
+      const dim3 jg{unsigned(join_blocks)};
+      if (vec)
+        hipLaunchKernelGGL((embed_join_kernel<Q, V>), jg, block, 0, s, O, W);
+      else
+        hipLaunchKernelGGL((embed_join_kernel<Q, 1>), jg, block, 0, s, O, W);
+    });
+  });
+  return check_launch(what);
+}

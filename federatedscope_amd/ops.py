@@ -1699,3 +1699,335 @@ def normbound_prescale(sq, bound):
         sq.data_ptr(), sq.shape[0], sq.shape[1], float(_np.float32(bound)),
         pre.data_ptr(), _stream(sq.device)), 'fsagg_normbound_prescale_f32')
     return pre
+
+
+# -- learning operators: Newton-Schulz, Muon, embedding rows -------------------
+_FLOAT_CODE = {torch.float32: L.FSAGG_F32, torch.float16: L.FSAGG_F16,
+               torch.bfloat16: L.FSAGG_BF16}
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_MUON_ADJUST = {None: L.FSAGG_MUON_ORIGINAL,
+                'original': L.FSAGG_MUON_ORIGINAL,
+                'match_rms_adamw': L.FSAGG_MUON_MATCH_RMS}
+
+
+class _OnDevice:
+    """Makes ``device`` current for a launch on its stream (a no-op when it
+    already is)."""
+    __slots__ = ('guard', )
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() \
+            else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _extent(t):
+    """[first, last) byte addresses a strided tensor covers."""
+    p = t.data_ptr()
+    if t.is_contiguous():
+        return p, p + t.numel() * t.element_size()
+    span = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return p, p + (span + 1) * t.element_size()
+
+
+def _overlap(a, b):
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (al, ah), (bl, bh) = _extent(a), _extent(b)
+    return al < bh and bl < ah
+
+
+def _check_float_cuda(t, what, device=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError('%s must be a torch.Tensor' % what)
+    if t.device.type != 'cuda':
+        raise ValueError('%s must live on a GPU (got %s)' % (what, t.device))
+    if device is not None and t.device != device:
+        raise ValueError('%s on %s, expected %s' % (what, t.device, device))
+    if t.dtype not in _FLOAT_CODE:
+        raise ValueError('%s must be float32, float16 or bfloat16 (got %s)' %
+                         (what, t.dtype))
+
+
+def _scratch(device, nbytes):
+    """Per-call workspace from torch's allocator, on the current stream: no
+    two calls, streams or captured graphs share one."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8,
+                       device=device)
+
+
+def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7,
+                  out=None):
+    """Orthogonalise update matrices by Newton-Schulz products: with X = the
+    wide orientation of G / max(|G|_F, eps), ``steps`` times A = X X^T,
+    X <- aX + (bA + cA^2)X, turned back (the singular vectors of G with
+    singular values near 1).
+
+    ``g``: a matrix [rows, cols], a batch [n, rows, cols], or a list of
+    matrices and batches of any shapes (one run of launches for all of them);
+    float32, float16 or bfloat16, any strides.  Returns a new contiguous
+    tensor (list) of g's dtype, or ``out`` (contiguous, of any of the three
+    dtypes, not overlapping any input).  The arithmetic is as exact as
+    float32 products.  NaN or infinity anywhere in a matrix makes all of it
+    NaN; a zero matrix stays zero.  Not differentiable."""
+    many = isinstance(g, (list, tuple))
+    gs = list(g) if many else [g]
+    if not gs:
+        return []
+    outs = [None] * len(gs) if out is None else (
+        list(out) if many else [out])
+    if len(outs) != len(gs):
+        raise ValueError('%d outputs for %d inputs' % (len(outs), len(gs)))
+    coef = [float(x) for x in coefficients]
+    if len(coef) != 3:
+        raise ValueError('coefficients must be exactly 3 values')
+    dev = None
+    lib = L.load()
+    table = (L.NsMat * len(gs))()
+    need = 0
+    for i, x in enumerate(gs):
+        _check_float_cuda(x, 'matrix %d' % i, dev)
+        dev = x.device
+        if x.dim() not in (2, 3):
+            raise ValueError('matrix %d must be [rows, cols] or [n, rows, '
+                             'cols] (got %s)' % (i, tuple(x.shape)))
+        o = outs[i]
+        if o is None:
+            o = outs[i] = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        else:
+            _check_float_cuda(o, 'out %d' % i, dev)
+            if o.shape != x.shape or not o.is_contiguous():
+                raise ValueError('out %d must be a contiguous %s tensor' %
+                                 (i, tuple(x.shape)))
+        batch = x.shape[0] if x.dim() == 3 else 1
+        rows, cols = x.shape[-2:]
+        t = table[i]
+        t.g, t.out = x.data_ptr(), o.data_ptr()
+        t.rows, t.cols, t.batch = rows, cols, batch
+        t.batch_stride = x.stride(0) if x.dim() == 3 else 0
+        t.row_stride, t.col_stride = x.stride(-2), x.stride(-1)
+        t.dtype, t.out_dtype = _FLOAT_CODE[x.dtype], _FLOAT_CODE[o.dtype]
+        need += lib.fsagg_newton_schulz_workspace_bytes(rows, cols, batch)
+    if out is not None:
+        for i, o in enumerate(outs):
+            if any(_overlap(o, x) for x in gs) or \
+                    any(_overlap(o, p) for p in outs[:i]):
+                raise ValueError('out %d overlaps another tensor' % i)
+    with _OnDevice(dev):
+        ws = _scratch(dev, need)
+        L.check(lib.fsagg_newton_schulz(
+            table, len(gs), int(steps), (ctypes.c_double * 3)(*coef),
+            float(eps), ws.data_ptr(), ws.numel(), _stream(dev)),
+                'fsagg_newton_schulz')
+    return outs if many else outs[0]
+
+
+def muon_step(params, avgs, bufs, lr, momentum=0.95, nesterov=True,
+              weight_decay=0.1, steps=5, coefficients=NS_COEFFICIENTS,
+              eps=1e-7, adjust_lr=None, maximize=False):
+    """One Muon step of matrix parameters toward their averages, in place on
+    ``params`` and their momentum ``bufs`` (zero before the first step):
+    g = param - avg (negated for ``maximize``), buf += (1 - momentum)
+    (g - buf), u = g + momentum (buf - g) if ``nesterov`` else buf,
+    param = (1 - lr weight_decay) param - lr' newton_schulz(u), with
+    lr' = lr sqrt(max(1, rows / cols)) (``adjust_lr`` None or 'original') or
+    0.2 lr sqrt(max(rows, cols)) ('match_rms_adamw').
+
+    Lists of contiguous float32 GPU tensors; params are [rows, cols], avgs
+    and bufs hold as many elements in any shape.  No written tensor may
+    overlap another."""
+    if not len(params) == len(avgs) == len(bufs):
+        raise ValueError('%d params, %d averages, %d momentum buffers' %
+                         (len(params), len(avgs), len(bufs)))
+    if adjust_lr not in _MUON_ADJUST:
+        raise ValueError('Adjust learning rate function %s is not supported' %
+                         (adjust_lr, ))
+    coef = [float(x) for x in coefficients]
+    if len(coef) != 3:
+        raise ValueError('coefficients must be exactly 3 values')
+    if not params:
+        return
+    lib = L.load()
+    dev = None
+    table = (L.MuonMat * len(params))()
+    need = 0
+    for i, (p, a, b) in enumerate(zip(params, avgs, bufs)):
+        for t, what in ((p, 'param'), (a, 'average'), (b, 'momentum')):
+            _check_f32_cuda(t, '%s %d' % (what, i), align=4)
+            if dev is not None and t.device != dev:
+                raise ValueError('%s %d on %s, expected %s' %
+                                 (what, i, t.device, dev))
+            dev = t.device
+            if t.numel() != p.numel():
+                raise ValueError('%s %d has %d elements, its param %d' %
+                                 (what, i, t.numel(), p.numel()))
+        if p.dim() != 2:
+            raise ValueError('Muon only supports 2D parameters whereas we '
+                             'found a parameter with size: %s' % (p.shape, ))
+        m = table[i]
+        m.param, m.avg, m.momentum = p.data_ptr(), a.data_ptr(), b.data_ptr()
+        m.rows, m.cols = p.shape
+        need += lib.fsagg_newton_schulz_workspace_bytes(*p.shape, 1)
+    _check_disjoint(list(params) + list(bufs), list(avgs))
+    hp = L.MuonParams(float(lr), float(momentum), float(weight_decay), *coef,
+                      float(eps), int(steps), int(bool(nesterov)),
+                      int(bool(maximize)), _MUON_ADJUST[adjust_lr])
+    with _OnDevice(dev):
+        ws = _scratch(dev, need)
+        L.check(lib.fsagg_muon_step_f32(table, len(params), ctypes.byref(hp),
+                                        ws.data_ptr(), ws.numel(),
+                                        _stream(dev)), 'fsagg_muon_step_f32')
+
+
+def _check_disjoint(written, read):
+    """No written tensor overlaps any other (the read ones may coincide)."""
+    spans = sorted([_extent(t) + (1, ) for t in written if t.numel()] +
+                   [_extent(t) + (0, ) for t in read if t.numel()])
+    end, wend = 0, 0     # furthest end so far, of all and of written ones
+    for lo, hi, w in spans:
+        if lo < (end if w else wend):
+            raise ValueError('a tensor that is written overlaps another')
+        end = max(end, hi)
+        if w:
+            wend = max(wend, hi)
+
+
+def _check_ids(ids, what, device):
+    if not isinstance(ids, torch.Tensor):
+        raise TypeError('%s must be a torch.Tensor' % what)
+    if ids.device != device:
+        raise ValueError('%s on %s, expected %s' % (what, ids.device, device))
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError('%s must be int64 or int32 (got %s)' %
+                         (what, ids.dtype))
+    if not ids.is_contiguous():
+        raise ValueError('%s must be contiguous' % what)
+
+
+def _check_rows(t, what):
+    """A 2-D tensor whose rows are contiguous (any distance apart)."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError('%s must be 2-D with contiguous rows' % what)
+
+
+def embedding_lookup(table, ids, scale=1.0, out=None):
+    """out[..., :] = scale * table[ids[...], :], the product in float32 and
+    rounded once to the table's dtype (float32, float16, bfloat16).  A token
+    outside [0, len(table)) is padding: a zero row.  ``table`` is 2-D with
+    contiguous rows, ``ids`` a contiguous int64 or int32 tensor of any shape
+    on the same GPU; ``out`` (contiguous, not overlapping either) or a new
+    tensor [*ids.shape, dim] is returned.  Its gradient with respect to the
+    table is :func:`embedding_grad`."""
+    _check_float_cuda(table, 'table')
+    _check_rows(table, 'table')
+    dev = table.device
+    _check_ids(ids, 'ids', dev)
+    vocab, dim = table.shape
+    shape = tuple(ids.shape) + (dim, )
+    if out is None:
+        out = torch.empty(shape, dtype=table.dtype, device=dev)
+    else:
+        _check_float_cuda(out, 'out', dev)
+        if out.dtype != table.dtype or tuple(out.shape) != shape or \
+                not out.is_contiguous():
+            raise ValueError('out must be a contiguous %s tensor of shape %s' %
+                             (table.dtype, shape))
+        if _overlap(out, table) or _overlap(out, ids):
+            raise ValueError('out overlaps an input')
+    with _OnDevice(dev):
+        L.check(L.load().fsagg_embed_lookup(
+            table.data_ptr(), vocab, dim, table.stride(0),
+            _FLOAT_CODE[table.dtype], ids.data_ptr(),
+            int(ids.dtype == torch.int64), ids.numel(), float(scale),
+            out.data_ptr(), _stream(dev)), 'fsagg_embed_lookup')
+    return out
+
+
+def embedding_grad(ids, grad, num_rows, scale=1.0, weights=None, out=None,
+                   accumulate=False):
+    """The gradient of :func:`embedding_lookup` with respect to its table,
+    and the reduction of row-sparse client updates:
+    out[v] = [out[v] +] sum over t with ids[t] = v of scale * w * grad[t].
+
+    ``ids`` and ``grad`` are one token tensor and its rows ([*ids.shape,
+    dim]), or lists of them (one entry per client, read in place) with
+    ``weights`` one float per entry (default 1).  Tokens outside
+    [0, num_rows) are padding: their rows are not read.  Sums are float32, in
+    token order whatever the timing, and rounded once.  ``out`` [num_rows,
+    dim] (contiguous rows; any of the three float dtypes; default: new, of
+    grad's dtype) gets zeros in the rows no token names; with ``accumulate``
+    the sums are added to ``out`` (required) and its other rows are not
+    touched."""
+    many = isinstance(ids, (list, tuple))
+    ids = list(ids) if many else [ids]
+    grad = list(grad) if many else [grad]
+    if len(ids) != len(grad) or not ids:
+        raise ValueError('%d token tensors, %d gradients' %
+                         (len(ids), len(grad)))
+    if weights is None:
+        weights = [1.0] * len(ids)
+    if len(weights) != len(ids):
+        raise ValueError('%d weights for %d token tensors' %
+                         (len(weights), len(ids)))
+    num_rows = int(num_rows)
+    if num_rows < 0:
+        raise ValueError('num_rows must not be negative')
+    if accumulate and out is None:
+        raise ValueError('accumulate needs out')
+    lib = L.load()
+    dev = dt = dim = None
+    parts = (L.EmbedPart * len(ids))()
+    tokens = 0
+    for i, (x, g) in enumerate(zip(ids, grad)):
+        _check_float_cuda(g, 'gradient %d' % i, dev)
+        if dev is None:
+            dev, dt = g.device, g.dtype
+            if g.dim() < 1:
+                raise ValueError('gradient 0 must have at least 1 dimension')
+            dim = g.shape[-1]
+        elif g.dtype != dt:
+            raise ValueError('gradient %d is %s, the first %s' %
+                             (i, g.dtype, dt))
+        _check_ids(x, 'ids %d' % i, dev)
+        if tuple(g.shape) != tuple(x.shape) + (dim, ):
+            raise ValueError('gradient %d has shape %s for tokens %s of %d '
+                             'columns' % (i, tuple(g.shape), tuple(x.shape),
+                                          dim))
+        if g.dim() != 2:
+            if not g.is_contiguous():
+                raise ValueError('gradient %d must be contiguous' % i)
+            g = g.reshape(x.numel(), dim)
+        _check_rows(g, 'gradient %d' % i)
+        p = parts[i]
+        p.ids, p.rows = x.data_ptr(), g.data_ptr()
+        p.tokens, p.row_stride = x.numel(), g.stride(0)
+        p.coef = float(scale) * float(weights[i])
+        p.ids64 = int(x.dtype == torch.int64)
+        tokens += x.numel()
+    if out is None:
+        out = torch.empty((num_rows, dim), dtype=dt, device=dev)
+    else:
+        _check_float_cuda(out, 'out', dev)
+        if tuple(out.shape) != (num_rows, dim):
+            raise ValueError('out has shape %s, expected %s' %
+                             (tuple(out.shape), (num_rows, dim)))
+        _check_rows(out, 'out')
+        if out.numel() and out.shape[0] > 1 and out.stride(0) < dim:
+            raise ValueError('the rows of out overlap')
+        if any(_overlap(out, t) for t in ids + grad):
+            raise ValueError('out overlaps an input')
+    with _OnDevice(dev):
+        need = lib.fsagg_embed_grad_workspace_bytes(tokens, dim, num_rows)
+        ws = _scratch(dev, need)
+        L.check(lib.fsagg_embed_grad(
+            parts, len(ids), _FLOAT_CODE[dt], num_rows, dim, out.data_ptr(),
+            _FLOAT_CODE[out.dtype], out.stride(0), int(bool(accumulate)),
+            ws.data_ptr(), ws.numel(), _stream(dev)), 'fsagg_embed_grad')
+    return out

@@ -232,6 +232,123 @@ int fsagg_server_opt_step_f64(double *param, const double *avg,
                               fsagg_stream_t stream);
 
 /*
+ * Newton-Schulz orthogonalisation of update matrices (no reference
+ * counterpart of its own: torch.optim's Muon, which the reference's
+ * get_optimizer builds by name, core/auxiliaries/optimizer_builder.py:53-56,
+ * orthogonalises its momentum this way).  For each matrix G, m = min and
+ * n = max of its sides, X = the m x n orientation of G / max(|G|_F, eps):
+ *     A = X X^T,  X <- a X + (b A + c A^2) X      `steps` times,
+ * stored back in G's own orientation.  The arithmetic is as exact as fp32
+ * products (two fp16 limbs per value, fp32 sums, the norm in fp64); the
+ * result is rounded once to out_dtype.  A NaN or an infinity in a matrix
+ * makes the whole of that matrix NaN; a zero matrix gives zeros.
+ *   mats (host): nmat entries, each `batch` matrices of one shape; element
+ *     (i, j) of matrix z is g[z*batch_stride + i*row_stride + j*col_stride]
+ *     (elements; 0 and negative strides are allowed); out (device) is
+ *     contiguous [batch][rows][cols] and does not overlap any g.  dtype /
+ *     out_dtype: FSAGG_F32, FSAGG_F16 or FSAGG_BF16.  An entry with a side
+ *     or batch of 0 does nothing.
+ *   coefficients (host): a, b, c; refused when they let the iterates grow
+ *     past 15 (the usual 3.4445, -4.7750, 2.0315 stay below 1.3).
+ *   Workspace: the sum over the entries of
+ *     fsagg_newton_schulz_workspace_bytes(rows, cols, batch), 16-byte
+ *     aligned; its contents need not be set and nothing is kept in it.
+ */
+#define FSAGG_NS_MAX_SHORT 16384
+#define FSAGG_NS_MAX_LONG 1048576
+#define FSAGG_NS_MAX_ELEMS 1073741824
+typedef struct fsagg_ns_mat {
+  const void *g; /* (device) */
+  void *out;     /* (device) */
+  int64_t rows, cols, batch;
+  int64_t batch_stride, row_stride, col_stride;
+  int32_t dtype, out_dtype;
+} fsagg_ns_mat;
+size_t fsagg_newton_schulz_workspace_bytes(int64_t rows, int64_t cols,
+                                           int64_t batch);
+int fsagg_newton_schulz(const fsagg_ns_mat *mats, int nmat, int steps,
+                        const double *coefficients, double eps,
+                        void *workspace, size_t workspace_bytes,
+                        fsagg_stream_t stream);
+
+/*
+ * FedOpt's server step with Muon on matrix parameters, in place
+ * (fedopt_aggregator.py:26-44 with the torch.optim optimizer of that name):
+ *     g = param - avg                     (negated for maximize)
+ *     momentum <- momentum + (1 - mu) (g - momentum)
+ *     u = nesterov ? g + mu (momentum - g) : momentum
+ *     param <- (1 - lr wd) param - lr' NS(u)
+ * with NS as fsagg_newton_schulz and lr' = lr sqrt(max(1, rows / cols))
+ * (FSAGG_MUON_ORIGINAL) or 0.2 lr sqrt(max(rows, cols))
+ * (FSAGG_MUON_MATCH_RMS).  mats (host): nmat contiguous fp32 matrices, no
+ * two of which overlap; the momentum starts at zero.  Workspace as above
+ * with batch 1.
+ */
+enum fsagg_muon_adjust { FSAGG_MUON_ORIGINAL = 0, FSAGG_MUON_MATCH_RMS = 1 };
+typedef struct fsagg_muon_mat {
+  float *param;     /* (device) rows x cols */
+  const float *avg; /* (device) */
+  float *momentum;  /* (device) */
+  int64_t rows, cols;
+} fsagg_muon_mat;
+typedef struct fsagg_muon_params {
+  double lr, momentum, weight_decay, a, b, c, eps;
+  int32_t steps, nesterov, maximize, adjust;
+} fsagg_muon_params;
+int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
+                        const fsagg_muon_params *hp, void *workspace,
+                        size_t workspace_bytes, fsagg_stream_t stream);
+
+/*
+ * Rows of an embedding table by token:  out[t] = round(scale * E[ids[t]]),
+ * the product in fp32.  A token outside [0, vocab) is padding: a zero row.
+ * What a server sends a client that needs only its tokens' rows (the
+ * reference sends whole state dicts, core/workers/server.py:591-650).
+ *   table (device) vocab rows of dim elements of `dtype` (FSAGG_F32, _F16,
+ *     _BF16), row_stride elements apart; ids (device) int64 (ids64 != 0) or
+ *     int32; out (device) contiguous [tokens][dim] of the table's dtype,
+ *     not overlapping it.  Any alignment; 16-byte aligned rows are read 16
+ *     bytes at a time.
+ */
+int fsagg_embed_lookup(const void *table, int64_t vocab, int64_t dim,
+                       int64_t row_stride, int dtype, const void *ids,
+                       int ids64, int64_t tokens, float scale, void *out,
+                       fsagg_stream_t stream);
+
+/*
+ * The lookup's gradient, and the reduction of row-sparse uploads: the
+ * weighted sum of rows by token,
+ *     out[v] = [accumulate: out[v] +] sum over t, ids[t] = v, of
+ *              coef(part of t) * rows[t],
+ * the parts' tokens in order, in fp32, rounded once to out_dtype; without
+ * `accumulate` rows that no token names become zero, with it they are not
+ * touched.  Tokens outside [0, vocab) are padding: their rows are not read.
+ * The result does not depend on timing (tokens are sorted stably, sums split
+ * by the sizes alone).  Stands in for the dense per-key average of
+ * clients_avg_aggregator.py:60-100 where a client changed few rows.
+ *   parts (host): nparts entries (one per client); ids (device) int64 or
+ *     int32, rows (device) of `dtype`, row_stride elements apart; out
+ *     (device) vocab rows, out_stride elements apart, overlapping no part.
+ *   Workspace: fsagg_embed_grad_workspace_bytes(all tokens, dim, vocab),
+ *     16-byte aligned; nothing is kept in it.
+ */
+#define FSAGG_EMBED_MAX_ROWS 2147483646
+#define FSAGG_EMBED_MAX_TOKENS 268435456
+typedef struct fsagg_embed_part {
+  const void *ids;  /* (device) */
+  const void *rows; /* (device) */
+  int64_t tokens, row_stride;
+  float coef;
+  int32_t ids64;
+} fsagg_embed_part;
+size_t fsagg_embed_grad_workspace_bytes(int64_t tokens, int64_t dim,
+                                        int64_t vocab);
+int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts, int dtype,
+                     int64_t vocab, int64_t dim, void *out, int out_dtype,
+                     int64_t out_stride, int accumulate, void *workspace,
+                     size_t workspace_bytes, fsagg_stream_t stream);
+
+/*
  * Quantised / packed upload → fp32 client-stack row, in one launch.
  * `src` (device) holds one client's packed wire bytes; `segs` (device) is an
  * array of nseg records (32 B each, naturally aligned):

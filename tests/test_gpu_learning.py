@@ -1,0 +1,613 @@
+"""The learning operators on the GPU against plain 64-bit forms: the
+Newton-Schulz orthogonalisation, the Muon step, the embedding lookup and its
+gradient.
+
+Tolerances.  A value held in two fp16 limbs is off by at most 2^-22 of it
+(half a step of each: 2^-11 2^-11), a float32 one by 2^-24, and both chains
+add up products in float32: so the Newton-Schulz error (2-norm) is four times
+that of the same chain in float32 where that one's roundings are many and
+average out.  Where they are few (a 1 x 1 matrix has five steps of three
+values) the float32 chain may happen to be exact, so the limbs' own roundings
+are added as they come at worst: a step maps a singular value s to
+a s + b s^3 + c s^5; X is off by 2^-22 of it, A = X^2 by 2 + 1 of those, A^2
+by 6, Q by one more, so the terms are off by 1, 4 and 8 of those at most, and
+the error that s brings along is scaled by the step's slope at s
+(_limb_error).  Last comes half a step of the result's type.  A sum of c products in float32 is off by at most (c + 1)
+2^-24 of the sum of the absolute products, and half a step of its type."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+A, B, C = 3.4445, -4.7750, 2.0315
+HALF = {torch.float32: 2.0**-24, torch.float16: 2.0**-11,
+        torch.bfloat16: 2.0**-8}
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _chain(g, dt, steps=5, coef=(A, B, C), eps=1e-7):
+    a, b, c = coef
+    x = g.detach().cpu().double()
+    x = (x / max(float(x.norm()), eps)).to(dt)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T if tall else x
+    for _ in range(steps):
+        gram = x @ x.T
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return (x.T if tall else x).double()
+
+
+def _limb_error(g, steps, coef, eps):
+    """2-norm over the singular values of the limb roundings' worst sum."""
+    a, b, c = coef
+    x = g.detach().cpu().double()
+    s = torch.linalg.svdvals(x) / max(float(x.norm()), eps)
+    e = 2.0**-22 * s
+    for _ in range(steps):
+        slope = (a + 3 * b * s**2 + 5 * c * s**4).abs()
+        e = slope * e + 2.0**-22 * (abs(a) * s + 4 * abs(b) * s**3 +
+                                    8 * abs(c) * s**5)
+        s = a * s + b * s**3 + c * s**5
+        e = e + 2.0**-22 * s.abs()
+    return float(e.norm())
+
+
+def _matrix(rows, cols, seed, scale=1e-2):
+    """A decaying spectrum over noise, as momentum has it."""
+    t = torch.Generator().manual_seed(seed)
+    q = max(1, min(rows, cols) // 4)
+    u = torch.randn(rows, q, generator=t) * torch.exp(
+        torch.arange(q) * (-6.0 / q))
+    x = u @ torch.randn(q, cols, generator=t) / math.sqrt(q)
+    return (x + 0.05 * torch.randn(rows, cols, generator=t)) * scale
+
+
+def _check_ns(got, g, steps=5, coef=(A, B, C), eps=1e-7):
+    want = _chain(g, torch.float64, steps, coef, eps)
+    got64 = got.detach().cpu().double()
+    assert got64.shape == want.shape
+    off32 = _chain(g, torch.float32, steps, coef, eps) - want
+    norm = float(want.norm())
+    half = HALF[got.dtype] if got.dtype != torch.float32 else 2.0**-24
+    limb = _limb_error(g, steps, coef, eps)
+    tol = 4 * float(off32.norm()) + limb + half * norm
+    assert float((got64 - want).norm()) <= tol
+    # no single element is far off: the largest float32 error with the same
+    # factor twice, and no element's error is more than the whole 2-norm's
+    el = 8 * float(off32.abs().max()) + limb
+    # fp16 below its normal range rounds to multiples of 2^-24
+    el = el + half * want.abs() + (2.0**-25 if got.dtype == torch.float16
+                                   else 0.0)
+    assert bool(((got64 - want).abs() <= el).all())
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 200), (62, 2048), (2048, 62),
+          (63, 65), (64, 64), (128, 128), (129, 127), (130, 700),
+          (300, 1000), (1000, 300), (257, 513)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', SHAPES)
+def test_newton_schulz(shape, dtype):
+    from federatedscope_amd import ops
+    g = _matrix(*shape, seed=sum(shape)).to(dtype).cuda()
+    keep = g.clone()
+    got = ops.newton_schulz(g)
+    assert got.dtype == dtype and torch.equal(g, keep)
+    _check_ns(got, g)
+    again = ops.newton_schulz(g)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize('steps', [1, 2, 3, 8])
+def test_newton_schulz_steps(steps):
+    from federatedscope_amd import ops
+    g = _matrix(90, 150, 3).cuda()
+    _check_ns(ops.newton_schulz(g, steps=steps), g, steps=steps)
+
+
+def test_newton_schulz_other_coefficients():
+    from federatedscope_amd import ops
+    g = _matrix(90, 150, 4).cuda()
+    coef = (15 / 8, -10 / 8, 3 / 8)
+    _check_ns(ops.newton_schulz(g, steps=7, coefficients=coef), g, steps=7,
+              coef=coef)
+
+
+@pytest.mark.parametrize('scale', [1e-30, 1e-6, 1e30])
+def test_newton_schulz_scale_of_the_input_does_not_matter(scale):
+    from federatedscope_amd import ops
+    g = (_matrix(70, 200, 5, 1.0).double() * scale).float().cuda()
+    _check_ns(ops.newton_schulz(g, eps=1e-35), g, eps=1e-35)
+
+
+def test_newton_schulz_below_eps_is_divided_by_eps():
+    from federatedscope_amd import ops
+    g = _matrix(40, 60, 6, 1e-9).cuda()
+    _check_ns(ops.newton_schulz(g, eps=1e-5), g, eps=1e-5)
+
+
+def test_newton_schulz_zero_nan_and_infinity():
+    from federatedscope_amd import ops
+    z = torch.zeros(40, 70, device='cuda')
+    assert torch.equal(ops.newton_schulz(z), z)
+    for bad in (float('nan'), float('inf'), -float('inf')):
+        g = _matrix(40, 70, 7).cuda()
+        g[39, 69] = bad
+        good = _matrix(50, 70, 8).cuda()
+        got = ops.newton_schulz([good, g])
+        assert bool(got[1].isnan().all())
+        _check_ns(got[0], good)        # its neighbour is not touched
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_newton_schulz_strides(dtype):
+    """Transposed views, column ranges, every other row, a broadcast batch
+    (stride 0): read in place."""
+    from federatedscope_amd import ops
+    big = _matrix(150, 260, 9).to(dtype).cuda()
+    for g in (big.T, big[:, 3:200], big[::2], big[1::3, 5::7], big[:, :1],
+              big[5:6]):
+        _check_ns(ops.newton_schulz(g), g)
+    wide = big[None].expand(3, -1, -1)
+    got = ops.newton_schulz(wide)
+    assert got.shape == (3, 150, 260)
+    for z in range(3):
+        _check_ns(got[z], big)
+    perm = torch.stack([big, big.flip(0)]).permute(0, 2, 1)
+    got = ops.newton_schulz(perm)
+    for z in range(2):
+        _check_ns(got[z], perm[z])
+
+
+def test_newton_schulz_list_of_many():
+    """More entries than one launch takes, shapes, types and batches mixed;
+    each equals its own call."""
+    from federatedscope_amd import ops
+    gs = []
+    for i in range(30):
+        g = _matrix(3 + 17 * (i % 7), 5 + 29 * (i % 5), i).to(DTYPES[i % 3])
+        gs.append(g.cuda())
+    gs.append(torch.stack([_matrix(33, 20, 50), _matrix(33, 20, 51)]).cuda())
+    gs.append(torch.zeros(0, 5, device='cuda'))
+    gs.append(torch.zeros(2, 5, 0, device='cuda'))
+    got = ops.newton_schulz(gs)
+    for g, o in zip(gs, got):
+        assert o.shape == g.shape and o.dtype == g.dtype
+        if g.numel():
+            for a, b in zip(g if g.dim() == 3 else [g],
+                            o if g.dim() == 3 else [o]):
+                _check_ns(b, a)
+
+
+@pytest.mark.parametrize('odt', DTYPES)
+def test_newton_schulz_out_type(odt):
+    from federatedscope_amd import ops
+    g = _matrix(65, 90, 10).cuda()
+    out = torch.empty(65, 90, dtype=odt, device='cuda')
+    assert ops.newton_schulz(g, out=out) is out
+    _check_ns(out, g)
+
+
+def test_newton_schulz_refusals_on_device():
+    from federatedscope_amd import ops
+    g = _matrix(20, 30, 11).cuda()
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.newton_schulz(g, out=g)
+    buf = torch.empty(2, 20, 30, device='cuda')
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.newton_schulz([g, g], out=[buf[0], buf[0]])
+    with pytest.raises(ValueError):
+        ops.newton_schulz(g, out=buf)
+    with pytest.raises(ValueError):
+        ops.newton_schulz(g, out=torch.empty(30, 20, device='cuda').T)
+    with pytest.raises(ValueError):
+        ops.newton_schulz(g.double())
+    with pytest.raises(ValueError):
+        ops.newton_schulz(g[0])
+    with pytest.raises(Exception, match='steps'):
+        ops.newton_schulz(g, steps=0)
+    with pytest.raises(Exception, match='coefficients'):
+        ops.newton_schulz(g, coefficients=(9.0, 9.0, 9.0))
+
+
+# -- Muon ----------------------------------------------------------------------
+def _muon64(p, a, m, lr, mu, nesterov, wd, adjust, maximize):
+    p, a, m = (t.detach().cpu().double() for t in (p, a, m))
+    g = (a - p) if maximize else (p - a)
+    old = m
+    m = m + (1 - mu) * (g - m)
+    u = g + mu * (m - g) if nesterov else m
+    y = _chain(u, torch.float64)
+    off = float((_chain(u, torch.float32) - y).abs().max())
+    rows, cols = p.shape
+    k = 0.2 * math.sqrt(max(rows, cols)) if adjust == 'match_rms_adamw' \
+        else math.sqrt(max(1.0, rows / cols))
+    return (1 - lr * wd) * p - lr * k * y, m, lr * k * (
+        8 * off + _limb_error(u, 5, (A, B, C), 1e-7)), g, old
+
+
+@pytest.mark.parametrize('adjust', [None, 'original', 'match_rms_adamw'])
+@pytest.mark.parametrize('nesterov,maximize,mu,wd', [
+    (True, False, 0.95, 0.1), (False, False, 0.9, 0.0),
+    (True, True, 0.0, 0.5), (False, True, 0.5, 0.1)])
+def test_muon_step(nesterov, maximize, mu, wd, adjust):
+    from federatedscope_amd import ops
+    shapes = [(62, 512), (512, 62), (33, 33), (1, 9), (130, 257)]
+    ps = [_matrix(*s, seed=i, scale=0.1).cuda() for i, s in
+          enumerate(shapes)]
+    bs = [torch.zeros_like(p) for p in ps]
+    lr = 0.05
+    for rnd in range(3):
+        avgs = [p - _matrix(*s, seed=40 * rnd + i).cuda() for i, (p, s) in
+                enumerate(zip(ps, shapes))]
+        want = [_muon64(p, a, b, lr, mu, nesterov, wd, adjust, maximize)
+                for p, a, b in zip(ps, avgs, bs)]
+        ops.muon_step(ps, [a.view(-1) for a in avgs],
+                      [b.view(-1) for b in bs], lr=lr, momentum=mu,
+                      nesterov=nesterov, weight_decay=wd, adjust_lr=adjust,
+                      maximize=maximize)
+        for p, b, (wp, wb, tol, g, old) in zip(ps, bs, want):
+            # float32 operations: g = p - avg, the difference to the old
+            # momentum, its product with a rounded factor, the sum
+            btol = 2.0**-24 * (wb.abs() + 2 * g.abs() +
+                               3 * (g - old).abs())
+            assert bool(((b.cpu().double() - wb).abs() <= btol).all())
+            # the parameter: scaled, and the fused sum; lr in float32
+            ptol = tol + 2.0**-23 * (wp.abs() + (wp - p.cpu()).abs() +
+                                     p.cpu().abs()) + 2.0**-23 * lr
+            assert bool(((p.cpu().double() - wp).abs() <= ptol).all())
+
+
+def test_muon_agrees_with_torch_optim():
+    """torch.optim.Muon orthogonalises in bfloat16: the same step within that
+    type's error (steps of 2^-8 over five products, a tenth of the update)."""
+    from federatedscope_amd import ops
+    for shape in ((24, 40), (40, 24), (32, 32)):
+        for adjust in (None, 'match_rms_adamw'):
+            w = torch.nn.Parameter(_matrix(*shape, seed=1, scale=1.0))
+            p = w.detach().clone().cuda()
+            b = torch.zeros_like(p)
+            opt = torch.optim.Muon([w], lr=0.1, weight_decay=0.1,
+                                   momentum=0.9, adjust_lr_fn=adjust)
+            for r in range(2):
+                g = _matrix(*shape, seed=5 + r, scale=1.0)
+                before = w.detach().clone()
+                w.grad = g
+                opt.step()
+                pb = p.clone()
+                ops.muon_step([p], [p - g.cuda()], [b], lr=0.1,
+                              momentum=0.9, adjust_lr=adjust)
+                step = (w.detach() - before).norm()
+                mine = (p - pb).cpu()
+                assert (mine - (w.detach() - before)).norm() <= 0.1 * step
+
+
+def test_muon_refusals_on_device():
+    from federatedscope_amd import ops
+    p, a, b = (torch.randn(6, 8, device='cuda') for _ in range(3))
+    with pytest.raises(ValueError, match='2D'):
+        ops.muon_step([p[0]], [a[0]], [b[0]], lr=0.1)
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.muon_step([p, p], [a, a], [b, torch.zeros_like(b)], lr=0.1)
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.muon_step([p], [a], [p], lr=0.1)
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.muon_step([p], [p], [b], lr=0.1)
+    with pytest.raises(ValueError, match='contiguous'):
+        ops.muon_step([p.T], [a], [b], lr=0.1)
+    with pytest.raises(ValueError, match='elements'):
+        ops.muon_step([p], [a[:5]], [b], lr=0.1)
+    with pytest.raises(ValueError, match='float32'):
+        ops.muon_step([p.half()], [a], [b], lr=0.1)
+    with pytest.raises(ValueError):
+        ops.muon_step([p], [a, a], [b], lr=0.1)
+
+
+# -- embedding rows --------------------------------------------------------------
+def _ids(count, vocab, seed, pad=0.1, dtype=torch.int64):
+    """Skewed tokens with padding of every kind among them."""
+    r = np.random.default_rng(seed)
+    x = np.minimum((np.exp(r.random(count) * math.log(vocab + 1)) - 1)
+                   .astype(np.int64), vocab - 1)
+    out = r.random(count) < pad
+    x[out] = r.choice([-1, -vocab, vocab, vocab + 7, 2**31 - 1, -2**31],
+                      size=int(out.sum()))
+    return torch.from_numpy(x).to(dtype).cuda()
+
+
+def _lookup_ref(table, ids, scale):
+    t, i = table.cpu(), ids.cpu().long()
+    ok = (i >= 0) & (i < len(t))
+    rows = (t[torch.where(ok, i, 0)].float() *
+            np.float32(scale)).to(t.dtype)
+    return torch.where(ok[..., None], rows, torch.zeros((), dtype=t.dtype))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [1, 5, 8, 129, 300, 1024, 1032, 4100])
+@pytest.mark.parametrize('shape', [(0, ), (1, ), (7, ), (3, 50)])
+def test_embedding_lookup(shape, dim, dtype):
+    from federatedscope_amd import ops
+    table = torch.randn(211, dim).to(dtype).cuda()
+    n = int(np.prod(shape))
+    for idt in (torch.int64, torch.int32):
+        ids = _ids(n, 211, dim, dtype=idt).reshape(shape)
+        for scale in (1.0, math.sqrt(dim)):
+            got = ops.embedding_lookup(table, ids, scale=scale)
+            assert got.shape == shape + (dim, )
+            assert torch.equal(got.cpu(), _lookup_ref(table, ids, scale))
+
+
+def test_embedding_lookup_views_and_special_values():
+    from federatedscope_amd import ops
+    big = torch.randn(50, 100, device='cuda')
+    big[3, 10:20] = float('nan')
+    big[4, 10] = float('inf')
+    ids = torch.tensor([3, 4, -1, 49, 50, 0, 3], device='cuda')
+    for t in (big[:, 8:72], big[:, 1:60], big[::2], big[:40], big[:0],
+              big[:, :0]):
+        got = ops.embedding_lookup(t, ids, scale=2.0)
+        want = _lookup_ref(t, ids, 2.0) if len(t) else torch.zeros(7, 100)
+        assert torch.equal(got.cpu().nan_to_num(7.0), want.nan_to_num(7.0))
+    out = torch.full((7, 100), 9.0, device='cuda')
+    assert ops.embedding_lookup(big, ids, out=out) is out
+    assert torch.equal(out.cpu().nan_to_num(7.0),
+                       _lookup_ref(big, ids, 1.0).nan_to_num(7.0))
+    for bad in (dict(out=out.T), dict(out=out.half()), dict(out=big[:7])):
+        with pytest.raises(ValueError):
+            ops.embedding_lookup(big, ids, **bad)
+    with pytest.raises(ValueError):
+        ops.embedding_lookup(big.T, ids)
+    with pytest.raises(ValueError):
+        ops.embedding_lookup(big, ids.float())
+    with pytest.raises(ValueError):
+        ops.embedding_lookup(big, ids[::2])
+    with pytest.raises(ValueError):
+        ops.embedding_lookup(big, ids.cpu())
+
+
+def _grad_ref(ids, grad, vocab, weights, scale):
+    """(sums, sums of absolute products, counts), in 64 bits."""
+    dim = grad[0].shape[-1]
+    tot = torch.zeros(vocab, dim, dtype=torch.float64)
+    mag = torch.zeros(vocab, dim, dtype=torch.float64)
+    cnt = torch.zeros(vocab, dtype=torch.float64)
+    for i, g, w in zip(ids, grad, weights):
+        i, g = i.cpu().long().reshape(-1), g.cpu().reshape(-1, dim)
+        ok = (i >= 0) & (i < vocab)
+        x = g[ok].double() * (scale * w)
+        tot.index_add_(0, i[ok], x)
+        mag.index_add_(0, i[ok], x.abs())
+        cnt.index_add_(0, i[ok], torch.ones(int(ok.sum()),
+                                            dtype=torch.float64))
+    return tot, mag, cnt
+
+
+def _check_grad(got, ids, grad, vocab, weights=None, scale=1.0, base=None):
+    weights = weights or [1.0] * len(ids)
+    tot, mag, cnt = _grad_ref(ids, grad, vocab, weights, scale)
+    want = tot
+    # the coefficient's own rounding and the sum's
+    tol = (cnt[:, None] + 2) * 2.0**-24 * mag
+    if base is not None:
+        want = tot + base.cpu().double()
+        tol = tol + 2.0**-24 * want.abs()
+        rest = cnt == 0
+        assert torch.equal(got.cpu()[rest], base.cpu()[rest])
+    else:
+        assert not got.cpu()[cnt == 0].any()
+    tol = tol * (1 + 2 * HALF[got.dtype]) + HALF[got.dtype] * want.abs()
+    if got.dtype == torch.float16:
+        tol = tol + 2.0**-25
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('tokens,vocab,dim', [
+    (1, 1, 1), (1, 9, 8), (5, 3, 4), (31, 40, 300), (32, 7, 16), (33, 1, 5),
+    (64, 1000, 129), (65, 64, 64), (700, 50, 40), (4096, 300, 24),
+    (4097, 2000, 9), (9000, 5, 17), (20000, 70000, 8), (6000, 1100000, 4)])
+def test_embedding_grad(tokens, vocab, dim, dtype):
+    from federatedscope_amd import ops
+    ids = _ids(tokens, vocab, tokens)
+    grad = torch.randn(tokens, dim, device='cuda').to(dtype)
+    got = ops.embedding_grad(ids, grad, vocab, scale=0.5)
+    assert got.shape == (vocab, dim) and got.dtype == dtype
+    _check_grad(got, [ids], [grad], vocab, scale=0.5)
+    assert torch.equal(got, ops.embedding_grad(ids, grad, vocab, scale=0.5))
+    base = torch.randn(vocab, dim, device='cuda').to(dtype)
+    out = base.clone()
+    assert ops.embedding_grad(ids, grad, vocab, scale=0.5, out=out,
+                              accumulate=True) is out
+    _check_grad(out, [ids], [grad], vocab, scale=0.5, base=base)
+
+
+@pytest.mark.parametrize('parts', [1, 3, 64, 65, 150])
+def test_embedding_grad_of_many_clients(parts):
+    """Uneven clients (some empty), int32 and int64 tokens, weights, a
+    float32 table of bfloat16 rows."""
+    from federatedscope_amd import ops
+    vocab, dim = 500, 48
+    ids = [_ids((i * 37) % 90, vocab, i, dtype=torch.int64 if i % 2 else
+                torch.int32) for i in range(parts)]
+    grad = [torch.randn(len(i), dim, device='cuda').bfloat16() for i in ids]
+    w = [(1 + i % 5) / 7 for i in range(parts)]
+    got = ops.embedding_grad(ids, grad, vocab, weights=w)
+    _check_grad(got, ids, grad, vocab, w)
+    base = torch.randn(vocab, dim, device='cuda')
+    out = base.clone()
+    ops.embedding_grad(ids, grad, vocab, weights=w, scale=3.0, out=out,
+                       accumulate=True)
+    _check_grad(out, ids, grad, vocab, w, 3.0, base)
+
+
+def test_embedding_grad_of_one_row():
+    """Every token the same row, over many chunks; no token at all; padding
+    alone."""
+    from federatedscope_amd import ops
+    ids = torch.full((10000, ), 2, device='cuda')
+    grad = torch.randn(10000, 260, device='cuda')
+    _check_grad(ops.embedding_grad(ids, grad, 4), [ids], [grad], 4)
+    none = torch.empty(0, dtype=torch.long, device='cuda')
+    got = ops.embedding_grad(none, grad[:0], 3)
+    assert got.shape == (3, 260) and not got.any()
+    got = ops.embedding_grad(ids * 0 - 1, grad, 3)
+    assert not got.any()
+    out = torch.ones(3, 260, device='cuda')
+    ops.embedding_grad(ids * 0 - 1, grad, 3, out=out, accumulate=True)
+    assert bool((out == 1).all())
+    assert ops.embedding_grad(ids, grad, 0).shape == (0, 260)
+
+
+def test_embedding_grad_does_not_read_padding():
+    from federatedscope_amd import ops
+    ids = torch.tensor([0, -1, 1, 5, 1, 9], device='cuda')
+    grad = torch.randn(6, 33, device='cuda')
+    clean = grad.clone()
+    for t in (1, 3, 5):
+        grad[t] = float('nan')
+        clean[t] = 0
+    got = ops.embedding_grad(ids, grad, 5)
+    assert torch.equal(got, ops.embedding_grad(ids, clean, 5))
+    grad[2, 7] = float('inf')
+    grad[0, 3] = float('nan')
+    got = ops.embedding_grad(ids, grad, 5)
+    assert got[1, 7] == float('inf') and bool(got[0, 3].isnan())
+    assert int(got.isfinite().logical_not().sum()) == 2
+
+
+def test_embedding_grad_views():
+    from federatedscope_amd import ops
+    ids = _ids(80, 30, 1)
+    wide = torch.randn(80, 200, device='cuda')
+    for g in (wide[:, 8:72], wide[:, 3:50], wide[:, :1]):
+        _check_grad(ops.embedding_grad(ids, g, 30), [ids], [g], 30)
+    many = torch.randn(160, 64, device='cuda')
+    _check_grad(ops.embedding_grad(ids, many[::2], 30), [ids], [many[::2]],
+                30)
+    flat = torch.randn(8, 10, 64, device='cuda')
+    _check_grad(ops.embedding_grad(ids.view(8, 10), flat, 30), [ids], [flat],
+                30)
+    buf = torch.full((30, 100), 5.0, device='cuda')
+    out = buf[:, 10:74]
+    ops.embedding_grad(ids, many[:80], 30, out=out)
+    _check_grad(out, [ids], [many[:80]], 30)
+    assert bool((buf[:, :10] == 5).all()) and bool((buf[:, 74:] == 5).all())
+    row = torch.randn(1, 64, device='cuda').expand(80, 64)
+    _check_grad(ops.embedding_grad(ids, row, 30), [ids], [row], 30)
+    with pytest.raises(ValueError, match='overlap'):
+        ops.embedding_grad(ids, many[:80], 30, out=many[80:81].expand(30, 64))
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.embedding_grad(ids, many[:80], 80, out=many[:80])
+    with pytest.raises(ValueError):
+        ops.embedding_grad([ids, ids], [many[:80], many[:80].half()], 30)
+    with pytest.raises(ValueError):
+        ops.embedding_grad(ids, many[:79], 30)
+    with pytest.raises(ValueError):
+        ops.embedding_grad([ids], [many[:80]], 30, weights=[1.0, 2.0])
+
+
+def test_embedding_grad_is_the_lookups_gradient():
+    """Against differences: the lookup is linear in its table, so a step of
+    any size gives the derivative, to the rounding of its float32 products
+    (64-bit sums of them here)."""
+    from federatedscope_amd import ops
+    vocab, dim, scale = 12, 6, 1.5
+    ids = torch.tensor([3, 0, 3, -1, 11, 3, 12, 0], device='cuda')
+    table = torch.randn(vocab, dim, device='cuda')
+    up = torch.randn(len(ids), dim, device='cuda')
+    got = ops.embedding_grad(ids, up, vocab, scale=scale)
+    for v in range(vocab):
+        for c in (0, 5):
+            t2 = table.clone()
+            t2[v, c] += 1.0
+            d = (ops.embedding_lookup(t2, ids, scale=scale).double() -
+                 ops.embedding_lookup(table, ids, scale=scale).double())
+            step = float(t2[v, c].double() - table[v, c].double())
+            fd = float((d * up.double()).sum()) / step
+            n = int((ids == v).sum())
+            tol = 2.0**-22 * max(1, n) * scale * (
+                float(up.abs().max()) * (2 + float(table.abs().max())))
+            assert abs(fd - float(got[v, c])) <= tol
+
+
+# -- streams and graphs ------------------------------------------------------------
+def _calls(seed):
+    """One of each operator, writing its own outputs."""
+    from federatedscope_amd import ops
+    g = _matrix(100, 150, seed).cuda()
+    p, a, m = (_matrix(70, 40, seed + i).cuda() for i in range(3))
+    table = torch.randn(300, 64, device='cuda')
+    ids = _ids(500, 300, seed)
+    rows = torch.randn(500, 64, device='cuda')
+    o1 = torch.empty_like(g)
+    o2 = torch.empty(500, 64, device='cuda')
+    o3 = torch.empty(300, 64, device='cuda')
+
+    def run():
+        ops.newton_schulz(g, out=o1)
+        ops.muon_step([p], [a], [m], lr=0.1)
+        ops.embedding_lookup(table, ids, scale=2.0, out=o2)
+        ops.embedding_grad(ids, rows, 300, out=o3)
+        ops.embedding_grad(ids, o2, 300, out=table, accumulate=True)
+    return run, [g, p, a, m, table, rows, o1, o2, o3]
+
+
+def test_operators_on_two_streams():
+    """Two runs at once on two streams equal the same runs one by one."""
+    want = []
+    for s in (1, 2):
+        run, bufs = _calls(s)
+        start = [b.clone() for b in bufs]
+        for _ in range(3):
+            run()
+        torch.cuda.synchronize()
+        want.append([b.clone() for b in bufs])
+        for b, c in zip(bufs, start):
+            b.copy_(c)
+        want[-1] = (run, bufs, want[-1])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in want]
+    for _ in range(3):
+        for s, (run, _, _) in zip(streams, want):
+            with torch.cuda.stream(s):
+                run()
+    torch.cuda.synchronize()
+    for _, bufs, w in want:
+        for b, x in zip(bufs, w):
+            assert torch.equal(b, x)
+
+
+def test_operators_in_captured_graphs():
+    """Two graphs, replayed in turn with eager work and synchronizations
+    between them; every replay equals the eager run."""
+    made = []
+    for seed in (3, 4):
+        run, bufs = _calls(seed)
+        start = [b.clone() for b in bufs]
+        states = []
+        for _ in range(4):
+            run()
+            torch.cuda.synchronize()
+            states.append([b.clone() for b in bufs])
+        for b, c in zip(bufs, start):
+            b.copy_(c)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+        torch.cuda.synchronize()
+        made.append((graph, bufs, states))
+    for k in range(4):
+        for graph, bufs, states in made:
+            graph.replay()
+            junk = torch.randn(1000, 1000, device='cuda')
+            junk = junk @ junk
+            torch.cuda.synchronize()
+            for b, x in zip(bufs, states[k]):
+                assert torch.equal(b, x)
