@@ -44,8 +44,63 @@ class ClientsAvgAggregator(DeviceEngine, _ModelIO, Aggregator):
             return self._ss_avg(models, recover_fun)
         weights = self._weights(models)
         out_dev = _first_device(models[0][1])
-        layout, flat, extra, keys = self._weighted_avg_device(models, weights)
+        layout, flat, extra, keys = self._avg_with_rows(models, weights)
         return self._emit(layout, flat, keys, out_dev, extra)
+
+    # keys the last round's clients sent as row-sparse updates
+    _row_keys = ()
+
+    def _avg_with_rows(self, models, weights):
+        """_weighted_avg_device, with the keys that client 0 sends as sparse
+        COO tensors (one sparse dimension: the gradient layout of
+        nn.Embedding(sparse=True)) taken as row-sparse *updates* of the
+        server model's value: model + sum of w_i * update_i, through
+        ops.embedding_grad.  Rows no client touched keep the model's value;
+        a client that lacks the key adds nothing.  The reference's loop has
+        no sparse form (clients_avg_aggregator.py:69-98 reduces dense
+        tensors)."""
+        self._row_keys = sparse_keys(models[0][1])
+        if not self._row_keys:
+            return self._weighted_avg_device(models, weights)
+        sums = OrderedDict((k, self._row_sum(k, models, weights))
+                           for k in self._row_keys)
+        dense = [(s, OrderedDict((k, v) for k, v in m.items()
+                                 if k not in sums)) for s, m in models]
+        layout, flat, extra, _ = self._weighted_avg_device(dense, weights)
+        extra.update(sums)
+        return layout, flat, extra, list(models[0][1].keys())
+
+    def _row_sum(self, key, models, weights):
+        dev = self.compute_device
+        if self.model is None:
+            raise ValueError('the row-sparse update of key %r needs the '
+                             "server's model" % key)
+        base = self.model.state_dict()[key]
+        rows = base.shape[0] if base.dim() else 0
+        ids, vals, w = [], [], []
+        for i, (_, m) in enumerate(models):
+            if key not in m:
+                continue
+            x = m[key]
+            if not (isinstance(x, torch.Tensor) and x.is_sparse and
+                    x.sparse_dim() == 1 and x.shape == base.shape):
+                raise ValueError(
+                    'client %d: key %r must be a sparse COO update of shape '
+                    '%s with one sparse dimension, as the first client '
+                    'sends it' % (i, key, tuple(base.shape)))
+            # (_indices / _values: uncoalesced tensors, too)
+            ids.append(x._indices()[0].to(dev).contiguous())
+            vals.append(x._values().to(dev).reshape(ids[-1].numel(),
+                                                    -1).contiguous()
+                        if ids[-1].numel() else
+                        x._values().to(dev).reshape(
+                            0, base[0].numel() if rows else 0))
+            w.append(weights[i])
+        out = base.to(dev, copy=True).contiguous()
+        if out.numel():
+            ops.embedding_grad(ids, vals, rows, weights=w,
+                               out=out.view(rows, -1), accumulate=True)
+        return out
 
     def _ss_avg(self, models, recover_fun):
         """The use_ss branch (clients_avg_aggregator.py:79-98): every upload
@@ -78,6 +133,14 @@ class ClientsAvgAggregator(DeviceEngine, _ModelIO, Aggregator):
                                           float(total),
                                           weight=w).to(out_dev)
         return avg
+
+
+def sparse_keys(model):
+    """The keys of a client's dict that are sparse COO tensors."""
+    if not isinstance(model, dict):      # a StagedUpdate holds dense rows
+        return ()
+    return [k for k, v in model.items()
+            if getattr(v, 'is_sparse', False)]
 
 
 def _share_to_device(x, dev):

@@ -8,7 +8,11 @@ configured optimizer — SGD (momentum, dampening, nesterov), Adam / AdamW
 (amsgrad), Adagrad (lr_decay, initial accumulator) or RMSprop (momentum,
 centered); weight decay and maximize for all — to the server model's
 parameters and the per-parameter optimizer state, which stays resident in
-HBM across rounds.  The updated parameters are written back into ``self.model`` and
+HBM across rounds.  Muon (momentum, nesterov, weight_decay, ns_steps,
+ns_coefficients, eps, adjust_lr_fn as torch.optim.Muon) steps all matrix
+parameters in one ops.muon_step; like torch.optim's it takes matrices only,
+unless ``aux`` = {type, lr, **kwargs} names another of these optimizers for
+the other parameters (biases, convolutions).  The updated parameters are written back into ``self.model`` and
 ``self.model.state_dict()`` is returned, as the reference does.
 
 Optimizer config: ``config.fedopt.optimizer`` = {type, lr, **kwargs} as in
@@ -17,10 +21,12 @@ StepLR(step_size, gamma) stepped once per aggregation (:14-22, :43-44).
 """
 import ctypes
 from collections import OrderedDict
+from types import SimpleNamespace
 
 import torch
 
 from ... import _lib as L
+from ... import ops
 from ...ops import _check_f32_cuda, _stream
 from ._engine import fedavg_weights
 from .clients_avg_aggregator import ClientsAvgAggregator
@@ -28,7 +34,7 @@ from .clients_avg_aggregator import ClientsAvgAggregator
 # torch.optim optimizers the device step implements (optimizer_builder.py:
 # 53-56 builds any torch.optim class by name; these are the ones with a
 # single-tensor elementwise step)
-_SUPPORTED = ('SGD', 'Adam', 'AdamW', 'Adagrad', 'RMSprop')
+_SUPPORTED = ('SGD', 'Adam', 'AdamW', 'Adagrad', 'RMSprop', 'Muon')
 # keyword arguments that do not change the arithmetic of a single-tensor CPU
 # step (the reference's optimizer runs on CPU tensors)
 _IGNORED = ('foreach', 'fused', 'capturable', 'differentiable')
@@ -43,6 +49,18 @@ def _opt_cfg(optimizer_cfg):
     for k in ('__help_info__', '__cfg_check_funcs__', 'is_ready_for_run'):
         d.pop(k, None)
     return d
+
+
+def _with_optimizer(config, optimizer):
+    """A view of ``config`` whose FedOpt optimizer is another one."""
+    fo = config.fedopt
+    return SimpleNamespace(
+        federate=config.federate,
+        fedopt=SimpleNamespace(
+            optimizer=optimizer,
+            annealing=getattr(fo, 'annealing', False),
+            annealing_step_size=getattr(fo, 'annealing_step_size', 2000),
+            annealing_gamma=getattr(fo, 'annealing_gamma', 0.5)))
 
 
 class FedOptAggregator(ClientsAvgAggregator):
@@ -63,8 +81,9 @@ class FedOptAggregator(ClientsAvgAggregator):
         self.maximize = bool(opt.pop('maximize', False))
         t = self.opt_type
         # torch.optim defaults per class
-        self.weight_decay = float(opt.pop('weight_decay',
-                                          1e-2 if t == 'AdamW' else 0.0))
+        self.weight_decay = float(opt.pop(
+            'weight_decay', {'AdamW': 1e-2, 'Muon': 0.1}.get(t, 0.0)))
+        self._aux = None
         self.amsgrad = False
         if t == 'SGD':
             self.momentum = float(opt.pop('momentum', 0.0))
@@ -81,6 +100,25 @@ class FedOptAggregator(ClientsAvgAggregator):
             self.lr_decay = float(opt.pop('lr_decay', 0.0))
             self.init_acc = float(opt.pop('initial_accumulator_value', 0.0))
             self.eps = float(opt.pop('eps', 1e-10))
+        elif t == 'Muon':
+            self.momentum = float(opt.pop('momentum', 0.95))
+            self.nesterov = bool(opt.pop('nesterov', True))
+            self.ns_coefficients = tuple(
+                float(x) for x in opt.pop('ns_coefficients',
+                                          ops.NS_COEFFICIENTS))
+            self.eps = float(opt.pop('eps', 1e-7))
+            self.ns_steps = int(opt.pop('ns_steps', 5))
+            self.adjust_lr_fn = opt.pop('adjust_lr_fn', None)
+            aux = opt.pop('aux', None)
+            if aux is not None:
+                aux = _opt_cfg(aux)
+                if aux.get('type') == 'Muon':
+                    raise ValueError('the aux optimizer takes what Muon '
+                                     'does not: it cannot be Muon')
+                # a second optimizer over the same model, stepping the
+                # parameters Muon does not take
+                self._aux = FedOptAggregator(
+                    _with_optimizer(config, aux), model, device)
         else:   # RMSprop
             self.alpha = float(opt.pop('alpha', 0.99))
             self.eps = float(opt.pop('eps', 1e-8))
@@ -108,6 +146,33 @@ class FedOptAggregator(ClientsAvgAggregator):
         def need(ok, msg, v):
             if not ok:
                 raise ValueError(msg % (v, ))
+        if t == 'Muon':
+            cfg = self.opt_kwargs
+            need(0.0 <= self.lr0, 'Learning rate should be >= 0 but is: %s',
+                 self.lr0)
+            need(0.0 <= self.momentum, 'momentum should be >= 0 but is: %s',
+                 cfg.get('momentum'))
+            need(0.0 <= self.weight_decay,
+                 'weight decay should be >= 0 but is: %s',
+                 cfg.get('weight_decay'))
+            need(self.adjust_lr_fn in ops._MUON_ADJUST,
+                 'Adjust learning rate function %s is not supported',
+                 self.adjust_lr_fn)
+            # torch.optim refuses these in step()
+            need(self.ns_steps < 100, 'Number of steps must be less than '
+                 '100 for computational efficiency%s', '')
+            need(len(self.ns_coefficients) == 3,
+                 'Coefficients must be a tuple of exactly 3 values%s', '')
+            # and these have no device form
+            need(self.ns_steps >= 1, 'ns_steps should be >= 1 but is: %s',
+                 self.ns_steps)
+            need(self.eps > 0.0, 'eps should be > 0 but is: %s', self.eps)
+            if self._aux is None and self.model is not None:
+                for p in self.model.parameters():
+                    need(p.dim() == 2, 'Muon only supports 2D parameters '
+                         'whereas we found a parameter with size: %s',
+                         p.shape)
+            return
         need(0.0 <= self.lr0, 'Invalid learning rate: %s', self.lr0)
         if t in ('Adam', 'AdamW', 'Adagrad', 'RMSprop'):
             need(0.0 <= self.eps, 'Invalid epsilon value: %s', self.eps)
@@ -156,7 +221,7 @@ class FedOptAggregator(ClientsAvgAggregator):
             return layout, self._bucket(layout, avg), extra
         weights = fedavg_weights([s for s, _ in models],
                                  self.cfg.federate.ignore_weight)
-        layout, avg, extra, _ = self._weighted_avg_device(models, weights)
+        layout, avg, extra, _ = self._avg_with_rows(models, weights)
         return layout, avg, extra
 
     def _states(self, key, like):
@@ -166,7 +231,9 @@ class FedOptAggregator(ClientsAvgAggregator):
         if st is None:
             t = self.opt_type
             z = lambda: torch.zeros_like(like)  # noqa: E731
-            if t == 'SGD':
+            if t == 'Muon':
+                st = [z(), None, None]
+            elif t == 'SGD':
                 st = [z() if self.momentum != 0.0 else None, None, None]
             elif t in ('Adam', 'AdamW'):
                 st = [z(), z(), z() if self.amsgrad else None]
@@ -178,6 +245,35 @@ class FedOptAggregator(ClientsAvgAggregator):
             st.append(0)
             self._state[key] = st
         return st
+
+    def _step_keys(self, keys, views):
+        """One optimizer step of the fp32 parameters ``keys``;
+        ``views(k)`` gives a parameter's (shape, contiguous device values,
+        average), both flat.  Muon takes the matrices in one call, its aux
+        optimizer the rest."""
+        fn = L.load().fsagg_server_opt_step_f32
+        mats = []
+        for k in keys:
+            shape, param, avg = views(k)
+            _check_f32_cuda(param, 'FedOpt parameter', align=4)
+            _check_f32_cuda(avg, 'FedOpt bucket')
+            opt = self
+            if self.opt_type == 'Muon':
+                if len(shape) == 2:
+                    st = self._states(k, avg)
+                    mats.append((param.view(shape), avg, st[0]))
+                    st[3] += 1
+                    continue
+                opt = self._aux
+            opt._step(fn, param, avg, opt._states(k, avg))
+        if mats:
+            ops.muon_step(*map(list, zip(*mats)), lr=self._lr(),
+                          momentum=self.momentum, nesterov=self.nesterov,
+                          weight_decay=self.weight_decay,
+                          steps=self.ns_steps,
+                          coefficients=self.ns_coefficients, eps=self.eps,
+                          adjust_lr=self.adjust_lr_fn,
+                          maximize=self.maximize)
 
     def _step(self, fn, param, avg, st):
         """One optimizer step of a contiguous device parameter range."""
@@ -191,16 +287,29 @@ class FedOptAggregator(ClientsAvgAggregator):
 
     def aggregate(self, agg_info):
         layout, avg, extra = self._new_model(agg_info)
-        lib = L.load()
         named = OrderedDict(self.model.named_parameters())
+        # averages of row-sparse uploads (fp32, beside the bucket)
+        rows = {k: extra.pop(k) for k in self._row_keys if k in extra}
         # parameters the aggregate holds (fedopt_aggregator.py:37-40); other
         # state_dict entries (buffers) are returned unchanged
-        step_keys = [k for k in named if k in layout.keys]
+        step_keys = [k for k in named if k in layout.keys or k in rows]
         for k in named:
-            if k in extra and extra[k].dtype != torch.float64:
+            if (k in extra and extra[k].dtype != torch.float64) or \
+                    (k in rows and (rows[k].dtype != torch.float32 or
+                                    named[k].dtype != torch.float32)):
                 raise NotImplementedError(
-                    'FedOpt on %s parameter %r' % (extra[k].dtype, k))
+                    'FedOpt on %s parameter %r' % (named[k].dtype, k))
+            if k in extra and self.opt_type == 'Muon' and \
+                    (self._aux is None or named[k].dim() == 2):
+                raise NotImplementedError('Muon on %s parameter %r' %
+                                          (extra[k].dtype, k))
         dev = self.compute_device
+
+        def avg_of(k):
+            if k in rows:
+                return rows[k].view(-1)
+            return avg[layout.offsets[k]:layout.offsets[k] +
+                       layout.numels[k]]
         inplace = bool(step_keys) and all(
             named[k].device == dev and named[k].dtype == torch.float32 and
             named[k].is_contiguous() and named[k].data_ptr() % 16 == 0
@@ -209,36 +318,37 @@ class FedOptAggregator(ClientsAvgAggregator):
             # parameters already on the compute device: the optimizer steps
             # them in place (as torch.optim's step does), no bucket copy of
             # the model in or out
-            for k in step_keys:
-                o, m = layout.offsets[k], layout.numels[k]
-                _check_f32_cuda(avg[o:o + m], 'FedOpt bucket')
-                self._step(lib.fsagg_server_opt_step_f32,
-                           named[k].data.view(-1), avg[o:o + m],
-                           self._states(k, avg[o:o + m]))
+            self._step_keys(step_keys, lambda k: (
+                named[k].shape, named[k].data.view(-1), avg_of(k)))
         elif step_keys:
+            dense = [k for k in step_keys if k not in rows]
             param = self._bucket(layout, OrderedDict(
                 (k, named[k].detach() if k in named else torch.zeros(
                     layout.shapes[k])) for k in layout.keys))
-            for k in step_keys:      # per key: params the optimizer owns
-                o, m = layout.offsets[k], layout.numels[k]
-                for t in (param, avg):
-                    _check_f32_cuda(t[o:o + m], 'FedOpt bucket')
-                self._step(lib.fsagg_server_opt_step_f32, param[o:o + m],
-                           avg[o:o + m], self._states(k, avg[o:o + m]))
-            views = layout.unpack(param)
+            flat = {k: param[layout.offsets[k]:layout.offsets[k] +
+                             layout.numels[k]] for k in dense}
+            for k in step_keys:
+                if k in rows:
+                    flat[k] = named[k].detach().to(
+                        dev, torch.float32, copy=True).reshape(-1)
+            self._step_keys(step_keys, lambda k: (named[k].shape, flat[k],
+                                                  avg_of(k)))
             with torch.no_grad():
                 for k in step_keys:
-                    named[k].data.copy_(views[k])
+                    named[k].data.copy_(flat[k].view(named[k].shape))
         for k in named:              # float64 parameters, one key each
             if k not in extra:
                 continue
+            opt = self._aux if self._aux is not None else self
             p64 = named[k].detach().to(dev, torch.float64).contiguous()
             a64 = extra[k].to(dev, torch.float64).contiguous()
-            self._step(lib.fsagg_server_opt_step_f64, p64, a64,
-                       self._states(k, p64.view(-1)))
+            opt._step(L.load().fsagg_server_opt_step_f64, p64, a64,
+                      opt._states(k, p64.view(-1)))
             with torch.no_grad():
                 named[k].data.copy_(p64)
         self._rounds += 1
+        if self._aux is not None:
+            self._aux._rounds += 1
         return self.model.state_dict()
 
     def _params(self, first, step):

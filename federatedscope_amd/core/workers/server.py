@@ -19,6 +19,9 @@ wait for the remaining clients instead of sitting inside aggregate().
 """
 from collections import deque
 
+from ... import ops
+from ..aggregators._engine import compute_device
+from ..aggregators.clients_avg_aggregator import sparse_keys
 from ..auxiliaries.utils import merge_param_dict
 from .ingress import DeviceIngress
 
@@ -75,6 +78,8 @@ class AggregationServer:
         """Stage model ``idx``'s part of an upload on arrival (or keep it as
         it came when its layout differs from the round's)."""
         staged_quant = self.dequantize
+        if not staged_quant and sparse_keys(para):
+            return para         # row-sparse updates are read where they lie
         ing = self.ingresses[idx]
         if ing is None:
             ing = self.ingresses[idx] = DeviceIngress(
@@ -123,6 +128,18 @@ class AggregationServer:
         if self.online_aggr:
             self.aggregator.inc(content)
         return self.check_and_move_on()
+
+    def select_rows(self, key, ids, scale=1.0, model_idx=0):
+        """The rows of the embedding table ``key`` that a client's tokens
+        ``ids`` name (ops.embedding_lookup: scaled, zero rows for padding),
+        on the compute device — what a client that trains a few rows of a
+        large table is sent instead of the whole of it (the reference
+        broadcasts whole state dicts, server.py:636-714); it answers with a
+        row-sparse update (ClientsAvgAggregator)."""
+        dev = compute_device(self.device)
+        table = self.models[model_idx].state_dict()[key].to(dev)
+        return ops.embedding_lookup(table, ids.to(dev).contiguous(),
+                                    scale=scale)
 
     # -- server.py:315-383 (count-based) ---------------------------------------
     def check_and_move_on(self):

@@ -75,10 +75,10 @@ template <int DT, int VEC>
 __device__ __forceinline__ void load_vec(const void *p, float (&v)[VEC]) {
   using T = typename Elem<DT>::type;
   if constexpr (VEC == 1) {
-    v[0] = Elem<DT>::get(*static_cast<const T *>(p));
+    v[0] = Elem<DT>::get(gld(static_cast<const T *>(p)));
   } else {
     typedef T tv __attribute__((ext_vector_type(VEC)));
-    const tv x = *static_cast<const tv *>(p);
+    const tv x = gld(static_cast<const tv *>(p));
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = Elem<DT>::get(x[e]);
   }

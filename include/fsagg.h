@@ -303,7 +303,7 @@ int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
  * Rows of an embedding table by token:  out[t] = round(scale * E[ids[t]]),
  * the product in fp32.  A token outside [0, vocab) is padding: a zero row.
  * What a server sends a client that needs only its tokens' rows (the
- * reference sends whole state dicts, core/workers/server.py:591-650).
+ * reference sends whole state dicts, core/workers/server.py:636-714).
  *   table (device) vocab rows of dim elements of `dtype` (FSAGG_F32, _F16,
  *     _BF16), row_stride elements apart; ids (device) int64 (ids64 != 0) or
  *     int32; out (device) contiguous [tokens][dim] of the table's dtype,

@@ -164,3 +164,59 @@ def test_disjoint_check():
         with pytest.raises(ValueError, match='overlaps'):
             ops._check_disjoint(w, r)
     ops._check_disjoint([a, buf[5:5]], [buf[7:7]])
+
+
+def _fedopt(opt, model=None):
+    from federatedscope_amd.core.aggregators import FedOptAggregator
+    cfg = SimpleNamespace(
+        federate=SimpleNamespace(ignore_weight=False, use_ss=False),
+        fedopt=SimpleNamespace(optimizer=dict(opt), annealing=False))
+    return FedOptAggregator(config=cfg, model=model or torch.nn.Linear(
+        3, 2, bias=False))
+
+
+@pytest.mark.parametrize('kw', [
+    dict(lr=-1), dict(lr=0.1, momentum=-1), dict(lr=0.1, weight_decay=-1),
+    dict(lr=0.1, adjust_lr_fn='x')])
+def test_fedopt_muon_rejects_what_torch_optim_rejects(kw):
+    with pytest.raises(ValueError) as want:
+        torch.optim.Muon([torch.zeros(2, 3, requires_grad=True)], **kw)
+    with pytest.raises(ValueError) as got:
+        _fedopt(dict(type='Muon', **kw))
+    # torch prints the number as it was given
+    assert str(got.value).split(':')[0] == str(want.value).split(':')[0]
+
+
+def test_fedopt_muon_config():
+    agg = _fedopt(dict(type='Muon', lr=0.1))
+    assert (agg.momentum, agg.nesterov, agg.weight_decay, agg.ns_steps,
+            agg.eps, agg.ns_coefficients) == (0.95, True, 0.1, 5, 1e-7, COEF)
+    with pytest.raises(ValueError, match='2D') as got:
+        _fedopt(dict(type='Muon', lr=0.1), torch.nn.Linear(3, 2))
+    with pytest.raises(ValueError) as want:
+        torch.optim.Muon([torch.zeros(2, requires_grad=True)])
+    assert str(got.value) == str(want.value)
+    for bad in (dict(ns_steps=100), dict(ns_steps=0), dict(eps=0.0),
+                dict(ns_coefficients=(1.0, 2.0)),
+                dict(aux=dict(type='Muon', lr=0.1))):
+        with pytest.raises(ValueError):
+            _fedopt(dict(type='Muon', lr=0.1, **bad))
+    with pytest.raises(TypeError, match='unexpected'):
+        _fedopt(dict(type='Muon', lr=0.1, betas=(0.9, 0.99)))
+    with pytest.raises(NotImplementedError):
+        _fedopt(dict(type='Muon', lr=0.1, aux=dict(type='LBFGS', lr=1.0)))
+    agg = _fedopt(dict(type='Muon', lr=0.1, aux=dict(type='Adam', lr=0.2)),
+                  torch.nn.Linear(3, 2))
+    assert agg._aux.opt_type == 'Adam' and agg._aux.lr0 == 0.2
+
+
+def test_sparse_keys_are_seen_and_host_packing_refuses_them():
+    from federatedscope_amd.core.aggregators.clients_avg_aggregator import \
+        sparse_keys
+    sp = torch.sparse_coo_tensor(torch.tensor([[1, 3]]), torch.ones(2, 4),
+                                 (5, 4))
+    assert sparse_keys({'a': torch.zeros(2), 'b': sp, 'c': 'text',
+                        'd': [1.0]}) == ['b']
+    dst = torch.zeros(20)
+    assert L.host().host_pack_dict(
+        {'b': sp}, [('b', 0, 80, 6, 0)], [], dst.data_ptr()) is False
