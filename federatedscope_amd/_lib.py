@@ -236,8 +236,8 @@ class EmbedPart(ctypes.Structure):
 
 
 FSAGG_MUON_ORIGINAL, FSAGG_MUON_MATCH_RMS = 0, 1
-SIGNATURES['fsagg_newton_schulz_workspace_bytes'] = (
-    _c_sz, [_c_i64, _c_i64, _c_i64])
+SIGNATURES['fsagg_newton_schulz_workspace_bytes'] = (_c_sz, [_c_p, _c_i])
+SIGNATURES['fsagg_muon_workspace_bytes'] = (_c_sz, [_c_p, _c_i])
 SIGNATURES['fsagg_newton_schulz'] = (
     _c_i, [_c_p, _c_i, _c_i, _c_p, _c_d, _c_p, _c_sz, _c_p])
 SIGNATURES['fsagg_muon_step_f32'] = (

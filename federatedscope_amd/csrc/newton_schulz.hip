@@ -29,13 +29,12 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMaxGroup = 24;     // matrices per launch (kernel arguments)
 constexpr int kNormBlock = 256;
-constexpr int kNormElems = 8192;  // update elements per norm workgroup
 constexpr int kMaxNorm = 256;     // norm workgroups per matrix
-constexpr int kPad = 128;         // workspace sides are multiples of this
 constexpr int kBK = 32;           // k per LDS stage
 constexpr float kS = 4096.0f;     // limb scale
 constexpr float kInvS = 1.0f / 4096.0f;
@@ -51,6 +50,7 @@ struct Mat {
   int32_t rows, cols, batch;
   int32_t m, n, mp, np;  // short and long side, and padded
   int32_t nb;            // norm workgroups per matrix
+  int32_t slabs, each;   // narrow matrices: slabs, and 64-column chunks of one
   int16_t dt, odt;
 };
 
@@ -93,6 +93,31 @@ __device__ __forceinline__ Planes planes_of(const Mat &M, int z) {
   return P;
 }
 
+// A narrow matrix (m <= kNarrow) keeps the iterate as fp32, a column's 64
+// rows together, and the slabs' shares of the Gram matrix, of this step and
+// the next.
+constexpr int kNarrow = 64;
+constexpr int kNarrowLong = 16384;
+constexpr int kMaxEach = 4;
+#ifndef NS_E1
+#define NS_E1 32
+#define NS_E2 64
+#endif
+constexpr int kGramElems = kNarrow * kNarrow;
+struct Narrow {
+  double *norm;
+  float *u, *x, *gram;
+};
+__device__ __forceinline__ Narrow narrow_of(const Mat &M, int z) {
+  char *p = M.ws + z * M.wstride;
+  Narrow N;
+  N.norm = reinterpret_cast<double *>(p);
+  N.x = reinterpret_cast<float *>(p + 8 * kMaxNorm);
+  N.gram = N.x + int64_t(M.np) * kNarrow;
+  N.u = N.gram + 2 * int64_t(M.slabs) * kGramElems;
+  return N;
+}
+
 struct Group {
   int nmat;
   int start[kMaxGroup + 1];  // first workgroup of each entry
@@ -111,6 +136,14 @@ struct MuonScalars {
   float keep, mu, lr, decay;  // 1 - momentum, momentum, lr, 1 - lr * wd
   int nesterov, maximize, adjust;
 };
+
+// the matrix's own learning rate
+__device__ __forceinline__ float muon_lr(const Mat &M, const MuonScalars &S) {
+  const float r = float(M.rows), k = float(M.cols);
+  if (S.adjust == FSAGG_MUON_MATCH_RMS)
+    return S.lr * (0.2f * __fsqrt_rn(r > k ? r : k));
+  return r > k ? S.lr * __fsqrt_rn(__fdiv_rn(r, k)) : S.lr;
+}
 
 __device__ __forceinline__ float load_as_f32(const void *p, int64_t i,
                                              int dt) {
@@ -134,55 +167,117 @@ __device__ __forceinline__ void store_from_f32(void *p, int64_t i, int dt,
   else static_cast<uint16_t *>(p)[i] = to_bf16(v);
 }
 
+// Results y of rows i .. i + 3, column j of matrix z (m x n orientation).
+template <bool MUON>
+__device__ __forceinline__ void store_result(const Mat &M,
+                                             const MuonScalars &S, int z,
+                                             int i, int j, const float *y) {
+  if (j >= M.n) return;
+  const bool tall = M.rows > M.cols;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (i + e >= M.m) continue;
+    const int64_t o = tall ? int64_t(j) * M.cols + i + e
+                           : int64_t(i + e) * M.cols + j;
+    if constexpr (MUON) {
+      float *p = static_cast<float *>(M.out) + o;
+      *p = __builtin_fmaf(-muon_lr(M, S), y[e], __fmul_rn(*p, S.decay));
+    } else {
+      store_from_f32(M.out, int64_t(z) * M.rows * M.cols + o, M.odt, y[e]);
+    }
+  }
+}
+
 __device__ __forceinline__ void split(float v, _Float16 &h, _Float16 &l) {
   h = _Float16(v);
   l = _Float16(v - float(h));
 }
 
-// Pass 1: the fp32 update u, rows x cols contiguous, and a workgroup's sum
-// of u^2 in fp64 (squares of fp32 neither overflow nor vanish there).
+// The update at element e = (i, j) of matrix z.
 //   MUON: g = p - avg (negated for maximize); buf += (1 - mu)(g - buf);
 //         u = nesterov ? g + mu (buf - g) : buf.
 template <bool MUON>
+__device__ __forceinline__ float update_at(const Mat &M, const MuonScalars &S,
+                                           int z, int64_t e, int64_t i,
+                                           int64_t j) {
+  if constexpr (!MUON)
+    return load_as_f32(M.g, z * M.sz + i * M.si + j * M.sj, M.dt);
+  const float p = static_cast<const float *>(M.out)[e];
+  float g = __fsub_rn(p, static_cast<const float *>(M.g)[e]);
+  if (S.maximize) g = -g;
+  const float o = M.buf[e];
+  // the torch.lerp forms: exact at both ends (mu = 0 gives g)
+  const float d = __fsub_rn(g, o);
+  const float n = S.keep < 0.5f
+                      ? __builtin_fmaf(S.keep, d, o)
+                      : __fsub_rn(g, __fmul_rn(d, 1.0f - S.keep));
+  M.buf[e] = n;
+  return S.nesterov ? __builtin_fmaf(S.mu, __fsub_rn(n, g), g) : n;
+}
+
+// Sum of the workgroup's kThreads values, in a fixed order, in every thread.
+template <int kThreads>
+__device__ __forceinline__ double block_sum(double v, double *part) {
+  part[threadIdx.x] = v;
+  __syncthreads();
+  for (int s = kThreads / 2; s > 0; s >>= 1) {
+    if (int(threadIdx.x) < s) part[threadIdx.x] += part[threadIdx.x + s];
+    __syncthreads();
+  }
+  return part[0];
+}
+
+// kS / max(norm, eps); NaN for a NaN norm, as dividing by it would give
+__device__ __forceinline__ double limb_scale(double sq, double eps) {
+  const double norm = sqrt(sq);
+  return double(kS) / (norm < eps ? eps : norm);
+}
+
+// Pass 1: the fp32 update u, rows x cols contiguous, and a workgroup's sum
+// of u^2 in fp64 (squares of fp32 neither overflow nor vanish there).
+template <bool MUON, bool NARROW>
 __global__ __launch_bounds__(kNormBlock) void ns_update_kernel(
     Group G, MuonScalars S) {
   int rel;
   const Mat &M = G.mat[find_mat(G, blockIdx.x, rel)];
   const int z = rel / M.nb, b = rel % M.nb;
-  const Planes P = planes_of(M, z);
-  float *u = reinterpret_cast<float *>(P.th(1));
-  const int64_t total = int64_t(M.rows) * M.cols;
+  float *u;
+  double *norm;
+  if constexpr (NARROW) {
+    const Narrow N = narrow_of(M, z);
+    u = N.u;
+    norm = N.norm;
+  } else {
+    const Planes P = planes_of(M, z);
+    u = reinterpret_cast<float *>(P.th(1));
+    norm = P.norm;
+  }
+  const uint32_t total = uint32_t(M.rows) * uint32_t(M.cols);
+  const uint32_t step = uint32_t(M.nb) * kNormBlock;
   double sq = 0.0;
-  for (int64_t e = int64_t(b) * kNormBlock + threadIdx.x; e < total;
-       e += int64_t(M.nb) * kNormBlock) {
-    float v;
-    if constexpr (MUON) {
-      const float p = static_cast<const float *>(M.out)[e];
-      float g = __fsub_rn(p, static_cast<const float *>(M.g)[e]);
-      if (S.maximize) g = -g;
-      const float o = M.buf[e];
-      // the torch.lerp forms: exact at both ends (mu = 0 gives g)
-      const float d = __fsub_rn(g, o);
-      const float n = S.keep < 0.5f
-                          ? __builtin_fmaf(S.keep, d, o)
-                          : __fsub_rn(g, __fmul_rn(d, 1.0f - S.keep));
-      M.buf[e] = n;
-      v = S.nesterov ? __builtin_fmaf(S.mu, __fsub_rn(n, g), g) : n;
-    } else {
-      const int64_t i = e / M.cols, j = e - i * M.cols;
-      v = load_as_f32(M.g, z * M.sz + i * M.si + j * M.sj, M.dt);
+  constexpr int kAhead = 4;
+  for (uint32_t e0 = uint32_t(b) * kNormBlock + threadIdx.x; e0 < total;
+       e0 += kAhead * step) {
+    float v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const uint32_t e = e0 + k * step;
+      v[k] = 0.0f;
+      if (e < total) {
+        const uint32_t i = MUON ? 0u : e / uint32_t(M.cols);
+        v[k] = update_at<MUON>(M, S, z, e, i, e - i * uint32_t(M.cols));
+      }
     }
-    u[e] = v;
-    sq += double(v) * double(v);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const uint32_t e = e0 + k * step;
+      if (e < total) u[e] = v[k];
+      sq += double(v[k]) * double(v[k]);
+    }
   }
   __shared__ double part[kNormBlock];
-  part[threadIdx.x] = sq;
-  __syncthreads();
-  for (int s = kNormBlock / 2; s > 0; s >>= 1) {
-    if (int(threadIdx.x) < s) part[threadIdx.x] += part[threadIdx.x + s];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) P.norm[b] = part[0];
+  sq = block_sum<kNormBlock>(sq, part);
+  if (threadIdx.x == 0) norm[b] = sq;
 }
 
 // Pass 2: X and T limbs of u / max(|u|, eps), zero in the padding.  One
@@ -198,15 +293,10 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
   const float *u = reinterpret_cast<const float *>(P.th(1));
   __shared__ double part[256];
   __shared__ float tile[64][65];
-  part[threadIdx.x] = int(threadIdx.x) < M.nb ? P.norm[threadIdx.x] : 0.0;
-  __syncthreads();
-  for (int s = 128; s > 0; s >>= 1) {
-    if (int(threadIdx.x) < s) part[threadIdx.x] += part[threadIdx.x + s];
-    __syncthreads();
-  }
-  const double norm = sqrt(part[0]);
-  // NaN norm: every value becomes NaN, as dividing by it would
-  const double scale = double(kS) / (norm < eps ? eps : norm);
+  const double scale = limb_scale(
+      block_sum<256>(int(threadIdx.x) < M.nb ? P.norm[threadIdx.x] : 0.0,
+                     part),
+      eps);
   const int i0 = (t / tn) * 64, j0 = (t % tn) * 64;
   const bool tall = M.rows > M.cols;
   // u's own rows r and columns c of this tile
@@ -236,242 +326,701 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
 
 enum Mode { kGram, kSquare, kApply, kLast, kLastMuon };
 
-// One BM x BN tile of C = P R^T (k contiguous in both) in limbs, 4 waves of
-// WM x WN.  A stage is kBK of k of both operands' limbs, written to LDS by
-// 16-byte direct loads: 64-byte rows, the four 16-byte slots of row r
-// permuted by (r / 4) % 4 so that a fragment read of 16 rows touches all 64
-// banks once.  Two stages: one is loaded while the other is multiplied.
+constexpr bool symmetric(int mode) { return mode == kGram || mode == kSquare; }
+
+// Tiles of one matrix and stages (of kBK) of a tile.
+template <int MODE, int BM, int BN>
+__host__ __device__ __forceinline__ int mode_tiles(const Mat &M) {
+  const int tm = M.mp / BM;
+  return symmetric(MODE) ? tm * (tm + 1) / 2 : tm * (M.np / BN);
+}
+template <int MODE>
+__host__ __device__ __forceinline__ int mode_stages(const Mat &M) {
+  return (MODE == kGram ? M.np : M.mp) / kBK;
+}
+
+// Tile t of a matrix.  Neighbours in t share operands, so that the
+// workgroups of one XCD read few rows: bands of kBand tile rows, column by
+// column.  A symmetric product has the tiles with ti <= tj only.
+constexpr int kBand = 4;
+template <int MODE, int BM, int BN>
+__device__ __forceinline__ void tile_of(const Mat &M, int t, int &ti,
+                                        int &tj) {
+  const int tm = M.mp / BM;
+  if constexpr (symmetric(MODE)) {
+    int b = 0;  // first tile row of the band
+    for (;;) {
+      const int h = tm - b < kBand ? tm - b : kBand;
+      // a triangle of h rows, then full columns
+      const int tri = h * (h + 1) / 2, n = tri + h * (tm - b - h);
+      if (t >= n) {
+        t -= n;
+        b += h;
+        continue;
+      }
+      if (t < tri) {
+        int c = 0;
+        while (t > c) {
+          t -= c + 1;
+          ++c;
+        }
+        ti = b + t;
+        tj = b + c;
+      } else {
+        t -= tri;
+        ti = b + t % h;
+        tj = b + h + t / h;
+      }
+      return;
+    }
+  } else {
+    const int tn = M.np / BN;
+    const int b = t / (kBand * tn) * kBand;
+    const int h = tm - b < kBand ? tm - b : kBand;
+    t -= b * tn;
+    ti = b + t % h;
+    tj = t / h;
+  }
+}
+
+// The stages of a group's product in one line: entry after entry, tile after
+// tile.  Workgroup q of `workers` takes stages [q, q + 1) * total / workers.
+struct Line {
+  int total, workers;
+  float *partial;  // [workers][first, later][BM * BN]
+};
+__device__ __forceinline__ int line_at(const Line &L, int q) {
+  return int(int64_t(q) * L.total / L.workers);
+}
+
+// One tile of C = P R^T (k contiguous in both), from stage k0 to stage k1.  A
+// stage is kBK of k of both operands' limbs, written to LDS by 16-byte direct
+// loads: 64-byte rows, the four 16-byte slots of row r permuted by (r / 4) %
+// 4 so that a fragment read of 16 rows touches all 64 banks once.  NBUF
+// stages of LDS: one is multiplied while NBUF - 1 are on their way.
 //
 // Rows and columns of the padding are zero in every plane (the prepare pass
 // writes them, products of zero rows are zero), so no tile is ragged inside
 // the workspace; only the last step checks its stores against the matrix.
-template <int BM, int BN, int WM, int WN, int MODE>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ns_gemm_kernel(
-    Group G, int src, float b, float c, float a, MuonScalars S) {
-  constexpr int kWaves = (BM / WM) * (BN / WN);
-  constexpr int kLoads = (BM + BN) * 2 * kBK * 2 / 1024;  // 1 KiB each
-  constexpr int kPer = kLoads / kWaves;
+template <int BM, int BN, int WM, int WN, int NBUF, int LIMBS>
+struct Tile {
+  static constexpr int kBM = BM, kBN = BN;
+  static constexpr int kWaves = (BM / WM) * (BN / WN);
+  static constexpr int kThreads = kWaves * 64;
+  static constexpr int MI = WM / 32, NJ = WN / 32;
+  static constexpr int kLoads = (BM + BN) * LIMBS * kBK * 2 / 1024;  // 1 KiB
+  static constexpr int kPer = kLoads / kWaves;
+  static constexpr int kStage = (BM + BN) * LIMBS * kBK;  // halfs
+  static constexpr int kLds = NBUF * kStage;
   static_assert(kPer * kWaves == kLoads, "loads divide over the waves");
-  constexpr int MI = WM / 32, NJ = WN / 32;
-  constexpr int kStage = (BM + BN) * 2 * kBK;  // halfs
-  __shared__ __attribute__((aligned(1024))) _Float16 lds[2 * kStage];
 
-  int rel;
-  const Mat &M = G.mat[find_mat(G, blockIdx.x, rel)];
-  const int tm = M.mp / BM;
-  int z, ti, tj;
-  if constexpr (MODE == kGram || MODE == kSquare) {
-    static_assert(BM == BN || (MODE != kGram && MODE != kSquare),
-                  "square tiles of a symmetric product");
-    const int tiles = tm * (tm + 1) / 2;
-    z = rel / tiles;
-    int t = rel % tiles;
-    ti = 0;
-    while (t >= tm - ti) {
-      t -= tm - ti;
-      ++ti;
-    }
-    tj = ti + t;
-  } else {
-    const int tn = M.np / BN, tiles = tm * tn;
-    z = rel / tiles;
-    const int t = rel % tiles;
-    ti = t % tm;
-    tj = t / tm;
-  }
-  const Planes P = planes_of(M, z);
-  const _Float16 *ph, *pl, *rh, *rl;
-  int ld, K;
-  if constexpr (MODE == kGram) {
-    ph = rh = P.xh;
-    pl = rl = P.xl;
-    ld = K = M.np;
-  } else if constexpr (MODE == kSquare) {
-    ph = rh = P.ah;
-    pl = rl = P.al;
-    ld = K = M.mp;
-  } else {
-    ph = P.qh;
-    pl = P.ql;
-    rh = P.th(src);
-    rl = P.tl(src);
-    ld = K = M.mp;
-  }
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-  const int i0 = ti * BM, j0 = tj * BN;
-
-  // this wave's loads of a stage: LDS order is [P.h][P.l][R.h][R.l] rows of
-  // 64 bytes, 16 rows per instruction
-  const _Float16 *gsrc[kPer];
-  int ldst[kPer];
-#pragma unroll
-  for (int q = 0; q < kPer; ++q) {
-    const int k = wave * kPer + q;
-    const int row16 = k * 16;
-    const bool right = row16 >= 2 * BM;
-    const int in = right ? row16 - 2 * BM : row16;
-    const int side = right ? BN : BM;
-    const _Float16 *base =
-        in < side ? (right ? rh : ph) : (right ? rl : pl);
-    const int g0 = (right ? j0 : i0) + (in < side ? in : in - side);
-    const int r = lane >> 2, slot = (lane & 3) ^ ((r >> 2) & 3);
-    gsrc[q] = base + int64_t(g0 + r) * ld + slot * 8;
-    ldst[q] = row16 * kBK;
-  }
-  auto issue = [&](int k0, int buf) {
-#pragma unroll
-    for (int q = 0; q < kPer; ++q)
-      __builtin_amdgcn_global_load_lds(
-          (__attribute__((address_space(1))) void *)(gsrc[q] + k0),
-          (__attribute__((address_space(3))) void *)(uintptr_t)(
-              lds + buf * kStage + ldst[q]),
-          16, 0, 0);
-  };
-
-  const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
-  const int fr = lane & 31, fk = lane >> 5;
   f32x16 acc[MI][NJ];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  int lane, wave, wm, wn;
 
-  issue(0, 0);
-  for (int k0 = 0, buf = 0; k0 < K; k0 += kBK, buf ^= 1) {
-    // this stage has landed for every wave, and the other is read out
+  __device__ __forceinline__ Tile() {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+    wm = (wave % (BM / WM)) * WM;
+    wn = (wave / (BM / WM)) * WN;
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  }
+
+  __device__ __forceinline__ void multiply(_Float16 *lds, const _Float16 *ph,
+                                           const _Float16 *pl,
+                                           const _Float16 *rh,
+                                           const _Float16 *rl, int ld, int i0,
+                                           int j0, int k0, int k1) {
+    // this wave's loads of a stage: LDS order is [P.h][P.l][R.h][R.l] rows
+    // of 64 bytes, 16 rows per instruction
+    const _Float16 *gsrc[kPer];
+    int ldst[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      const int row16 = (wave * kPer + q) * 16;
+      const bool right = row16 >= LIMBS * BM;
+      const int in = right ? row16 - LIMBS * BM : row16;
+      const int side = right ? BN : BM;
+      const _Float16 *base =
+          in < side ? (right ? rh : ph) : (right ? rl : pl);
+      const int g0 = (right ? j0 : i0) + (in < side ? in : in - side);
+      const int r = lane >> 2, slot = (lane & 3) ^ ((r >> 2) & 3);
+      gsrc[q] = base + int64_t(g0 + r) * ld + slot * 8;
+      ldst[q] = row16 * kBK;
+    }
+    auto issue = [&](int k) {
+      const int buf = k % NBUF;
+#pragma unroll
+      for (int q = 0; q < kPer; ++q)
+        __builtin_amdgcn_global_load_lds(
+            (__attribute__((address_space(1))) void *)(gsrc[q] + k * kBK),
+            (__attribute__((address_space(3))) void *)(uintptr_t)(
+                lds + buf * kStage + ldst[q]),
+            16, 0, 0);
+    };
+    const int fr = lane & 31, fk = lane >> 5;
+    clear();
+    // nothing of the previous tile is on its way, and every wave has read its
+    // last stage
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (k0 + kBK < K) issue(k0 + kBK, buf ^ 1);
-    const _Float16 *st = lds + buf * kStage;
 #pragma unroll
-    for (int kk = 0; kk < kBK / 16; ++kk) {
-      half8 fah[MI], fal[MI], fbh[NJ], fbl[NJ];
+    for (int n = 0; n < NBUF - 1; ++n)
+      if (k0 + n < k1) issue(k0 + n);
+    for (int k = k0; k < k1; ++k) {
+      // this stage has landed for every wave (later ones may be on their
+      // way), and the one before it is read out
+      if (NBUF > 2 && k + NBUF - 1 <= k1)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
+                         (NBUF - 2) * kPer)
+                     : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" :::
+                         "memory");
+      if (k + NBUF - 1 < k1) issue(k + NBUF - 1);
+      const _Float16 *st = lds + (k % NBUF) * kStage;
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int r = wm + i * 32 + fr;
-        const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
-        fah[i] = *reinterpret_cast<const half8 *>(st + o);
-        fal[i] = *reinterpret_cast<const half8 *>(st + BM * kBK + o);
-      }
+      for (int kk = 0; kk < kBK / 16; ++kk) {
+        half8 fa[LIMBS][MI], fb[LIMBS][NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int r = wn + j * 32 + fr;
-        const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
-        fbh[j] = *reinterpret_cast<const half8 *>(st + 2 * BM * kBK + o);
-        fbl[j] =
-            *reinterpret_cast<const half8 *>(st + (2 * BM + BN) * kBK + o);
-      }
+        for (int i = 0; i < MI; ++i) {
+          const int r = wm + i * 32 + fr;
+          const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+          for (int l = 0; l < LIMBS; ++l)
+            fa[l][i] =
+                *reinterpret_cast<const half8 *>(st + l * BM * kBK + o);
+        }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              fal[i], fbh[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              fah[i], fbl[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              fah[i], fbh[j], acc[i][j], 0, 0, 0);
+          const int r = wn + j * 32 + fr;
+          const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
+#pragma unroll
+          for (int l = 0; l < LIMBS; ++l)
+            fb[l][j] = *reinterpret_cast<const half8 *>(
+                st + (LIMBS * BM + l * BN) * kBK + o);
+        }
+        // l h, h l, h h (the small terms first)
+#pragma unroll
+        for (int t = LIMBS == 2 ? 0 : 2; t < 3; ++t)
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                  fa[t == 0 ? LIMBS - 1 : 0][i],
+                  fb[t == 1 ? LIMBS - 1 : 0][j], acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+
+  // block (i, j) of the accumulators as it lies in the threads, 16 bytes at
+  // a time
+  __device__ __forceinline__ void put_partial(float *p) const {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+          reinterpret_cast<f32x4 *>(
+              p)[((i * NJ + j) * 4 + q) * kThreads + threadIdx.x] = v;
+        }
+  }
+  static __device__ __forceinline__ void add_partial(f32x16 &x,
+                                                     const float *p,
+                                                     int block) {
+    f32x4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      v[q] = reinterpret_cast<const f32x4 *>(
+          p)[(block * 4 + q) * kThreads + threadIdx.x];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = __fadd_rn(x[r], v[r / 4][r % 4]);
+  }
+
+  template <int MODE>
+  __device__ __forceinline__ void finish(const Mat &M, const Planes &P, int z,
+                                         int ti, int tj, int src, float a,
+                                         float b, float c,
+                                         const MuonScalars &S) const {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        finish_block<MODE>(acc[i][j], M, P, z, ti, tj, i, j, src, a, b, c, S);
+  }
+
+  // what the product is for, for one 32 x 32 block: a lane holds column gj
+  // and rows gi .. gi + 3 of each quad
+  template <int MODE>
+  __device__ __forceinline__ void finish_block(
+      const f32x16 &x, const Mat &M, const Planes &P, int z, int ti, int tj,
+      int i, int j, int src, float a, float b, float c,
+      const MuonScalars &S) const {
+    const int fr = lane & 31, fk = lane >> 5;
+    const int gi0 = ti * BM + wm + i * 32 + 4 * fk;
+    const int gj = tj * BN + wn + j * 32 + fr;
+    half4 oh[4], ol[4];
+    if constexpr (MODE != kGram) {
+      // A is symmetric: its column gj is row gj; X's column is T's row
+      const _Float16 *bh = MODE == kSquare ? P.ah : P.th(src);
+      const _Float16 *bl = MODE == kSquare ? P.al : P.tl(src);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t o = int64_t(gj) * M.mp + gi0 + 8 * q;
+        oh[q] = *reinterpret_cast<const half4 *>(bh + o);
+        ol[q] = *reinterpret_cast<const half4 *>(bl + o);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int gi = gi0 + 8 * q;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = x[4 * q + e] * kInvS;
+        if constexpr (MODE == kSquare)
+          v[e] = b * (float(oh[q][e]) + float(ol[q][e])) + c * v[e];
+        else if constexpr (MODE != kGram)
+          v[e] = a * (float(oh[q][e]) + float(ol[q][e])) + v[e];
+      }
+      if constexpr (MODE == kLast || MODE == kLastMuon) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= kInvS;
+        store_result<MODE == kLastMuon>(M, S, z, gi, gj, v);
+      } else {
+        half4 h, l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          _Float16 u, w;
+          split(v[e], u, w);
+          h[e] = u;
+          l[e] = w;
+        }
+        _Float16 *ch, *cl, *dh, *dl;  // C by rows, and C^T
+        int ldc, ldd;
+        if constexpr (MODE == kApply) {
+          ch = P.xh;
+          cl = P.xl;
+          ldc = M.np;
+          dh = P.th(src ^ 1);
+          dl = P.tl(src ^ 1);
+          ldd = M.mp;
+        } else {
+          ch = MODE == kGram ? P.ah : P.qh;
+          cl = MODE == kGram ? P.al : P.ql;
+          ldc = ldd = M.mp;
+          dh = ch;
+          dl = cl;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t o = int64_t(gi + e) * ldc + gj;
+          ch[o] = h[e];
+          if (LIMBS == 2 || MODE == kGram) cl[o] = l[e];
+        }
+        if (MODE == kApply || ti != tj) {
+          const int64_t o = int64_t(gj) * ldd + gi;
+          *reinterpret_cast<half4 *>(dh + o) = h;
+          if (LIMBS == 2 || MODE != kSquare)
+            *reinterpret_cast<half4 *>(dl + o) = l;
+        }
+      }
+    }
+  }
+};
+
+template <int MODE, class T>
+__device__ __forceinline__ void multiply_of(T &tile, _Float16 *lds,
+                                            const Mat &M, const Planes &P,
+                                            int src, int i0, int j0, int k0,
+                                            int k1) {
+  if constexpr (MODE == kGram)
+    tile.multiply(lds, P.xh, P.xl, P.xh, P.xl, M.np, i0, j0, k0, k1);
+  else if constexpr (MODE == kSquare)
+    tile.multiply(lds, P.ah, P.al, P.ah, P.al, M.mp, i0, j0, k0, k1);
+  else
+    tile.multiply(lds, P.qh, P.ql, P.th(src), P.tl(src), M.mp, i0, j0, k0,
+                  k1);
+}
+
+// Workgroup b's place when the workgroups, which go round robin over the 8
+// XCDs, shall take a contiguous stretch of the work per XCD.
+__device__ __forceinline__ int xcd_place(int b, int n) {
+  const int per = n / 8, more = n % 8, x = b % 8;
+  return x * per + (x < more ? x : more) + b / 8;
+}
+
+// A product, one workgroup per tile (G.start counts tiles).
+template <class T, int MODE>
+__global__ __launch_bounds__(T::kThreads) void ns_gemm_kernel(
+    Group G, int src, float a, float b, float c, MuonScalars S) {
+  __shared__ __attribute__((aligned(1024))) _Float16 lds[T::kLds];
+  int rel;
+  const Mat &M =
+      G.mat[find_mat(G, xcd_place(int(blockIdx.x), int(gridDim.x)), rel)];
+  const int tiles = mode_tiles<MODE, T::kBM, T::kBN>(M);
+  const int z = rel / tiles;
+  int ti, tj;
+  tile_of<MODE, T::kBM, T::kBN>(M, rel % tiles, ti, tj);
+  const Planes P = planes_of(M, z);
+  T tile;
+  multiply_of<MODE>(tile, lds, M, P, src, ti * T::kBM, tj * T::kBN, 0,
+                    mode_stages<MODE>(M));
+  tile.template finish<MODE>(M, P, z, ti, tj, src, a, b, c, S);
+}
+
+// A product over the line of stages (G.start counts stages): whole tiles are
+// finished here, a tile that two or more workgroups share leaves its parts
+// in `partial`.
+template <class T, int MODE>
+__global__ __launch_bounds__(T::kThreads) void ns_line_kernel(
+    Group G, Line L, int src, float a, float b, float c, MuonScalars S) {
+  __shared__ __attribute__((aligned(1024))) _Float16 lds[T::kLds];
+  const int q = xcd_place(int(blockIdx.x), L.workers);
+  int at = line_at(L, q);
+  const int end = line_at(L, q + 1);
+  T tile;
+  for (int seg = 0; at < end; ++seg) {
+    int rel;
+    const Mat &M = G.mat[find_mat(G, at, rel)];
+    const int stages = mode_stages<MODE>(M);
+    const int tiles = mode_tiles<MODE, T::kBM, T::kBN>(M);
+    const int t = rel / stages, k0 = rel % stages;
+    const int left = end - at;
+    const int k1 = stages - k0 < left ? stages : k0 + left;
+    const int z = t / tiles;
+    int ti, tj;
+    tile_of<MODE, T::kBM, T::kBN>(M, t % tiles, ti, tj);
+    const Planes P = planes_of(M, z);
+    multiply_of<MODE>(tile, lds, M, P, src, ti * T::kBM, tj * T::kBN, k0, k1);
+    if (k0 == 0 && k1 == stages)
+      tile.template finish<MODE>(M, P, z, ti, tj, src, a, b, c, S);
+    else
+      tile.put_partial(L.partial +
+                       (int64_t(q) * 2 + (seg > 0)) * (T::kBM * T::kBN));
+    at += k1 - k0;
+  }
+}
+
+// Tiles that workgroups shared: workgroup (w, block) looks at the boundary
+// between workers w and w + 1 and, when it is the first one inside a tile,
+// adds the tile's parts in order, one 32 x 32 block of every wave.
+template <class T, int MODE>
+__global__ __launch_bounds__(T::kThreads) void ns_join_kernel(
+    Group G, Line L, int src, float a, float b, float c, MuonScalars S) {
+  int w = int(blockIdx.x);
+  const int block = int(blockIdx.y);
+  const int cut = line_at(L, w + 1);
+  int rel;
+  const Mat &M = G.mat[find_mat(G, cut, rel)];
+  const int stages = mode_stages<MODE>(M);
+  const int tiles = mode_tiles<MODE, T::kBM, T::kBN>(M);
+  const int t = rel / stages, first = cut - rel % stages;
+  if (cut == first || line_at(L, w) > first) return;
+  f32x16 x;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+  for (; w < L.workers && line_at(L, w) < first + stages; ++w)
+    if (line_at(L, w) < line_at(L, w + 1))
+      T::add_partial(x,
+                     L.partial + (int64_t(w) * 2 + (line_at(L, w) < first)) *
+                                     (T::kBM * T::kBN),
+                     block);
+  const int z = t / tiles;
+  int ti, tj;
+  tile_of<MODE, T::kBM, T::kBN>(M, t % tiles, ti, tj);
+  T tile;
+  tile.template finish_block<MODE>(x, M, planes_of(M, z), z, ti, tj,
+                                   block / T::NJ, block % T::NJ, src, a, b, c,
+                                   S);
+}
+
+// -- narrow matrices ---------------------------------------------------------
+// m <= 64: A and Q are one 64 x 64 tile, and what a step costs is reading the
+// columns and handing the Gram matrix over.  A workgroup of 4 waves owns a
+// slab of up to kMaxEach chunks of 64 columns, a wave one 32 x 32 block of
+// every product; the slab's columns stay in its registers for the step.  A
+// launch sums the slabs' Gram shares of the step before (every workgroup the
+// same, in order), forms Q, applies it and leaves its share of the next one:
+// one launch per step, where the tiled products take three.  A matrix of one
+// slab needs no exchange: all its steps are one launch.
+__device__ __forceinline__ int swz(int r, int chunk) {
+  return r * 64 + ((chunk ^ ((r >> 1) & 7)) * 8);
+}
+
+struct Slab {
+  int lane, fr, fk, bi, bj;
+  __device__ __forceinline__ Slab() {
+    lane = threadIdx.x & 63;
+    fr = lane & 31;
+    fk = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+    bi = (wave & 1) * 32;
+    bj = (wave >> 1) * 32;
+  }
+  // rows of quad q of this lane, and its column
+  __device__ __forceinline__ int row(int q) const {
+    return bi + 8 * q + 4 * fk;
+  }
+  __device__ __forceinline__ int col() const { return bj + fr; }
+
+  // x += P R^T over 64 of k; planes [64][64], limbs l at + 4096
+  __device__ __forceinline__ void multiply(const _Float16 *p,
+                                           const _Float16 *r,
+                                           f32x16 &x) const {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const int op = swz(bi + fr, kk * 2 + fk), oq = swz(bj + fr, kk * 2 + fk);
+      const half8 ph = *reinterpret_cast<const half8 *>(p + op);
+      const half8 pl = *reinterpret_cast<const half8 *>(p + 4096 + op);
+      const half8 rh = *reinterpret_cast<const half8 *>(r + oq);
+      const half8 rl = *reinterpret_cast<const half8 *>(r + 4096 + oq);
+      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, rh, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rl, x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rh, x, 0, 0, 0);
+    }
+  }
+  // limbs of the block's values (times kS), transposed: row col(), the rows
+  // of a quad side by side
+  __device__ __forceinline__ void put_columns(_Float16 *p,
+                                              const f32x16 &x) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      half4 h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        _Float16 u, w;
+        split(x[4 * q + e], u, w);
+        h[e] = u;
+        l[e] = w;
+      }
+      const int o = swz(col(), row(q) >> 3) + (row(q) & 7);
+      *reinterpret_cast<half4 *>(p + o) = h;
+      *reinterpret_cast<half4 *>(p + 4096 + o) = l;
+    }
+  }
+  // the same by rows
+  __device__ __forceinline__ void put_rows(_Float16 *p,
+                                           const f32x16 &x) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        _Float16 u, w;
+        split(x[4 * q + e], u, w);
+        const int o = swz(row(q) + e, col() >> 3) + (col() & 7);
+        p[o] = u;
+        p[4096 + o] = w;
+      }
+  }
+};
+
+// Launch k of a narrow matrix: 0 scales the update; k = 1 .. steps is step
+// k, the last of which stores the result.  WHOLE: everything in one launch.
+template <bool MUON, bool WHOLE>
+__global__ __launch_bounds__(256) void ns_narrow_kernel(
+    Group G, int k, int steps, float a, float b, float c, double eps,
+    MuonScalars S) {
+  __shared__ __attribute__((aligned(1024))) _Float16 lds[3 * 2 * 4096];
+  __shared__ double part[256];
+  _Float16 *const lq = lds, *const lt = lds + 8192, *const lx = lds + 16384;
+  int rel;
+  const Mat &M = G.mat[find_mat(G, blockIdx.x, rel)];
+  const int slabs = WHOLE ? 1 : M.slabs;
+  const int z = rel / slabs, slab = rel % slabs;
+  const int chunk0 = slab * M.each, chunks = M.np / 64;
+  const int have = chunks - chunk0 < M.each ? chunks - chunk0 : M.each;
+  const Narrow N = narrow_of(M, z);
+  const Slab W;
+  const bool tall = M.rows > M.cols;
+  f32x16 x[kMaxEach];  // kS times the columns
+
+  f32x16 gram;
+  auto clear = [](f32x16 &v) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = 0.0f;
+  };
+  clear(gram);
+  if (WHOLE || k == 0) {
+    // the update, scaled
+    double sq = 0.0;
+#pragma unroll
+    for (int ch = 0; ch < kMaxEach; ++ch) {
+      if (ch >= have) break;
+      const int j = (chunk0 + ch) * 64 + W.col();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = W.row(q) + e;
+          float v = 0.0f;
+          if (i < M.m && j < M.n) {
+            const int r = tall ? j : i, cc = tall ? i : j;
+            const int64_t o = int64_t(r) * M.cols + cc;
+            v = WHOLE ? update_at<MUON>(M, S, z, o, r, cc) : N.u[o];
+          }
+          x[ch][4 * q + e] = v;
+          if (WHOLE) sq += double(v) * double(v);
+        }
+    }
+    if (!WHOLE)
+      sq = int(threadIdx.x) < M.nb ? N.norm[threadIdx.x] : 0.0;
+    const double scale = limb_scale(block_sum<256>(sq, part), eps);
+#pragma unroll
+    for (int ch = 0; ch < kMaxEach; ++ch) {
+      if (ch >= have) break;
+      // (padding stays zero whatever the scale)
+      const int j = (chunk0 + ch) * 64 + W.col();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = W.row(r / 4) + r % 4;
+        x[ch][r] = i < M.m && j < M.n ? float(double(x[ch][r]) * scale)
+                                      : 0.0f;
+      }
+      W.put_rows(lx, x[ch]);
+      __syncthreads();
+      W.multiply(lx, lx, gram);
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int ch = 0; ch < kMaxEach; ++ch) {
+      if (ch >= have) break;
+      const float *p = N.x + (int64_t(chunk0 + ch) * 64 + W.col()) * kNarrow;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(p + W.row(q));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[ch][4 * q + e] = v[e];
+      }
+    }
+    // every slab's share of the Gram matrix, in order
+    const f32x4 *g = reinterpret_cast<const f32x4 *>(
+        N.gram + int64_t((k - 1) & 1) * slabs * kGramElems);
+    constexpr int kAhead = 4;
+    for (int s0 = 0; s0 < slabs; s0 += kAhead) {
+      f32x4 v[kAhead][4];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (s0 + u < slabs)
+            v[u][q] = g[(s0 + u) * (kGramElems / 4) + q * 256 + threadIdx.x];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (s0 + u < slabs) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            gram[r] = __fadd_rn(gram[r], v[u][r / 4][r % 4]);
         }
     }
   }
 
-  // a lane holds column j and rows i .. i + 3 of each quad
+  for (int step = WHOLE ? 1 : k;; ++step) {
+    if (step > 0) {
+      // Q = bA + cA^2 from the Gram sum (kS^2 A)
+      f32x16 t;
+      clear(t);
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+      for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
+      W.put_columns(lt, gram);
+      __syncthreads();
+      W.multiply(lt, lt, t);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+      for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
+      W.put_columns(lq, t);
+      clear(gram);
+      __syncthreads();
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int gi = i0 + wm + i * 32 + 8 * q + 4 * fk;
-        const int gj = j0 + wn + j * 32 + fr;
-        float v[4];
+      for (int ch = 0; ch < kMaxEach; ++ch) {
+        if (ch >= have) break;
+        W.put_columns(lt, x[ch]);
+        __syncthreads();
+        clear(t);
+        W.multiply(lq, lt, t);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * kInvS;
-        if constexpr (MODE == kSquare) {
-          // A is symmetric: its column gj is row gj
-          const int64_t o = int64_t(gj) * M.mp + gi;
-          const half4 h = *reinterpret_cast<const half4 *>(P.ah + o);
-          const half4 l = *reinterpret_cast<const half4 *>(P.al + o);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = b * (float(h[e]) + float(l[e])) + c * v[e];
-        }
-        if constexpr (MODE == kApply || MODE == kLast || MODE == kLastMuon) {
-          const int64_t o = int64_t(gj) * M.mp + gi;
-          const half4 h = *reinterpret_cast<const half4 *>(P.th(src) + o);
-          const half4 l = *reinterpret_cast<const half4 *>(P.tl(src) + o);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = a * (float(h[e]) + float(l[e])) + v[e];
-        }
-        if constexpr (MODE == kLast || MODE == kLastMuon) {
-          if (gj >= M.n) continue;
-          const bool tall = M.rows > M.cols;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (gi + e >= M.m) continue;
-            const int64_t o = tall ? int64_t(gj) * M.cols + gi + e
-                                   : int64_t(gi + e) * M.cols + gj;
-            const float y = v[e] * kInvS;
-            if constexpr (MODE == kLast) {
-              store_from_f32(M.out, int64_t(z) * M.rows * M.cols + o, M.odt,
-                             y);
-            } else {
-              const float r = float(M.rows), k = float(M.cols);
-              const float lr =
-                  S.lr * (S.adjust == FSAGG_MUON_MATCH_RMS
-                              ? 0.2f * __fsqrt_rn(r > k ? r : k)
-                              : (r > k ? __fsqrt_rn(__fdiv_rn(r, k)) : 1.0f));
-              float *p = static_cast<float *>(M.out) + o;
-              *p = __builtin_fmaf(-lr, y, __fmul_rn(*p, S.decay));
-            }
-          }
+        for (int r = 0; r < 16; ++r)
+          x[ch][r] = a * x[ch][r] + t[r] * kInvS;
+        if (step < steps) {
+          W.put_rows(lx, x[ch]);
+          __syncthreads();
+          W.multiply(lx, lx, gram);
         } else {
-          half4 h, l;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            _Float16 x, y;
-            split(v[e], x, y);
-            h[e] = x;
-            l[e] = y;
-          }
-          _Float16 *ch, *cl, *dh, *dl;  // C by rows, and C^T
-          int ldc, ldd;
-          if constexpr (MODE == kApply) {
-            ch = P.xh;
-            cl = P.xl;
-            ldc = M.np;
-            dh = P.th(src ^ 1);
-            dl = P.tl(src ^ 1);
-            ldd = M.mp;
-          } else {
-            ch = MODE == kGram ? P.ah : P.qh;
-            cl = MODE == kGram ? P.al : P.ql;
-            ldc = ldd = M.mp;
-            dh = ch;
-            dl = cl;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int64_t o = int64_t(gi + e) * ldc + gj;
-            ch[o] = h[e];
-            cl[o] = l[e];
-          }
-          if (MODE == kApply || ti != tj) {
-            const int64_t o = int64_t(gj) * ldd + gi;
-            *reinterpret_cast<half4 *>(dh + o) = h;
-            *reinterpret_cast<half4 *>(dl + o) = l;
-          }
+          __syncthreads();
         }
       }
+    }
+    if (!WHOLE || step >= steps) break;
+  }
+
+  if (!WHOLE && k < steps) {
+#pragma unroll
+    for (int ch = 0; ch < kMaxEach; ++ch) {
+      if (ch >= have) break;
+      float *p = N.x + (int64_t(chunk0 + ch) * 64 + W.col()) * kNarrow;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = x[ch][4 * q + e];
+        *reinterpret_cast<f32x4 *>(p + W.row(q)) = v;
+      }
+    }
+    f32x4 *g = reinterpret_cast<f32x4 *>(
+        N.gram + (int64_t(k & 1) * slabs + slab) * kGramElems);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = gram[4 * q + e];
+      g[q * 256 + threadIdx.x] = v;
+    }
+    return;
+  }
+#pragma unroll
+  for (int ch = 0; ch < kMaxEach; ++ch) {
+    if (ch >= have) break;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = x[ch][4 * q + e] * kInvS;
+      store_result<MUON>(M, S, z, W.row(q),
+                         (chunk0 + ch) * 64 + W.col(), y);
+    }
+  }
 }
 
-int64_t round_pad(int64_t v) { return (v + kPad - 1) / kPad * kPad; }
+// -- host --------------------------------------------------------------------
+// Tiles: 256 x 256 keeps a CU's matrix cores at about 80 % of what a large
+// library product reaches, where there is work for all of them; 64 x 64 is
+// for matrices too small for that, where a tile's latency counts.  One limb
+// suffices for a bf16 result (below).
+using BigTile = Tile<256, 256, 128, 64, 2, 2>;
+using BigTile1 = Tile<256, 256, 128, 64, 4, 1>;
+using MidTile = Tile<64, 64, 32, 32, 4, 2>;
+constexpr int kBigWorkers = 256;   // one workgroup of a big tile per CU
+constexpr int kMidWorkers = 512;
+constexpr int kBigSide = 256, kMidSide = 64;
 
-// Fills the derived fields; 0 on success.
-int plan_mat(Mat &M, int64_t rows, int64_t cols, int64_t batch,
+// How an entry is computed: in one launch, by slabs, or by tiled products.
+enum Way { kWhole, kNarrowSlabs, kMid, kBig, kBigOne, kWays };
+
+int64_t round_to(int64_t v, int64_t p) { return (v + p - 1) / p * p; }
+
+// Checks the sizes and fills in what does not depend on the other entries.
+int size_mat(Mat &M, int64_t rows, int64_t cols, int64_t batch,
              const char *what) {
   if (rows < 0 || cols < 0 || batch < 0) {
     set_error("%s: negative size", what);
@@ -491,15 +1040,83 @@ int plan_mat(Mat &M, int64_t rows, int64_t cols, int64_t batch,
   M.batch = int32_t(batch);
   M.m = int32_t(m);
   M.n = int32_t(n);
-  M.mp = int32_t(round_pad(m));
-  M.np = int32_t(round_pad(n));
-  int64_t nb = (rows * cols + kNormElems - 1) / kNormElems;
-  M.nb = int32_t(nb < 1 ? 1 : nb > kMaxNorm ? kMaxNorm : nb);
-  M.wstride = (ws_bytes_of(M.mp, M.np) + 1023) / 1024 * 1024;
+  // a launch counts its work items in 32 bits: 64 x 64 tiles (the prepare
+  // pass has most) of all entries of a group
+  if (batch * (round_to(m, kBigSide) / 64) * (round_to(n, kBigSide) / 64) >
+      (int64_t(1) << 24) / kMaxGroup) {
+    set_error("%s: a batch of %lld %lld x %lld matrices is too large for one "
+              "call", what, (long long)batch, (long long)rows,
+              (long long)cols);
+    return FSAGG_EINVAL;
+  }
   return FSAGG_OK;
 }
 
 bool empty(const Mat &M) { return M.m == 0 || M.batch == 0; }
+
+// Stages of the last product of an entry in big tiles.
+int64_t big_stages(const Mat &M) {
+  return M.batch * (round_to(M.m, kBigSide) / kBigSide) *
+         (round_to(M.n, kBigSide) / kBigSide) *
+         (round_to(M.m, kBigSide) / kBK);
+}
+
+// Big tiles pay from about 8 stages for each of the 256 workgroups on.
+constexpr int64_t kBigStages = 2048;
+constexpr int kBigShort = 512;
+
+Way way_of(const Mat &M, const int64_t (&work)[2]) {
+  if (M.m <= kNarrow && M.n <= kNarrowLong)
+    return M.n <= 64 * kMaxEach ? kWhole : kNarrowSlabs;
+  if (M.m >= kBigShort) {
+    const int one = M.odt == FSAGG_BF16;
+    if (work[one] >= kBigStages) return one ? kBigOne : kBig;
+  }
+  return kMid;
+}
+
+// The derived fields of an entry computed that way.
+void plan_mat(Mat &M, Way way) {
+  const int64_t total = int64_t(M.rows) * M.cols;
+  int64_t bytes;
+  M.slabs = M.each = 1;
+  int64_t nb = (total + 4 * kNormBlock - 1) / (4 * kNormBlock);
+  M.nb = int32_t(nb > kMaxNorm ? kMaxNorm : nb);
+  if (way == kWhole || way == kNarrowSlabs) {
+    M.mp = kNarrow;
+    M.np = int32_t(round_to(M.n, 64));
+    const int chunks = M.np / 64;
+    // a launch reads slabs x 16 KiB of Gram shares per workgroup, and works
+    // a chunk in about the time of 13 of those
+    if (way == kWhole) M.each = chunks;
+    else M.each = chunks <= NS_E1 ? 1 : chunks <= NS_E2 ? 2 : kMaxEach;
+    M.slabs = (chunks + M.each - 1) / M.each;
+    bytes = way == kWhole ? 0
+                          : 8 * kMaxNorm +
+                                4 * (int64_t(M.np) * kNarrow +
+                                     2 * int64_t(M.slabs) * kGramElems +
+                                     total);
+  } else {
+    const int side = way == kMid ? kMidSide : kBigSide;
+    M.mp = int32_t(round_to(M.m, side));
+    M.np = int32_t(round_to(M.n, side));
+    bytes = ws_bytes_of(M.mp, M.np);
+  }
+  M.wstride = round_to(bytes, 1024);
+}
+
+// Parts that the workgroups of one product may leave.
+int64_t partial_bytes(Way way) {
+  switch (way) {
+    case kBig:
+    case kBigOne:
+      return int64_t(2) * kBigWorkers * kBigSide * kBigSide * 4;
+    case kMid:
+      return int64_t(2) * kMidWorkers * kMidSide * kMidSide * 4;
+    default:
+      return 0;
+  }
+}
 
 // The largest |x|, |x|^2 and |q| that the iteration's limbs have to hold,
 // from the scalar iteration on a grid of the singular values in [0, 1]
@@ -524,65 +1141,187 @@ bool coefficients_fit(double a, double b, double c, int steps) {
   return true;
 }
 
-template <int MODE>
-void launch_gemm(Group &G, int src, float a, float b, float c,
-                 const MuonScalars &S, hipStream_t s) {
-  constexpr int B = 128, W = 64;
+struct Step {
+  float a, b, c;
+  double eps;
+  int steps;
+  MuonScalars S;
+  hipStream_t stream;
+};
+
+// One product of the whole group: one workgroup per tile, or the line of
+// stages shared by as many workgroups as the GPU holds, each with at least
+// kMinStages of them.  Sharing saves the stages that the last round of whole
+// tiles (or the longest tile, where there are fewer tiles than workgroups)
+// leaves idle, and costs a join: parts written and read again, about
+// kJoinStages stages' time with either tile.
+constexpr int kMinStages = 8, kJoinStages = 16;
+template <class T, int MODE>
+void launch_product(Group &G, int workers, float *partial, int src,
+                    const Step &st) {
+  int64_t tiles = 0, stages = 0;
+  for (int i = 0; i < G.nmat; ++i) {
+    const Mat &M = G.mat[i];
+    const int64_t t = int64_t(M.batch) * mode_tiles<MODE, T::kBM, T::kBN>(M);
+    tiles += t;
+    stages += t * mode_stages<MODE>(M);
+  }
+  int64_t w = stages / kMinStages;
+  if (w > workers) w = workers;
+  if (w < 1) w = 1;
+  const int64_t rounds = (tiles + workers - 1) / workers;
+  const bool share = rounds * (stages / tiles) - stages / w > kJoinStages;
+  Line L;
+  L.workers = int(w);
+  L.partial = partial;
+  L.total = int(stages);
   int total = 0;
   for (int i = 0; i < G.nmat; ++i) {
     const Mat &M = G.mat[i];
-    const int tm = M.mp / B;
     G.start[i] = total;
-    total += M.batch * (MODE == kGram || MODE == kSquare
-                            ? tm * (tm + 1) / 2
-                            : tm * (M.np / B));
+    total += M.batch * mode_tiles<MODE, T::kBM, T::kBN>(M) *
+             (share ? mode_stages<MODE>(M) : 1);
   }
   G.start[G.nmat] = total;
-  hipLaunchKernelGGL((ns_gemm_kernel<B, B, W, W, MODE>), dim3(total),
-                     dim3(256), 0, s, G, src, b, c, a, S);
+  if (!share) {
+    hipLaunchKernelGGL((ns_gemm_kernel<T, MODE>), dim3(total),
+                       dim3(T::kThreads), 0, st.stream, G, src, st.a, st.b,
+                       st.c, st.S);
+    return;
+  }
+  hipLaunchKernelGGL((ns_line_kernel<T, MODE>), dim3(L.workers),
+                     dim3(T::kThreads), 0, st.stream, G, L, src, st.a, st.b,
+                     st.c, st.S);
+  hipLaunchKernelGGL((ns_join_kernel<T, MODE>),
+                     dim3(L.workers - 1, T::MI * T::NJ), dim3(T::kThreads), 0,
+                     st.stream, G, L, src, st.a, st.b, st.c, st.S);
 }
 
-template <bool MUON>
-int run_group(Group &G, int steps, float a, float b, float c, double eps,
-              const MuonScalars &S, hipStream_t s, const char *what) {
+template <class T, bool MUON>
+void run_products(Group &G, int workers, float *partial, const Step &st) {
   int total = 0;
   for (int i = 0; i < G.nmat; ++i) {
     G.start[i] = total;
     total += G.mat[i].batch * G.mat[i].nb;
   }
   G.start[G.nmat] = total;
-  hipLaunchKernelGGL(ns_update_kernel<MUON>, dim3(total), dim3(kNormBlock), 0,
-                     s, G, S);
+  hipLaunchKernelGGL((ns_update_kernel<MUON, false>), dim3(total),
+                     dim3(kNormBlock), 0, st.stream, G, st.S);
   total = 0;
   for (int i = 0; i < G.nmat; ++i) {
     G.start[i] = total;
     total += G.mat[i].batch * (G.mat[i].mp / 64) * (G.mat[i].np / 64);
   }
   G.start[G.nmat] = total;
-  hipLaunchKernelGGL(ns_prepare_kernel, dim3(total), dim3(256), 0, s, G, eps);
+  hipLaunchKernelGGL(ns_prepare_kernel, dim3(total), dim3(256), 0, st.stream,
+                     G, st.eps);
   int src = 0;
-  for (int k = 0; k < steps; ++k) {
-    launch_gemm<kGram>(G, src, a, b, c, S, s);
-    launch_gemm<kSquare>(G, src, a, b, c, S, s);
-    if (k + 1 < steps) launch_gemm<kApply>(G, src, a, b, c, S, s);
-    else if (MUON) launch_gemm<kLastMuon>(G, src, a, b, c, S, s);
-    else launch_gemm<kLast>(G, src, a, b, c, S, s);
-    src ^= 1;
+  for (int k = 0; k < st.steps; ++k, src ^= 1) {
+    launch_product<T, kGram>(G, workers, partial, src, st);
+    launch_product<T, kSquare>(G, workers, partial, src, st);
+    if (k + 1 < st.steps)
+      launch_product<T, kApply>(G, workers, partial, src, st);
+    else
+      launch_product<T, MUON ? kLastMuon : kLast>(G, workers, partial, src,
+                                                  st);
   }
-  return check_launch(what);
 }
 
-// Workgroups of the widest launch: the prepare pass, 64 x 64 tiles.
-int64_t most_blocks(const Mat &M) {
-  return int64_t(M.batch) * (M.mp / 64) * (M.np / 64) +
-         int64_t(M.batch) * M.nb;
+template <bool MUON>
+void run_narrow(Group &G, const Step &st) {
+  int total = 0;
+  for (int i = 0; i < G.nmat; ++i) {
+    G.start[i] = total;
+    total += G.mat[i].batch * G.mat[i].nb;
+  }
+  G.start[G.nmat] = total;
+  hipLaunchKernelGGL((ns_update_kernel<MUON, true>), dim3(total),
+                     dim3(kNormBlock), 0, st.stream, G, st.S);
+  total = 0;
+  for (int i = 0; i < G.nmat; ++i) {
+    G.start[i] = total;
+    total += G.mat[i].batch * G.mat[i].slabs;
+  }
+  G.start[G.nmat] = total;
+  for (int k = 0; k <= st.steps; ++k)
+    hipLaunchKernelGGL((ns_narrow_kernel<MUON, false>), dim3(total),
+                       dim3(256), 0, st.stream, G, k, st.steps, st.a, st.b,
+                       st.c, st.eps, st.S);
 }
 
-// Entries in order, up to kMaxGroup per run.
+template <bool MUON>
+void run_whole(Group &G, const Step &st) {
+  int total = 0;
+  for (int i = 0; i < G.nmat; ++i) {
+    G.start[i] = total;
+    total += G.mat[i].batch;
+  }
+  G.start[G.nmat] = total;
+  hipLaunchKernelGGL((ns_narrow_kernel<MUON, true>), dim3(total), dim3(256),
+                     0, st.stream, G, 0, st.steps, st.a, st.b, st.c, st.eps,
+                     st.S);
+}
+
+template <bool MUON>
+void run_group(Group &G, Way way, float *partial, const Step &st) {
+  if (way == kWhole) run_whole<MUON>(G, st);
+  else if (way == kNarrowSlabs) run_narrow<MUON>(G, st);
+  else if (way == kMid)
+    run_products<MidTile, MUON>(G, kMidWorkers, partial, st);
+  else if (way == kBig)
+    run_products<BigTile, MUON>(G, kBigWorkers, partial, st);
+  else if constexpr (!MUON)  // (a parameter is fp32)
+    run_products<BigTile1, MUON>(G, kBigWorkers, partial, st);
+}
+
+// f(group, way, bytes of its entries) for every group of entries, in turn;
+// entries of one way go together.  `fill(i, M)` sets entry i's sizes, types
+// and pointers.
+template <typename Fill, typename F>
+int each_group(int nmat, Fill fill, Group &G, F f) {
+  int64_t work[2] = {0, 0};
+  for (int i = 0; i < nmat; ++i) {
+    Mat M;
+    const int rc = fill(i, M);
+    if (rc != FSAGG_OK) return rc;
+    if (!empty(M) && M.m >= kBigShort)
+      work[M.odt == FSAGG_BF16] += big_stages(M);
+  }
+  for (int way = 0; way < kWays; ++way) {
+    G.nmat = 0;
+    size_t bytes = 0;
+    for (int i = 0; i < nmat; ++i) {
+      Mat &M = G.mat[G.nmat];
+      fill(i, M);
+      if (empty(M) || way_of(M, work) != way) continue;
+      plan_mat(M, Way(way));
+      bytes += size_t(M.wstride) * M.batch;
+      if (++G.nmat == kMaxGroup) {
+        f(G, Way(way), bytes);
+        G.nmat = 0;
+        bytes = 0;
+      }
+    }
+    if (G.nmat) f(G, Way(way), bytes);
+  }
+  return FSAGG_OK;
+}
+
+// The groups run one after the other, so they share the workspace.
+template <typename Fill>
+int workspace_of(int nmat, Fill fill, size_t &need) {
+  Group G;
+  need = 0;
+  return each_group(nmat, fill, G, [&](Group &, Way way, size_t bytes) {
+    const size_t b = bytes + partial_bytes(way);
+    if (b > need) need = b;
+  });
+}
+
 template <bool MUON, typename Fill>
 int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
-            const MuonScalars &S, void *ws, size_t ws_bytes, hipStream_t s,
-            const char *what) {
+            const MuonScalars &S, void *ws, size_t ws_bytes,
+            hipStream_t stream, const char *what) {
   if (steps < 1 || steps > 99) {
     set_error("%s: steps must be in [1, 99], got %d", what, steps);
     return FSAGG_EINVAL;
@@ -598,21 +1337,9 @@ int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
   }
   // everything is checked before anything is launched
   size_t need = 0;
-  for (int i = 0; i < nmat; ++i) {
-    Mat M;
-    const int rc = fill(i, M);
-    if (rc != FSAGG_OK) return rc;
-    if (empty(M)) continue;
-    need += size_t(M.wstride) * M.batch;
-    // a launch counts its work items in 32 bits
-    if (most_blocks(M) > (int64_t(1) << 24) / kMaxGroup) {
-      set_error("%s: matrix %d: a batch of %d is too large for one call",
-                what, i, M.batch);
-      return FSAGG_EINVAL;
-    }
-  }
-  if (need == 0) return FSAGG_OK;
-  if (!ws || ws_bytes < need) {
+  int rc = workspace_of(nmat, fill, need);
+  if (rc != FSAGG_OK) return rc;
+  if (need > 0 && (!ws || ws_bytes < need)) {
     set_error("%s: workspace of %zu bytes, %zu needed", what,
               ws ? ws_bytes : size_t(0), need);
     return FSAGG_ESPACE;
@@ -621,29 +1348,67 @@ int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
     set_error("%s: workspace must be 16-byte aligned", what);
     return FSAGG_EINVAL;
   }
-  char *at = static_cast<char *>(ws);
+  const Step st = {float(coef[0]), float(coef[1]), float(coef[2]), eps,
+                   steps,          S,              stream};
   Group G;
-  G.nmat = 0;
-  for (int i = 0; i < nmat; ++i) {
-    Mat &M = G.mat[G.nmat];
-    fill(i, M);
-    if (empty(M)) continue;
-    M.ws = at;
-    at += size_t(M.wstride) * M.batch;
-    if (++G.nmat == kMaxGroup) {
-      const int rc = run_group<MUON>(G, steps, float(coef[0]), float(coef[1]),
-                                     float(coef[2]), eps, S, s, what);
-      if (rc != FSAGG_OK) return rc;
-      G.nmat = 0;
+  each_group(nmat, fill, G, [&](Group &g, Way way, size_t bytes) {
+    char *at = static_cast<char *>(ws);
+    for (int i = 0; i < g.nmat; ++i) {
+      g.mat[i].ws = at;
+      at += size_t(g.mat[i].wstride) * g.mat[i].batch;
     }
-  }
-  if (G.nmat == 0) return FSAGG_OK;
-  return run_group<MUON>(G, steps, float(coef[0]), float(coef[1]),
-                         float(coef[2]), eps, S, s, what);
+    run_group<MUON>(g, way,
+                    reinterpret_cast<float *>(static_cast<char *>(ws) + bytes),
+                    st);
+  });
+  return check_launch(what);
 }
 
 bool float_dtype(int dt) {
   return dt == FSAGG_F32 || dt == FSAGG_F16 || dt == FSAGG_BF16;
+}
+
+// Entry i of either table: sizes and types, and (for a run) its pointers.
+auto ns_fill(const fsagg_ns_mat *mats, bool pointers, const char *what) {
+  return [=](int i, Mat &M) {
+    const fsagg_ns_mat &d = mats[i];
+    const int rc = size_mat(M, d.rows, d.cols, d.batch, what);
+    if (rc != FSAGG_OK) return rc;
+    if (!float_dtype(d.dtype) || !float_dtype(d.out_dtype) ||
+        (pointers && !empty(M) && (!d.g || !d.out))) {
+      set_error("%s: matrix %d: null pointer or unknown dtype", what, i);
+      return int(FSAGG_EINVAL);
+    }
+    M.g = d.g;
+    M.out = d.out;
+    M.buf = nullptr;
+    M.ws = nullptr;
+    M.sz = d.batch_stride;
+    M.si = d.row_stride;
+    M.sj = d.col_stride;
+    M.dt = int16_t(d.dtype);
+    M.odt = int16_t(d.out_dtype);
+    return int(FSAGG_OK);
+  };
+}
+
+auto muon_fill(const fsagg_muon_mat *mats, bool pointers, const char *what) {
+  return [=](int i, Mat &M) {
+    const fsagg_muon_mat &d = mats[i];
+    const int rc = size_mat(M, d.rows, d.cols, 1, what);
+    if (rc != FSAGG_OK) return rc;
+    if (pointers && !empty(M) && (!d.param || !d.avg || !d.momentum)) {
+      set_error("%s: matrix %d: null pointer", what, i);
+      return int(FSAGG_EINVAL);
+    }
+    M.g = d.avg;
+    M.out = d.param;
+    M.buf = d.momentum;
+    M.ws = nullptr;
+    M.sz = M.si = M.sj = 0;
+    M.dt = M.odt = FSAGG_F32;
+    return int(FSAGG_OK);
+  };
 }
 
 }  // namespace
@@ -651,15 +1416,14 @@ bool float_dtype(int dt) {
 
 using namespace fsagg;
 
-extern "C" size_t fsagg_newton_schulz_workspace_bytes(int64_t rows,
-                                                      int64_t cols,
-                                                      int64_t batch) {
-  Mat M;
-  if (plan_mat(M, rows, cols, batch, "fsagg_newton_schulz_workspace_bytes") !=
-          FSAGG_OK ||
-      empty(M))
+extern "C" size_t fsagg_newton_schulz_workspace_bytes(
+    const fsagg_ns_mat *mats, int nmat) {
+  const char *what = "fsagg_newton_schulz_workspace_bytes";
+  size_t need = 0;
+  if (nmat <= 0 || !mats ||
+      workspace_of(nmat, ns_fill(mats, false, what), need) != FSAGG_OK)
     return 0;
-  return size_t(M.wstride) * M.batch;
+  return need;
 }
 
 extern "C" int fsagg_newton_schulz(const fsagg_ns_mat *mats, int nmat,
@@ -672,27 +1436,19 @@ extern "C" int fsagg_newton_schulz(const fsagg_ns_mat *mats, int nmat,
     set_error("%s: invalid argument", what);
     return FSAGG_EINVAL;
   }
-  auto fill = [&](int i, Mat &M) {
-    const fsagg_ns_mat &d = mats[i];
-    const int rc = plan_mat(M, d.rows, d.cols, d.batch, what);
-    if (rc != FSAGG_OK) return rc;
-    if (empty(M)) return int(FSAGG_OK);
-    if (!d.g || !d.out || !float_dtype(d.dtype) || !float_dtype(d.out_dtype)) {
-      set_error("%s: matrix %d: null pointer or unknown dtype", what, i);
-      return int(FSAGG_EINVAL);
-    }
-    M.g = d.g;
-    M.out = d.out;
-    M.buf = nullptr;
-    M.sz = d.batch_stride;
-    M.si = d.row_stride;
-    M.sj = d.col_stride;
-    M.dt = int16_t(d.dtype);
-    M.odt = int16_t(d.out_dtype);
-    return int(FSAGG_OK);
-  };
-  return run_all<false>(nmat, fill, steps, coefficients, eps, MuonScalars{},
-                        workspace, workspace_bytes, as_stream(stream), what);
+  return run_all<false>(nmat, ns_fill(mats, true, what), steps, coefficients,
+                        eps, MuonScalars{}, workspace, workspace_bytes,
+                        as_stream(stream), what);
+}
+
+extern "C" size_t fsagg_muon_workspace_bytes(const fsagg_muon_mat *mats,
+                                             int nmat) {
+  const char *what = "fsagg_muon_workspace_bytes";
+  size_t need = 0;
+  if (nmat <= 0 || !mats ||
+      workspace_of(nmat, muon_fill(mats, false, what), need) != FSAGG_OK)
+    return 0;
+  return need;
 }
 
 extern "C" int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
@@ -704,26 +1460,11 @@ extern "C" int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
     set_error("%s: invalid argument", what);
     return FSAGG_EINVAL;
   }
-  if (hp->adjust != FSAGG_MUON_ORIGINAL && hp->adjust != FSAGG_MUON_MATCH_RMS) {
+  if (hp->adjust != FSAGG_MUON_ORIGINAL &&
+      hp->adjust != FSAGG_MUON_MATCH_RMS) {
     set_error("%s: unknown learning-rate adjustment %d", what, hp->adjust);
     return FSAGG_EINVAL;
   }
-  auto fill = [&](int i, Mat &M) {
-    const fsagg_muon_mat &d = mats[i];
-    const int rc = plan_mat(M, d.rows, d.cols, 1, what);
-    if (rc != FSAGG_OK) return rc;
-    if (empty(M)) return int(FSAGG_OK);
-    if (!d.param || !d.avg || !d.momentum) {
-      set_error("%s: matrix %d: null pointer", what, i);
-      return int(FSAGG_EINVAL);
-    }
-    M.g = d.avg;
-    M.out = d.param;
-    M.buf = d.momentum;
-    M.sz = M.si = M.sj = 0;
-    M.dt = M.odt = FSAGG_F32;
-    return int(FSAGG_OK);
-  };
   MuonScalars S;
   S.keep = float(1.0 - hp->momentum);
   S.mu = float(hp->momentum);
@@ -733,6 +1474,7 @@ extern "C" int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
   S.maximize = hp->maximize;
   S.adjust = hp->adjust;
   const double coef[3] = {hp->a, hp->b, hp->c};
-  return run_all<true>(nmat, fill, hp->steps, coef, hp->eps, S, workspace,
-                       workspace_bytes, as_stream(stream), what);
+  return run_all<true>(nmat, muon_fill(mats, true, what), hp->steps, coef,
+                       hp->eps, S, workspace, workspace_bytes,
+                       as_stream(stream), what);
 }

@@ -1791,7 +1791,6 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7,
     dev = None
     lib = L.load()
     table = (L.NsMat * len(gs))()
-    need = 0
     for i, x in enumerate(gs):
         _check_float_cuda(x, 'matrix %d' % i, dev)
         dev = x.device
@@ -1814,12 +1813,12 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7,
         t.batch_stride = x.stride(0) if x.dim() == 3 else 0
         t.row_stride, t.col_stride = x.stride(-2), x.stride(-1)
         t.dtype, t.out_dtype = _FLOAT_CODE[x.dtype], _FLOAT_CODE[o.dtype]
-        need += lib.fsagg_newton_schulz_workspace_bytes(rows, cols, batch)
     if out is not None:
         for i, o in enumerate(outs):
             if any(_overlap(o, x) for x in gs) or \
                     any(_overlap(o, p) for p in outs[:i]):
                 raise ValueError('out %d overlaps another tensor' % i)
+    need = lib.fsagg_newton_schulz_workspace_bytes(table, len(gs))
     with _OnDevice(dev):
         ws = _scratch(dev, need)
         L.check(lib.fsagg_newton_schulz(
@@ -1857,7 +1856,6 @@ def muon_step(params, avgs, bufs, lr, momentum=0.95, nesterov=True,
     lib = L.load()
     dev = None
     table = (L.MuonMat * len(params))()
-    need = 0
     for i, (p, a, b) in enumerate(zip(params, avgs, bufs)):
         for t, what in ((p, 'param'), (a, 'average'), (b, 'momentum')):
             _check_f32_cuda(t, '%s %d' % (what, i), align=4)
@@ -1874,11 +1872,11 @@ def muon_step(params, avgs, bufs, lr, momentum=0.95, nesterov=True,
         m = table[i]
         m.param, m.avg, m.momentum = p.data_ptr(), a.data_ptr(), b.data_ptr()
         m.rows, m.cols = p.shape
-        need += lib.fsagg_newton_schulz_workspace_bytes(*p.shape, 1)
     _check_disjoint(list(params) + list(bufs), list(avgs))
     hp = L.MuonParams(float(lr), float(momentum), float(weight_decay), *coef,
                       float(eps), int(steps), int(bool(nesterov)),
                       int(bool(maximize)), _MUON_ADJUST[adjust_lr])
+    need = lib.fsagg_muon_workspace_bytes(table, len(params))
     with _OnDevice(dev):
         ws = _scratch(dev, need)
         L.check(lib.fsagg_muon_step_f32(table, len(params), ctypes.byref(hp),

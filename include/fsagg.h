@@ -250,9 +250,10 @@ int fsagg_server_opt_step_f64(double *param, const double *avg,
  *     or batch of 0 does nothing.
  *   coefficients (host): a, b, c; refused when they let the iterates grow
  *     past 15 (the usual 3.4445, -4.7750, 2.0315 stay below 1.3).
- *   Workspace: the sum over the entries of
- *     fsagg_newton_schulz_workspace_bytes(rows, cols, batch), 16-byte
- *     aligned; its contents need not be set and nothing is kept in it.
+ *   Workspace: fsagg_newton_schulz_workspace_bytes of the same entries
+ *     (pointers and strides do not matter to it; 0 also for sizes that the
+ *     call refuses), 16-byte aligned; its contents need not be set and
+ *     nothing is kept in it.
  */
 #define FSAGG_NS_MAX_SHORT 16384
 #define FSAGG_NS_MAX_LONG 1048576
@@ -264,8 +265,8 @@ typedef struct fsagg_ns_mat {
   int64_t batch_stride, row_stride, col_stride;
   int32_t dtype, out_dtype;
 } fsagg_ns_mat;
-size_t fsagg_newton_schulz_workspace_bytes(int64_t rows, int64_t cols,
-                                           int64_t batch);
+size_t fsagg_newton_schulz_workspace_bytes(const fsagg_ns_mat *mats,
+                                           int nmat);
 int fsagg_newton_schulz(const fsagg_ns_mat *mats, int nmat, int steps,
                         const double *coefficients, double eps,
                         void *workspace, size_t workspace_bytes,
@@ -281,8 +282,8 @@ int fsagg_newton_schulz(const fsagg_ns_mat *mats, int nmat, int steps,
  * with NS as fsagg_newton_schulz and lr' = lr sqrt(max(1, rows / cols))
  * (FSAGG_MUON_ORIGINAL) or 0.2 lr sqrt(max(rows, cols))
  * (FSAGG_MUON_MATCH_RMS).  mats (host): nmat contiguous fp32 matrices, no
- * two of which overlap; the momentum starts at zero.  Workspace as above
- * with batch 1.
+ * two of which overlap; the momentum starts at zero.  Workspace:
+ * fsagg_muon_workspace_bytes of the same entries, 16-byte aligned.
  */
 enum fsagg_muon_adjust { FSAGG_MUON_ORIGINAL = 0, FSAGG_MUON_MATCH_RMS = 1 };
 typedef struct fsagg_muon_mat {
@@ -295,6 +296,7 @@ typedef struct fsagg_muon_params {
   double lr, momentum, weight_decay, a, b, c, eps;
   int32_t steps, nesterov, maximize, adjust;
 } fsagg_muon_params;
+size_t fsagg_muon_workspace_bytes(const fsagg_muon_mat *mats, int nmat);
 int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
                         const fsagg_muon_params *hp, void *workspace,
                         size_t workspace_bytes, fsagg_stream_t stream);

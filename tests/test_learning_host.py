@@ -52,21 +52,27 @@ def test_newton_schulz_refuses_matrices(kw):
 
 def test_newton_schulz_workspace():
     lib = L.load()
-    need = lib.fsagg_newton_schulz_workspace_bytes(62, 2048, 3)
-    assert need > 0 and need % 16 == 0
     m = _mat(62, 2048, 3)
+
+    def bytes_of(*mats):
+        return lib.fsagg_newton_schulz_workspace_bytes(
+            (L.NsMat * len(mats))(*mats), len(mats))
+    need = bytes_of(m)
+    assert need > 0 and need % 16 == 0
     assert _ns([m]) == -3 and 'workspace' in _err()
     assert _ns([m], ws=4096, ws_bytes=need - 1) == -3
     assert _ns([m], ws=4104, ws_bytes=need + 64) == -1
     # nothing to do needs nothing
-    assert lib.fsagg_newton_schulz_workspace_bytes(0, 5, 1) == 0
+    assert bytes_of(_mat(0, 5), _mat(5, 0), _mat(batch=0)) == 0
     assert _ns([_mat(0, 5), _mat(5, 0), _mat(batch=0)]) == 0
     assert _ns([]) == 0
+    # refused sizes
+    assert bytes_of(m, _mat(rows=-1)) == 0
 
 
 def test_newton_schulz_accepts_tame_coefficients():
     """The bound is on the iterates, not on the coefficients themselves."""
-    m = _mat()
+    m = _mat(4, 600)
     for coef in (COEF, (2.0, -1.5, 0.5), (1.5, -0.5, 0.0), (15 / 8, -10 / 8,
                                                             3 / 8)):
         assert _ns([m], coef=coef) == -3      # only the workspace is missing
@@ -75,7 +81,9 @@ def test_newton_schulz_accepts_tame_coefficients():
 def test_muon_abi_refusals():
     lib = L.load()
     hp = L.MuonParams(0.1, 0.9, 0.1, *COEF, 1e-7, 5, 1, 0, 0)
-    t = (L.MuonMat * 1)(L.MuonMat(4096, 8192, 16384, 4, 6))
+    t = (L.MuonMat * 1)(L.MuonMat(4096, 8192, 16384, 4, 600))
+    assert lib.fsagg_muon_workspace_bytes(t, 1) > 0
+    assert lib.fsagg_muon_workspace_bytes(None, 1) == 0
     assert lib.fsagg_muon_step_f32(t, 1, None, None, 0, None) == -1
     assert lib.fsagg_muon_step_f32(None, 1, ctypes.byref(hp), None, 0,
                                    None) == -1
