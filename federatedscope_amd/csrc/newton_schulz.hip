@@ -413,6 +413,8 @@ struct Tile {
   static constexpr int kStage = (BM + BN) * LIMBS * kBK;  // halfs
   static constexpr int kLds = NBUF * kStage;
   static_assert(kPer * kWaves == kLoads, "loads divide over the waves");
+  static_assert(BM % (kPer * 16) == 0 && BN % (kPer * 16) == 0,
+                "a wave loads one plane's rows");
 
   f32x16 acc[MI][NJ];
   int lane, wave, wm, wn;
@@ -439,85 +441,109 @@ struct Tile {
                                            const _Float16 *rl, int ld, int i0,
                                            int j0, int k0, int k1) {
     // this wave's loads of a stage: LDS order is [P.h][P.l][R.h][R.l] rows
-    // of 64 bytes, 16 rows per instruction
-    const _Float16 *gsrc[kPer];
-    int ldst[kPer];
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-      const int row16 = (wave * kPer + q) * 16;
-      const bool right = row16 >= LIMBS * BM;
-      const int in = right ? row16 - LIMBS * BM : row16;
-      const int side = right ? BN : BM;
-      const _Float16 *base =
-          in < side ? (right ? rh : ph) : (right ? rl : pl);
-      const int g0 = (right ? j0 : i0) + (in < side ? in : in - side);
-      const int r = lane >> 2, slot = (lane & 3) ^ ((r >> 2) & 3);
-      gsrc[q] = base + int64_t(g0 + r) * ld + slot * 8;
-      ldst[q] = row16 * kBK;
-    }
+    // of 64 bytes, 16 rows per instruction, one plane per wave
+    const int row0 = wave * (kPer * 16);
+    const bool right = row0 >= LIMBS * BM;
+    const int in = right ? row0 - LIMBS * BM : row0;
+    const int side = right ? BN : BM;
+    const _Float16 *base = in < side ? (right ? rh : ph) : (right ? rl : pl);
+    const int g0 = (right ? j0 : i0) + (in < side ? in : in - side);
+    // (a buffer descriptor: one 32-bit offset per lane instead of a 64-bit
+    // address per load)
+    __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<_Float16 *>(base + int64_t(g0) * ld), short(0),
+        kPer * 16 * ld * 2, 0x00020000);
+    const int lr = lane >> 2;
+    const int goff = (lr * ld + (((lane & 3) ^ ((lr >> 2) & 3)) * 8)) * 2;
+    // (past the last stage: offsets outside the descriptor, which fetch
+    // nothing; so every stage has as many loads on their way, and the loop
+    // has no branch)
     auto issue = [&](int k) {
-      const int buf = k % NBUF;
+      _Float16 *st = lds + (k % NBUF) * kStage + row0 * kBK;
+      const int off = k < k1 ? goff : 0x7FFFFFF0;
+      const int at = k < k1 ? k * kBK * 2 : 0;
 #pragma unroll
       for (int q = 0; q < kPer; ++q)
-        __builtin_amdgcn_global_load_lds(
-            (__attribute__((address_space(1))) void *)(gsrc[q] + k * kBK),
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc,
             (__attribute__((address_space(3))) void *)(uintptr_t)(
-                lds + buf * kStage + ldst[q]),
-            16, 0, 0);
+                st + q * 16 * kBK),
+            16, off, q * 16 * ld * 2 + at, 0, 0);
     };
     const int fr = lane & 31, fk = lane >> 5;
+    struct Frags {
+      half8 a[LIMBS][MI], b[LIMBS][NJ];
+    };
+    auto read = [&](Frags &f, int k, int kk) {
+      const _Float16 *st = lds + (k % NBUF) * kStage;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int r = wm + i * 32 + fr;
+        const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
+#pragma unroll
+        for (int l = 0; l < LIMBS; ++l)
+          f.a[l][i] = *reinterpret_cast<const half8 *>(st + l * BM * kBK + o);
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int r = wn + j * 32 + fr;
+        const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
+#pragma unroll
+        for (int l = 0; l < LIMBS; ++l)
+          f.b[l][j] = *reinterpret_cast<const half8 *>(
+              st + (LIMBS * BM + l * BN) * kBK + o);
+      }
+    };
+    // l h, h l, h h (the small terms first)
+    auto mul = [&](const Frags &f) {
+#pragma unroll
+      for (int t = LIMBS == 2 ? 0 : 2; t < 3; ++t)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                f.a[t == 0 ? LIMBS - 1 : 0][i],
+                f.b[t == 1 ? LIMBS - 1 : 0][j], acc[i][j], 0, 0, 0);
+    };
     clear();
     // nothing of the previous tile is on its way, and every wave has read its
     // last stage
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int n = 0; n < NBUF - 1; ++n)
-      if (k0 + n < k1) issue(k0 + n);
-    for (int k = k0; k < k1; ++k) {
-      // this stage has landed for every wave (later ones may be on their
-      // way), and the one before it is read out
-      if (NBUF > 2 && k + NBUF - 1 <= k1)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
-                         (NBUF - 2) * kPer)
-                     : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" :::
-                         "memory");
-      if (k + NBUF - 1 < k1) issue(k + NBUF - 1);
-      const _Float16 *st = lds + (k % NBUF) * kStage;
-#pragma unroll
-      for (int kk = 0; kk < kBK / 16; ++kk) {
-        half8 fa[LIMBS][MI], fb[LIMBS][NJ];
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          const int r = wm + i * 32 + fr;
-          const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
-#pragma unroll
-          for (int l = 0; l < LIMBS; ++l)
-            fa[l][i] =
-                *reinterpret_cast<const half8 *>(st + l * BM * kBK + o);
-        }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int r = wn + j * 32 + fr;
-          const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
-#pragma unroll
-          for (int l = 0; l < LIMBS; ++l)
-            fb[l][j] = *reinterpret_cast<const half8 *>(
-                st + (LIMBS * BM + l * BN) * kBK + o);
-        }
-        // l h, h l, h h (the small terms first)
-#pragma unroll
-        for (int t = LIMBS == 2 ? 0 : 2; t < 3; ++t)
-#pragma unroll
-          for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                  fa[t == 0 ? LIMBS - 1 : 0][i],
-                  fb[t == 1 ? LIMBS - 1 : 0][j], acc[i][j], 0, 0, 0);
-      }
+    for (int n = 0; n < NBUF; ++n) issue(k0 + n);
+    // The fragments of the next half stage are read while the present one is
+    // multiplied.  In the middle of stage k every wave has read all of it:
+    // past that barrier its buffer takes stage k + NBUF.
+    Frags f0, f1;
+    wait_and_meet<(NBUF - 1) * kPer>();
+    read(f0, k0, 0);
+    for (int k = k0; k + 1 < k1; ++k) {
+      read(f1, k, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      mul(f0);
+      __builtin_amdgcn_sched_barrier(0);
+      wait_and_meet<(NBUF - 2) * kPer>();
+      issue(k + NBUF);
+      read(f0, k + 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      mul(f1);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    read(f1, k1 - 1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    mul(f0);
+    mul(f1);
+    // (nothing may be on its way to LDS when the workgroup ends)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+
+  // all but the last N of this wave's direct loads have landed, and every
+  // wave says so; LDS reads before it are done
+  template <int N>
+  static __device__ __forceinline__ void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N)
+                 : "memory");
   }
 
   // block (i, j) of the accumulators as it lies in the threads, 16 bytes at
@@ -1318,6 +1344,16 @@ int workspace_of(int nmat, Fill fill, size_t &need) {
   });
 }
 
+template <typename Fill>
+bool nothing(int nmat, Fill fill) {
+  for (int i = 0; i < nmat; ++i) {
+    Mat M;
+    fill(i, M);
+    if (!empty(M)) return false;
+  }
+  return true;
+}
+
 template <bool MUON, typename Fill>
 int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
             const MuonScalars &S, void *ws, size_t ws_bytes,
@@ -1348,6 +1384,7 @@ int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
     set_error("%s: workspace must be 16-byte aligned", what);
     return FSAGG_EINVAL;
   }
+  if (need == 0 && nothing(nmat, fill)) return FSAGG_OK;
   const Step st = {float(coef[0]), float(coef[1]), float(coef[2]), eps,
                    steps,          S,              stream};
   Group G;
