@@ -520,14 +520,14 @@ struct Tile {
     read(f0, k0, 0);
     for (int k = k0; k + 1 < k1; ++k) {
       read(f1, k, 1);
-      __builtin_amdgcn_sched_barrier(0);
       mul(f0);
+      spread<0>();
       __builtin_amdgcn_sched_barrier(0);
       wait_and_meet<(NBUF - 2) * kPer>();
-      issue(k + NBUF);
       read(f0, k + 1, 0);
-      __builtin_amdgcn_sched_barrier(0);
+      issue(k + NBUF);
       mul(f1);
+      spread<kPer>();
       __builtin_amdgcn_sched_barrier(0);
     }
     read(f1, k1 - 1, 1);
@@ -536,6 +536,28 @@ struct Tile {
     mul(f1);
     // (nothing may be on its way to LDS when the workgroup ends)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+
+  // Order of a half stage: the fragment reads, then LOADS direct loads, one
+  // at a time between the matrix instructions, so that the waves do not queue
+  // for the LDS and the memory pipe while the matrix cores wait.
+  template <int LOADS>
+  static __device__ __forceinline__ void spread() {
+    constexpr int kMfma = MI * NJ * (LIMBS == 2 ? 3 : 1);
+    constexpr int kReads = LIMBS * (MI + NJ);
+    constexpr int kEach = kMfma > kReads + LOADS ? kMfma / (kReads + LOADS)
+                                                 : 1;
+#pragma unroll
+    for (int n = 0; n < kReads; ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kMfma, 0);
   }
 
   // all but the last N of this wave's direct loads have landed, and every
