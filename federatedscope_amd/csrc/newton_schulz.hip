@@ -608,48 +608,62 @@ struct Tile {
         finish_block<MODE>(acc[i][j], M, P, z, ti, tj, i, j, src, a, b, c, S);
   }
 
-  // what the product is for, for one 32 x 32 block: a lane holds column gj
-  // and rows gi .. gi + 3 of each quad
+  // what the product is for, for one 32 x 32 block.  The matrix cores leave
+  // a lane column gj and four runs of 4 rows; lanes l and l + 32 exchange two
+  // of them, so that a lane has two runs of 8 rows (gi .. gi + 7, + 16) and
+  // the transposed planes move 16 bytes a lane.
   template <int MODE>
   __device__ __forceinline__ void finish_block(
-      const f32x16 &x, const Mat &M, const Planes &P, int z, int ti, int tj,
-      int i, int j, int src, float a, float b, float c,
+      const f32x16 &acc16, const Mat &M, const Planes &P, int z, int ti,
+      int tj, int i, int j, int src, float a, float b, float c,
       const MuonScalars &S) const {
     const int fr = lane & 31, fk = lane >> 5;
-    const int gi0 = ti * BM + wm + i * 32 + 4 * fk;
+    const int gi0 = ti * BM + wm + i * 32 + 8 * fk;
     const int gj = tj * BN + wn + j * 32 + fr;
-    half4 oh[4], ol[4];
+    half8 oh[2], ol[2];
     if constexpr (MODE != kGram) {
       // A is symmetric: its column gj is row gj; X's column is T's row
       const _Float16 *bh = MODE == kSquare ? P.ah : P.th(src);
       const _Float16 *bl = MODE == kSquare ? P.al : P.tl(src);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t o = int64_t(gj) * M.mp + gi0 + 8 * q;
-        oh[q] = *reinterpret_cast<const half4 *>(bh + o);
-        ol[q] = *reinterpret_cast<const half4 *>(bl + o);
+      for (int p = 0; p < 2; ++p) {
+        const int64_t o = int64_t(gj) * M.mp + gi0 + 16 * p;
+        oh[p] = *reinterpret_cast<const half8 *>(bh + o);
+        ol[p] = *reinterpret_cast<const half8 *>(bl + o);
       }
     }
+    f32x16 x = acc16;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int gi = gi0 + 8 * q;
-      float v[4];
+    for (int p = 0; p < 2; ++p)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] = x[4 * q + e] * kInvS;
+        const auto s = __builtin_amdgcn_permlane32_swap(
+            __float_as_uint(x[8 * p + e]), __float_as_uint(x[8 * p + 4 + e]),
+            false, false);
+        x[8 * p + e] = __uint_as_float(s[0]);
+        x[8 * p + 4 + e] = __uint_as_float(s[1]);
+      }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int gi = gi0 + 16 * p;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = x[8 * p + e] * kInvS;
         if constexpr (MODE == kSquare)
-          v[e] = b * (float(oh[q][e]) + float(ol[q][e])) + c * v[e];
+          v[e] = b * (float(oh[p][e]) + float(ol[p][e])) + c * v[e];
         else if constexpr (MODE != kGram)
-          v[e] = a * (float(oh[q][e]) + float(ol[q][e])) + v[e];
+          v[e] = a * (float(oh[p][e]) + float(ol[p][e])) + v[e];
       }
       if constexpr (MODE == kLast || MODE == kLastMuon) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= kInvS;
+        for (int e = 0; e < 8; ++e) v[e] *= kInvS;
         store_result<MODE == kLastMuon>(M, S, z, gi, gj, v);
+        store_result<MODE == kLastMuon>(M, S, z, gi + 4, gj, v + 4);
       } else {
-        half4 h, l;
+        half8 h, l;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
           _Float16 u, w;
           split(v[e], u, w);
           h[e] = u;
@@ -671,18 +685,19 @@ struct Tile {
           dh = ch;
           dl = cl;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t o = int64_t(gi + e) * ldc + gj;
-          ch[o] = h[e];
-          if (LIMBS == 2 || MODE == kGram) cl[o] = l[e];
-        }
+        // a tile on the diagonal is its own transpose
         if (MODE == kApply || ti != tj) {
-          const int64_t o = int64_t(gj) * ldd + gi;
-          *reinterpret_cast<half4 *>(dh + o) = h;
-          if (LIMBS == 2 || MODE != kSquare)
-            *reinterpret_cast<half4 *>(dl + o) = l;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int64_t o = int64_t(gi + e) * ldc + gj;
+            ch[o] = h[e];
+            if (LIMBS == 2 || MODE == kGram) cl[o] = l[e];
+          }
         }
+        const int64_t o = int64_t(gj) * ldd + gi;
+        *reinterpret_cast<half8 *>(dh + o) = h;
+        if (LIMBS == 2 || MODE != kSquare)
+          *reinterpret_cast<half8 *>(dl + o) = l;
       }
     }
   }
