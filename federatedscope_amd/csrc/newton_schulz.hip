@@ -34,7 +34,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMaxGroup = 24;     // matrices per launch (kernel arguments)
 constexpr int kNormBlock = 256;
-constexpr int kMaxNorm = 256;     // norm workgroups per matrix
+constexpr int kMaxNorm = 1024;    // norm workgroups per matrix
 constexpr int kBK = 32;           // k per LDS stage
 constexpr float kS = 4096.0f;     // limb scale
 constexpr float kInvS = 1.0f / 4096.0f;
@@ -51,6 +51,7 @@ struct Mat {
   int32_t m, n, mp, np;  // short and long side, and padded
   int32_t nb;            // norm workgroups per matrix
   int32_t slabs, each;   // narrow matrices: slabs, and 64-column chunks of one
+  int32_t vec;           // 8 results side by side may be stored at once
   int16_t dt, odt;
 };
 
@@ -98,11 +99,7 @@ __device__ __forceinline__ Planes planes_of(const Mat &M, int z) {
 // the next.
 constexpr int kNarrow = 64;
 constexpr int kNarrowLong = 16384;
-constexpr int kMaxEach = 4;
-#ifndef NS_E1
-#define NS_E1 32
-#define NS_E2 64
-#endif
+constexpr int kMaxEach = 4, kMaxWhole = 4;
 constexpr int kGramElems = kNarrow * kNarrow;
 struct Narrow {
   double *norm;
@@ -160,30 +157,86 @@ __device__ __forceinline__ uint16_t to_bf16(float v) {
   return uint16_t((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
 }
 
-__device__ __forceinline__ void store_from_f32(void *p, int64_t i, int dt,
-                                               float v) {
-  if (dt == FSAGG_F32) static_cast<float *>(p)[i] = v;
-  else if (dt == FSAGG_F16) static_cast<_Float16 *>(p)[i] = _Float16(v);
-  else static_cast<uint16_t *>(p)[i] = to_bf16(v);
+template <int DT>
+__device__ __forceinline__ void store_from_f32(void *p, int64_t i, float v) {
+  if constexpr (DT == FSAGG_F32) static_cast<float *>(p)[i] = v;
+  else if constexpr (DT == FSAGG_F16)
+    static_cast<_Float16 *>(p)[i] = _Float16(v);
+  else
+    static_cast<uint16_t *>(p)[i] = to_bf16(v);
 }
 
-// Results y of rows i .. i + 3, column j of matrix z (m x n orientation).
-template <bool MUON>
+// Results y of rows i .. i + N - 1 (N = 4 or 8, i a multiple of N), column j
+// of matrix z (m x n orientation), as type DT.  A tall matrix has them side
+// by side.
+template <bool MUON, int DT, int N>
 __device__ __forceinline__ void store_result(const Mat &M,
                                              const MuonScalars &S, int z,
                                              int i, int j, const float *y) {
-  if (j >= M.n) return;
+  if (j >= M.n || i >= M.m) return;
   const bool tall = M.rows > M.cols;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (i + e >= M.m) continue;
-    const int64_t o = tall ? int64_t(j) * M.cols + i + e
-                           : int64_t(i + e) * M.cols + j;
+  const int64_t zo = MUON ? 0 : int64_t(z) * M.rows * M.cols;
+  if (tall && M.vec) {
+    const int64_t o = zo + int64_t(j) * M.cols + i;
     if constexpr (MUON) {
-      float *p = static_cast<float *>(M.out) + o;
-      *p = __builtin_fmaf(-muon_lr(M, S), y[e], __fmul_rn(*p, S.decay));
+      f32x4 *p = reinterpret_cast<f32x4 *>(static_cast<float *>(M.out) + o);
+      const float lr = muon_lr(M, S);
+      f32x4 v[N / 4];
+#pragma unroll
+      for (int q = 0; q < N / 4; ++q) v[q] = p[q];
+#pragma unroll
+      for (int q = 0; q < N / 4; ++q) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[q][e] = __builtin_fmaf(-lr, y[4 * q + e],
+                                   __fmul_rn(v[q][e], S.decay));
+        p[q] = v[q];
+      }
+    } else if constexpr (DT == FSAGG_F32) {
+      f32x4 *p = reinterpret_cast<f32x4 *>(static_cast<float *>(M.out) + o);
+#pragma unroll
+      for (int q = 0; q < N / 4; ++q)
+        p[q] = f32x4{y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]};
     } else {
-      store_from_f32(M.out, int64_t(z) * M.rows * M.cols + o, M.odt, y[e]);
+      typedef uint32_t un __attribute__((ext_vector_type(N / 2)));
+      un v;
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        uint32_t h[2];
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+          h[d] = DT == FSAGG_F16
+                     ? __builtin_bit_cast(uint16_t, _Float16(y[e + d]))
+                     : to_bf16(y[e + d]);
+        v[e / 2] = h[0] | (h[1] << 16);
+      }
+      *reinterpret_cast<un *>(static_cast<uint16_t *>(M.out) + o) = v;
+    }
+    return;
+  }
+  if constexpr (MUON) {
+    float *const out = static_cast<float *>(M.out);
+    const float lr = muon_lr(M, S);
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int64_t o = tall ? int64_t(j) * M.cols + i + e
+                             : int64_t(i + e) * M.cols + j;
+      v[e] = i + e < M.m ? out[o] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int64_t o = tall ? int64_t(j) * M.cols + i + e
+                             : int64_t(i + e) * M.cols + j;
+      if (i + e < M.m)
+        out[o] = __builtin_fmaf(-lr, y[e], __fmul_rn(v[e], S.decay));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int64_t o = tall ? int64_t(j) * M.cols + i + e
+                             : int64_t(i + e) * M.cols + j;
+      if (i + e < M.m) store_from_f32<DT>(M.out, zo + o, y[e]);
     }
   }
 }
@@ -227,6 +280,14 @@ __device__ __forceinline__ double block_sum(double v, double *part) {
   return part[0];
 }
 
+// The sum of the norm workgroups' shares.
+__device__ __forceinline__ double norm_sum(const double *norm, int nb,
+                                           double *part) {
+  double v = 0.0;
+  for (int i = threadIdx.x; i < nb; i += 256) v += norm[i];
+  return block_sum<256>(v, part);
+}
+
 // kS / max(norm, eps); NaN for a NaN norm, as dividing by it would give
 __device__ __forceinline__ double limb_scale(double sq, double eps) {
   const double norm = sqrt(sq);
@@ -255,7 +316,7 @@ __global__ __launch_bounds__(kNormBlock) void ns_update_kernel(
   const uint32_t total = uint32_t(M.rows) * uint32_t(M.cols);
   const uint32_t step = uint32_t(M.nb) * kNormBlock;
   double sq = 0.0;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 8;
   for (uint32_t e0 = uint32_t(b) * kNormBlock + threadIdx.x; e0 < total;
        e0 += kAhead * step) {
     float v[kAhead];
@@ -293,10 +354,7 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
   const float *u = reinterpret_cast<const float *>(P.th(1));
   __shared__ double part[256];
   __shared__ float tile[64][65];
-  const double scale = limb_scale(
-      block_sum<256>(int(threadIdx.x) < M.nb ? P.norm[threadIdx.x] : 0.0,
-                     part),
-      eps);
+  const double scale = limb_scale(norm_sum(P.norm, M.nb, part), eps);
   const int i0 = (t / tn) * 64, j0 = (t % tn) * 64;
   const bool tall = M.rows > M.cols;
   // u's own rows r and columns c of this tile
@@ -596,23 +654,36 @@ struct Tile {
     for (int r = 0; r < 16; ++r) x[r] = __fadd_rn(x[r], v[r / 4][r % 4]);
   }
 
+  template <int MODE, int DT>
+  __device__ __forceinline__ void finish_as(const Mat &M, const Planes &P,
+                                            int z, int ti, int tj, int src,
+                                            float a, float b, float c,
+                                            const MuonScalars &S) const {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        finish_block<MODE, DT>(acc[i][j], M, P, z, ti, tj, i, j, src, a, b, c,
+                               S);
+  }
   template <int MODE>
   __device__ __forceinline__ void finish(const Mat &M, const Planes &P, int z,
                                          int ti, int tj, int src, float a,
                                          float b, float c,
                                          const MuonScalars &S) const {
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        finish_block<MODE>(acc[i][j], M, P, z, ti, tj, i, j, src, a, b, c, S);
+    if (MODE == kLast && M.odt == FSAGG_BF16)
+      finish_as<MODE, FSAGG_BF16>(M, P, z, ti, tj, src, a, b, c, S);
+    else if (MODE == kLast && M.odt == FSAGG_F16)
+      finish_as<MODE, FSAGG_F16>(M, P, z, ti, tj, src, a, b, c, S);
+    else
+      finish_as<MODE, FSAGG_F32>(M, P, z, ti, tj, src, a, b, c, S);
   }
 
   // what the product is for, for one 32 x 32 block.  The matrix cores leave
   // a lane column gj and four runs of 4 rows; lanes l and l + 32 exchange two
   // of them, so that a lane has two runs of 8 rows (gi .. gi + 7, + 16) and
-  // the transposed planes move 16 bytes a lane.
-  template <int MODE>
+  // the transposed planes move 16 bytes a lane.  DT: the result's type.
+  template <int MODE, int DT>
   __device__ __forceinline__ void finish_block(
       const f32x16 &acc16, const Mat &M, const Planes &P, int z, int ti,
       int tj, int i, int j, int src, float a, float b, float c,
@@ -658,8 +729,7 @@ struct Tile {
       if constexpr (MODE == kLast || MODE == kLastMuon) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= kInvS;
-        store_result<MODE == kLastMuon>(M, S, z, gi, gj, v);
-        store_result<MODE == kLastMuon>(M, S, z, gi + 4, gj, v + 4);
+        store_result<MODE == kLastMuon, DT, 8>(M, S, z, gi, gj, v);
       } else {
         half8 h, l;
 #pragma unroll
@@ -803,21 +873,31 @@ __global__ __launch_bounds__(T::kThreads) void ns_join_kernel(
   const int z = t / tiles;
   int ti, tj;
   tile_of<MODE, T::kBM, T::kBN>(M, t % tiles, ti, tj);
-  T tile;
-  tile.template finish_block<MODE>(x, M, planes_of(M, z), z, ti, tj,
-                                   block / T::NJ, block % T::NJ, src, a, b, c,
-                                   S);
+  const T tile;
+  const Planes P = planes_of(M, z);
+  const int i = block / T::NJ, j = block % T::NJ;
+  if (MODE == kLast && M.odt == FSAGG_BF16)
+    tile.template finish_block<MODE, FSAGG_BF16>(x, M, P, z, ti, tj, i, j, src,
+                                                 a, b, c, S);
+  else if (MODE == kLast && M.odt == FSAGG_F16)
+    tile.template finish_block<MODE, FSAGG_F16>(x, M, P, z, ti, tj, i, j, src,
+                                                a, b, c, S);
+  else
+    tile.template finish_block<MODE, FSAGG_F32>(x, M, P, z, ti, tj, i, j, src,
+                                                a, b, c, S);
 }
 
 // -- narrow matrices ---------------------------------------------------------
-// m <= 64: A and Q are one 64 x 64 tile, and what a step costs is reading the
-// columns and handing the Gram matrix over.  A workgroup of 4 waves owns a
-// slab of up to kMaxEach chunks of 64 columns, a wave one 32 x 32 block of
-// every product; the slab's columns stay in its registers for the step.  A
-// launch sums the slabs' Gram shares of the step before (every workgroup the
-// same, in order), forms Q, applies it and leaves its share of the next one:
-// one launch per step, where the tiled products take three.  A matrix of one
-// slab needs no exchange: all its steps are one launch.
+// m <= 64: A and Q are one 64 x 64 tile, and what a step costs is latency:
+// reading the columns, three small products one after the other, and handing
+// the Gram matrix over.  A group of 4 waves owns up to kMaxEach chunks of 64
+// columns, a wave one 32 x 32 block of every product; the columns stay in
+// its registers for the step.  Up to kMaxWhole chunks are the groups of one
+// workgroup, which takes all steps in one launch (the Gram shares meet in
+// LDS).  Beyond that a workgroup is one group: a launch sums the slabs' Gram
+// shares of the step before (every workgroup the same, in order), forms Q,
+// applies it and leaves its share of the next one, so a step is one launch
+// where the tiled products take three.
 __device__ __forceinline__ int swz(int r, int chunk) {
   return r * 64 + ((chunk ^ ((r >> 1) & 7)) * 8);
 }
@@ -830,7 +910,7 @@ struct Slab {
     fk = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
     bi = (wave & 1) * 32;
-    bj = (wave >> 1) * 32;
+    bj = (wave & 2) * 16;
   }
   // rows of quad q of this lane, and its column
   __device__ __forceinline__ int row(int q) const {
@@ -838,10 +918,15 @@ struct Slab {
   }
   __device__ __forceinline__ int col() const { return bj + fr; }
 
-  // x += P R^T over 64 of k; planes [64][64], limbs l at + 4096
+  // x += P R^T over 64 of k; planes [64][64], limbs l at + 4096.  The three
+  // limb products go to accumulators of their own (a chain of dependent
+  // matrix instructions is what a product this small waits for).
   __device__ __forceinline__ void multiply(const _Float16 *p,
                                            const _Float16 *r,
                                            f32x16 &x) const {
+    f32x16 s, t;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = t[e] = 0.0f;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       const int op = swz(bi + fr, kk * 2 + fk), oq = swz(bj + fr, kk * 2 + fk);
@@ -849,10 +934,13 @@ struct Slab {
       const half8 pl = *reinterpret_cast<const half8 *>(p + 4096 + op);
       const half8 rh = *reinterpret_cast<const half8 *>(r + oq);
       const half8 rl = *reinterpret_cast<const half8 *>(r + 4096 + oq);
-      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, rh, x, 0, 0, 0);
-      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rl, x, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, rh, s, 0, 0, 0);
+      t = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rl, t, 0, 0, 0);
       x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rh, x, 0, 0, 0);
     }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      x[e] = __fadd_rn(x[e], __fadd_rn(s[e], t[e]));
   }
   // limbs of the block's values (times kS), transposed: row col(), the rows
   // of a quad side by side
@@ -889,68 +977,178 @@ struct Slab {
   }
 };
 
-// Launch k of a narrow matrix: 0 scales the update; k = 1 .. steps is step
-// k, the last of which stores the result.  WHOLE: everything in one launch.
+// The scaled update of chunk `ch` (kS times), zero in the padding whatever
+// the scale; raw: the update itself.
 template <bool MUON, bool WHOLE>
+__device__ __forceinline__ void load_update(const Mat &M, const Narrow &N,
+                                            const Slab &W,
+                                            const MuonScalars &S, int z,
+                                            int ch, f32x16 &x) {
+  const bool tall = M.rows > M.cols;
+  const int j = ch * 64 + W.col();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int i = W.row(r / 4) + r % 4;
+    float v = 0.0f;
+    if (i < M.m && j < M.n) {
+      const int a = tall ? j : i, b = tall ? i : j;
+      const int64_t o = int64_t(a) * M.cols + b;
+      v = WHOLE ? update_at<MUON>(M, S, z, o, a, b) : N.u[o];
+    }
+    x[r] = v;
+  }
+}
+__device__ __forceinline__ void scale_update(const Mat &M, const Slab &W,
+                                             int ch, double scale,
+                                             f32x16 &x) {
+  const int j = ch * 64 + W.col();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int i = W.row(r / 4) + r % 4;
+    x[r] = i < M.m && j < M.n ? float(double(x[r]) * scale) : 0.0f;
+  }
+}
+template <bool MUON, int DT>
+__device__ __forceinline__ void store_chunk_as(const Mat &M, const Slab &W,
+                                               const MuonScalars &S, int z,
+                                               int ch, const f32x16 &x) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = x[4 * q + e] * kInvS;
+    store_result<MUON, DT, 4>(M, S, z, W.row(q), ch * 64 + W.col(), y);
+  }
+}
+template <bool MUON>
+__device__ __forceinline__ void store_chunk(const Mat &M, const Slab &W,
+                                            const MuonScalars &S, int z,
+                                            int ch, const f32x16 &x) {
+  if (!MUON && M.odt == FSAGG_BF16)
+    store_chunk_as<MUON, FSAGG_BF16>(M, W, S, z, ch, x);
+  else if (!MUON && M.odt == FSAGG_F16)
+    store_chunk_as<MUON, FSAGG_F16>(M, W, S, z, ch, x);
+  else
+    store_chunk_as<MUON, FSAGG_F32>(M, W, S, z, ch, x);
+}
+__device__ __forceinline__ void clear16(f32x16 &v) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) v[r] = 0.0f;
+}
+// kS Q = b kS A + c kS A^2 from kS^2 A; `la` takes A's limbs
+__device__ __forceinline__ f32x16 square(const Slab &W, f32x16 gram,
+                                         _Float16 *la, float b, float c) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
+  W.put_columns(la, gram);
+  __syncthreads();
+  f32x16 t;
+  clear16(t);
+  W.multiply(la, la, t);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
+  return t;
+}
+
+// A whole matrix of up to kMaxWhole chunks, group g the chunk g.
+template <bool MUON>
+__global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
+    Group G, int steps, float a, float b, float c, double eps,
+    MuonScalars S) {
+  // Q, and per group the columns' limbs by columns and by rows
+  __shared__ __attribute__((aligned(1024)))
+  _Float16 lds[8192 * (1 + 2 * kMaxWhole)];
+  __shared__ double part[256 * kMaxWhole];
+  int z;
+  const Mat &M = G.mat[find_mat(G, blockIdx.x, z)];
+  const Narrow N = {};
+  const Slab W;
+  const int g = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 8);
+  const int t256 = threadIdx.x & 255;
+  const int chunks = M.np / 64;
+  _Float16 *const lq = lds, *const lt = lds + 8192 * (1 + 2 * g);
+  _Float16 *const lx = lt + 8192;
+  f32x16 x, gram, t;
+  double sq = 0.0;
+  load_update<MUON, true>(M, N, W, S, z, g, x);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) sq += double(x[r]) * double(x[r]);
+  scale_update(M, W, g,
+               limb_scale(block_sum<256 * kMaxWhole>(sq, part), eps), x);
+  for (int step = 1; step <= steps; ++step) {
+    clear16(gram);
+    if (g < chunks) W.put_rows(lx, x);
+    __syncthreads();
+    if (g < chunks) W.multiply(lx, lx, gram);
+    __syncthreads();
+    // the groups' shares, in order
+    if (chunks > 1) {
+      f32x4 *mine = reinterpret_cast<f32x4 *>(lx);
+      if (g < chunks) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          mine[q * 256 + t256] = f32x4{gram[4 * q], gram[4 * q + 1],
+                                       gram[4 * q + 2], gram[4 * q + 3]};
+      }
+      __syncthreads();
+      clear16(gram);
+      for (int k = 0; k < chunks; ++k) {
+        const f32x4 *other = reinterpret_cast<const f32x4 *>(
+            lds + 8192 * (2 + 2 * k));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 v = other[q * 256 + t256];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            gram[4 * q + e] = __fadd_rn(gram[4 * q + e], v[e]);
+        }
+      }
+    }
+    t = square(W, gram, lt, b, c);
+    if (g == 0) W.put_columns(lq, t);
+    __syncthreads();
+    if (g < chunks) W.put_columns(lt, x);
+    __syncthreads();
+    if (g < chunks) {
+      clear16(t);
+      W.multiply(lq, lt, t);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = a * x[r] + t[r] * kInvS;
+    }
+  }
+  if (g < chunks) store_chunk<MUON>(M, W, S, z, g, x);
+}
+
+// Launch k of a narrow matrix in slabs: 0 scales the update; k = 1 .. steps
+// is step k, the last of which stores the result.
+template <bool MUON>
 __global__ __launch_bounds__(256) void ns_narrow_kernel(
     Group G, int k, int steps, float a, float b, float c, double eps,
     MuonScalars S) {
-  __shared__ __attribute__((aligned(1024))) _Float16 lds[3 * 2 * 4096];
+  __shared__ __attribute__((aligned(1024))) _Float16 lds[3 * 8192];
   __shared__ double part[256];
   _Float16 *const lq = lds, *const lt = lds + 8192, *const lx = lds + 16384;
   int rel;
   const Mat &M = G.mat[find_mat(G, blockIdx.x, rel)];
-  const int slabs = WHOLE ? 1 : M.slabs;
+  const int slabs = M.slabs;
   const int z = rel / slabs, slab = rel % slabs;
   const int chunk0 = slab * M.each, chunks = M.np / 64;
   const int have = chunks - chunk0 < M.each ? chunks - chunk0 : M.each;
   const Narrow N = narrow_of(M, z);
   const Slab W;
-  const bool tall = M.rows > M.cols;
   f32x16 x[kMaxEach];  // kS times the columns
-
-  f32x16 gram;
-  auto clear = [](f32x16 &v) {
+  f32x16 gram, t;
+  clear16(gram);
+  if (k == 0) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) v[r] = 0.0f;
-  };
-  clear(gram);
-  if (WHOLE || k == 0) {
-    // the update, scaled
-    double sq = 0.0;
+    for (int ch = 0; ch < kMaxEach; ++ch)
+      if (ch < have)
+        load_update<MUON, false>(M, N, W, S, z, chunk0 + ch, x[ch]);
+    const double scale = limb_scale(norm_sum(N.norm, M.nb, part), eps);
 #pragma unroll
     for (int ch = 0; ch < kMaxEach; ++ch) {
       if (ch >= have) break;
-      const int j = (chunk0 + ch) * 64 + W.col();
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = W.row(q) + e;
-          float v = 0.0f;
-          if (i < M.m && j < M.n) {
-            const int r = tall ? j : i, cc = tall ? i : j;
-            const int64_t o = int64_t(r) * M.cols + cc;
-            v = WHOLE ? update_at<MUON>(M, S, z, o, r, cc) : N.u[o];
-          }
-          x[ch][4 * q + e] = v;
-          if (WHOLE) sq += double(v) * double(v);
-        }
-    }
-    if (!WHOLE)
-      sq = int(threadIdx.x) < M.nb ? N.norm[threadIdx.x] : 0.0;
-    const double scale = limb_scale(block_sum<256>(sq, part), eps);
-#pragma unroll
-    for (int ch = 0; ch < kMaxEach; ++ch) {
-      if (ch >= have) break;
-      // (padding stays zero whatever the scale)
-      const int j = (chunk0 + ch) * 64 + W.col();
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = W.row(r / 4) + r % 4;
-        x[ch][r] = i < M.m && j < M.n ? float(double(x[ch][r]) * scale)
-                                      : 0.0f;
-      }
+      scale_update(M, W, chunk0 + ch, scale, x[ch]);
       W.put_rows(lx, x[ch]);
       __syncthreads();
       W.multiply(lx, lx, gram);
@@ -971,7 +1169,7 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
     // every slab's share of the Gram matrix, in order
     const f32x4 *g = reinterpret_cast<const f32x4 *>(
         N.gram + int64_t((k - 1) & 1) * slabs * kGramElems);
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     for (int s0 = 0; s0 < slabs; s0 += kAhead) {
       f32x4 v[kAhead][4];
 #pragma unroll
@@ -988,81 +1186,50 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
             gram[r] = __fadd_rn(gram[r], v[u][r / 4][r % 4]);
         }
     }
-  }
-
-  for (int step = WHOLE ? 1 : k;; ++step) {
-    if (step > 0) {
-      // Q = bA + cA^2 from the Gram sum (kS^2 A)
-      f32x16 t;
-      clear(t);
+    t = square(W, gram, lt, b, c);
+    W.put_columns(lq, t);
+    clear16(gram);
+    __syncthreads();
 #pragma unroll
-      for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
-      W.put_columns(lt, gram);
+    for (int ch = 0; ch < kMaxEach; ++ch) {
+      if (ch >= have) break;
+      W.put_columns(lt, x[ch]);
       __syncthreads();
-      W.multiply(lt, lt, t);
+      clear16(t);
+      W.multiply(lq, lt, t);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
-      W.put_columns(lq, t);
-      clear(gram);
-      __syncthreads();
-#pragma unroll
-      for (int ch = 0; ch < kMaxEach; ++ch) {
-        if (ch >= have) break;
-        W.put_columns(lt, x[ch]);
+      for (int r = 0; r < 16; ++r) x[ch][r] = a * x[ch][r] + t[r] * kInvS;
+      if (k < steps) {
+        W.put_rows(lx, x[ch]);
         __syncthreads();
-        clear(t);
-        W.multiply(lq, lt, t);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          x[ch][r] = a * x[ch][r] + t[r] * kInvS;
-        if (step < steps) {
-          W.put_rows(lx, x[ch]);
-          __syncthreads();
-          W.multiply(lx, lx, gram);
-        } else {
-          __syncthreads();
-        }
+        W.multiply(lx, lx, gram);
+      } else {
+        __syncthreads();
       }
     }
-    if (!WHOLE || step >= steps) break;
   }
-
-  if (!WHOLE && k < steps) {
+  if (k < steps) {
 #pragma unroll
     for (int ch = 0; ch < kMaxEach; ++ch) {
       if (ch >= have) break;
       float *p = N.x + (int64_t(chunk0 + ch) * 64 + W.col()) * kNarrow;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = x[ch][4 * q + e];
-        *reinterpret_cast<f32x4 *>(p + W.row(q)) = v;
-      }
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4 *>(p + W.row(q)) =
+            f32x4{x[ch][4 * q], x[ch][4 * q + 1], x[ch][4 * q + 2],
+                  x[ch][4 * q + 3]};
     }
     f32x4 *g = reinterpret_cast<f32x4 *>(
         N.gram + (int64_t(k & 1) * slabs + slab) * kGramElems);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = gram[4 * q + e];
-      g[q * 256 + threadIdx.x] = v;
-    }
+    for (int q = 0; q < 4; ++q)
+      g[q * 256 + threadIdx.x] = f32x4{gram[4 * q], gram[4 * q + 1],
+                                       gram[4 * q + 2], gram[4 * q + 3]};
     return;
   }
 #pragma unroll
-  for (int ch = 0; ch < kMaxEach; ++ch) {
-    if (ch >= have) break;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = x[ch][4 * q + e] * kInvS;
-      store_result<MUON>(M, S, z, W.row(q),
-                         (chunk0 + ch) * 64 + W.col(), y);
-    }
-  }
+  for (int ch = 0; ch < kMaxEach; ++ch)
+    if (ch < have) store_chunk<MUON>(M, W, S, z, chunk0 + ch, x[ch]);
 }
 
 // -- host --------------------------------------------------------------------
@@ -1130,7 +1297,7 @@ constexpr int kBigShort = 512;
 
 Way way_of(const Mat &M, const int64_t (&work)[2]) {
   if (M.m <= kNarrow && M.n <= kNarrowLong)
-    return M.n <= 64 * kMaxEach ? kWhole : kNarrowSlabs;
+    return M.n <= 64 * kMaxWhole ? kWhole : kNarrowSlabs;
   if (M.m >= kBigShort) {
     const int one = M.odt == FSAGG_BF16;
     if (work[one] >= kBigStages) return one ? kBigOne : kBig;
@@ -1149,10 +1316,10 @@ void plan_mat(Mat &M, Way way) {
     M.mp = kNarrow;
     M.np = int32_t(round_to(M.n, 64));
     const int chunks = M.np / 64;
-    // a launch reads slabs x 16 KiB of Gram shares per workgroup, and works
-    // a chunk in about the time of 13 of those
-    if (way == kWhole) M.each = chunks;
-    else M.each = chunks <= NS_E1 ? 1 : chunks <= NS_E2 ? 2 : kMaxEach;
+    // a launch reads 16 KiB of Gram shares per slab into every workgroup,
+    // and works its chunks one after the other: 8 slabs' shares cost about
+    // what a chunk does
+    M.each = way == kWhole ? 1 : chunks <= 32 ? 1 : chunks <= 96 ? 2 : 4;
     M.slabs = (chunks + M.each - 1) / M.each;
     bytes = way == kWhole ? 0
                           : 8 * kMaxNorm +
@@ -1307,9 +1474,9 @@ void run_narrow(Group &G, const Step &st) {
   }
   G.start[G.nmat] = total;
   for (int k = 0; k <= st.steps; ++k)
-    hipLaunchKernelGGL((ns_narrow_kernel<MUON, false>), dim3(total),
-                       dim3(256), 0, st.stream, G, k, st.steps, st.a, st.b,
-                       st.c, st.eps, st.S);
+    hipLaunchKernelGGL(ns_narrow_kernel<MUON>, dim3(total), dim3(256), 0,
+                       st.stream, G, k, st.steps, st.a, st.b, st.c, st.eps,
+                       st.S);
 }
 
 template <bool MUON>
@@ -1320,9 +1487,9 @@ void run_whole(Group &G, const Step &st) {
     total += G.mat[i].batch;
   }
   G.start[G.nmat] = total;
-  hipLaunchKernelGGL((ns_narrow_kernel<MUON, true>), dim3(total), dim3(256),
-                     0, st.stream, G, 0, st.steps, st.a, st.b, st.c, st.eps,
-                     st.S);
+  hipLaunchKernelGGL(ns_whole_kernel<MUON>, dim3(total),
+                     dim3(256 * kMaxWhole), 0, st.stream, G, st.steps, st.a,
+                     st.b, st.c, st.eps, st.S);
 }
 
 template <bool MUON>
@@ -1455,6 +1622,7 @@ auto ns_fill(const fsagg_ns_mat *mats, bool pointers, const char *what) {
     }
     M.g = d.g;
     M.out = d.out;
+    M.vec = aligned16(d.out) && d.cols % 8 == 0;
     M.buf = nullptr;
     M.ws = nullptr;
     M.sz = d.batch_stride;
@@ -1477,6 +1645,7 @@ auto muon_fill(const fsagg_muon_mat *mats, bool pointers, const char *what) {
     }
     M.g = d.avg;
     M.out = d.param;
+    M.vec = aligned16(d.param) && d.cols % 8 == 0;
     M.buf = d.momentum;
     M.ws = nullptr;
     M.sz = M.si = M.sj = 0;
