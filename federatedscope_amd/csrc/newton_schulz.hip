@@ -29,6 +29,8 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -241,9 +243,25 @@ __device__ __forceinline__ void store_result(const Mat &M,
   }
 }
 
-__device__ __forceinline__ void split(float v, _Float16 &h, _Float16 &l) {
-  h = _Float16(v);
-  l = _Float16(v - float(h));
+// Limbs of two values (one conversion instruction rounds both).
+__device__ __forceinline__ void split2(float v0, float v1, half2 &h,
+                                       half2 &l) {
+  h = __builtin_convertvector((f32x2){v0, v1}, half2);
+  l = __builtin_convertvector((f32x2){v0 - float(h[0]), v1 - float(h[1])},
+                              half2);
+}
+// Limbs of N values, side by side.
+template <int N, typename H>
+__device__ __forceinline__ void split_n(const float *v, H &h, H &l) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    half2 x, y;
+    split2(v[e], v[e + 1], x, y);
+    h[e] = x[0];
+    h[e + 1] = x[1];
+    l[e] = y[0];
+    l[e + 1] = y[1];
+  }
 }
 
 // The update at element e = (i, j) of matrix z.
@@ -368,17 +386,23 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
     else tile[r][c] = v;
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-    const int r = k / 64, c = k % 64;
-    _Float16 h, l;
-    split(tile[r][c], h, l);
+  // 8 values a thread, in both orientations
+  for (int k = threadIdx.x; k < 64 * 8; k += 256) {
+    const int r = k / 8, c = k % 8 * 8;
+    float v[8];
+    half8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+    split_n<8>(v, h, l);
     const int64_t x = int64_t(i0 + r) * M.np + j0 + c;
-    P.xh[x] = h;
-    P.xl[x] = l;
-    split(tile[c][r], h, l);
+    *reinterpret_cast<half8 *>(P.xh + x) = h;
+    *reinterpret_cast<half8 *>(P.xl + x) = l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
+    split_n<8>(v, h, l);
     const int64_t y = int64_t(j0 + r) * M.mp + i0 + c;
-    P.th(0)[y] = h;
-    P.tl(0)[y] = l;
+    *reinterpret_cast<half8 *>(P.th(0) + y) = h;
+    *reinterpret_cast<half8 *>(P.tl(0) + y) = l;
   }
 }
 
@@ -732,13 +756,7 @@ struct Tile {
         store_result<MODE == kLastMuon, DT, 8>(M, S, z, gi, gj, v);
       } else {
         half8 h, l;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          _Float16 u, w;
-          split(v[e], u, w);
-          h[e] = u;
-          l[e] = w;
-        }
+        split_n<8>(v, h, l);
         _Float16 *ch, *cl, *dh, *dl;  // C by rows, and C^T
         int ldc, ldd;
         if constexpr (MODE == kApply) {
@@ -918,15 +936,15 @@ struct Slab {
   }
   __device__ __forceinline__ int col() const { return bj + fr; }
 
-  // x += P R^T over 64 of k; planes [64][64], limbs l at + 4096.  The three
-  // limb products go to accumulators of their own (a chain of dependent
+  // x += P R^T over 64 of k; planes [64][64], limbs l at + 4096.  The small
+  // limb products go to an accumulator of their own (a chain of dependent
   // matrix instructions is what a product this small waits for).
   __device__ __forceinline__ void multiply(const _Float16 *p,
                                            const _Float16 *r,
                                            f32x16 &x) const {
-    f32x16 s, t;
+    f32x16 s;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = t[e] = 0.0f;
+    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       const int op = swz(bi + fr, kk * 2 + fk), oq = swz(bj + fr, kk * 2 + fk);
@@ -935,12 +953,11 @@ struct Slab {
       const half8 rh = *reinterpret_cast<const half8 *>(r + oq);
       const half8 rl = *reinterpret_cast<const half8 *>(r + 4096 + oq);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, rh, s, 0, 0, 0);
-      t = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rl, t, 0, 0, 0);
       x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rh, x, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rl, s, 0, 0, 0);
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      x[e] = __fadd_rn(x[e], __fadd_rn(s[e], t[e]));
+    for (int e = 0; e < 16; ++e) x[e] = __fadd_rn(x[e], s[e]);
   }
   // limbs of the block's values (times kS), transposed: row col(), the rows
   // of a quad side by side
@@ -948,14 +965,9 @@ struct Slab {
                                               const f32x16 &x) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
+      const float v[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
       half4 h, l;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        _Float16 u, w;
-        split(x[4 * q + e], u, w);
-        h[e] = u;
-        l[e] = w;
-      }
+      split_n<4>(v, h, l);
       const int o = swz(col(), row(q) >> 3) + (row(q) & 7);
       *reinterpret_cast<half4 *>(p + o) = h;
       *reinterpret_cast<half4 *>(p + 4096 + o) = l;
@@ -965,15 +977,17 @@ struct Slab {
   __device__ __forceinline__ void put_rows(_Float16 *p,
                                            const f32x16 &x) const {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < 4; ++q) {
+      const float v[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+      half4 h, l;
+      split_n<4>(v, h, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        _Float16 u, w;
-        split(x[4 * q + e], u, w);
         const int o = swz(row(q) + e, col() >> 3) + (col() & 7);
-        p[o] = u;
-        p[4096 + o] = w;
+        p[o] = h[e];
+        p[4096 + o] = l[e];
       }
+    }
   }
 };
 
@@ -1035,21 +1049,6 @@ __device__ __forceinline__ void clear16(f32x16 &v) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) v[r] = 0.0f;
 }
-// kS Q = b kS A + c kS A^2 from kS^2 A; `la` takes A's limbs
-__device__ __forceinline__ f32x16 square(const Slab &W, f32x16 gram,
-                                         _Float16 *la, float b, float c) {
-#pragma unroll
-  for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
-  W.put_columns(la, gram);
-  __syncthreads();
-  f32x16 t;
-  clear16(t);
-  W.multiply(la, la, t);
-#pragma unroll
-  for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
-  return t;
-}
-
 // A whole matrix of up to kMaxWhole chunks, group g the chunk g.
 template <bool MUON>
 __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
@@ -1091,8 +1090,8 @@ __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
                                        gram[4 * q + 2], gram[4 * q + 3]};
       }
       __syncthreads();
-      clear16(gram);
-      for (int k = 0; k < chunks; ++k) {
+      if (g == 0) clear16(gram);
+      for (int k = 0; g == 0 && k < chunks; ++k) {
         const f32x4 *other = reinterpret_cast<const f32x4 *>(
             lds + 8192 * (2 + 2 * k));
 #pragma unroll
@@ -1104,10 +1103,25 @@ __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
         }
       }
     }
-    t = square(W, gram, lt, b, c);
-    if (g == 0) W.put_columns(lq, t);
+    // Q by the first group, which others wait for: all of them at it would
+    // share the one CU's vector units
+    if (g == 0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
+      W.put_columns(lq, gram);
+    } else if (g < chunks) {
+      W.put_columns(lt, x);
+    }
     __syncthreads();
-    if (g < chunks) W.put_columns(lt, x);
+    if (g == 0) {
+      clear16(t);
+      W.multiply(lq, lq, t);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
+      W.put_columns(lt, x);
+    }
+    __syncthreads();
+    if (g == 0) W.put_columns(lq, t);
     __syncthreads();
     if (g < chunks) {
       clear16(t);
@@ -1186,7 +1200,15 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
             gram[r] = __fadd_rn(gram[r], v[u][r / 4][r % 4]);
         }
     }
-    t = square(W, gram, lt, b, c);
+    // kS Q = b kS A + c kS A^2 from kS^2 A
+#pragma unroll
+    for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
+    W.put_columns(lt, gram);
+    __syncthreads();
+    clear16(t);
+    W.multiply(lt, lt, t);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
     W.put_columns(lq, t);
     clear16(gram);
     __syncthreads();
