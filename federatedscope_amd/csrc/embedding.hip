@@ -27,12 +27,15 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWave;
-constexpr int kMaxParts = 64;     // parts per key launch (kernel arguments)
+constexpr int kMaxParts = 112;    // parts per key launch (kernel arguments)
 constexpr int kTile = 4096;       // tokens per sorting workgroup
 constexpr int kSortBlock = 1024;
 constexpr int kSortWaves = kSortBlock / kWave;
 constexpr int kRounds = kTile / kSortBlock;  // 64-token rounds of a wave
 constexpr int kMaxDigit = 10;     // bits per radix pass
+#ifndef EM_WAVES
+#define EM_WAVES 2048
+#endif
 // a launch counts its work items in 32 bits
 constexpr int64_t kMaxGrid = (int64_t(1) << 32) / kBlock - 1;
 
@@ -149,16 +152,16 @@ __global__ __launch_bounds__(kBlock) void embed_lookup_kernel(
 struct Part {
   const void *ids;
   const char *rows;
-  int64_t row_bytes;
-  int64_t start;  // first token of the part
+  uint32_t start;   // first token of the part
+  uint32_t stride;  // elements between rows; the top bit: int64 ids
   float coef;
-  int32_t ids64;
 };
 struct Parts {
-  int n;
-  int64_t end;  // tokens up to the end of the last part here
+  int n, elem;
+  uint32_t end;  // tokens up to the end of the last part here
   Part part[kMaxParts];
 };
+constexpr uint32_t kIds64 = 0x80000000u;
 
 // Arrays of a call, in its workspace.
 struct Sort {
@@ -170,25 +173,32 @@ struct Sort {
   float *partial;    // [chunk][head, tail][dim]
 };
 
-// Key of every token of these parts: its row, or V for padding.
+// Key of token t: its row, or V for padding; its row of values and factor
+// are noted.
+__device__ __forceinline__ uint32_t token_key(const Parts &P, const Sort &W,
+                                              uint32_t t, uint32_t vocab) {
+  int lo = 0, hi = P.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (P.part[mid].start <= t) lo = mid;
+    else hi = mid;
+  }
+  const Part &p = P.part[lo];
+  const int64_t i = t - p.start;
+  const int64_t id = load_id(p.ids, i, (p.stride & kIds64) != 0);
+  W.row[t] = p.rows + i * int64_t(p.stride & ~kIds64) * P.elem;
+  W.coef[t] = p.coef;
+  return id >= 0 && id < int64_t(vocab) ? uint32_t(id) : vocab;
+}
+
+// Keys of these parts' tokens (a call of more parts than fit one launch).
 __global__ __launch_bounds__(kBlock) void embed_key_kernel(Parts P, Sort W,
                                                            uint32_t vocab) {
-  for (int64_t t = P.part[0].start + int64_t(blockIdx.x) * kBlock +
-                   threadIdx.x;
+  for (int64_t t = int64_t(P.part[0].start) +
+                   int64_t(blockIdx.x) * kBlock + threadIdx.x;
        t < P.end; t += int64_t(gridDim.x) * kBlock) {
-    int lo = 0, hi = P.n;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (P.part[mid].start <= t) lo = mid;
-      else hi = mid;
-    }
-    const Part &p = P.part[lo];
-    const int64_t i = t - p.start;
-    const int64_t id = load_id(p.ids, i, p.ids64);
-    W.key[0][t] = id >= 0 && id < int64_t(vocab) ? uint32_t(id) : vocab;
+    W.key[0][t] = token_key(P, W, uint32_t(t), vocab);
     W.tok[0][t] = uint32_t(t);
-    W.row[t] = p.rows + i * p.row_bytes;
-    W.coef[t] = p.coef;
   }
 }
 
@@ -202,8 +212,9 @@ __device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
                                            uint32_t (&rank)[kRounds]) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const uint32_t mask = (1u << bits) - 1u;
-  for (int i = threadIdx.x; i < (kSortWaves << bits); i += kSortBlock)
-    cnt[i] = 0;
+  uint32_t *cnt32 = reinterpret_cast<uint32_t *>(cnt);
+  for (int i = threadIdx.x; i < (kSortWaves << bits) / 2; i += kSortBlock)
+    cnt32[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
@@ -226,36 +237,17 @@ __device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
   __syncthreads();
 }
 
-__device__ __forceinline__ void load_tile(const Sort &W, int src,
-                                          int64_t tokens, uint32_t (&key)[4],
-                                          uint32_t (&tok)[4], bool (&in)[4],
-                                          int64_t base) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+// Turns digit d's counts by wave into the counts of the waves before; the
+// digit's total.
+__device__ __forceinline__ uint32_t wave_prefix(uint16_t *cnt, int d) {
+  uint32_t total = 0;
 #pragma unroll
-  for (int k = 0; k < kRounds; ++k) {
-    const int64_t t = base + wave * (kRounds * kWave) + k * kWave + lane;
-    in[k] = t < tokens;
-    key[k] = in[k] ? W.key[src][t] : 0u;
-    tok[k] = in[k] ? W.tok[src][t] : 0u;
+  for (int w = 0; w < kSortWaves; ++w) {
+    const uint32_t n = cnt[d * kSortWaves + w];
+    cnt[d * kSortWaves + w] = uint16_t(total);
+    total += n;
   }
-}
-
-// hist[digit][block]
-__global__ __launch_bounds__(kSortBlock) void embed_hist_kernel(
-    Sort W, int src, int64_t tokens, int shift, int bits, int blocks) {
-  __shared__ uint32_t h[1 << kMaxDigit];
-  const int digits = 1 << bits;
-  for (int i = threadIdx.x; i < digits; i += kSortBlock) h[i] = 0;
-  __syncthreads();
-  const int64_t base = int64_t(blockIdx.x) * kTile;
-  for (int k = 0; k < kRounds; ++k) {
-    const int64_t t = base + k * kSortBlock + threadIdx.x;
-    if (t < tokens)
-      atomicAdd(&h[(W.key[src][t] >> shift) & (digits - 1)], 1u);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < digits; i += kSortBlock)
-    W.hist[int64_t(i) * blocks + blockIdx.x] = h[i];
+  return total;
 }
 
 // Exclusive sum over the workgroup's kSortBlock values, in thread order.
@@ -276,16 +268,59 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v,
   return before + s - v;
 }
 
+// token k of this thread's rounds in the tile at `base`
+__device__ __forceinline__ int64_t tile_token(int64_t base, int k) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  return base + wave * (kRounds * kWave) + k * kWave + lane;
+}
+
+// hist[digit][block] of the first digit, of the keys as they are (P.n = 0)
+// or as they are made here.
+__global__ __launch_bounds__(kSortBlock) void embed_hist_kernel(
+    Parts P, Sort W, int src, int64_t tokens, uint32_t vocab, int shift,
+    int bits, int blocks) {
+  __shared__ uint32_t h[1 << kMaxDigit];
+  const int digits = 1 << bits;
+  for (int i = threadIdx.x; i < digits; i += kSortBlock) h[i] = 0;
+  __syncthreads();
+  const int64_t base = int64_t(blockIdx.x) * kTile;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t t = tile_token(base, k);
+    if (t >= tokens) continue;
+    uint32_t key;
+    if (P.n > 0) {
+      key = token_key(P, W, uint32_t(t), vocab);
+      W.key[0][t] = key;
+      W.tok[0][t] = uint32_t(t);
+    } else {
+      key = W.key[src][t];
+    }
+    atomicAdd(&h[(key >> shift) & (digits - 1)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < digits; i += kSortBlock)
+    W.hist[int64_t(i) * blocks + blockIdx.x] = h[i];
+}
+
 // One stable pass: every token of tile b goes to the digit's start plus the
 // digit's tokens in earlier tiles and waves plus its rank.
 __global__ __launch_bounds__(kSortBlock) void embed_scatter_kernel(
     Sort W, int src, int64_t tokens, int shift, int bits, int blocks) {
-  __shared__ uint16_t cnt[kSortWaves << kMaxDigit];
+  __shared__ __attribute__((aligned(16)))
+  uint16_t cnt[kSortWaves << kMaxDigit];
   __shared__ uint32_t at[1 << kMaxDigit];
   __shared__ uint32_t scratch[kSortWaves];
   uint32_t key[kRounds], tok[kRounds], rank[kRounds];
   bool in[kRounds];
-  load_tile(W, src, tokens, key, tok, in, int64_t(blockIdx.x) * kTile);
+  const int64_t base = int64_t(blockIdx.x) * kTile;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t t = tile_token(base, k);
+    in[k] = t < tokens;
+    key[k] = in[k] ? W.key[src][t] : 0u;
+    tok[k] = in[k] ? W.tok[src][t] : 0u;
+  }
   const int digits = 1 << bits;
   // thread d: digit d's total and its tokens in earlier tiles
   uint32_t total = 0, mine = 0;
@@ -297,17 +332,79 @@ __global__ __launch_bounds__(kSortBlock) void embed_scatter_kernel(
     }
   }
   const uint32_t first = block_exclusive(total, scratch);
-  if (int(threadIdx.x) < digits) at[threadIdx.x] = first + mine;
   tile_ranks(key, in, shift, bits, cnt, rank);
+  if (int(threadIdx.x) < digits) {
+    at[threadIdx.x] = first + mine;
+    wave_prefix(cnt, threadIdx.x);
+  }
+  __syncthreads();
   const int wave = threadIdx.x / kWave;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
     if (!in[k]) continue;
     const uint32_t d = (key[k] >> shift) & (digits - 1);
-    uint32_t o = at[d] + rank[k];
-    for (int w = 0; w < wave; ++w) o += cnt[d * kSortWaves + w];
+    const uint32_t o = at[d] + cnt[d * kSortWaves + wave] + rank[k];
     W.key[src ^ 1][o] = key[k];
     W.tok[src ^ 1][o] = tok[k];
+  }
+}
+
+// Keys and sort of one tile's tokens in one launch, through LDS.
+__global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(
+    Parts P, Sort W, int src, int64_t tokens, uint32_t vocab, int passes,
+    int bits) {
+  __shared__ __attribute__((aligned(16)))
+  uint16_t cnt[kSortWaves << kMaxDigit];
+  __shared__ uint32_t at[1 << kMaxDigit];
+  __shared__ uint32_t scratch[kSortWaves];
+  __shared__ uint32_t skey[kTile], stok[kTile];
+  uint32_t key[kRounds], tok[kRounds], rank[kRounds];
+  bool in[kRounds];
+  const int wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t t = tile_token(0, k);
+    in[k] = t < tokens;
+    key[k] = tok[k] = 0u;
+    if (in[k]) {
+      key[k] = P.n > 0 ? token_key(P, W, uint32_t(t), vocab) : W.key[0][t];
+      tok[k] = uint32_t(t);
+    }
+  }
+  const int digits = 1 << bits;
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    tile_ranks(key, in, shift, bits, cnt, rank);
+    const uint32_t total =
+        int(threadIdx.x) < digits ? wave_prefix(cnt, threadIdx.x) : 0u;
+    const uint32_t first = block_exclusive(total, scratch);
+    if (int(threadIdx.x) < digits) at[threadIdx.x] = first;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      if (!in[k]) continue;
+      const uint32_t d = (key[k] >> shift) & (digits - 1);
+      const uint32_t o = at[d] + cnt[d * kSortWaves + wave] + rank[k];
+      skey[o] = key[k];
+      stok[o] = tok[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const int t = int(tile_token(0, k));
+      if (in[k]) {
+        key[k] = skey[t];
+        tok[k] = stok[t];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t t = tile_token(0, k);
+    if (in[k]) {
+      W.key[src][t] = key[k];
+      W.tok[src][t] = tok[k];
+    }
   }
 }
 
@@ -341,6 +438,8 @@ __device__ __forceinline__ int64_t wave_lower_bound(const uint32_t *key,
   return lo;
 }
 
+constexpr int kZeroRows = kBlock;  // most rows of a zero workgroup
+
 // Row sums of one chunk of sorted tokens and one slice of columns per wave;
 // workgroups past those write the zero rows that no token names.
 template <int GT, int OT, int VEC>
@@ -353,13 +452,26 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
   const int wave =
       __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   if (int(blockIdx.x) >= sum_blocks) {
+    // the rows of this stretch that a token names: one search per thread,
+    // inside the stretch's own tokens
+    __shared__ uint8_t named[kZeroRows];
     const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * zero_rows;
     const int64_t r1 = r0 + zero_rows < O.vocab ? r0 + zero_rows : O.vocab;
     const int64_t a = wave_lower_bound(O.key, 0, O.tokens, uint32_t(r0));
     const int64_t b = wave_lower_bound(O.key, a, O.tokens, uint32_t(r1));
+    if (r0 + int64_t(threadIdx.x) < r1) {
+      const uint32_t r = uint32_t(r0) + threadIdx.x;
+      int64_t lo = a, hi = b;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (O.key[mid] < r) lo = mid + 1;
+        else hi = mid;
+      }
+      named[threadIdx.x] = lo < b && O.key[lo] == r;
+    }
+    __syncthreads();
     for (int64_t r = r0 + wave; r < r1; r += kWaves) {
-      const int64_t p = wave_lower_bound(O.key, a, b, uint32_t(r));
-      if (p < b && O.key[p] == uint32_t(r)) continue;
+      if (named[r - r0]) continue;
       char *dst = O.out + r * O.row_bytes;
       const float z[VEC] = {};
       for (int64_t c = int64_t(lane) * VEC; c < O.dim; c += kWave * VEC)
@@ -467,17 +579,34 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(Out O, Sort W) {
   if (O.key[chunk * O.chunk] == key && chunk > 0 &&
       O.key[chunk * O.chunk - 1] == key)
     return;
-  // chunks after this one that the row reaches
-  int64_t last = chunk + 1;
-  while (last + 1 < O.chunks && O.key[(last + 1) * O.chunk] == key) ++last;
+  // chunks after this one that the row reaches: those that begin with it
+  // (a lane looks at one)
+  int64_t last = chunk;
+  for (;;) {
+    const int64_t q = last + 1 + lane;
+    const uint64_t same =
+        __ballot(q < O.chunks && O.key[q * O.chunk] == key);
+    const int n = same == ~0ull ? kWave : __builtin_ctzll(~same);
+    last += n;
+    if (n < kWave) break;
+  }
   if (c >= O.dim) return;
   float acc[VEC];
   load_vec<FSAGG_F32, VEC>(W.partial + (chunk * 2 + 1) * O.dim + c, acc);
-  for (int64_t q = chunk + 1; q <= last; ++q) {
-    float v[VEC];
-    load_vec<FSAGG_F32, VEC>(W.partial + q * 2 * O.dim + c, v);
+  constexpr int kAhead = 8;
+  for (int64_t q0 = chunk + 1; q0 <= last; q0 += kAhead) {
+    float v[kAhead][VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = __fadd_rn(acc[e], v[e]);
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t q = q0 + u <= last ? q0 + u : last;
+      load_vec<FSAGG_F32, VEC>(W.partial + q * 2 * O.dim + c, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (q0 + u <= last) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = __fadd_rn(acc[e], v[u][e]);
+      }
   }
   char *dst = O.out + int64_t(key) * O.row_bytes + c * kOE;
   if (O.accumulate) {
@@ -503,9 +632,14 @@ void with_dtype(int dt, F f) {
   else f(std::integral_constant<int, FSAGG_BF16>());
 }
 
-int64_t chunk_tokens(int64_t tokens) {
-  (void)tokens;
-  return 32;
+// Tokens per chunk: long chunks leave fewer partial sums, short ones make
+// enough waves where tokens are few.
+int chunk_tokens(int64_t tokens, int64_t dim) {
+  if (tokens <= kWave) return kWave;  // one chunk, no join
+  const int64_t slices = (dim + 511) / 512;
+  int chunk = kWave;
+  while (chunk > 8 && tokens * slices < int64_t(chunk) * EM_WAVES) chunk /= 2;
+  return chunk;
 }
 
 struct Sizes {
@@ -519,7 +653,7 @@ Sizes sizes_of(int64_t tokens, int64_t dim, int64_t vocab) {
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   Z.tokens = tokens;
   Z.dim = dim;
-  Z.chunk = chunk_tokens(tokens);
+  Z.chunk = chunk_tokens(tokens, dim);
   Z.chunks = (tokens + Z.chunk - 1) / Z.chunk;
   Z.blocks = (tokens + kTile - 1) / kTile;
   Z.bits = 1;
@@ -616,7 +750,8 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   int64_t tokens = 0;
   for (int i = 0; i < nparts; ++i) {
     const fsagg_embed_part &p = parts[i];
-    if (p.tokens < 0 || (p.tokens > 0 && dim > 0 && (!p.ids || !p.rows))) {
+    if (p.tokens < 0 || (p.tokens > 0 && dim > 0 && (!p.ids || !p.rows)) ||
+        p.row_stride < 0 || p.row_stride >= int64_t(kIds64)) {
       set_error("%s: part %d: invalid argument", what, i);
       return FSAGG_EINVAL;
     }
@@ -657,39 +792,48 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
     W.hist = reinterpret_cast<uint32_t *>(take(Z.hist));
     W.partial = reinterpret_cast<float *>(take(Z.partial));
   }
-  int64_t start = 0;
-  for (int i = 0; i < nparts;) {
-    Parts P;
-    P.n = 0;
-    const int64_t first = start;
-    for (; i < nparts && P.n < kMaxParts; ++i) {
-      const fsagg_embed_part &p = parts[i];
-      if (p.tokens == 0) continue;
-      Part &q = P.part[P.n++];
-      q.ids = p.ids;
-      q.rows = static_cast<const char *>(p.rows);
-      q.row_bytes = p.row_stride * e;
-      q.start = start;
-      q.coef = p.coef;
-      q.ids64 = p.ids64;
-      start += p.tokens;
+  // the parts that hold tokens, up to kMaxParts at a time
+  Parts P;
+  P.n = 0;
+  P.elem = e;
+  P.end = 0;
+  int nonempty = 0;
+  for (int i = 0; i < nparts; ++i) nonempty += parts[i].tokens > 0;
+  const bool one_launch = nonempty <= kMaxParts;
+  for (int i = 0; i < nparts; ++i) {
+    const fsagg_embed_part &p = parts[i];
+    if (p.tokens == 0) continue;
+    Part &q = P.part[P.n++];
+    q.ids = p.ids;
+    q.rows = static_cast<const char *>(p.rows);
+    q.start = P.end;
+    q.stride = uint32_t(p.row_stride) | (p.ids64 ? kIds64 : 0u);
+    q.coef = p.coef;
+    P.end += uint32_t(p.tokens);
+    if (!one_launch && (P.n == kMaxParts || P.end == uint32_t(tokens))) {
+      hipLaunchKernelGGL(embed_key_kernel,
+                         dim3(stream_grid(P.end - P.part[0].start, kBlock,
+                                          2048)),
+                         dim3(kBlock), 0, s, P, W, uint32_t(vocab));
+      P.n = 0;
     }
-    P.end = start;
-    if (P.n == 0) continue;
-    hipLaunchKernelGGL(embed_key_kernel,
-                       dim3(stream_grid(start - first, kBlock, 2048)),
-                       dim3(kBlock), 0, s, P, W, uint32_t(vocab));
   }
   int src = 0;
-  if (tokens > 0)
+  if (tokens > 0 && tokens <= kTile) {
+    src = 1;
+    hipLaunchKernelGGL(embed_sort_kernel, dim3(1), dim3(kSortBlock), 0, s, P,
+                       W, src, tokens, uint32_t(vocab), Z.passes, Z.digit);
+  } else if (tokens > 0) {
     for (int p = 0; p < Z.passes; ++p, src ^= 1) {
       hipLaunchKernelGGL(embed_hist_kernel, dim3(Z.blocks), dim3(kSortBlock),
-                         0, s, W, src, tokens, p * Z.digit, Z.digit,
-                         int(Z.blocks));
+                         0, s, P, W, src, tokens, uint32_t(vocab),
+                         p * Z.digit, Z.digit, int(Z.blocks));
+      P.n = 0;  // the keys are there
       hipLaunchKernelGGL(embed_scatter_kernel, dim3(Z.blocks),
                          dim3(kSortBlock), 0, s, W, src, tokens, p * Z.digit,
                          Z.digit, int(Z.blocks));
     }
+  }
   Out O;
   O.out = static_cast<char *>(out);
   O.row_bytes = out_stride * oe;
@@ -707,7 +851,7 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   // rows per zero workgroup: about 64 KiB
   int64_t zero_rows = 65536 / (dim * oe);
   if (zero_rows < kWaves) zero_rows = kWaves;
-  if (zero_rows > 1024) zero_rows = 1024;
+  if (zero_rows > kZeroRows) zero_rows = kZeroRows;
   const int64_t zero_blocks =
       accumulate ? 0 : (vocab + zero_rows - 1) / zero_rows;
   const int64_t join_blocks =

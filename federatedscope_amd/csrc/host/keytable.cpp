@@ -45,6 +45,7 @@ PyObject *b64_frame(PyObject *, PyObject *args);
 PyObject *b64_frame_many(PyObject *, PyObject *args);
 // host/krumcert.cpp: the Krum selection certificate
 PyObject *gram_select(PyObject *, PyObject *args);
+PyObject *embed_parts(PyObject *, PyObject *args);
 
 namespace {
 
@@ -706,6 +707,9 @@ PyMethodDef kMethods[] = {
     {"gram_select", gram_select, METH_VARARGS,
      "gram_select(buf, nseg, f, m, ordered) -> None or (scores, order, "
      "ambiguous)"},
+    {"embed_parts", embed_parts, METH_VARARGS,
+     "embed_parts(ids, grads, coefs, out_lo, out_hi) -> (table, tokens, dim, "
+     "dtype_code) or None"},
     {"key_table", key_table, METH_VARARGS,
      "key_table(dicts, keys, shapes, device_index[, offs4]) -> (bytes, "
      "missing, aligned16) or None"},

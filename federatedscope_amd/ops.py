@@ -1963,15 +1963,17 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, weights=None, out=None,
     grad's dtype) gets zeros in the rows no token names; with ``accumulate``
     the sums are added to ``out`` (required) and its other rows are not
     touched."""
-    many = isinstance(ids, (list, tuple))
-    ids = list(ids) if many else [ids]
-    grad = list(grad) if many else [grad]
+    if not isinstance(ids, (list, tuple)):
+        ids, grad = [ids], [grad]
+    ids, grad = list(ids), list(grad)
     if len(ids) != len(grad) or not ids:
         raise ValueError('%d token tensors, %d gradients' %
                          (len(ids), len(grad)))
     if weights is None:
-        weights = [1.0] * len(ids)
-    if len(weights) != len(ids):
+        coefs = [float(scale)] * len(ids)
+    elif len(weights) == len(ids):
+        coefs = [float(scale) * float(w) for w in weights]
+    else:
         raise ValueError('%d weights for %d token tensors' %
                          (len(weights), len(ids)))
     num_rows = int(num_rows)
@@ -1979,7 +1981,38 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, weights=None, out=None,
         raise ValueError('num_rows must not be negative')
     if accumulate and out is None:
         raise ValueError('accumulate needs out')
+    lo, hi = (0, 0) if out is None or not isinstance(out, torch.Tensor) or \
+        not out.numel() else _extent(out)
+    got = L.host().embed_parts(ids, grad, coefs, lo, hi)
+    if got is None:
+        got = _embed_parts(ids, grad, coefs, out)
+    parts, tokens, dim, code = got
+    dev = grad[0].device
+    if out is None:
+        out = torch.empty((num_rows, dim), dtype=grad[0].dtype, device=dev)
+    else:
+        _check_float_cuda(out, 'out', dev)
+        if tuple(out.shape) != (num_rows, dim):
+            raise ValueError('out has shape %s, expected %s' %
+                             (tuple(out.shape), (num_rows, dim)))
+        _check_rows(out, 'out')
+        if num_rows > 1 and dim and out.stride(0) < dim:
+            raise ValueError('the rows of out overlap')
     lib = L.load()
+    with _OnDevice(dev):
+        ws = _scratch(dev, lib.fsagg_embed_grad_workspace_bytes(
+            tokens, dim, num_rows))
+        L.check(lib.fsagg_embed_grad(
+            parts, len(ids), code, num_rows, dim, out.data_ptr(),
+            _FLOAT_CODE[out.dtype], out.stride(0), int(bool(accumulate)),
+            ws.data_ptr(), ws.numel(), _stream(dev)), 'fsagg_embed_grad')
+    return out
+
+
+def _embed_parts(ids, grad, coefs, out):
+    """The parts table of fsagg_embed_grad, with a message for what is wrong
+    (_fsagg_host.embed_parts takes the plain form and gives up on the
+    rest)."""
     dev = dt = dim = None
     parts = (L.EmbedPart * len(ids))()
     tokens = 0
@@ -2003,29 +2036,11 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, weights=None, out=None,
                 raise ValueError('gradient %d must be contiguous' % i)
             g = g.reshape(x.numel(), dim)
         _check_rows(g, 'gradient %d' % i)
+        if out is not None and (_overlap(out, g) or _overlap(out, x)):
+            raise ValueError('out overlaps an input')
         p = parts[i]
         p.ids, p.rows = x.data_ptr(), g.data_ptr()
         p.tokens, p.row_stride = x.numel(), g.stride(0)
-        p.coef = float(scale) * float(weights[i])
-        p.ids64 = int(x.dtype == torch.int64)
+        p.coef, p.ids64 = coefs[i], int(x.dtype == torch.int64)
         tokens += x.numel()
-    if out is None:
-        out = torch.empty((num_rows, dim), dtype=dt, device=dev)
-    else:
-        _check_float_cuda(out, 'out', dev)
-        if tuple(out.shape) != (num_rows, dim):
-            raise ValueError('out has shape %s, expected %s' %
-                             (tuple(out.shape), (num_rows, dim)))
-        _check_rows(out, 'out')
-        if out.numel() and out.shape[0] > 1 and out.stride(0) < dim:
-            raise ValueError('the rows of out overlap')
-        if any(_overlap(out, t) for t in ids + grad):
-            raise ValueError('out overlaps an input')
-    with _OnDevice(dev):
-        need = lib.fsagg_embed_grad_workspace_bytes(tokens, dim, num_rows)
-        ws = _scratch(dev, need)
-        L.check(lib.fsagg_embed_grad(
-            parts, len(ids), _FLOAT_CODE[dt], num_rows, dim, out.data_ptr(),
-            _FLOAT_CODE[out.dtype], out.stride(0), int(bool(accumulate)),
-            ws.data_ptr(), ws.numel(), _stream(dev)), 'fsagg_embed_grad')
-    return out
+    return parts, tokens, dim, _FLOAT_CODE[dt]
