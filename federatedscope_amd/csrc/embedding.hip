@@ -22,20 +22,24 @@
 
 #include <hip/hip_fp16.h>
 
+#ifndef EM_WAVES
+#define EM_WAVES 2048
+#define EM_SB 8
+#endif
 namespace fsagg {
 namespace {
 
 constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWave;
 constexpr int kMaxParts = 112;    // parts per key launch (kernel arguments)
-constexpr int kTile = 4096;       // tokens per sorting workgroup
-constexpr int kSortBlock = 1024;
-constexpr int kSortWaves = kSortBlock / kWave;
-constexpr int kRounds = kTile / kSortBlock;  // 64-token rounds of a wave
+// Sorting: a thread holds kRounds tokens.  Up to kOneTile tokens are one
+// workgroup's; else tiles of 1024 tokens, small enough that many sort at
+// once.
+constexpr int kRounds = 4;
+constexpr int kOneThreads = 1024, kOneTile = kOneThreads * kRounds;
+constexpr int kTileThreads = 256, kTile = kTileThreads * kRounds;
+constexpr int kSumBlocks = EM_SB;   // tiles whose counts a tile adds up itself
 constexpr int kMaxDigit = 10;     // bits per radix pass
-#ifndef EM_WAVES
-#define EM_WAVES 2048
-#endif
 // a launch counts its work items in 32 bits
 constexpr int64_t kMaxGrid = (int64_t(1) << 32) / kBlock - 1;
 
@@ -73,18 +77,33 @@ struct Elem<FSAGG_BF16> {
   }
 };
 
-// VEC elements as fp32: one 16-byte load (or less), or single elements
+// VEC elements as they lie: one 16-byte load (or less), or a single element
 template <int DT, int VEC>
-__device__ __forceinline__ void load_vec(const void *p, float (&v)[VEC]) {
-  using T = typename Elem<DT>::type;
+struct Raw {
+  typedef typename Elem<DT>::type type __attribute__((ext_vector_type(VEC)));
+};
+template <int DT>
+struct Raw<DT, 1> {
+  using type = typename Elem<DT>::type;
+};
+template <int DT, int VEC>
+__device__ __forceinline__ typename Raw<DT, VEC>::type load_raw(
+    const void *p) {
+  return gld(static_cast<const typename Raw<DT, VEC>::type *>(p));
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void widen(
+    const typename Raw<DT, VEC>::type &x, float (&v)[VEC]) {
   if constexpr (VEC == 1) {
-    v[0] = Elem<DT>::get(gld(static_cast<const T *>(p)));
+    v[0] = Elem<DT>::get(x);
   } else {
-    typedef T tv __attribute__((ext_vector_type(VEC)));
-    const tv x = gld(static_cast<const tv *>(p));
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = Elem<DT>::get(x[e]);
   }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void load_vec(const void *p, float (&v)[VEC]) {
+  widen<DT, VEC>(load_raw<DT, VEC>(p), v);
 }
 template <int DT, int VEC>
 __device__ __forceinline__ void store_vec(void *p, const float (&v)[VEC]) {
@@ -167,16 +186,18 @@ constexpr uint32_t kIds64 = 0x80000000u;
 struct Sort {
   uint32_t *key[2];
   uint32_t *tok[2];
-  const char **row;  // by token
-  float *coef;       // by token
+  const char **row, **srow;  // by token, and as sorted
+  float *coef, *scoef;
   uint32_t *hist;    // [digits][blocks]
+  uint32_t *total;   // [digits]
   float *partial;    // [chunk][head, tail][dim]
 };
 
-// Key of token t: its row, or V for padding; its row of values and factor
-// are noted.
-__device__ __forceinline__ uint32_t token_key(const Parts &P, const Sort &W,
-                                              uint32_t t, uint32_t vocab) {
+// Key of token t: its row, or V for padding; and its row of values and
+// factor.
+__device__ __forceinline__ uint32_t token_key(const Parts &P, uint32_t t,
+                                              uint32_t vocab,
+                                              const char *&row, float &coef) {
   int lo = 0, hi = P.n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -186,9 +207,21 @@ __device__ __forceinline__ uint32_t token_key(const Parts &P, const Sort &W,
   const Part &p = P.part[lo];
   const int64_t i = t - p.start;
   const int64_t id = load_id(p.ids, i, (p.stride & kIds64) != 0);
-  W.row[t] = p.rows + i * int64_t(p.stride & ~kIds64) * P.elem;
-  W.coef[t] = p.coef;
+  row = p.rows + i * int64_t(p.stride & ~kIds64) * P.elem;
+  coef = p.coef;
   return id >= 0 && id < int64_t(vocab) ? uint32_t(id) : vocab;
+}
+
+__device__ __forceinline__ uint32_t note_token(const Parts &P, const Sort &W,
+                                               uint32_t t, uint32_t vocab) {
+  const char *row;
+  float coef;
+  const uint32_t key = token_key(P, t, vocab, row, coef);
+  W.key[0][t] = key;
+  W.tok[0][t] = t;
+  W.row[t] = row;
+  W.coef[t] = coef;
+  return key;
 }
 
 // Keys of these parts' tokens (a call of more parts than fit one launch).
@@ -196,25 +229,32 @@ __global__ __launch_bounds__(kBlock) void embed_key_kernel(Parts P, Sort W,
                                                            uint32_t vocab) {
   for (int64_t t = int64_t(P.part[0].start) +
                    int64_t(blockIdx.x) * kBlock + threadIdx.x;
-       t < P.end; t += int64_t(gridDim.x) * kBlock) {
-    W.key[0][t] = token_key(P, W, uint32_t(t), vocab);
-    W.tok[0][t] = uint32_t(t);
-  }
+       t < P.end; t += int64_t(gridDim.x) * kBlock)
+    note_token(P, W, uint32_t(t), vocab);
+}
+
+// token k of this thread's rounds in the tile at `base`: wave w owns tokens
+// [256 w, 256 w + 256) in rounds of 64
+__device__ __forceinline__ int64_t tile_token(int64_t base, int k) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  return base + wave * (kRounds * kWave) + k * kWave + lane;
 }
 
 // Rank of every token of a workgroup's tile among the tile's tokens of the
-// same digit, in order: wave w owns tokens [256 w, 256 w + 256) in rounds of
-// 64; cnt[digit][wave] ends as the wave's count of the digit.
+// same digit in the same wave, in order; cnt[digit][wave] ends as the wave's
+// count of the digit.
+template <int TH>
 __device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
                                            const bool (&in)[kRounds],
                                            int shift, int bits,
                                            uint16_t *cnt,
                                            uint32_t (&rank)[kRounds]) {
+  constexpr int kW = TH / kWave;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const uint32_t mask = (1u << bits) - 1u;
-  uint32_t *cnt32 = reinterpret_cast<uint32_t *>(cnt);
-  for (int i = threadIdx.x; i < (kSortWaves << bits) / 2; i += kSortBlock)
-    cnt32[i] = 0;
+  u32x4 *cnt4 = reinterpret_cast<u32x4 *>(cnt);
+  for (int i = threadIdx.x; i < (kW << bits) / 8; i += TH)
+    cnt4[i] = u32x4{0, 0, 0, 0};
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
@@ -224,7 +264,7 @@ __device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
       const uint64_t m = __ballot((d >> b) & 1u);
       same &= ((d >> b) & 1u) ? m : ~m;
     }
-    uint16_t *c = cnt + d * kSortWaves + wave;
+    uint16_t *c = cnt + d * kW + wave;
     const uint32_t before = in[k] ? *c : 0u;
     rank[k] = before + __popcll(same & ((1ull << lane) - 1ull));
     // the whole wave has read its counters (one instruction stream); the
@@ -239,78 +279,112 @@ __device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
 
 // Turns digit d's counts by wave into the counts of the waves before; the
 // digit's total.
+template <int TH>
 __device__ __forceinline__ uint32_t wave_prefix(uint16_t *cnt, int d) {
+  constexpr int kW = TH / kWave;
+  uint16_t n[kW];
+#pragma unroll
+  for (int w = 0; w < kW; ++w) n[w] = cnt[d * kW + w];
   uint32_t total = 0;
 #pragma unroll
-  for (int w = 0; w < kSortWaves; ++w) {
-    const uint32_t n = cnt[d * kSortWaves + w];
-    cnt[d * kSortWaves + w] = uint16_t(total);
-    total += n;
+  for (int w = 0; w < kW; ++w) {
+    cnt[d * kW + w] = uint16_t(total);
+    total += n[w];
   }
   return total;
 }
 
-// Exclusive sum over the workgroup's kSortBlock values, in thread order.
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t v,
-                                                    uint32_t *scratch) {
+// Exclusive sums over digits: at[d] = v(0) + .. + v(d - 1), v by thread
+// (digit d = c TH + thread; 1 << kMaxDigit digits at most).
+template <int TH, typename F>
+__device__ __forceinline__ void digit_starts(int digits, F v, uint32_t *at,
+                                             uint32_t *scratch) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  uint32_t s = v;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const uint32_t u = __shfl_up(s, o);
-    if (lane >= o) s += u;
-  }
-  if (lane == kWave - 1) scratch[wave] = s;
-  __syncthreads();
   uint32_t before = 0;
-  for (int w = 0; w < wave; ++w) before += scratch[w];
-  __syncthreads();
-  return before + s - v;
+  for (int c = 0; c < digits; c += TH) {
+    const int d = c + int(threadIdx.x);
+    const uint32_t n = d < digits ? v(d) : 0u;
+    uint32_t s = n;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t u = __shfl_up(s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == kWave - 1) scratch[wave] = s;
+    __syncthreads();
+    uint32_t sum = before;
+    for (int w = 0; w < TH / kWave; ++w) {
+      if (w == wave && d < digits) at[d] = sum + s - n;
+      sum += scratch[w];
+    }
+    before = sum;
+    __syncthreads();
+  }
 }
 
-// token k of this thread's rounds in the tile at `base`
-__device__ __forceinline__ int64_t tile_token(int64_t base, int k) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  return base + wave * (kRounds * kWave) + k * kWave + lane;
-}
-
-// hist[digit][block] of the first digit, of the keys as they are (P.n = 0)
-// or as they are made here.
-__global__ __launch_bounds__(kSortBlock) void embed_hist_kernel(
+// hist[digit][block], of the keys as they are (P.n = 0) or as they are made
+// here.
+__global__ __launch_bounds__(kTileThreads) void embed_hist_kernel(
     Parts P, Sort W, int src, int64_t tokens, uint32_t vocab, int shift,
     int bits, int blocks) {
   __shared__ uint32_t h[1 << kMaxDigit];
   const int digits = 1 << bits;
-  for (int i = threadIdx.x; i < digits; i += kSortBlock) h[i] = 0;
+  for (int i = threadIdx.x; i < digits; i += kTileThreads) h[i] = 0;
   __syncthreads();
   const int64_t base = int64_t(blockIdx.x) * kTile;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
     const int64_t t = tile_token(base, k);
     if (t >= tokens) continue;
-    uint32_t key;
-    if (P.n > 0) {
-      key = token_key(P, W, uint32_t(t), vocab);
-      W.key[0][t] = key;
-      W.tok[0][t] = uint32_t(t);
-    } else {
-      key = W.key[src][t];
-    }
+    const uint32_t key = P.n > 0 ? note_token(P, W, uint32_t(t), vocab)
+                                 : W.key[src][t];
     atomicAdd(&h[(key >> shift) & (digits - 1)], 1u);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < digits; i += kSortBlock)
+  for (int i = threadIdx.x; i < digits; i += kTileThreads)
     W.hist[int64_t(i) * blocks + blockIdx.x] = h[i];
 }
 
+// Where there are many tiles: a digit's counts become the counts of the
+// tiles before, and its total is noted (one workgroup per digit).
+__global__ __launch_bounds__(kTileThreads) void embed_scan_kernel(
+    Sort W, int blocks) {
+  __shared__ uint32_t scratch[kTileThreads / kWave];
+  uint32_t *h = W.hist + int64_t(blockIdx.x) * blocks;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  uint32_t before = 0;
+  for (int b0 = 0; b0 < blocks; b0 += kTileThreads) {
+    const int b = b0 + int(threadIdx.x);
+    const uint32_t n = b < blocks ? h[b] : 0u;
+    uint32_t s = n;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t u = __shfl_up(s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == kWave - 1) scratch[wave] = s;
+    __syncthreads();
+    uint32_t sum = before;
+    for (int w = 0; w < kTileThreads / kWave; ++w) {
+      if (w == wave && b < blocks) h[b] = sum + s - n;
+      sum += scratch[w];
+    }
+    before = sum;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) W.total[blockIdx.x] = before;
+}
+
 // One stable pass: every token of tile b goes to the digit's start plus the
-// digit's tokens in earlier tiles and waves plus its rank.
-__global__ __launch_bounds__(kSortBlock) void embed_scatter_kernel(
-    Sort W, int src, int64_t tokens, int shift, int bits, int blocks) {
-  __shared__ __attribute__((aligned(16)))
-  uint16_t cnt[kSortWaves << kMaxDigit];
-  __shared__ uint32_t at[1 << kMaxDigit];
-  __shared__ uint32_t scratch[kSortWaves];
+// digit's tokens in earlier tiles and waves plus its rank.  The last pass
+// takes the rows and factors along.
+__global__ __launch_bounds__(kTileThreads) void embed_scatter_kernel(
+    Sort W, int src, int64_t tokens, int shift, int bits, int blocks,
+    int scanned, int last) {
+  constexpr int kW = kTileThreads / kWave;
+  __shared__ __attribute__((aligned(16))) uint16_t cnt[kW << kMaxDigit];
+  __shared__ uint32_t at[1 << kMaxDigit], mine[1 << kMaxDigit];
+  __shared__ uint32_t scratch[kW];
   uint32_t key[kRounds], tok[kRounds], rank[kRounds];
   bool in[kRounds];
   const int64_t base = int64_t(blockIdx.x) * kTile;
@@ -322,20 +396,36 @@ __global__ __launch_bounds__(kSortBlock) void embed_scatter_kernel(
     tok[k] = in[k] ? W.tok[src][t] : 0u;
   }
   const int digits = 1 << bits;
-  // thread d: digit d's total and its tokens in earlier tiles
-  uint32_t total = 0, mine = 0;
-  if (int(threadIdx.x) < digits) {
-    const uint32_t *h = W.hist + int64_t(threadIdx.x) * blocks;
-    for (int b = 0; b < blocks; ++b) {
-      if (b == int(blockIdx.x)) mine = total;
-      total += h[b];
-    }
-  }
-  const uint32_t first = block_exclusive(total, scratch);
-  tile_ranks(key, in, shift, bits, cnt, rank);
-  if (int(threadIdx.x) < digits) {
-    at[threadIdx.x] = first + mine;
-    wave_prefix(cnt, threadIdx.x);
+  // a digit's total and its tokens in earlier tiles
+  digit_starts<kTileThreads>(
+      digits,
+      [&](int d) {
+        const uint32_t *h = W.hist + int64_t(d) * blocks;
+        if (scanned) {
+          mine[d] = h[blockIdx.x];
+          return W.total[d];
+        }
+        uint32_t total = 0, m = 0;
+        constexpr int kAhead = 8;
+        for (int b0 = 0; b0 < blocks; b0 += kAhead) {
+          uint32_t n[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            n[u] = b0 + u < blocks ? h[b0 + u] : 0u;
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            if (b0 + u == int(blockIdx.x)) m = total;
+            total += n[u];
+          }
+        }
+        mine[d] = m;
+        return total;
+      },
+      at, scratch);
+  tile_ranks<kTileThreads>(key, in, shift, bits, cnt, rank);
+  for (int d = threadIdx.x; d < digits; d += kTileThreads) {
+    at[d] += mine[d];
+    wave_prefix<kTileThreads>(cnt, d);
   }
   __syncthreads();
   const int wave = threadIdx.x / kWave;
@@ -343,50 +433,61 @@ __global__ __launch_bounds__(kSortBlock) void embed_scatter_kernel(
   for (int k = 0; k < kRounds; ++k) {
     if (!in[k]) continue;
     const uint32_t d = (key[k] >> shift) & (digits - 1);
-    const uint32_t o = at[d] + cnt[d * kSortWaves + wave] + rank[k];
+    const uint32_t o = at[d] + cnt[d * kW + wave] + rank[k];
     W.key[src ^ 1][o] = key[k];
-    W.tok[src ^ 1][o] = tok[k];
+    if (last) {
+      W.srow[o] = W.row[tok[k]];
+      W.scoef[o] = W.coef[tok[k]];
+    } else {
+      W.tok[src ^ 1][o] = tok[k];
+    }
   }
 }
 
-// Keys and sort of one tile's tokens in one launch, through LDS.
-__global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(
+// Keys and sort of one workgroup's tokens in one launch, through LDS.
+__global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
     Parts P, Sort W, int src, int64_t tokens, uint32_t vocab, int passes,
     int bits) {
-  __shared__ __attribute__((aligned(16)))
-  uint16_t cnt[kSortWaves << kMaxDigit];
+  constexpr int kW = kOneThreads / kWave;
+  __shared__ __attribute__((aligned(16))) uint16_t cnt[kW << kMaxDigit];
   __shared__ uint32_t at[1 << kMaxDigit];
-  __shared__ uint32_t scratch[kSortWaves];
-  __shared__ uint32_t skey[kTile], stok[kTile];
+  __shared__ uint32_t scratch[kW];
+  __shared__ uint32_t skey[kOneTile];
+  __shared__ uint16_t stok[kOneTile];
+  __shared__ const char *srow[kOneTile];
+  __shared__ float scoef[kOneTile];
   uint32_t key[kRounds], tok[kRounds], rank[kRounds];
   bool in[kRounds];
   const int wave = threadIdx.x / kWave;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const int64_t t = tile_token(0, k);
+    const int t = int(tile_token(0, k));
     in[k] = t < tokens;
     key[k] = tok[k] = 0u;
-    if (in[k]) {
-      key[k] = P.n > 0 ? token_key(P, W, uint32_t(t), vocab) : W.key[0][t];
-      tok[k] = uint32_t(t);
+    if (!in[k]) continue;
+    tok[k] = uint32_t(t);
+    if (P.n > 0) {
+      key[k] = token_key(P, uint32_t(t), vocab, srow[t], scoef[t]);
+    } else {
+      key[k] = W.key[0][t];
+      srow[t] = W.row[t];
+      scoef[t] = W.coef[t];
     }
   }
   const int digits = 1 << bits;
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
-    tile_ranks(key, in, shift, bits, cnt, rank);
-    const uint32_t total =
-        int(threadIdx.x) < digits ? wave_prefix(cnt, threadIdx.x) : 0u;
-    const uint32_t first = block_exclusive(total, scratch);
-    if (int(threadIdx.x) < digits) at[threadIdx.x] = first;
-    __syncthreads();
+    tile_ranks<kOneThreads>(key, in, shift, bits, cnt, rank);
+    digit_starts<kOneThreads>(
+        digits, [&](int d) { return wave_prefix<kOneThreads>(cnt, d); }, at,
+        scratch);
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {
       if (!in[k]) continue;
       const uint32_t d = (key[k] >> shift) & (digits - 1);
-      const uint32_t o = at[d] + cnt[d * kSortWaves + wave] + rank[k];
+      const uint32_t o = at[d] + cnt[d * kW + wave] + rank[k];
       skey[o] = key[k];
-      stok[o] = tok[k];
+      stok[o] = uint16_t(tok[k]);
     }
     __syncthreads();
 #pragma unroll
@@ -403,7 +504,8 @@ __global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(
     const int64_t t = tile_token(0, k);
     if (in[k]) {
       W.key[src][t] = key[k];
-      W.tok[src][t] = tok[k];
+      W.srow[t] = srow[tok[k]];
+      W.scoef[t] = scoef[tok[k]];
     }
   }
 }
@@ -414,7 +516,7 @@ struct Out {
   int64_t row_bytes, dim, vocab, tokens;
   int chunk, slices, accumulate;
   int64_t chunks;
-  const uint32_t *key, *tok;
+  const uint32_t *key;
 };
 
 // first position in key[lo, hi) with key >= x, by the whole wave: 64 probes
@@ -494,11 +596,8 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
   float coef = 0.0f;
   if (lane < cnt) {
     k = O.key[p0 + lane];
-    if (k != none) {
-      const uint32_t t = O.tok[p0 + lane];
-      row = W.row[t];
-      coef = W.coef[t];
-    }
+    row = W.srow[p0 + lane];
+    coef = W.scoef[p0 + lane];
   }
   // padding sorts last
   const int valid = __popcll(__ballot(k != none));
@@ -510,9 +609,9 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
   bool head = __builtin_amdgcn_readlane(k, 0) == prev;
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 16;
   for (int i0 = 0; i0 < valid; i0 += kAhead) {
-    float v[kAhead][VEC];
+    typename Raw<GT, VEC>::type raw[kAhead] = {};
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u < valid ? i0 + u : valid - 1;
@@ -521,9 +620,7 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
       const uint32_t ahi = __builtin_amdgcn_readlane(uint32_t(a >> 32), i);
       const char *src =
           reinterpret_cast<const char *>((uint64_t(ahi) << 32) | alo);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[u][e] = 0.0f;
-      if (mine) load_vec<GT, VEC>(src + c * kGE, v[u]);
+      if (mine) raw[u] = load_raw<GT, VEC>(src + c * kGE);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -531,8 +628,10 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
       if (i >= valid) break;
       const float w =
           __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(coef), i));
+      float v[VEC];
+      widen<GT, VEC>(raw[u], v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] = __builtin_fmaf(v[u][e], w, acc[e]);
+      for (int e = 0; e < VEC; ++e) acc[e] = __builtin_fmaf(v[e], w, acc[e]);
       const uint32_t key = __builtin_amdgcn_readlane(k, i);
       const uint32_t after =
           i + 1 < valid ? __builtin_amdgcn_readlane(k, i + 1) : next;
@@ -645,7 +744,7 @@ int chunk_tokens(int64_t tokens, int64_t dim) {
 struct Sizes {
   int64_t tokens, dim, chunk, chunks, blocks;
   int bits, passes, digit;
-  size_t key, row, coef, hist, partial, total;
+  size_t key, row, coef, hist, digits, partial, total;
 };
 
 Sizes sizes_of(int64_t tokens, int64_t dim, int64_t vocab) {
@@ -665,7 +764,9 @@ Sizes sizes_of(int64_t tokens, int64_t dim, int64_t vocab) {
   Z.coef = up(4 * tokens);
   Z.hist = up(size_t(4) * Z.blocks << Z.digit);
   Z.partial = Z.chunks > 1 ? up(size_t(8) * Z.chunks * dim) : 0;
-  Z.total = 4 * Z.key + Z.row + Z.coef + Z.hist + Z.partial;
+  Z.digits = up(size_t(4) << Z.digit);
+  Z.total = 4 * Z.key + 2 * Z.row + 2 * Z.coef + Z.hist + Z.digits +
+            Z.partial;
   return Z;
 }
 
@@ -788,8 +889,11 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
       W.tok[i] = reinterpret_cast<uint32_t *>(take(Z.key));
     }
     W.row = reinterpret_cast<const char **>(take(Z.row));
+    W.srow = reinterpret_cast<const char **>(take(Z.row));
     W.coef = reinterpret_cast<float *>(take(Z.coef));
+    W.scoef = reinterpret_cast<float *>(take(Z.coef));
     W.hist = reinterpret_cast<uint32_t *>(take(Z.hist));
+    W.total = reinterpret_cast<uint32_t *>(take(Z.digits));
     W.partial = reinterpret_cast<float *>(take(Z.partial));
   }
   // the parts that hold tokens, up to kMaxParts at a time
@@ -819,19 +923,25 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
     }
   }
   int src = 0;
-  if (tokens > 0 && tokens <= kTile) {
+  if (tokens > 0 && tokens <= kOneTile) {
     src = 1;
-    hipLaunchKernelGGL(embed_sort_kernel, dim3(1), dim3(kSortBlock), 0, s, P,
+    hipLaunchKernelGGL(embed_sort_kernel, dim3(1), dim3(kOneThreads), 0, s, P,
                        W, src, tokens, uint32_t(vocab), Z.passes, Z.digit);
   } else if (tokens > 0) {
+    const int scanned = Z.blocks > kSumBlocks;
     for (int p = 0; p < Z.passes; ++p, src ^= 1) {
-      hipLaunchKernelGGL(embed_hist_kernel, dim3(Z.blocks), dim3(kSortBlock),
-                         0, s, P, W, src, tokens, uint32_t(vocab),
-                         p * Z.digit, Z.digit, int(Z.blocks));
+      hipLaunchKernelGGL(embed_hist_kernel, dim3(Z.blocks),
+                         dim3(kTileThreads), 0, s, P, W, src, tokens,
+                         uint32_t(vocab), p * Z.digit, Z.digit,
+                         int(Z.blocks));
       P.n = 0;  // the keys are there
+      if (scanned)
+        hipLaunchKernelGGL(embed_scan_kernel, dim3(1 << Z.digit),
+                           dim3(kTileThreads), 0, s, W, int(Z.blocks));
       hipLaunchKernelGGL(embed_scatter_kernel, dim3(Z.blocks),
-                         dim3(kSortBlock), 0, s, W, src, tokens, p * Z.digit,
-                         Z.digit, int(Z.blocks));
+                         dim3(kTileThreads), 0, s, W, src, tokens,
+                         p * Z.digit, Z.digit, int(Z.blocks), scanned,
+                         int(p + 1 == Z.passes));
     }
   }
   Out O;
@@ -844,7 +954,6 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   O.chunks = Z.chunks;
   O.accumulate = accumulate;
   O.key = W.key[src];
-  O.tok = W.tok[src];
   const int v = vec ? vec_elems : 1;
   O.slices = int((dim + int64_t(kWave) * v - 1) / (int64_t(kWave) * v));
   const int64_t sum_blocks = (Z.chunks * O.slices + kWaves - 1) / kWaves;

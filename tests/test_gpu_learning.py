@@ -410,7 +410,8 @@ def _check_grad(got, ids, grad, vocab, weights=None, scale=1.0, base=None):
 @pytest.mark.parametrize('tokens,vocab,dim', [
     (1, 1, 1), (1, 9, 8), (5, 3, 4), (31, 40, 300), (32, 7, 16), (33, 1, 5),
     (64, 1000, 129), (65, 64, 64), (700, 50, 40), (4096, 300, 24),
-    (4097, 2000, 9), (9000, 5, 17), (20000, 70000, 8), (6000, 1100000, 4)])
+    (4097, 2000, 9), (9000, 5, 17), (20000, 70000, 8), (6000, 1100000, 4),
+    (140001, 900, 4)])
 def test_embedding_grad(tokens, vocab, dim, dtype):
     from federatedscope_amd import ops
     ids = _ids(tokens, vocab, tokens)
@@ -426,13 +427,15 @@ def test_embedding_grad(tokens, vocab, dim, dtype):
     _check_grad(out, [ids], [grad], vocab, scale=0.5, base=base)
 
 
-@pytest.mark.parametrize('parts', [1, 3, 64, 65, 150])
-def test_embedding_grad_of_many_clients(parts):
+@pytest.mark.parametrize('parts,most', [(1, 90), (3, 90), (64, 90), (65, 90),
+                                        (112, 90), (113, 90), (150, 90),
+                                        (150, 20), (300, 5)])
+def test_embedding_grad_of_many_clients(parts, most):
     """Uneven clients (some empty), int32 and int64 tokens, weights, a
     float32 table of bfloat16 rows."""
     from federatedscope_amd import ops
     vocab, dim = 500, 48
-    ids = [_ids((i * 37) % 90, vocab, i, dtype=torch.int64 if i % 2 else
+    ids = [_ids((i * 37) % most, vocab, i, dtype=torch.int64 if i % 2 else
                 torch.int32) for i in range(parts)]
     grad = [torch.randn(len(i), dim, device='cuda').bfloat16() for i in ids]
     w = [(1 + i % 5) / 7 for i in range(parts)]
