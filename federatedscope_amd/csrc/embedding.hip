@@ -22,10 +22,6 @@
 
 #include <hip/hip_fp16.h>
 
-#ifndef EM_WAVES
-#define EM_WAVES 2048
-#define EM_SB 8
-#endif
 namespace fsagg {
 namespace {
 
@@ -38,7 +34,8 @@ constexpr int kMaxParts = 112;    // parts per key launch (kernel arguments)
 constexpr int kRounds = 4;
 constexpr int kOneThreads = 1024, kOneTile = kOneThreads * kRounds;
 constexpr int kTileThreads = 256, kTile = kTileThreads * kRounds;
-constexpr int kSumBlocks = EM_SB;   // tiles whose counts a tile adds up itself
+constexpr int kSumBlocks = 8;     // tiles whose counts a tile adds up itself
+constexpr int kFew = kBlock;      // tokens that every workgroup sorts itself
 constexpr int kMaxDigit = 10;     // bits per radix pass
 // a launch counts its work items in 32 bits
 constexpr int64_t kMaxGrid = (int64_t(1) << 32) / kBlock - 1;
@@ -195,13 +192,14 @@ struct Sort {
 
 // Key of token t: its row, or V for padding; and its row of values and
 // factor.
-__device__ __forceinline__ uint32_t token_key(const Parts &P, uint32_t t,
-                                              uint32_t vocab,
+__device__ __forceinline__ uint32_t token_key(const Parts &P,
+                                              const uint32_t *starts,
+                                              uint32_t t, uint32_t vocab,
                                               const char *&row, float &coef) {
   int lo = 0, hi = P.n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (P.part[mid].start <= t) lo = mid;
+    if (starts[mid] <= t) lo = mid;
     else hi = mid;
   }
   const Part &p = P.part[lo];
@@ -212,11 +210,19 @@ __device__ __forceinline__ uint32_t token_key(const Parts &P, uint32_t t,
   return id >= 0 && id < int64_t(vocab) ? uint32_t(id) : vocab;
 }
 
-__device__ __forceinline__ uint32_t note_token(const Parts &P, const Sort &W,
-                                               uint32_t t, uint32_t vocab) {
+// The parts' first tokens, for token_key, in LDS (the caller synchronises).
+__device__ __forceinline__ void stage_starts(const Parts &P,
+                                             uint32_t *starts) {
+  if (int(threadIdx.x) < P.n) starts[threadIdx.x] = P.part[threadIdx.x].start;
+}
+
+__device__ __forceinline__ uint32_t note_token(const Parts &P,
+                                               const uint32_t *starts,
+                                               const Sort &W, uint32_t t,
+                                               uint32_t vocab) {
   const char *row;
   float coef;
-  const uint32_t key = token_key(P, t, vocab, row, coef);
+  const uint32_t key = token_key(P, starts, t, vocab, row, coef);
   W.key[0][t] = key;
   W.tok[0][t] = t;
   W.row[t] = row;
@@ -227,10 +233,13 @@ __device__ __forceinline__ uint32_t note_token(const Parts &P, const Sort &W,
 // Keys of these parts' tokens (a call of more parts than fit one launch).
 __global__ __launch_bounds__(kBlock) void embed_key_kernel(Parts P, Sort W,
                                                            uint32_t vocab) {
+  __shared__ uint32_t starts[kMaxParts];
+  stage_starts(P, starts);
+  __syncthreads();
   for (int64_t t = int64_t(P.part[0].start) +
                    int64_t(blockIdx.x) * kBlock + threadIdx.x;
        t < P.end; t += int64_t(gridDim.x) * kBlock)
-    note_token(P, W, uint32_t(t), vocab);
+    note_token(P, starts, W, uint32_t(t), vocab);
 }
 
 // token k of this thread's rounds in the tile at `base`: wave w owns tokens
@@ -328,16 +337,19 @@ __global__ __launch_bounds__(kTileThreads) void embed_hist_kernel(
     Parts P, Sort W, int src, int64_t tokens, uint32_t vocab, int shift,
     int bits, int blocks) {
   __shared__ uint32_t h[1 << kMaxDigit];
+  __shared__ uint32_t starts[kMaxParts];
   const int digits = 1 << bits;
   for (int i = threadIdx.x; i < digits; i += kTileThreads) h[i] = 0;
+  stage_starts(P, starts);
   __syncthreads();
   const int64_t base = int64_t(blockIdx.x) * kTile;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
     const int64_t t = tile_token(base, k);
     if (t >= tokens) continue;
-    const uint32_t key = P.n > 0 ? note_token(P, W, uint32_t(t), vocab)
-                                 : W.key[src][t];
+    const uint32_t key = P.n > 0
+                             ? note_token(P, starts, W, uint32_t(t), vocab)
+                             : W.key[src][t];
     atomicAdd(&h[(key >> shift) & (digits - 1)], 1u);
   }
   __syncthreads();
@@ -456,6 +468,9 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
   __shared__ uint16_t stok[kOneTile];
   __shared__ const char *srow[kOneTile];
   __shared__ float scoef[kOneTile];
+  __shared__ uint32_t starts[kMaxParts];
+  stage_starts(P, starts);
+  __syncthreads();
   uint32_t key[kRounds], tok[kRounds], rank[kRounds];
   bool in[kRounds];
   const int wave = threadIdx.x / kWave;
@@ -467,7 +482,8 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
     if (!in[k]) continue;
     tok[k] = uint32_t(t);
     if (P.n > 0) {
-      key[k] = token_key(P, uint32_t(t), vocab, srow[t], scoef[t]);
+      key[k] =
+          token_key(P, starts, uint32_t(t), vocab, srow[t], scoef[t]);
     } else {
       key[k] = W.key[0][t];
       srow[t] = W.row[t];
@@ -518,6 +534,12 @@ struct Out {
   int64_t chunks;
   const uint32_t *key;
 };
+
+// lanes from the first on that say yes
+__device__ __forceinline__ int run_length(bool yes) {
+  const uint64_t m = __ballot(yes);
+  return m == ~0ull ? kWave : __builtin_ctzll(~m);
+}
 
 // first position in key[lo, hi) with key >= x, by the whole wave: 64 probes
 // a round
@@ -659,6 +681,103 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
   }
 }
 
+// A call of few tokens, in one launch: every workgroup sorts them itself (a
+// token's place is the number of tokens that come before it), then a wave
+// adds up one row's tokens in one slice of columns; workgroups past those
+// write the zero rows.
+template <int GT, int OT, int VEC>
+__global__ __launch_bounds__(kBlock) void embed_few_kernel(Parts P, Out O,
+                                                           int sum_blocks,
+                                                           int zero_rows) {
+  constexpr int kGE = sizeof(typename Elem<GT>::type);
+  constexpr int kOE = sizeof(typename Elem<OT>::type);
+  __shared__ uint32_t starts[kMaxParts];
+  __shared__ uint32_t key[kFew], skey[kFew];
+  __shared__ const char *srow[kFew];
+  __shared__ float scoef[kFew];
+  __shared__ uint8_t named[kZeroRows];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave =
+      __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int tokens = int(O.tokens), t = threadIdx.x;
+  const uint32_t none = uint32_t(O.vocab);
+  stage_starts(P, starts);
+  named[t] = 0;
+  __syncthreads();
+  const char *row = nullptr;
+  float coef = 0.0f;
+  uint32_t k = ~0u;
+  if (t < tokens) k = token_key(P, starts, uint32_t(t), none, row, coef);
+  key[t] = k;
+  __syncthreads();
+  if (int(blockIdx.x) >= sum_blocks) {
+    const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * zero_rows;
+    const int64_t r1 = r0 + zero_rows < O.vocab ? r0 + zero_rows : O.vocab;
+    if (t < tokens && int64_t(k) >= r0 && int64_t(k) < r1) named[k - r0] = 1;
+    __syncthreads();
+    for (int64_t r = r0 + wave; r < r1; r += kWaves) {
+      if (named[r - r0]) continue;
+      char *dst = O.out + r * O.row_bytes;
+      const float z[VEC] = {};
+      for (int64_t c = int64_t(lane) * VEC; c < O.dim; c += kWave * VEC)
+        store_vec<OT, VEC>(dst + c * kOE, z);
+    }
+    return;
+  }
+  if (t < tokens) {
+    int place = 0;
+    for (int j = 0; j < tokens; ++j)
+      place += key[j] < k || (key[j] == k && j < t);
+    skey[place] = k;
+    srow[place] = row;
+    scoef[place] = coef;
+  }
+  __syncthreads();
+  const int64_t unit = int64_t(blockIdx.x) * kWaves + wave;
+  const int p = int(unit / O.slices);
+  if (p >= tokens) return;
+  const uint32_t mine = skey[p];
+  if (mine == none || (p > 0 && skey[p - 1] == mine)) return;
+  int end = p;
+  for (;;) {
+    const int q = end + lane;
+    const int n = run_length(q < tokens && skey[q] == mine);
+    end += n;
+    if (n < kWave) break;
+  }
+  const int64_t c = ((unit % O.slices) * kWave + lane) * VEC;
+  if (c >= O.dim) return;
+  float acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+  constexpr int kAhead = 8;
+  for (int i0 = p; i0 < end; i0 += kAhead) {
+    typename Raw<GT, VEC>::type raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      raw[u] = load_raw<GT, VEC>(srow[i0 + u < end ? i0 + u : end - 1] +
+                                 c * kGE);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (i0 + u < end) {
+        const float w = scoef[i0 + u];
+        float v[VEC];
+        widen<GT, VEC>(raw[u], v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          acc[e] = __builtin_fmaf(v[e], w, acc[e]);
+      }
+  }
+  char *dst = O.out + int64_t(mine) * O.row_bytes + c * kOE;
+  if (O.accumulate) {
+    float o[VEC];
+    load_vec<OT, VEC>(dst, o);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = __fadd_rn(o[e], acc[e]);
+  }
+  store_vec<OT, VEC>(dst, acc);
+}
+
 // Rows whose tokens cross chunks: the wave of the chunk in which the row
 // begins adds the later chunks' partial sums in order.
 template <int OT, int VEC>
@@ -683,9 +802,7 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(Out O, Sort W) {
   int64_t last = chunk;
   for (;;) {
     const int64_t q = last + 1 + lane;
-    const uint64_t same =
-        __ballot(q < O.chunks && O.key[q * O.chunk] == key);
-    const int n = same == ~0ull ? kWave : __builtin_ctzll(~same);
+    const int n = run_length(q < O.chunks && O.key[q * O.chunk] == key);
     last += n;
     if (n < kWave) break;
   }
@@ -733,11 +850,11 @@ void with_dtype(int dt, F f) {
 
 // Tokens per chunk: long chunks leave fewer partial sums, short ones make
 // enough waves where tokens are few.
+constexpr int64_t kManyWaves = 2048;
 int chunk_tokens(int64_t tokens, int64_t dim) {
-  if (tokens <= kWave) return kWave;  // one chunk, no join
   const int64_t slices = (dim + 511) / 512;
   int chunk = kWave;
-  while (chunk > 8 && tokens * slices < int64_t(chunk) * EM_WAVES) chunk /= 2;
+  while (chunk > 8 && tokens * slices < int64_t(chunk) * kManyWaves) chunk /= 2;
   return chunk;
 }
 
@@ -922,12 +1039,57 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
       P.n = 0;
     }
   }
+  Out O;
+  O.out = static_cast<char *>(out);
+  O.row_bytes = out_stride * oe;
+  O.dim = dim;
+  O.vocab = vocab;
+  O.tokens = tokens;
+  O.chunk = int(Z.chunk);
+  O.chunks = Z.chunks;
+  O.accumulate = accumulate;
+  const int v = vec ? vec_elems : 1;
+  O.slices = int((dim + int64_t(kWave) * v - 1) / (int64_t(kWave) * v));
+  const bool few = tokens <= kFew && one_launch;
+  const int64_t sum_units = few ? tokens : Z.chunks;
+  const int64_t sum_blocks = (sum_units * O.slices + kWaves - 1) / kWaves;
+  // rows per zero workgroup: about 64 KiB
+  int64_t zero_rows = 65536 / (dim * oe);
+  if (zero_rows < kWaves) zero_rows = kWaves;
+  if (zero_rows > kZeroRows) zero_rows = kZeroRows;
+  const int64_t zero_blocks =
+      accumulate ? 0 : (vocab + zero_rows - 1) / zero_rows;
+  const int64_t join_blocks =
+      Z.chunks > 1 && !few
+          ? ((Z.chunks - 1) * O.slices + kWaves - 1) / kWaves
+          : 0;
+  if (sum_blocks + zero_blocks > kMaxGrid) {
+    set_error("%s: %lld tokens of %lld columns are too many for one call",
+              what, (long long)tokens, (long long)dim);
+    return FSAGG_EINVAL;
+  }
+  if (few) {
+    with_dtype(dtype, [&](auto gt) {
+      with_dtype(out_dtype, [&](auto ot) {
+        constexpr int D = decltype(gt)::value, Q = decltype(ot)::value;
+        const dim3 grid(unsigned(sum_blocks + zero_blocks)), block(kBlock);
+        if (vec)
+          hipLaunchKernelGGL((embed_few_kernel<D, Q, Elem<D>::kVec>), grid,
+                             block, 0, s, P, O, int(sum_blocks),
+                             int(zero_rows));
+        else
+          hipLaunchKernelGGL((embed_few_kernel<D, Q, 1>), grid, block, 0, s,
+                             P, O, int(sum_blocks), int(zero_rows));
+      });
+    });
+    return check_launch(what);
+  }
   int src = 0;
-  if (tokens > 0 && tokens <= kOneTile) {
+  if (tokens <= kOneTile) {
     src = 1;
     hipLaunchKernelGGL(embed_sort_kernel, dim3(1), dim3(kOneThreads), 0, s, P,
                        W, src, tokens, uint32_t(vocab), Z.passes, Z.digit);
-  } else if (tokens > 0) {
+  } else {
     const int scanned = Z.blocks > kSumBlocks;
     for (int p = 0; p < Z.passes; ++p, src ^= 1) {
       hipLaunchKernelGGL(embed_hist_kernel, dim3(Z.blocks),
@@ -944,32 +1106,7 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
                          int(p + 1 == Z.passes));
     }
   }
-  Out O;
-  O.out = static_cast<char *>(out);
-  O.row_bytes = out_stride * oe;
-  O.dim = dim;
-  O.vocab = vocab;
-  O.tokens = tokens;
-  O.chunk = int(Z.chunk);
-  O.chunks = Z.chunks;
-  O.accumulate = accumulate;
   O.key = W.key[src];
-  const int v = vec ? vec_elems : 1;
-  O.slices = int((dim + int64_t(kWave) * v - 1) / (int64_t(kWave) * v));
-  const int64_t sum_blocks = (Z.chunks * O.slices + kWaves - 1) / kWaves;
-  // rows per zero workgroup: about 64 KiB
-  int64_t zero_rows = 65536 / (dim * oe);
-  if (zero_rows < kWaves) zero_rows = kWaves;
-  if (zero_rows > kZeroRows) zero_rows = kZeroRows;
-  const int64_t zero_blocks =
-      accumulate ? 0 : (vocab + zero_rows - 1) / zero_rows;
-  const int64_t join_blocks =
-      Z.chunks > 1 ? ((Z.chunks - 1) * O.slices + kWaves - 1) / kWaves : 0;
-  if (sum_blocks + zero_blocks > kMaxGrid) {
-    set_error("%s: %lld tokens of %lld columns are too many for one call",
-              what, (long long)tokens, (long long)dim);
-    return FSAGG_EINVAL;
-  }
   with_dtype(dtype, [&](auto gt) {
     with_dtype(out_dtype, [&](auto ot) {
       constexpr int D = decltype(gt)::value, Q = decltype(ot)::value;

@@ -409,7 +409,8 @@ def _check_grad(got, ids, grad, vocab, weights=None, scale=1.0, base=None):
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('tokens,vocab,dim', [
     (1, 1, 1), (1, 9, 8), (5, 3, 4), (31, 40, 300), (32, 7, 16), (33, 1, 5),
-    (64, 1000, 129), (65, 64, 64), (700, 50, 40), (4096, 300, 24),
+    (64, 1000, 129), (65, 64, 64), (255, 1, 6), (256, 3, 260),
+    (257, 90, 33), (700, 50, 40), (4096, 300, 24),
     (4097, 2000, 9), (9000, 5, 17), (20000, 70000, 8), (6000, 1100000, 4),
     (140001, 900, 4)])
 def test_embedding_grad(tokens, vocab, dim, dtype):
