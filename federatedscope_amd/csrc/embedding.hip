@@ -314,32 +314,39 @@ __device__ __forceinline__ uint32_t wave_prefix(uint16_t *cnt, int d) {
   return total;
 }
 
-// Exclusive sums over digits: at[d] = v(0) + .. + v(d - 1), v by thread
-// (digit d = c TH + thread; 1 << kMaxDigit digits at most).
+// Exclusive sums over digits: at[d] = v(0) + .. + v(d - 1), 1 << kMaxDigit
+// digits at most.  A thread has neighbouring digits, so that their counts
+// are read together and one scan does.
 template <int TH, typename F>
 __device__ __forceinline__ void digit_starts(int digits, F v, uint32_t *at,
                                              uint32_t *scratch) {
+  constexpr int kEach = (1 << kMaxDigit) / TH;
+  static_assert(kEach * TH == 1 << kMaxDigit, "digits divide over threads");
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  uint32_t before = 0;
-  for (int c = 0; c < digits; c += TH) {
-    const int d = c + int(threadIdx.x);
-    const uint32_t n = d < digits ? v(d) : 0u;
-    uint32_t s = n;
+  const int each = (digits + TH - 1) / TH;
+  const int d0 = int(threadIdx.x) * each;
+  uint32_t n[kEach], own = 0;
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const uint32_t u = __shfl_up(s, o);
-      if (lane >= o) s += u;
-    }
-    if (lane == kWave - 1) scratch[wave] = s;
-    __syncthreads();
-    uint32_t sum = before;
-    for (int w = 0; w < TH / kWave; ++w) {
-      if (w == wave && d < digits) at[d] = sum + s - n;
-      sum += scratch[w];
-    }
-    before = sum;
-    __syncthreads();
+  for (int i = 0; i < kEach; ++i)
+    n[i] = i < each && d0 + i < digits ? v(d0 + i) : 0u;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) own += n[i];
+  uint32_t s = own;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t u = __shfl_up(s, o);
+    if (lane >= o) s += u;
   }
+  if (lane == kWave - 1) scratch[wave] = s;
+  __syncthreads();
+  s -= own;
+  for (int w = 0; w < wave; ++w) s += scratch[w];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (i < each && d0 + i < digits) at[d0 + i] = s;
+    s += n[i];
+  }
+  __syncthreads();
 }
 
 // hist[digit][block], of the keys as they are (P.n = 0) or as they are made
@@ -552,28 +559,42 @@ __device__ __forceinline__ int run_length(bool yes) {
   return m == ~0ull ? kWave : __builtin_ctzll(~m);
 }
 
-// first position in key[lo, hi) with key >= x, by the whole wave: 64 probes
-// a round
-__device__ __forceinline__ int64_t wave_lower_bound(const uint32_t *key,
-                                                    int64_t lo, int64_t hi,
-                                                    uint32_t x) {
+// first positions a and b in key[0, n) with key >= x and key >= y, by the
+// whole wave: 64 probes a round for each, both on their way together
+__device__ __forceinline__ void wave_bounds(const uint32_t *key, int64_t n,
+                                            uint32_t x, uint32_t y,
+                                            int64_t &a, int64_t &b) {
   const int lane = threadIdx.x & (kWave - 1);
-  while (hi > lo) {
-    const int64_t step = (hi - lo + kWave - 1) / kWave;
-    const int64_t p = lo + lane * step;
-    // probes whose key is below x: all before the answer
-    const uint64_t below = __ballot(p < hi && key[p < hi ? p : hi - 1] < x);
-    const int c = __popcll(below);
-    if (c == 0) return lo;
-    const int64_t nlo = lo + (c - 1) * step + 1;
-    const int64_t nhi = lo + c * step;
-    hi = nhi < hi ? nhi : hi;
-    lo = nlo;
+  int64_t lo[2] = {0, 0}, hi[2] = {n, n};
+  while (lo[0] < hi[0] || lo[1] < hi[1]) {
+    int64_t step[2];
+    bool below[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      step[i] = (hi[i] - lo[i] + kWave - 1) / kWave;
+      const int64_t p = lo[i] + lane * step[i];
+      below[i] = false;
+      if (p < hi[i]) below[i] = key[p] < (i ? y : x);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // probes whose key is below: all before the answer
+      const int c = __popcll(__ballot(below[i]));
+      if (c == 0) {
+        hi[i] = lo[i];
+        continue;
+      }
+      const int64_t nhi = lo[i] + c * step[i];
+      lo[i] += (c - 1) * step[i] + 1;
+      hi[i] = nhi < hi[i] ? nhi : hi[i];
+    }
   }
-  return lo;
+  a = lo[0];
+  b = lo[1];
 }
 
 constexpr int kZeroRows = kBlock;  // most rows of a zero workgroup
+constexpr int64_t kScanKeys = 32 * kBlock;
 
 // Row sums of one chunk of sorted tokens and one slice of columns per wave;
 // workgroups past those write the zero rows that no token names.
@@ -587,14 +608,27 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
   const int wave =
       __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   if (int(blockIdx.x) >= sum_blocks) {
-    // the rows of this stretch that a token names: one search per thread,
-    // inside the stretch's own tokens
+    // the rows of this stretch that a token names, from the stretch's own
+    // tokens: all of them where they are few, else one search per thread
     __shared__ uint8_t named[kZeroRows];
     const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * zero_rows;
     const int64_t r1 = r0 + zero_rows < O.vocab ? r0 + zero_rows : O.vocab;
-    const int64_t a = wave_lower_bound(O.key, 0, O.tokens, uint32_t(r0));
-    const int64_t b = wave_lower_bound(O.key, a, O.tokens, uint32_t(r1));
-    if (r0 + int64_t(threadIdx.x) < r1) {
+    int64_t a, b;
+    wave_bounds(O.key, O.tokens, uint32_t(r0), uint32_t(r1), a, b);
+    named[threadIdx.x] = 0;
+    __syncthreads();
+    if (b - a <= kScanKeys) {
+      constexpr int kAhead = 8;
+      for (int64_t i0 = a + threadIdx.x; i0 < b; i0 += kAhead * kBlock) {
+        uint32_t r[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          r[u] = i0 + u * kBlock < b ? O.key[i0 + u * kBlock] : 0u;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (i0 + u * kBlock < b) named[r[u] - uint32_t(r0)] = 1;
+      }
+    } else if (r0 + int64_t(threadIdx.x) < r1) {
       const uint32_t r = uint32_t(r0) + threadIdx.x;
       int64_t lo = a, hi = b;
       while (lo < hi) {

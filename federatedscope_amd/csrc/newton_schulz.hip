@@ -24,6 +24,7 @@
 
 #include <cmath>
 #include <initializer_list>
+#include <type_traits>
 
 namespace fsagg {
 namespace {
@@ -1257,11 +1258,14 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
 
 // -- host --------------------------------------------------------------------
 // Tiles: 256 x 256 keeps a CU's matrix cores at about 80 % of what a large
-// library product reaches, where there is work for all of them; 64 x 64 is
-// for matrices too small for that, where a tile's latency counts.  One limb
-// suffices for a bf16 result (below).
+// library product reaches, where there is work for all of them; 128 x 128,
+// two workgroups to a CU, takes products that leave the last round of those
+// too empty (below); 64 x 64 is for matrices too small for that, where a
+// tile's latency counts.  One limb suffices for a bf16 result (below).
 using BigTile = Tile<256, 256, 128, 64, 2, 2>;
 using BigTile1 = Tile<256, 256, 128, 64, 4, 1>;
+using HalfTile = Tile<128, 128, 64, 64, 2, 2>;
+using HalfTile1 = Tile<128, 128, 64, 64, 4, 1>;
 using MidTile = Tile<64, 64, 32, 32, 4, 2>;
 constexpr int kBigWorkers = 256;   // one workgroup of a big tile per CU
 constexpr int kMidWorkers = 512;
@@ -1414,32 +1418,33 @@ struct Step {
   hipStream_t stream;
 };
 
-// One product of the whole group: one workgroup per tile, or the line of
-// stages shared by as many workgroups as the GPU holds, each with at least
-// kMinStages of them.  Sharing saves the stages that the last round of whole
-// tiles (or the longest tile, where there are fewer tiles than workgroups)
-// leaves idle, and costs a join: parts written and read again, about
-// kJoinStages stages' time with either tile.
-constexpr int kMinStages = 8, kJoinStages = 16;
-template <class T, int MODE>
-void launch_product(Group &G, int workers, float *partial, int src,
-                    const Step &st) {
+// The tiles of a group's product, its stages, and those of the longest tile.
+struct Count {
   int64_t tiles = 0, stages = 0;
+  int longest = 0;
+  // stages that the busiest of `workers` places works, a tile to a workgroup
+  int64_t whole(int workers) const {
+    const int64_t rounds = (tiles + workers - 1) / workers;
+    const int64_t s = rounds * (stages / tiles);
+    return s > longest ? s : longest;
+  }
+};
+template <class T, int MODE>
+Count count_tiles(const Group &G) {
+  Count c;
   for (int i = 0; i < G.nmat; ++i) {
     const Mat &M = G.mat[i];
     const int64_t t = int64_t(M.batch) * mode_tiles<MODE, T::kBM, T::kBN>(M);
-    tiles += t;
-    stages += t * mode_stages<MODE>(M);
+    c.tiles += t;
+    c.stages += t * mode_stages<MODE>(M);
+    if (mode_stages<MODE>(M) > c.longest) c.longest = mode_stages<MODE>(M);
   }
-  int64_t w = stages / kMinStages;
-  if (w > workers) w = workers;
-  if (w < 1) w = 1;
-  const int64_t rounds = (tiles + workers - 1) / workers;
-  const bool share = rounds * (stages / tiles) - stages / w > kJoinStages;
-  Line L;
-  L.workers = int(w);
-  L.partial = partial;
-  L.total = int(stages);
+  return c;
+}
+
+// Sets the entries' first workgroups (a workgroup per tile) or first stages.
+template <class T, int MODE>
+int place_tiles(Group &G, bool share) {
   int total = 0;
   for (int i = 0; i < G.nmat; ++i) {
     const Mat &M = G.mat[i];
@@ -1448,12 +1453,52 @@ void launch_product(Group &G, int workers, float *partial, int src,
              (share ? mode_stages<MODE>(M) : 1);
   }
   G.start[G.nmat] = total;
+  return total;
+}
+
+template <class T, int MODE>
+void launch_whole(Group &G, int src, const Step &st) {
+  const int total = place_tiles<T, MODE>(G, false);
+  hipLaunchKernelGGL((ns_gemm_kernel<T, MODE>), dim3(total),
+                     dim3(T::kThreads), 0, st.stream, G, src, st.a, st.b,
+                     st.c, st.S);
+}
+
+// One product of the whole group: one workgroup per tile, or the line of
+// stages shared by as many workgroups as the GPU holds, each with at least
+// kMinStages of them.  Sharing saves the stages that the last round of whole
+// tiles (or the longest tile, where there are fewer tiles than workgroups)
+// leaves idle, and costs a join: parts written and read again, about
+// kJoinStages stages' time with either tile.
+constexpr int kMinStages = 8, kJoinStages = 16, kTileEnd = 9;
+template <class T, int MODE, class H = void>
+void launch_product(Group &G, int workers, float *partial, int src,
+                    const Step &st) {
+  const Count n = count_tiles<T, MODE>(G);
+  int64_t w = n.stages / kMinStages;
+  if (w > workers) w = workers;
+  if (w < 1) w = 1;
+  const bool share = n.whole(workers) - n.stages / w > kJoinStages;
+  if constexpr (!std::is_void<H>::value) {
+    // A stage of half the tile, two workgroups to a CU, takes 1/1.8 of the
+    // time of one (2.9 -> 1.6 us, two limbs), a tile's end about 9 stages
+    // with either.
+    const int64_t mine = share ? n.stages / w + kJoinStages
+                               : n.whole(workers) + kTileEnd;
+    const Count m = count_tiles<H, MODE>(G);
+    if (m.whole(2 * workers) + kTileEnd < mine * 9 / 5) {
+      launch_whole<H, MODE>(G, src, st);
+      return;
+    }
+  }
   if (!share) {
-    hipLaunchKernelGGL((ns_gemm_kernel<T, MODE>), dim3(total),
-                       dim3(T::kThreads), 0, st.stream, G, src, st.a, st.b,
-                       st.c, st.S);
+    launch_whole<T, MODE>(G, src, st);
     return;
   }
+  Line L;
+  L.workers = int(w);
+  L.partial = partial;
+  L.total = place_tiles<T, MODE>(G, true);
   hipLaunchKernelGGL((ns_line_kernel<T, MODE>), dim3(L.workers),
                      dim3(T::kThreads), 0, st.stream, G, L, src, st.a, st.b,
                      st.c, st.S);
@@ -1462,7 +1507,7 @@ void launch_product(Group &G, int workers, float *partial, int src,
                      st.stream, G, L, src, st.a, st.b, st.c, st.S);
 }
 
-template <class T, bool MUON>
+template <class T, bool MUON, class H = void>
 void run_products(Group &G, int workers, float *partial, const Step &st) {
   int total = 0;
   for (int i = 0; i < G.nmat; ++i) {
@@ -1482,13 +1527,13 @@ void run_products(Group &G, int workers, float *partial, const Step &st) {
                      G, st.eps);
   int src = 0;
   for (int k = 0; k < st.steps; ++k, src ^= 1) {
-    launch_product<T, kGram>(G, workers, partial, src, st);
-    launch_product<T, kSquare>(G, workers, partial, src, st);
+    launch_product<T, kGram, H>(G, workers, partial, src, st);
+    launch_product<T, kSquare, H>(G, workers, partial, src, st);
     if (k + 1 < st.steps)
-      launch_product<T, kApply>(G, workers, partial, src, st);
+      launch_product<T, kApply, H>(G, workers, partial, src, st);
     else
-      launch_product<T, MUON ? kLastMuon : kLast>(G, workers, partial, src,
-                                                  st);
+      launch_product<T, MUON ? kLastMuon : kLast, H>(G, workers, partial, src,
+                                                     st);
   }
 }
 
@@ -1534,9 +1579,9 @@ void run_group(Group &G, Way way, float *partial, const Step &st) {
   else if (way == kMid)
     run_products<MidTile, MUON>(G, kMidWorkers, partial, st);
   else if (way == kBig)
-    run_products<BigTile, MUON>(G, kBigWorkers, partial, st);
+    run_products<BigTile, MUON, HalfTile>(G, kBigWorkers, partial, st);
   else if constexpr (!MUON)  // (a parameter is fp32)
-    run_products<BigTile1, MUON>(G, kBigWorkers, partial, st);
+    run_products<BigTile1, MUON, HalfTile1>(G, kBigWorkers, partial, st);
 }
 
 // f(group, way, bytes of its entries) for every group of entries, in turn;
