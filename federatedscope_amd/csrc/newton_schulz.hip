@@ -468,13 +468,14 @@ __device__ __forceinline__ void tile_of(const Mat &M, int t, int &ti,
 }
 
 // The stages of a group's product in one line: entry after entry, tile after
-// tile.  Workgroup q of `workers` takes stages [q, q + 1) * total / workers.
+// tile.  Each of `workers` workgroups takes `each` of them, the first `more`
+// one more (no division: in 64 bits it costs the join more than its sums).
 struct Line {
-  int total, workers;
+  int workers, each, more;
   float *partial;  // [workers][first, later][BM * BN]
 };
 __device__ __forceinline__ int line_at(const Line &L, int q) {
-  return int(int64_t(q) * L.total / L.workers);
+  return q * L.each + (q < L.more ? q : L.more);
 }
 
 // One tile of C = P R^T (k contiguous in both), from stage k0 to stage k1.  A
@@ -668,16 +669,13 @@ struct Tile {
               p)[((i * NJ + j) * 4 + q) * kThreads + threadIdx.x] = v;
         }
   }
-  static __device__ __forceinline__ void add_partial(f32x16 &x,
+  static __device__ __forceinline__ void get_partial(f32x4 (&v)[4],
                                                      const float *p,
                                                      int block) {
-    f32x4 v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       v[q] = reinterpret_cast<const f32x4 *>(
           p)[(block * 4 + q) * kThreads + threadIdx.x];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = __fadd_rn(x[r], v[r / 4][r % 4]);
   }
 
   template <int MODE, int DT>
@@ -884,12 +882,28 @@ __global__ __launch_bounds__(T::kThreads) void ns_join_kernel(
   f32x16 x;
 #pragma unroll
   for (int r = 0; r < 16; ++r) x[r] = 0.0f;
-  for (; w < L.workers && line_at(L, w) < first + stages; ++w)
-    if (line_at(L, w) < line_at(L, w + 1))
-      T::add_partial(x,
-                     L.partial + (int64_t(w) * 2 + (line_at(L, w) < first)) *
-                                     (T::kBM * T::kBN),
-                     block);
+  constexpr int kAhead = 4;
+  for (bool more = true; more; w += kAhead) {
+    f32x4 v[kAhead][4];
+    bool in[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      in[u] = w + u < L.workers && line_at(L, w + u) < first + stages;
+      if (in[u])
+        T::get_partial(v[u],
+                       L.partial + (int64_t(w + u) * 2 +
+                                    (line_at(L, w + u) < first)) *
+                                       (T::kBM * T::kBN),
+                       block);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (in[u]) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = __fadd_rn(x[r], v[u][r / 4][r % 4]);
+      }
+    more = in[kAhead - 1];
+  }
   const int z = t / tiles;
   int ti, tj;
   tile_of<MODE, T::kBM, T::kBN>(M, t % tiles, ti, tj);
@@ -1498,7 +1512,9 @@ void launch_product(Group &G, int workers, float *partial, int src,
   Line L;
   L.workers = int(w);
   L.partial = partial;
-  L.total = place_tiles<T, MODE>(G, true);
+  const int total = place_tiles<T, MODE>(G, true);
+  L.each = total / L.workers;
+  L.more = total % L.workers;
   hipLaunchKernelGGL((ns_line_kernel<T, MODE>), dim3(L.workers),
                      dim3(T::kThreads), 0, st.stream, G, L, src, st.a, st.b,
                      st.c, st.S);
