@@ -154,13 +154,18 @@ __global__ __launch_bounds__(kBlock) void embed_lookup_kernel(
   const bool ok = id >= 0 && id < vocab;
   const char *src = table + (ok ? id : 0) * row_bytes;
   char *dst = out + t * dim * kE;
-  float v[kLookVecs][VEC];
+  float v[kLookVecs][VEC] = {};
+  if (ok) {
+    // (lanes past the row read its start: a load under a condition is waited
+    // for before the next one goes out)
+    typename Raw<DT, VEC>::type raw[kLookVecs];
 #pragma unroll
-  for (int k = 0; k < kLookVecs; ++k) {
-    const int64_t c = c0 + (k * kWave + lane) * VEC;
+    for (int k = 0; k < kLookVecs; ++k) {
+      const int64_t c = c0 + (k * kWave + lane) * VEC;
+      raw[k] = load_raw<DT, VEC>(src + (c < dim ? c : 0) * kE);
+    }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[k][e] = 0.0f;
-    if (ok && c < dim) load_vec<DT, VEC>(src + c * kE, v[k]);
+    for (int k = 0; k < kLookVecs; ++k) widen<DT, VEC>(raw[k], v[k]);
   }
 #pragma unroll
   for (int k = 0; k < kLookVecs; ++k) {
@@ -201,44 +206,66 @@ struct Sort {
   float *partial;    // [chunk][head, tail][dim]
 };
 
-// Key of token t: its row, or V for padding; and its row of values and
-// factor.
-__device__ __forceinline__ uint32_t token_key(const Parts &P,
-                                              const uint32_t *starts,
-                                              uint32_t t, uint32_t vocab,
-                                              const char *&row, float &coef) {
-  int lo = 0, hi = P.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= t) lo = mid;
-    else hi = mid;
+// Keys of N tokens (each its row, or V for padding), their rows of values
+// and factors; the N chains of loads go side by side.
+template <int N>
+__device__ __forceinline__ void token_keys(const Parts &P,
+                                           const uint32_t *starts,
+                                           const uint32_t (&t)[N],
+                                           uint32_t vocab, uint32_t (&key)[N],
+                                           const char *(&row)[N],
+                                           float (&coef)[N]) {
+  static_assert(kMaxParts <= 128, "steps of the search");
+  int at[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) at[k] = 0;
+#pragma unroll
+  for (int step = 64; step > 0; step >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int next = at[k] + step;
+      const uint32_t first = starts[next < P.n ? next : 0];
+      at[k] = next < P.n && first <= t[k] ? next : at[k];
+    }
+  Part p[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) p[k] = P.part[at[k]];
+  // (both halves of an int64 id as words, so that one kind of load serves
+  // both types)
+  uint32_t lo[N], hi[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int64_t i = t[k] - p[k].start;
+    const bool wide = (p[k].stride & kIds64) != 0;
+    const uint32_t *q = static_cast<const uint32_t *>(p[k].ids) +
+                        (wide ? 2 * i : i);
+    lo[k] = gld(q);
+    hi[k] = gld(q + (wide ? 1 : 0));
   }
-  const Part &p = P.part[lo];
-  const int64_t i = t - p.start;
-  const int64_t id = load_id(p.ids, i, (p.stride & kIds64) != 0);
-  row = p.rows + i * int64_t(p.stride & ~kIds64) * P.elem;
-  coef = p.coef;
-  return id >= 0 && id < int64_t(vocab) ? uint32_t(id) : vocab;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int64_t i = t[k] - p[k].start;
+    const bool wide = (p[k].stride & kIds64) != 0;
+    row[k] = p[k].rows + i * int64_t(p[k].stride & ~kIds64) * P.elem;
+    coef[k] = p[k].coef;
+    // (a negative int32 id is above any row, too)
+    key[k] = (!wide || hi[k] == 0) && lo[k] < vocab ? lo[k] : vocab;
+  }
 }
 
-// The parts' first tokens, for token_key, in LDS (the caller synchronises).
+// The parts' first tokens, for token_keys, in LDS (the caller synchronises).
 __device__ __forceinline__ void stage_starts(const Parts &P,
                                              uint32_t *starts) {
   if (int(threadIdx.x) < P.n) starts[threadIdx.x] = P.part[threadIdx.x].start;
 }
 
-__device__ __forceinline__ uint32_t note_token(const Parts &P,
-                                               const uint32_t *starts,
-                                               const Sort &W, uint32_t t,
-                                               uint32_t vocab) {
-  const char *row;
-  float coef;
-  const uint32_t key = token_key(P, starts, t, vocab, row, coef);
+__device__ __forceinline__ void note_token(const Sort &W, uint32_t t,
+                                           uint32_t key, const char *row,
+                                           float coef) {
   W.key[0][t] = key;
   W.tok[0][t] = t;
   W.row[t] = row;
   W.coef[t] = coef;
-  return key;
 }
 
 // Keys of these parts' tokens (a call of more parts than fit one launch).
@@ -249,8 +276,14 @@ __global__ __launch_bounds__(kBlock) void embed_key_kernel(Parts P, Sort W,
   __syncthreads();
   for (int64_t t = int64_t(P.part[0].start) +
                    int64_t(blockIdx.x) * kBlock + threadIdx.x;
-       t < P.end; t += int64_t(gridDim.x) * kBlock)
-    note_token(P, starts, W, uint32_t(t), vocab);
+       t < P.end; t += int64_t(gridDim.x) * kBlock) {
+    const uint32_t at[1] = {uint32_t(t)};
+    uint32_t key[1];
+    const char *row[1];
+    float coef[1];
+    token_keys<1>(P, starts, at, vocab, key, row, coef);
+    note_token(W, at[0], key[0], row[0], coef[0]);
+  }
 }
 
 // token k of this thread's rounds in the tile at `base`: wave w owns tokens
@@ -361,15 +394,28 @@ __global__ __launch_bounds__(kTileThreads) void embed_hist_kernel(
   stage_starts(P, starts);
   __syncthreads();
   const int64_t base = int64_t(blockIdx.x) * kTile;
+  uint32_t t[kRounds], key[kRounds];
+  bool in[kRounds];
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const int64_t t = tile_token(base, k);
-    if (t >= tokens) continue;
-    const uint32_t key = P.n > 0
-                             ? note_token(P, starts, W, uint32_t(t), vocab)
-                             : W.key[src][t];
-    atomicAdd(&h[(key >> shift) & (digits - 1)], 1u);
+    const int64_t at = tile_token(base, k);
+    in[k] = at < tokens;
+    t[k] = uint32_t(in[k] ? at : tokens - 1);
   }
+  if (P.n > 0) {
+    const char *row[kRounds];
+    float coef[kRounds];
+    token_keys<kRounds>(P, starts, t, vocab, key, row, coef);
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k)
+      if (in[k]) note_token(W, t[k], key[k], row[k], coef[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) key[k] = W.key[src][t[k]];
+  }
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k)
+    if (in[k]) atomicAdd(&h[(key[k] >> shift) & (digits - 1)], 1u);
   __syncthreads();
   for (int i = threadIdx.x; i < digits; i += kTileThreads)
     W.hist[int64_t(i) * blocks + blockIdx.x] = h[i];
@@ -422,8 +468,8 @@ __global__ __launch_bounds__(kTileThreads) void embed_scatter_kernel(
   for (int k = 0; k < kRounds; ++k) {
     const int64_t t = tile_token(base, k);
     in[k] = t < tokens;
-    key[k] = in[k] ? W.key[src][t] : 0u;
-    tok[k] = in[k] ? W.tok[src][t] : 0u;
+    key[k] = W.key[src][in[k] ? t : tokens - 1];
+    tok[k] = W.tok[src][in[k] ? t : tokens - 1];
   }
   const int digits = 1 << bits;
   // a digit's total and its tokens in earlier tiles
@@ -459,6 +505,15 @@ __global__ __launch_bounds__(kTileThreads) void embed_scatter_kernel(
   }
   __syncthreads();
   const int wave = threadIdx.x / kWave;
+  const char *row[kRounds];
+  float coef[kRounds];
+  if (last) {
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      row[k] = W.row[tok[k]];
+      coef[k] = W.coef[tok[k]];
+    }
+  }
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
     if (!in[k]) continue;
@@ -466,8 +521,8 @@ __global__ __launch_bounds__(kTileThreads) void embed_scatter_kernel(
     const uint32_t o = at[d] + cnt[d * kW + wave] + rank[k];
     W.key[src ^ 1][o] = key[k];
     if (last) {
-      W.srow[o] = W.row[tok[k]];
-      W.scoef[o] = W.coef[tok[k]];
+      W.srow[o] = row[k];
+      W.scoef[o] = coef[k];
     } else {
       W.tok[src ^ 1][o] = tok[k];
     }
@@ -496,18 +551,26 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
   for (int k = 0; k < kRounds; ++k) {
     const int t = int(tile_token(0, k));
     in[k] = t < tokens;
-    key[k] = tok[k] = 0u;
-    if (!in[k]) continue;
-    tok[k] = uint32_t(t);
-    if (P.n > 0) {
-      key[k] =
-          token_key(P, starts, uint32_t(t), vocab, srow[t], scoef[t]);
-    } else {
-      key[k] = W.key[0][t];
-      srow[t] = W.row[t];
-      scoef[t] = W.coef[t];
+    tok[k] = uint32_t(in[k] ? t : int(tokens) - 1);
+  }
+  const char *row[kRounds];
+  float coef[kRounds];
+  if (P.n > 0) {
+    token_keys<kRounds>(P, starts, tok, vocab, key, row, coef);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      key[k] = W.key[0][tok[k]];
+      row[k] = W.row[tok[k]];
+      coef[k] = W.coef[tok[k]];
     }
   }
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k)
+    if (in[k]) {
+      srow[tok[k]] = row[k];
+      scoef[tok[k]] = coef[k];
+    }
   const int digits = 1 << bits;
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
@@ -652,6 +715,9 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
   const int64_t chunk = unit / O.slices;
   const int64_t c = ((unit % O.slices) * kWave + lane) * VEC;
   const bool mine = c < O.dim;
+  // (lanes past the row read its start: a load under a condition is waited
+  // for before the next one goes out)
+  const int64_t lc = mine ? c / VEC : 0;
   const int64_t p0 = chunk * O.chunk;
   const int64_t left = O.tokens - p0;
   const int cnt = int(left < O.chunk ? left : O.chunk);
@@ -677,7 +743,8 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
   bool head = __builtin_amdgcn_readlane(k, 0) == prev;
   constexpr int kAhead = 16;
   for (int i0 = 0; i0 < valid; i0 += kAhead) {
-    typename Raw<GT, VEC>::type raw[kAhead] = {};
+    typename Raw<GT, VEC>::type raw[kAhead];
+    typename Raw<OT, VEC>::type old[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u < valid ? i0 + u : valid - 1;
@@ -686,9 +753,18 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
       const uint32_t ahi = __builtin_amdgcn_readlane(uint32_t(a >> 32), i);
       const char *src =
           reinterpret_cast<const char *>((uint64_t(ahi) << 32) | alo);
-      if (mine)
-        raw[u] = gld_nt(reinterpret_cast<const typename Raw<GT, VEC>::type *>(
-            src + c * kGE));
+      raw[u] = gld_nt(
+          reinterpret_cast<const typename Raw<GT, VEC>::type *>(src) + lc);
+    }
+    // what the rows hold (of those that end here it is needed)
+    if (O.accumulate) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u < valid ? i0 + u : valid - 1;
+        old[u] = load_raw<OT, VEC>(
+            O.out + int64_t(__builtin_amdgcn_readlane(k, i)) * O.row_bytes +
+            lc * (VEC * kOE));
+      }
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -713,7 +789,7 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
           char *dst = O.out + int64_t(key) * O.row_bytes + c * kOE;
           if (O.accumulate) {
             float o[VEC];
-            load_vec<OT, VEC>(dst, o);
+            widen<OT, VEC>(old[u], o);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] = __fadd_rn(o[e], acc[e]);
           }
@@ -750,10 +826,15 @@ __global__ __launch_bounds__(kBlock) void embed_few_kernel(Parts P, Out O,
   stage_starts(P, starts);
   named[t] = 0;
   __syncthreads();
-  const char *row = nullptr;
-  float coef = 0.0f;
+  const char *rows[1];
+  float coefs[1];
   uint32_t k = ~0u;
-  if (t < tokens) k = token_key(P, starts, uint32_t(t), none, row, coef);
+  if (tokens > 0) {  // (else there is no part to look into)
+    const uint32_t at[1] = {uint32_t(t < tokens ? t : tokens - 1)};
+    uint32_t keys[1];
+    token_keys<1>(P, starts, at, none, keys, rows, coefs);
+    if (t < tokens) k = keys[0];
+  }
   key[t] = k;
   __syncthreads();
   if (int(blockIdx.x) >= sum_blocks) {
@@ -774,8 +855,8 @@ __global__ __launch_bounds__(kBlock) void embed_few_kernel(Parts P, Out O,
     for (int j = 0; j < tokens; ++j)
       place += key[j] < k || (key[j] == k && j < t);
     skey[place] = k;
-    srow[place] = row;
-    scoef[place] = coef;
+    srow[place] = rows[0];
+    scoef[place] = coefs[0];
   }
   __syncthreads();
   const int64_t unit = int64_t(blockIdx.x) * kWaves + wave;

@@ -146,12 +146,14 @@ __device__ __forceinline__ float muon_lr(const Mat &M, const MuonScalars &S) {
   return r > k ? S.lr * __fsqrt_rn(__fdiv_rn(r, k)) : S.lr;
 }
 
-__device__ __forceinline__ float load_as_f32(const void *p, int64_t i,
-                                             int dt) {
-  if (dt == FSAGG_F32) return static_cast<const float *>(p)[i];
-  if (dt == FSAGG_F16)
+template <int DT>
+__device__ __forceinline__ float load_as_f32(const void *p, int64_t i) {
+  if constexpr (DT == FSAGG_F32) return static_cast<const float *>(p)[i];
+  else if constexpr (DT == FSAGG_F16)
     return float(static_cast<const _Float16 *>(p)[i]);
-  return __uint_as_float(uint32_t(static_cast<const uint16_t *>(p)[i]) << 16);
+  else
+    return __uint_as_float(uint32_t(static_cast<const uint16_t *>(p)[i])
+                           << 16);
 }
 
 // round to nearest even, NaN kept (quieted)
@@ -266,26 +268,44 @@ __device__ __forceinline__ void split_n(const float *v, H &h, H &l) {
   }
 }
 
-// The update at element e = (i, j) of matrix z.
-//   MUON: g = p - avg (negated for maximize); buf += (1 - mu)(g - buf);
-//         u = nesterov ? g + mu (buf - g) : buf.
-template <bool MUON>
-__device__ __forceinline__ float update_at(const Mat &M, const MuonScalars &S,
-                                           int z, int64_t e, int64_t i,
-                                           int64_t j) {
+// What the update at a place is made of: the loads, apart from what follows
+// them so that those of several places go out together.
+struct Taken {
+  float g, p, o;  // update or average; parameter, momentum (muon)
+};
+template <bool MUON, int DT>
+__device__ __forceinline__ Taken take_at(const Mat &M, int z, int64_t e,
+                                         int64_t i, int64_t j) {
   if constexpr (!MUON)
-    return load_as_f32(M.g, z * M.sz + i * M.si + j * M.sj, M.dt);
-  const float p = static_cast<const float *>(M.out)[e];
-  float g = __fsub_rn(p, static_cast<const float *>(M.g)[e]);
+    return {load_as_f32<DT>(M.g, z * M.sz + i * M.si + j * M.sj), 0.0f, 0.0f};
+  return {static_cast<const float *>(M.g)[e],
+          static_cast<const float *>(M.out)[e], M.buf[e]};
+}
+
+// The update at element e: the input's own, or the momentum step from
+// parameter - average, whose new momentum is stored.
+template <bool MUON>
+__device__ __forceinline__ float update_of(const Mat &M, const MuonScalars &S,
+                                           int64_t e, const Taken &t) {
+  if constexpr (!MUON) return t.g;
+  float g = __fsub_rn(t.p, t.g);
   if (S.maximize) g = -g;
-  const float o = M.buf[e];
   // the torch.lerp forms: exact at both ends (mu = 0 gives g)
-  const float d = __fsub_rn(g, o);
+  const float d = __fsub_rn(g, t.o);
   const float n = S.keep < 0.5f
-                      ? __builtin_fmaf(S.keep, d, o)
+                      ? __builtin_fmaf(S.keep, d, t.o)
                       : __fsub_rn(g, __fmul_rn(d, 1.0f - S.keep));
   M.buf[e] = n;
   return S.nesterov ? __builtin_fmaf(S.mu, __fsub_rn(n, g), g) : n;
+}
+
+// f(integral constant): the update's type as a template argument
+template <bool MUON, typename F>
+__device__ __forceinline__ void with_update_type(const Mat &M, F f) {
+  if (!MUON && M.dt == FSAGG_F16) f(std::integral_constant<int, FSAGG_F16>());
+  else if (!MUON && M.dt == FSAGG_BF16)
+    f(std::integral_constant<int, FSAGG_BF16>());
+  else f(std::integral_constant<int, FSAGG_F32>());
 }
 
 // Sum of the workgroup's kThreads values, in a fixed order, in every thread.
@@ -337,25 +357,27 @@ __global__ __launch_bounds__(kNormBlock) void ns_update_kernel(
   const uint32_t step = uint32_t(M.nb) * kNormBlock;
   double sq = 0.0;
   constexpr int kAhead = 8;
-  for (uint32_t e0 = uint32_t(b) * kNormBlock + threadIdx.x; e0 < total;
-       e0 += kAhead * step) {
-    float v[kAhead];
+  with_update_type<MUON>(M, [&](auto dt) {
+    for (uint32_t e0 = uint32_t(b) * kNormBlock + threadIdx.x; e0 < total;
+         e0 += kAhead * step) {
+      Taken t[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const uint32_t e = e0 + k * step;
-      v[k] = 0.0f;
-      if (e < total) {
+      for (int k = 0; k < kAhead; ++k) {
+        const uint32_t e = e0 + k * step < total ? e0 + k * step : total - 1;
         const uint32_t i = MUON ? 0u : e / uint32_t(M.cols);
-        v[k] = update_at<MUON>(M, S, z, e, i, e - i * uint32_t(M.cols));
+        t[k] = take_at<MUON, decltype(dt)::value>(
+            M, z, e, i, e - i * uint32_t(M.cols));
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const uint32_t e = e0 + k * step;
+        if (e >= total) break;
+        const float v = update_of<MUON>(M, S, e, t[k]);
+        u[e] = v;
+        sq += double(v) * double(v);
       }
     }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const uint32_t e = e0 + k * step;
-      if (e < total) u[e] = v[k];
-      sq += double(v[k]) * double(v[k]);
-    }
-  }
+  });
   __shared__ double part[kNormBlock];
   sq = block_sum<kNormBlock>(sq, part);
   if (threadIdx.x == 0) norm[b] = sq;
@@ -374,16 +396,28 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
   const float *u = reinterpret_cast<const float *>(P.th(1));
   __shared__ double part[256];
   __shared__ float tile[64][65];
-  const double scale = limb_scale(norm_sum(P.norm, M.nb, part), eps);
   const int i0 = (t / tn) * 64, j0 = (t % tn) * 64;
   const bool tall = M.rows > M.cols;
   // u's own rows r and columns c of this tile
   const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
-  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-    const int r = k / 64, c = k % 64;
-    float v = 0.0f;
-    if (r0 + r < M.rows && c0 + c < M.cols)
-      v = float(double(u[int64_t(r0 + r) * M.cols + c0 + c]) * scale);
+  // (all on their way before the norm is waited for; places past the matrix
+  // read its last row or column: a load under a condition is waited for
+  // before the next one goes out)
+  const int c = threadIdx.x % 64;
+  float u0[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int r = r0 + k * 4 + int(threadIdx.x) / 64;
+    u0[k] = u[int64_t(r < M.rows ? r : M.rows - 1) * M.cols +
+              (c0 + c < M.cols ? c0 + c : M.cols - 1)];
+  }
+  const double scale = limb_scale(norm_sum(P.norm, M.nb, part), eps);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int r = k * 4 + int(threadIdx.x) / 64;
+    // (a place past the matrix stays zero under a scale of infinity or NaN)
+    const bool in = r0 + r < M.rows && c0 + c < M.cols;
+    const float v = in ? float(double(u0[k]) * scale) : 0.0f;
     if (tall) tile[c][r] = v;
     else tile[r][c] = v;
   }
@@ -678,6 +712,22 @@ struct Tile {
           p)[(block * 4 + q) * kThreads + threadIdx.x];
   }
 
+  // f(integral constant): the result's type as a template argument (one limb
+  // goes with bf16 results only)
+  template <int MODE, typename F>
+  static __device__ __forceinline__ void with_result_type(const Mat &M, F f) {
+    if constexpr (MODE == kLast && LIMBS == 1) {
+      f(std::integral_constant<int, FSAGG_BF16>());
+    } else if constexpr (MODE == kLast) {
+      if (M.odt == FSAGG_BF16) f(std::integral_constant<int, FSAGG_BF16>());
+      else if (M.odt == FSAGG_F16)
+        f(std::integral_constant<int, FSAGG_F16>());
+      else f(std::integral_constant<int, FSAGG_F32>());
+    } else {
+      f(std::integral_constant<int, FSAGG_F32>());
+    }
+  }
+
   template <int MODE, int DT>
   __device__ __forceinline__ void finish_as(const Mat &M, const Planes &P,
                                             int z, int ti, int tj, int src,
@@ -695,12 +745,9 @@ struct Tile {
                                          int ti, int tj, int src, float a,
                                          float b, float c,
                                          const MuonScalars &S) const {
-    if (MODE == kLast && M.odt == FSAGG_BF16)
-      finish_as<MODE, FSAGG_BF16>(M, P, z, ti, tj, src, a, b, c, S);
-    else if (MODE == kLast && M.odt == FSAGG_F16)
-      finish_as<MODE, FSAGG_F16>(M, P, z, ti, tj, src, a, b, c, S);
-    else
-      finish_as<MODE, FSAGG_F32>(M, P, z, ti, tj, src, a, b, c, S);
+    with_result_type<MODE>(M, [&](auto dt) {
+      finish_as<MODE, decltype(dt)::value>(M, P, z, ti, tj, src, a, b, c, S);
+    });
   }
 
   // what the product is for, for one 32 x 32 block.  The matrix cores leave
@@ -910,15 +957,11 @@ __global__ __launch_bounds__(T::kThreads) void ns_join_kernel(
   const T tile;
   const Planes P = planes_of(M, z);
   const int i = block / T::NJ, j = block % T::NJ;
-  if (MODE == kLast && M.odt == FSAGG_BF16)
-    tile.template finish_block<MODE, FSAGG_BF16>(x, M, P, z, ti, tj, i, j, src,
-                                                 a, b, c, S);
-  else if (MODE == kLast && M.odt == FSAGG_F16)
-    tile.template finish_block<MODE, FSAGG_F16>(x, M, P, z, ti, tj, i, j, src,
-                                                a, b, c, S);
-  else
-    tile.template finish_block<MODE, FSAGG_F32>(x, M, P, z, ti, tj, i, j, src,
-                                                a, b, c, S);
+  T::template with_result_type<MODE>(M, [&](auto dt) {
+    tile.template finish_block<MODE, decltype(dt)::value>(x, M, P, z, ti, tj,
+                                                          i, j, src, a, b, c,
+                                                          S);
+  });
 }
 
 // -- narrow matrices ---------------------------------------------------------
@@ -1016,17 +1059,42 @@ __device__ __forceinline__ void load_update(const Mat &M, const Narrow &N,
                                             int ch, f32x16 &x) {
   const bool tall = M.rows > M.cols;
   const int j = ch * 64 + W.col();
+  // (places past the matrix read its last row or column)
+  const int lj = j < M.n ? j : M.n - 1;
+  const auto place = [&](int i, int jj) {
+    return int64_t(tall ? jj : i) * M.cols + (tall ? i : jj);
+  };
+  if constexpr (!WHOLE) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int i = W.row(r / 4) + r % 4;
-    float v = 0.0f;
-    if (i < M.m && j < M.n) {
-      const int a = tall ? j : i, b = tall ? i : j;
-      const int64_t o = int64_t(a) * M.cols + b;
-      v = WHOLE ? update_at<MUON>(M, S, z, o, a, b) : N.u[o];
+    for (int r = 0; r < 16; ++r) {
+      const int i = W.row(r / 4) + r % 4;
+      x[r] = N.u[place(i < M.m ? i : M.m - 1, lj)];
     }
-    x[r] = v;
+  } else {
+    with_update_type<MUON>(M, [&](auto dt) {
+      // (4 at a time, and the addresses of 4: with 1024 threads there are no
+      // registers for all)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        int i0 = W.row(q);
+        asm volatile("" : "+v"(i0));
+        Taken t[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int li = i0 + r < M.m ? i0 + r : M.m - 1;
+          t[r] = take_at<MUON, decltype(dt)::value>(
+              M, z, place(li, lj), tall ? lj : li, tall ? li : lj);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (i0 + r < M.m && j < M.n)
+            x[4 * q + r] = update_of<MUON>(M, S, place(i0 + r, j), t[r]);
+      }
+    });
   }
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (W.row(r / 4) + r % 4 >= M.m || j >= M.n) x[r] = 0.0f;
 }
 __device__ __forceinline__ void scale_update(const Mat &M, const Slab &W,
                                              int ch, double scale,
