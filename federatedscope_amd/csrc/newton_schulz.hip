@@ -15,9 +15,11 @@
 // error 1e-6 .. 8e-6 against 64 bits by spectrum, both) at 3/16 of the cost
 // per product: 16-bit limbs run at 16 times the fp32 matrix rate.
 //
-// Every product is C = P R^T with both operands contiguous along k, so X is
-// kept as X (for A) and as T = X^T (for QX); A and Q are symmetric: the
-// tiles on and above the diagonal are computed and stored twice.
+// A = X X^T and A^2 are products C = P R^T with both operands contiguous along
+// k; A and Q are symmetric: the tiles on and above the diagonal are computed
+// and stored twice.  QX is computed as (QX)^T = X^T Q with X's fragments read
+// transposed from LDS, so that X is kept in one orientation and a lane's
+// results lie side by side in it.
 #include "common.h"
 
 #include <hip/hip_fp16.h>
@@ -59,25 +61,25 @@ struct Mat {
   int16_t dt, odt;
 };
 
-// Workspace of one matrix: X limbs, T limbs twice (a step reads one and
-// writes the other), A limbs, Q limbs, norm partials.  The fp32 update lies
-// in the second T until the first step writes it.
+// Workspace of one matrix: X limbs twice (a step reads one and writes the
+// other), A limbs, Q limbs, norm partials.  The fp32 update lies in the
+// second X until the first step writes it.
 struct Planes {
-  _Float16 *xh, *xl, *t, *ah, *al, *qh, *ql;
+  _Float16 *x, *ah, *al, *qh, *ql;
   int64_t e;
   double *norm;
   // (selected by arithmetic: an array indexed at run time would live in
   // scratch memory)
-  __device__ __forceinline__ _Float16 *th(int k) const {
-    return t + 2 * k * e;
+  __device__ __forceinline__ _Float16 *xh(int k) const {
+    return x + 2 * k * e;
   }
-  __device__ __forceinline__ _Float16 *tl(int k) const {
-    return t + (2 * k + 1) * e;
+  __device__ __forceinline__ _Float16 *xl(int k) const {
+    return x + (2 * k + 1) * e;
   }
 };
 
 __host__ __device__ inline int64_t ws_elems(int64_t mp, int64_t np) {
-  return 6 * mp * np + 4 * mp * mp;
+  return 4 * mp * np + 4 * mp * mp;
 }
 __host__ __device__ inline int64_t ws_bytes_of(int64_t mp, int64_t np) {
   return 2 * ws_elems(mp, np) + 8 * kMaxNorm;
@@ -86,11 +88,9 @@ __device__ __forceinline__ Planes planes_of(const Mat &M, int z) {
   _Float16 *p = reinterpret_cast<_Float16 *>(M.ws + z * M.wstride);
   const int64_t e = int64_t(M.mp) * M.np, s = int64_t(M.mp) * M.mp;
   Planes P;
-  P.xh = p;
-  P.xl = p + e;
-  P.t = p + 2 * e;
+  P.x = p;
   P.e = e;
-  P.ah = p + 6 * e;
+  P.ah = p + 4 * e;
   P.al = P.ah + s;
   P.qh = P.ah + 2 * s;
   P.ql = P.ah + 3 * s;
@@ -172,18 +172,20 @@ __device__ __forceinline__ void store_from_f32(void *p, int64_t i, float v) {
     static_cast<uint16_t *>(p)[i] = to_bf16(v);
 }
 
-// Results y of rows i .. i + N - 1 (N = 4 or 8, i a multiple of N), column j
-// of matrix z (m x n orientation), as type DT.  A tall matrix has them side
-// by side.
-template <bool MUON, int DT, int N>
+// N = 4 or 8 results y of matrix z (m x n orientation) from (i, j) on, as
+// type DT: rows i, i + 1, .. of column j (DOWN) or columns j, j + 1, .. of
+// row i.  They lie side by side if the matrix is tall, or not, respectively;
+// the first is then a multiple of N.
+template <bool MUON, int DT, int N, bool DOWN>
 __device__ __forceinline__ void store_result(const Mat &M,
                                              const MuonScalars &S, int z,
                                              int i, int j, const float *y) {
   if (j >= M.n || i >= M.m) return;
   const bool tall = M.rows > M.cols;
-  const int64_t zo = MUON ? 0 : int64_t(z) * M.rows * M.cols;
-  if (tall && M.vec) {
-    const int64_t o = zo + int64_t(j) * M.cols + i;
+  const int64_t o = (MUON ? 0 : int64_t(z) * M.rows * M.cols) +
+                    (tall ? int64_t(j) * M.cols + i
+                          : int64_t(i) * M.cols + j);
+  if (tall == DOWN && M.vec) {
     if constexpr (MUON) {
       f32x4 *p = reinterpret_cast<f32x4 *>(static_cast<float *>(M.out) + o);
       const float lr = muon_lr(M, S);
@@ -220,30 +222,22 @@ __device__ __forceinline__ void store_result(const Mat &M,
     }
     return;
   }
+  const int64_t step = tall == DOWN ? 1 : M.cols;
+  const int have = DOWN ? M.m - i : M.n - j;
   if constexpr (MUON) {
-    float *const out = static_cast<float *>(M.out);
+    float *const out = static_cast<float *>(M.out) + o;
     const float lr = muon_lr(M, S);
     float v[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int64_t o = tall ? int64_t(j) * M.cols + i + e
-                             : int64_t(i + e) * M.cols + j;
-      v[e] = i + e < M.m ? out[o] : 0.0f;
-    }
+    for (int e = 0; e < N; ++e) v[e] = out[(e < have ? e : have - 1) * step];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int64_t o = tall ? int64_t(j) * M.cols + i + e
-                             : int64_t(i + e) * M.cols + j;
-      if (i + e < M.m)
-        out[o] = __builtin_fmaf(-lr, y[e], __fmul_rn(v[e], S.decay));
-    }
+    for (int e = 0; e < N; ++e)
+      if (e < have)
+        out[e * step] = __builtin_fmaf(-lr, y[e], __fmul_rn(v[e], S.decay));
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int64_t o = tall ? int64_t(j) * M.cols + i + e
-                             : int64_t(i + e) * M.cols + j;
-      if (i + e < M.m) store_from_f32<DT>(M.out, zo + o, y[e]);
-    }
+    for (int e = 0; e < N; ++e)
+      if (e < have) store_from_f32<DT>(M.out, o + e * step, y[e]);
   }
 }
 
@@ -350,7 +344,7 @@ __global__ __launch_bounds__(kNormBlock) void ns_update_kernel(
     norm = N.norm;
   } else {
     const Planes P = planes_of(M, z);
-    u = reinterpret_cast<float *>(P.th(1));
+    u = reinterpret_cast<float *>(P.xh(1));
     norm = P.norm;
   }
   const uint32_t total = uint32_t(M.rows) * uint32_t(M.cols);
@@ -383,9 +377,9 @@ __global__ __launch_bounds__(kNormBlock) void ns_update_kernel(
   if (threadIdx.x == 0) norm[b] = sq;
 }
 
-// Pass 2: X and T limbs of u / max(|u|, eps), zero in the padding.  One
-// workgroup per 64 x 64 tile of the padded m x n orientation; the tile goes
-// through LDS so that both orientations are written in rows.
+// Pass 2: X limbs of u / max(|u|, eps), zero in the padding.  One workgroup
+// per 64 x 64 tile of the padded m x n orientation; the tile goes through LDS
+// so that it is read and written in rows, whichever way u lies.
 __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
                                                          double eps) {
   int rel;
@@ -393,7 +387,7 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
   const int tn = M.np / 64, tiles = (M.mp / 64) * tn;
   const int z = rel / tiles, t = rel % tiles;
   const Planes P = planes_of(M, z);
-  const float *u = reinterpret_cast<const float *>(P.th(1));
+  const float *u = reinterpret_cast<const float *>(P.xh(1));
   __shared__ double part[256];
   __shared__ float tile[64][65];
   const int i0 = (t / tn) * 64, j0 = (t % tn) * 64;
@@ -422,23 +416,17 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
     else tile[r][c] = v;
   }
   __syncthreads();
-  // 8 values a thread, in both orientations
+  // 8 values a thread
   for (int k = threadIdx.x; k < 64 * 8; k += 256) {
-    const int r = k / 8, c = k % 8 * 8;
+    const int r = k / 8, c8 = k % 8 * 8;
     float v[8];
     half8 h, l;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+    for (int e = 0; e < 8; ++e) v[e] = tile[r][c8 + e];
     split_n<8>(v, h, l);
-    const int64_t x = int64_t(i0 + r) * M.np + j0 + c;
-    *reinterpret_cast<half8 *>(P.xh + x) = h;
-    *reinterpret_cast<half8 *>(P.xl + x) = l;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
-    split_n<8>(v, h, l);
-    const int64_t y = int64_t(j0 + r) * M.mp + i0 + c;
-    *reinterpret_cast<half8 *>(P.th(0) + y) = h;
-    *reinterpret_cast<half8 *>(P.tl(0) + y) = l;
+    const int64_t x = int64_t(i0 + r) * M.np + j0 + c8;
+    *reinterpret_cast<half8 *>(P.xh(0) + x) = h;
+    *reinterpret_cast<half8 *>(P.xl(0) + x) = l;
   }
 }
 
@@ -518,6 +506,12 @@ __device__ __forceinline__ int line_at(const Line &L, int q) {
 // 4 so that a fragment read of 16 rows touches all 64 banks once.  NBUF
 // stages of LDS: one is multiplied while NBUF - 1 are on their way.
 //
+// With TR the left operand lies the other way, P^T with rows along k: a stage
+// is kBK rows of BM, and transposing reads (a group of 16 lanes takes 4 rows
+// of 16 columns, lane i the 4 values of column i) make the same fragments.
+// 32 lanes read 64 bytes of each of 4 rows, so the rows' 64-byte pieces are
+// permuted by the row, and again every bank is touched once.
+//
 // Rows and columns of the padding are zero in every plane (the prepare pass
 // writes them, products of zero rows are zero), so no tile is ragged inside
 // the workspace; only the last step checks its stores against the matrix.
@@ -554,11 +548,19 @@ struct Tile {
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
   }
 
+  // which 64-byte piece of row k of a transposed stage piece 0 goes to (rows
+  // of 64 have two pieces, and two rows fill the banks)
+  static __device__ __forceinline__ int piece(int k) {
+    return BM >= 128 ? k & 3 : (k >> 1) & 1;
+  }
+
+  template <bool TR>
   __device__ __forceinline__ void multiply(_Float16 *lds, const _Float16 *ph,
-                                           const _Float16 *pl,
+                                           const _Float16 *pl, int ldp,
                                            const _Float16 *rh,
-                                           const _Float16 *rl, int ld, int i0,
-                                           int j0, int k0, int k1) {
+                                           const _Float16 *rl, int ldr,
+                                           int i0, int j0, int k0, int k1,
+                                           int depth) {
     // this wave's loads of a stage: LDS order is [P.h][P.l][R.h][R.l] rows
     // of 64 bytes, 16 rows per instruction, one plane per wave
     const int row0 = wave * (kPer * 16);
@@ -569,25 +571,49 @@ struct Tile {
     const int g0 = (right ? j0 : i0) + (in < side ? in : in - side);
     // (a buffer descriptor: one 32-bit offset per lane instead of a 64-bit
     // address per load)
-    __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<_Float16 *>(base + int64_t(g0) * ld), short(0),
-        kPer * 16 * ld * 2, 0x00020000);
     const int lr = lane >> 2;
-    const int goff = (lr * ld + (((lane & 3) ^ ((lr >> 2) & 3)) * 8)) * 2;
-    // (past the last stage: offsets outside the descriptor, which fetch
+    const int ld = right ? ldr : ldp;
+    const _Float16 *first = base + int64_t(g0) * ld;
+    uint32_t extent = uint32_t(kPer * 16 * ld) * 2u;
+    // lane offsets of even and odd loads, bytes from load to load and from
+    // stage to stage
+    uint32_t goff0 = uint32_t(lr * ld + ((lane & 3) ^ ((lr >> 2) & 3)) * 8) *
+                     2u;
+    uint32_t goff1 = goff0, dload = uint32_t(16 * ld) * 2u, dstage = kBK * 2;
+    if constexpr (TR) {
+      if (!right) {
+        constexpr int kSlots = BM / 8;        // 16-byte slots of a row
+        constexpr int kRows = 64 / kSlots;    // rows of a load
+        const int r0 = (in < side ? in : in - side) / 16 * kRows;
+        const int r = lane / kSlots, slot = lane % kSlots;
+        first = base + int64_t(r0) * ld + i0;
+        extent = uint32_t(depth - r0) * uint32_t(ld) * 2u - uint32_t(i0) * 2u;
+        goff0 = uint32_t(r * ld + (slot ^ (piece(r0 + r) << 2)) * 8) * 2u;
+        goff1 = uint32_t(r * ld + (slot ^ (piece(r0 + kRows + r) << 2)) * 8) *
+                2u;
+        dload = uint32_t(kRows * ld) * 2u;
+        dstage = uint32_t(kBK * ld) * 2u;
+      }
+    }
+    __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<_Float16 *>(first), short(0), int(extent), 0x00020000);
+    // (past the last stage: an offset outside the descriptor, which fetches
     // nothing; so every stage has as many loads on their way, and the loop
-    // has no branch)
+    // has no branch.  A plane has at most 2.7 GB: FSAGG_NS_MAX_ELEMS halfs,
+    // and a quarter more of padding)
+    constexpr uint32_t kPast = 0xF0000000u;
     auto issue = [&](int k) {
       _Float16 *st = lds + (k % NBUF) * kStage + row0 * kBK;
-      const int off = k < k1 ? goff : 0x7FFFFFF0;
-      const int at = k < k1 ? k * kBK * 2 : 0;
+      const uint32_t off0 = k < k1 ? goff0 : kPast;
+      const uint32_t off1 = k < k1 ? goff1 : kPast;
+      const uint32_t at = k < k1 ? uint32_t(k) * dstage : 0u;
 #pragma unroll
       for (int q = 0; q < kPer; ++q)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rsrc,
             (__attribute__((address_space(3))) void *)(uintptr_t)(
                 st + q * 16 * kBK),
-            16, off, q * 16 * ld * 2 + at, 0, 0);
+            16, int(q & 1 ? off1 : off0), int(uint32_t(q) * dload + at), 0, 0);
     };
     const int fr = lane & 31, fk = lane >> 5;
     struct Frags {
@@ -597,6 +623,19 @@ struct Tile {
       const _Float16 *st = lds + (k % NBUF) * kStage;
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
+        if constexpr (TR) {
+          const int r = kk * 16 + fk * 8 + (lane & 15) / 4;
+          const int col = wm + i * 32 + (fr & 16) + (lane & 3) * 4;
+          const int o =
+              r * BM + (((col / 8) ^ (piece(r) << 2)) * 8) + col % 8;
+#pragma unroll
+          for (int l = 0; l < LIMBS; ++l) {
+            const half4 x = read_tr(st + l * BM * kBK + o);
+            const half4 y = read_tr(st + l * BM * kBK + o + 4 * BM);
+            f.a[l][i] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+          continue;
+        }
         const int r = wm + i * 32 + fr;
         const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
 #pragma unroll
@@ -640,13 +679,13 @@ struct Tile {
     for (int k = k0; k + 1 < k1; ++k) {
       read(f1, k, 1);
       mul(f0);
-      spread<0>();
+      spread<0, TR>();
       __builtin_amdgcn_sched_barrier(0);
       wait_and_meet<(NBUF - 2) * kPer>();
       read(f0, k + 1, 0);
       issue(k + NBUF);
       mul(f1);
-      spread<kPer>();
+      spread<kPer, TR>();
       __builtin_amdgcn_sched_barrier(0);
     }
     read(f1, k1 - 1, 1);
@@ -660,10 +699,10 @@ struct Tile {
   // Order of a half stage: the fragment reads, then LOADS direct loads, one
   // at a time between the matrix instructions, so that the waves do not queue
   // for the LDS and the memory pipe while the matrix cores wait.
-  template <int LOADS>
+  template <int LOADS, bool TR>
   static __device__ __forceinline__ void spread() {
     constexpr int kMfma = MI * NJ * (LIMBS == 2 ? 3 : 1);
-    constexpr int kReads = LIMBS * (MI + NJ);
+    constexpr int kReads = LIMBS * ((TR ? 2 : 1) * MI + NJ);
     constexpr int kEach = kMfma > kReads + LOADS ? kMfma / (kReads + LOADS)
                                                  : 1;
 #pragma unroll
@@ -677,6 +716,13 @@ struct Tile {
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, kMfma, 0);
+  }
+
+  static __device__ __forceinline__ half4 read_tr(const _Float16 *p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(
+        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   (__attribute__((address_space(3))) s4 *)(uintptr_t)p));
   }
 
   // all but the last N of this wave's direct loads have landed, and every
@@ -752,24 +798,26 @@ struct Tile {
 
   // what the product is for, for one 32 x 32 block.  The matrix cores leave
   // a lane column gj and four runs of 4 rows; lanes l and l + 32 exchange two
-  // of them, so that a lane has two runs of 8 rows (gi .. gi + 7, + 16) and
-  // the transposed planes move 16 bytes a lane.  DT: the result's type.
+  // of them, so that a lane has two runs of 8 rows (gi .. gi + 7, + 16).  Of
+  // (QX)^T these are 8 columns of X, 16 bytes a lane.  DT: the result's type.
   template <int MODE, int DT>
   __device__ __forceinline__ void finish_block(
       const f32x16 &acc16, const Mat &M, const Planes &P, int z, int ti,
       int tj, int i, int j, int src, float a, float b, float c,
       const MuonScalars &S) const {
+    constexpr bool kX = !symmetric(MODE);
     const int fr = lane & 31, fk = lane >> 5;
-    const int gi0 = ti * BM + wm + i * 32 + 8 * fk;
-    const int gj = tj * BN + wn + j * 32 + fr;
+    const int gi0 = (kX ? tj : ti) * BM + wm + i * 32 + 8 * fk;
+    const int gj = (kX ? ti : tj) * BN + wn + j * 32 + fr;
+    const int ld = kX ? M.np : M.mp;
     half8 oh[2], ol[2];
     if constexpr (MODE != kGram) {
-      // A is symmetric: its column gj is row gj; X's column is T's row
-      const _Float16 *bh = MODE == kSquare ? P.ah : P.th(src);
-      const _Float16 *bl = MODE == kSquare ? P.al : P.tl(src);
+      // (A is symmetric: its column gj is row gj)
+      const _Float16 *bh = MODE == kSquare ? P.ah : P.xh(src);
+      const _Float16 *bl = MODE == kSquare ? P.al : P.xl(src);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int64_t o = int64_t(gj) * M.mp + gi0 + 16 * p;
+        const int64_t o = int64_t(gj) * ld + gi0 + 16 * p;
         oh[p] = *reinterpret_cast<const half8 *>(bh + o);
         ol[p] = *reinterpret_cast<const half8 *>(bl + o);
       }
@@ -800,56 +848,49 @@ struct Tile {
       if constexpr (MODE == kLast || MODE == kLastMuon) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= kInvS;
-        store_result<MODE == kLastMuon, DT, 8>(M, S, z, gi, gj, v);
+        store_result<MODE == kLastMuon, DT, 8, false>(M, S, z, gj, gi, v);
       } else {
         half8 h, l;
         split_n<8>(v, h, l);
-        _Float16 *ch, *cl, *dh, *dl;  // C by rows, and C^T
-        int ldc, ldd;
-        if constexpr (MODE == kApply) {
-          ch = P.xh;
-          cl = P.xl;
-          ldc = M.np;
-          dh = P.th(src ^ 1);
-          dl = P.tl(src ^ 1);
-          ldd = M.mp;
-        } else {
-          ch = MODE == kGram ? P.ah : P.qh;
-          cl = MODE == kGram ? P.al : P.ql;
-          ldc = ldd = M.mp;
-          dh = ch;
-          dl = cl;
-        }
-        // a tile on the diagonal is its own transpose
-        if (MODE == kApply || ti != tj) {
+        _Float16 *ch = kX ? P.xh(src ^ 1) : MODE == kGram ? P.ah : P.qh;
+        _Float16 *cl = kX ? P.xl(src ^ 1) : MODE == kGram ? P.al : P.ql;
+        // (of one limb's products, Q has none to multiply; A and X are added,
+        // too)
+        constexpr bool kLow = LIMBS == 2 || MODE != kSquare;
+        // C's other half, unless the tile is its own transpose
+        if (!kX && ti != tj) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int64_t o = int64_t(gi + e) * ldc + gj;
+            const int64_t o = int64_t(gi + e) * ld + gj;
             ch[o] = h[e];
-            if (LIMBS == 2 || MODE == kGram) cl[o] = l[e];
+            if (kLow) cl[o] = l[e];
           }
         }
-        const int64_t o = int64_t(gj) * ldd + gi;
-        *reinterpret_cast<half8 *>(dh + o) = h;
-        if (LIMBS == 2 || MODE != kSquare)
-          *reinterpret_cast<half8 *>(dl + o) = l;
+        const int64_t o = int64_t(gj) * ld + gi;
+        *reinterpret_cast<half8 *>(ch + o) = h;
+        if (kLow) *reinterpret_cast<half8 *>(cl + o) = l;
       }
     }
   }
 };
 
+// Tile (ti, tj) of the mode's product, stages k0 to k1.
 template <int MODE, class T>
 __device__ __forceinline__ void multiply_of(T &tile, _Float16 *lds,
                                             const Mat &M, const Planes &P,
-                                            int src, int i0, int j0, int k0,
+                                            int src, int ti, int tj, int k0,
                                             int k1) {
   if constexpr (MODE == kGram)
-    tile.multiply(lds, P.xh, P.xl, P.xh, P.xl, M.np, i0, j0, k0, k1);
+    tile.template multiply<false>(lds, P.xh(src), P.xl(src), M.np, P.xh(src),
+                                  P.xl(src), M.np, ti * T::kBM, tj * T::kBN,
+                                  k0, k1, 0);
   else if constexpr (MODE == kSquare)
-    tile.multiply(lds, P.ah, P.al, P.ah, P.al, M.mp, i0, j0, k0, k1);
+    tile.template multiply<false>(lds, P.ah, P.al, M.mp, P.ah, P.al, M.mp,
+                                  ti * T::kBM, tj * T::kBN, k0, k1, 0);
   else
-    tile.multiply(lds, P.qh, P.ql, P.th(src), P.tl(src), M.mp, i0, j0, k0,
-                  k1);
+    tile.template multiply<true>(lds, P.xh(src), P.xl(src), M.np, P.qh, P.ql,
+                                 M.mp, tj * T::kBM, ti * T::kBN, k0, k1,
+                                 M.mp);
 }
 
 // Workgroup b's place when the workgroups, which go round robin over the 8
@@ -873,8 +914,7 @@ __global__ __launch_bounds__(T::kThreads) void ns_gemm_kernel(
   tile_of<MODE, T::kBM, T::kBN>(M, rel % tiles, ti, tj);
   const Planes P = planes_of(M, z);
   T tile;
-  multiply_of<MODE>(tile, lds, M, P, src, ti * T::kBM, tj * T::kBN, 0,
-                    mode_stages<MODE>(M));
+  multiply_of<MODE>(tile, lds, M, P, src, ti, tj, 0, mode_stages<MODE>(M));
   tile.template finish<MODE>(M, P, z, ti, tj, src, a, b, c, S);
 }
 
@@ -901,7 +941,7 @@ __global__ __launch_bounds__(T::kThreads) void ns_line_kernel(
     int ti, tj;
     tile_of<MODE, T::kBM, T::kBN>(M, t % tiles, ti, tj);
     const Planes P = planes_of(M, z);
-    multiply_of<MODE>(tile, lds, M, P, src, ti * T::kBM, tj * T::kBN, k0, k1);
+    multiply_of<MODE>(tile, lds, M, P, src, ti, tj, k0, k1);
     if (k0 == 0 && k1 == stages)
       tile.template finish<MODE>(M, P, z, ti, tj, src, a, b, c, S);
     else
@@ -1115,7 +1155,7 @@ __device__ __forceinline__ void store_chunk_as(const Mat &M, const Slab &W,
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = x[4 * q + e] * kInvS;
-    store_result<MUON, DT, 4>(M, S, z, W.row(q), ch * 64 + W.col(), y);
+    store_result<MUON, DT, 4, true>(M, S, z, W.row(q), ch * 64 + W.col(), y);
   }
 }
 template <bool MUON>
