@@ -779,12 +779,21 @@ struct Tile {
                                             int z, int ti, int tj, int src,
                                             float a, float b, float c,
                                             const MuonScalars &S) const {
+    // (what is added is read kAhead blocks before its turn)
+    constexpr int kBlocks = MI * NJ, kAhead = kBlocks < 2 ? kBlocks : 2;
+    Addend add[kAhead];
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int n = 0; n < kAhead; ++n)
+      add[n] = addend<MODE>(M, P, ti, tj, n / NJ, n % NJ, src);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        finish_block<MODE, DT>(acc[i][j], M, P, z, ti, tj, i, j, src, a, b, c,
-                               S);
+    for (int n = 0; n < kBlocks; ++n) {
+      const Addend now = add[n % kAhead];
+      if (n + kAhead < kBlocks)
+        add[n % kAhead] = addend<MODE>(M, P, ti, tj, (n + kAhead) / NJ,
+                                       (n + kAhead) % NJ, src);
+      finish_block<MODE, DT>(acc[n / NJ][n % NJ], now, M, P, z, ti, tj, n / NJ,
+                             n % NJ, src, a, b, c, S);
+    }
   }
   template <int MODE>
   __device__ __forceinline__ void finish(const Mat &M, const Planes &P, int z,
@@ -796,32 +805,54 @@ struct Tile {
     });
   }
 
-  // what the product is for, for one 32 x 32 block.  The matrix cores leave
-  // a lane column gj and four runs of 4 rows; lanes l and l + 32 exchange two
-  // of them, so that a lane has two runs of 8 rows (gi .. gi + 7, + 16).  Of
-  // (QX)^T these are 8 columns of X, 16 bytes a lane.  DT: the result's type.
-  template <int MODE, int DT>
-  __device__ __forceinline__ void finish_block(
-      const f32x16 &acc16, const Mat &M, const Planes &P, int z, int ti,
-      int tj, int i, int j, int src, float a, float b, float c,
-      const MuonScalars &S) const {
-    constexpr bool kX = !symmetric(MODE);
-    const int fr = lane & 31, fk = lane >> 5;
-    const int gi0 = (kX ? tj : ti) * BM + wm + i * 32 + 8 * fk;
-    const int gj = (kX ? ti : tj) * BN + wn + j * 32 + fr;
-    const int ld = kX ? M.np : M.mp;
-    half8 oh[2], ol[2];
+  // Block (i, j) of the accumulators: the matrix cores leave a lane column gj
+  // and four runs of 4 rows; lanes l and l + 32 exchange two of them, so that
+  // a lane has two runs of 8 rows (gi .. gi + 7, + 16).  Of (QX)^T these are
+  // 8 columns of X, 16 bytes a lane.
+  template <int MODE>
+  __device__ __forceinline__ int block_row(int ti, int tj, int i) const {
+    return (symmetric(MODE) ? ti : tj) * BM + wm + i * 32 + 8 * (lane >> 5);
+  }
+  template <int MODE>
+  __device__ __forceinline__ int block_column(int ti, int tj, int j) const {
+    return (symmetric(MODE) ? tj : ti) * BN + wn + j * 32 + (lane & 31);
+  }
+
+  // A or X where the block's results lie (A is symmetric: its column gj is
+  // row gj)
+  struct Addend {
+    half8 h[2], l[2];
+  };
+  template <int MODE>
+  __device__ __forceinline__ Addend addend(const Mat &M, const Planes &P,
+                                           int ti, int tj, int i, int j,
+                                           int src) const {
+    Addend v;
     if constexpr (MODE != kGram) {
-      // (A is symmetric: its column gj is row gj)
       const _Float16 *bh = MODE == kSquare ? P.ah : P.xh(src);
       const _Float16 *bl = MODE == kSquare ? P.al : P.xl(src);
+      const int64_t o = int64_t(block_column<MODE>(ti, tj, j)) *
+                            (MODE == kSquare ? M.mp : M.np) +
+                        block_row<MODE>(ti, tj, i);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int64_t o = int64_t(gj) * ld + gi0 + 16 * p;
-        oh[p] = *reinterpret_cast<const half8 *>(bh + o);
-        ol[p] = *reinterpret_cast<const half8 *>(bl + o);
+        v.h[p] = *reinterpret_cast<const half8 *>(bh + o + 16 * p);
+        v.l[p] = *reinterpret_cast<const half8 *>(bl + o + 16 * p);
       }
     }
+    return v;
+  }
+
+  // what the product is for, for one block.  DT: the result's type.
+  template <int MODE, int DT>
+  __device__ __forceinline__ void finish_block(
+      const f32x16 &acc16, const Addend &add, const Mat &M, const Planes &P,
+      int z, int ti, int tj, int i, int j, int src, float a, float b, float c,
+      const MuonScalars &S) const {
+    constexpr bool kX = !symmetric(MODE);
+    const int gi0 = block_row<MODE>(ti, tj, i);
+    const int gj = block_column<MODE>(ti, tj, j);
+    const int ld = kX ? M.np : M.mp;
     f32x16 x = acc16;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
@@ -841,9 +872,9 @@ struct Tile {
       for (int e = 0; e < 8; ++e) {
         v[e] = x[8 * p + e] * kInvS;
         if constexpr (MODE == kSquare)
-          v[e] = b * (float(oh[p][e]) + float(ol[p][e])) + c * v[e];
+          v[e] = b * (float(add.h[p][e]) + float(add.l[p][e])) + c * v[e];
         else if constexpr (MODE != kGram)
-          v[e] = a * (float(oh[p][e]) + float(ol[p][e])) + v[e];
+          v[e] = a * (float(add.h[p][e]) + float(add.l[p][e])) + v[e];
       }
       if constexpr (MODE == kLast || MODE == kLastMuon) {
 #pragma unroll
@@ -966,6 +997,13 @@ __global__ __launch_bounds__(T::kThreads) void ns_join_kernel(
   const int tiles = mode_tiles<MODE, T::kBM, T::kBN>(M);
   const int t = rel / stages, first = cut - rel % stages;
   if (cut == first || line_at(L, w) > first) return;
+  const int z = t / tiles;
+  int ti, tj;
+  tile_of<MODE, T::kBM, T::kBN>(M, t % tiles, ti, tj);
+  const T tile;
+  const Planes P = planes_of(M, z);
+  const int i = block / T::NJ, j = block % T::NJ;
+  const auto add = tile.template addend<MODE>(M, P, ti, tj, i, j, src);
   f32x16 x;
 #pragma unroll
   for (int r = 0; r < 16; ++r) x[r] = 0.0f;
@@ -991,16 +1029,9 @@ __global__ __launch_bounds__(T::kThreads) void ns_join_kernel(
       }
     more = in[kAhead - 1];
   }
-  const int z = t / tiles;
-  int ti, tj;
-  tile_of<MODE, T::kBM, T::kBN>(M, t % tiles, ti, tj);
-  const T tile;
-  const Planes P = planes_of(M, z);
-  const int i = block / T::NJ, j = block % T::NJ;
   T::template with_result_type<MODE>(M, [&](auto dt) {
-    tile.template finish_block<MODE, decltype(dt)::value>(x, M, P, z, ti, tj,
-                                                          i, j, src, a, b, c,
-                                                          S);
+    tile.template finish_block<MODE, decltype(dt)::value>(
+        x, add, M, P, z, ti, tj, i, j, src, a, b, c, S);
   });
 }
 
