@@ -12,7 +12,9 @@ are added as they come at worst: a step maps a singular value s to
 a s + b s^3 + c s^5; X is off by 2^-22 of it, A = X^2 by 2 + 1 of those, A^2
 by 6, Q by one more, so the terms are off by 1, 4 and 8 of those at most, and
 the error that s brings along is scaled by the step's slope at s
-(_limb_error).  Last comes half a step of the result's type.  A sum of c products in float32 is off by at most (c + 1)
+(_limb_error).  Large matrices with a bfloat16 result multiply the high limbs
+alone: A, A^2 and Q X then come with 2^-11 in place of 2^-22, a X and the
+iterate itself do not.  Last comes half a step of the result's type.  A sum of c products in float32 is off by at most (c + 1)
 2^-24 of the sum of the absolute products, and half a step of its type."""
 import math
 
@@ -28,28 +30,33 @@ HALF = {torch.float32: 2.0**-24, torch.float16: 2.0**-11,
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
-def _chain(g, dt, steps=5, coef=(A, B, C), eps=1e-7):
+def _chain(g, dt, steps=5, coef=(A, B, C), eps=1e-7, where='cpu'):
     a, b, c = coef
-    x = g.detach().cpu().double()
+    x = g.detach().to(where).double()
     x = (x / max(float(x.norm()), eps)).to(dt)
     tall = x.shape[0] > x.shape[1]
     x = x.T if tall else x
     for _ in range(steps):
         gram = x @ x.T
         x = a * x + (b * gram + c * (gram @ gram)) @ x
-    return (x.T if tall else x).double()
+    return (x.T if tall else x).double().cpu()
 
 
-def _limb_error(g, steps, coef, eps):
-    """2-norm over the singular values of the limb roundings' worst sum."""
+def _limb_error(g, steps, coef, eps, one=False, where='cpu'):
+    """2-norm over the singular values of the limb roundings' worst sum;
+    `one`: of products of the high limbs alone."""
     a, b, c = coef
-    x = g.detach().cpu().double()
-    s = torch.linalg.svdvals(x) / max(float(x.norm()), eps)
+    product = 2.0**-11 if one else 2.0**-22
+    x = g.detach().to(where).double()
+    x = x.T if x.shape[0] > x.shape[1] else x
+    s = (torch.linalg.svdvals(x) if where == 'cpu' else
+         torch.linalg.eigvalsh((x @ x.T).cpu()).clamp(min=0).sqrt())
+    s = s / max(float(x.norm()), eps)
     e = 2.0**-22 * s
     for _ in range(steps):
         slope = (a + 3 * b * s**2 + 5 * c * s**4).abs()
-        e = slope * e + 2.0**-22 * (abs(a) * s + 4 * abs(b) * s**3 +
-                                    8 * abs(c) * s**5)
+        e = slope * e + 2.0**-22 * abs(a) * s + product * (
+            4 * abs(b) * s**3 + 8 * abs(c) * s**5)
         s = a * s + b * s**3 + c * s**5
         e = e + 2.0**-22 * s.abs()
     return float(e.norm())
@@ -65,14 +72,15 @@ def _matrix(rows, cols, seed, scale=1e-2):
     return (x + 0.05 * torch.randn(rows, cols, generator=t)) * scale
 
 
-def _check_ns(got, g, steps=5, coef=(A, B, C), eps=1e-7):
-    want = _chain(g, torch.float64, steps, coef, eps)
+def _check_ns(got, g, steps=5, coef=(A, B, C), eps=1e-7, one=False,
+              where='cpu'):
+    want = _chain(g, torch.float64, steps, coef, eps, where)
     got64 = got.detach().cpu().double()
     assert got64.shape == want.shape
-    off32 = _chain(g, torch.float32, steps, coef, eps) - want
+    off32 = _chain(g, torch.float32, steps, coef, eps, where) - want
     norm = float(want.norm())
     half = HALF[got.dtype] if got.dtype != torch.float32 else 2.0**-24
-    limb = _limb_error(g, steps, coef, eps)
+    limb = _limb_error(g, steps, coef, eps, one, where)
     tol = 4 * float(off32.norm()) + limb + half * norm
     assert float((got64 - want).norm()) <= tol
     # no single element is far off: the largest float32 error with the same
@@ -183,6 +191,49 @@ def test_newton_schulz_list_of_many():
                 _check_ns(b, a)
 
 
+# the large tiles: whole 256 x 256 ones, shared ones with their joins, 128 x
+# 128 ones; sizes that end inside a tile
+LARGE = [(17, 1200, 1300), (1, 1200, 13000), (2, 515, 4100), (2, 4100, 515),
+         (1, 1100, 2600), (1, 2603, 1101)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', LARGE)
+def test_newton_schulz_large(shape, dtype):
+    from federatedscope_amd import ops
+    batch, rows, cols = shape
+    g = torch.stack([_matrix(rows, cols, z) for z in range(min(batch, 2))])
+    g = g.repeat((batch + 1) // 2, 1, 1)[:batch].to(dtype).cuda()
+    got = ops.newton_schulz(g)
+    for z in range(min(batch, 2)):
+        _check_ns(got[z], g[z], one=dtype == torch.bfloat16, where='cuda')
+    for z in range(2, batch):
+        assert torch.equal(got[z], got[z % 2])
+    assert torch.equal(got, ops.newton_schulz(g))
+
+
+def test_newton_schulz_planes_past_two_gigabytes():
+    """Every 256 columns of every row against a float32 chain: a tile read
+    or written at a wrong place is off by as much as it holds.  A product
+    here adds up at most 2^12 values in one accumulator (a workgroup's share
+    of the 2^16 matrix instructions along a row), so A is off by 2^-12 of
+    itself at worst, and the float32 chain's by no more if it splits the row
+    as far; a step scales that by its slope, 4 at most, and its terms count it
+    up to 4 times: under 4 2^-12 (1 + 4 + 16) = 2 % for the three steps."""
+    from federatedscope_amd import ops
+    t = torch.Generator(device='cuda').manual_seed(5)
+    g = torch.randn(1025, 4090 * 256, generator=t, device='cuda')
+    got = ops.newton_schulz(g, steps=3)
+    x = g / float(g.norm())
+    del g
+    for _ in range(3):
+        gram = x @ x.T
+        x = A * x + (B * gram + C * (gram @ gram)) @ x
+    got = (got - x).view(1025, 4090, 256).square().sum(-1)
+    x = x.view(1025, 4090, 256).square().sum(-1)
+    assert float((got / x).max()) <= 0.02**2
+
+
 @pytest.mark.parametrize('odt', DTYPES)
 def test_newton_schulz_out_type(odt):
     from federatedscope_amd import ops
@@ -215,19 +266,19 @@ def test_newton_schulz_refusals_on_device():
 
 
 # -- Muon ----------------------------------------------------------------------
-def _muon64(p, a, m, lr, mu, nesterov, wd, adjust, maximize):
+def _muon64(p, a, m, lr, mu, nesterov, wd, adjust, maximize, where='cpu'):
     p, a, m = (t.detach().cpu().double() for t in (p, a, m))
     g = (a - p) if maximize else (p - a)
     old = m
     m = m + (1 - mu) * (g - m)
     u = g + mu * (m - g) if nesterov else m
-    y = _chain(u, torch.float64)
-    off = float((_chain(u, torch.float32) - y).abs().max())
+    y = _chain(u, torch.float64, where=where)
+    off = float((_chain(u, torch.float32, where=where) - y).abs().max())
     rows, cols = p.shape
     k = 0.2 * math.sqrt(max(rows, cols)) if adjust == 'match_rms_adamw' \
         else math.sqrt(max(1.0, rows / cols))
     return (1 - lr * wd) * p - lr * k * y, m, lr * k * (
-        8 * off + _limb_error(u, 5, (A, B, C), 1e-7)), g, old
+        8 * off + _limb_error(u, 5, (A, B, C), 1e-7, where=where)), g, old
 
 
 @pytest.mark.parametrize('adjust', [None, 'original', 'match_rms_adamw'])
@@ -260,6 +311,31 @@ def test_muon_step(nesterov, maximize, mu, wd, adjust):
             ptol = tol + 2.0**-23 * (wp.abs() + (wp - p.cpu()).abs() +
                                      p.cpu().abs()) + 2.0**-23 * lr
             assert bool(((p.cpu().double() - wp).abs() <= ptol).all())
+
+
+@pytest.mark.parametrize('shapes', [
+    [(1200, 1300)] * 17, [(515, 4100), (4100, 515)], [(1100, 2600)],
+    [(2603, 1101)]])
+def test_muon_step_large(shapes):
+    """The large tiles (matrices 2 and on repeat the first two)."""
+    from federatedscope_amd import ops
+    ps = [_matrix(*s, seed=i % 2, scale=0.1).cuda()
+          for i, s in enumerate(shapes)]
+    avgs = [p - _matrix(*s, seed=40 + i % 2).cuda()
+            for i, (p, s) in enumerate(zip(ps, shapes))]
+    bs = [_matrix(*s, seed=80 + i % 2).cuda() for i, s in enumerate(shapes)]
+    want = [_muon64(p, a, b, 0.05, 0.9, True, 0.1, None, False, 'cuda')
+            for p, a, b in zip(ps[:2], avgs, bs)]
+    ops.muon_step(ps, avgs, bs, lr=0.05, momentum=0.9)
+    for p, b, (wp, wb, tol, g, old) in zip(ps, bs, want):
+        btol = 2.0**-24 * (wb.abs() + 2 * g.abs() + 3 * (g - old).abs())
+        assert bool(((b.cpu().double() - wb).abs() <= btol).all())
+        ptol = tol + 2.0**-23 * (wp.abs() + (wp - p.cpu()).abs() +
+                                 p.cpu().abs()) + 2.0**-23 * 0.05
+        assert bool(((p.cpu().double() - wp).abs() <= ptol).all())
+    for i in range(2, len(shapes)):
+        assert torch.equal(ps[i], ps[i % 2])
+        assert torch.equal(bs[i], bs[i % 2])
 
 
 def test_muon_agrees_with_torch_optim():
