@@ -1450,10 +1450,12 @@ int size_mat(Mat &M, int64_t rows, int64_t cols, int64_t batch,
   M.batch = int32_t(batch);
   M.m = int32_t(m);
   M.n = int32_t(n);
-  // a launch counts its work items in 32 bits: 64 x 64 tiles (the prepare
-  // pass has most) of all entries of a group
-  if (batch * (round_to(m, kBigSide) / 64) * (round_to(n, kBigSide) / 64) >
-      (int64_t(1) << 24) / kMaxGroup) {
+  // a launch counts its work items in 32 bits: workgroups of the update pass
+  // and 64 x 64 tiles of all entries of a group (where one workgroup takes a
+  // whole matrix, a batch has few enough)
+  if (!(m <= kNarrow && n <= 64 * kMaxWhole) &&
+      batch * (round_to(m, kBigSide) / 64) * (round_to(n, kBigSide) / 64) >
+          (int64_t(1) << 24) / kMaxGroup) {
     set_error("%s: a batch of %lld %lld x %lld matrices is too large for one "
               "call", what, (long long)batch, (long long)rows,
               (long long)cols);
@@ -1490,8 +1492,14 @@ void plan_mat(Mat &M, Way way) {
   const int64_t total = int64_t(M.rows) * M.cols;
   int64_t bytes;
   M.slabs = M.each = 1;
-  int64_t nb = (total + 4 * kNormBlock - 1) / (4 * kNormBlock);
-  M.nb = int32_t(nb > kMaxNorm ? kMaxNorm : nb);
+  // update workgroups of a matrix: 4 elements a thread while all of the batch
+  // are few, else 16 (no more of them than of 64 x 64 tiles)
+  const auto blocks = [&](int64_t each) {
+    const int64_t nb = (total + each - 1) / each;
+    return int32_t(nb > kMaxNorm ? kMaxNorm : nb);
+  };
+  M.nb = blocks(4 * kNormBlock);
+  if (int64_t(M.batch) * M.nb > 8 * kMaxNorm) M.nb = blocks(16 * kNormBlock);
   if (way == kWhole || way == kNarrowSlabs) {
     M.mp = kNarrow;
     M.np = int32_t(round_to(M.n, 64));

@@ -234,6 +234,26 @@ def test_newton_schulz_planes_past_two_gigabytes():
     assert float((got / x).max()) <= 0.02**2
 
 
+def test_newton_schulz_batches_of_many():
+    """As many matrices as a batch may hold (one, repeated with stride 0,
+    between two others)."""
+    from federatedscope_amd import ops
+    for rows, cols, batch in ((9, 14, 65535), (9, 300, 20000),
+                              (66, 70, 20000)):
+        a, b = _matrix(rows, cols, 1).cuda(), _matrix(rows, cols, 2).cuda()
+        g = a[None].expand(batch, -1, -1)
+        got = ops.newton_schulz(g)
+        one = ops.newton_schulz(a)
+        _check_ns(one, a)
+        _check_ns(got[0], a)
+        assert bool((got == got[0]).all())
+        g = g[:300].clone()
+        g[7] = b
+        got = ops.newton_schulz(g)
+        _check_ns(got[7], b)
+        _check_ns(got[8], a)
+
+
 @pytest.mark.parametrize('odt', DTYPES)
 def test_newton_schulz_out_type(odt):
     from federatedscope_amd import ops
@@ -613,6 +633,39 @@ def test_embedding_grad_is_the_lookups_gradient():
             tol = 2.0**-22 * max(1, n) * scale * (
                 float(up.abs().max()) * (2 + float(table.abs().max())))
             assert abs(fd - float(got[v, c])) <= tol
+
+
+def test_embedding_past_four_gigabytes():
+    """A table, and rows of tokens, whose offsets pass 32 bits."""
+    from federatedscope_amd import ops
+    vocab, dim = 1100000, 1000
+    table = torch.zeros(vocab, dim, device='cuda')
+    table[-3:] = torch.randn(3, dim, device='cuda')
+    ids = torch.tensor([vocab - 1, vocab - 3, 5, vocab, vocab - 1],
+                       device='cuda')
+    got = ops.embedding_lookup(table, ids)
+    assert torch.equal(got[[0, 1, 4]], table[[-1, -3, -1]])
+    assert not got[[2, 3]].any()
+    up = torch.randn(5, dim, device='cuda')
+    want = table[[-1, -3]] + torch.stack([up[0] + up[4], up[1]])
+    ops.embedding_grad(ids, up, vocab, out=table, accumulate=True)
+    assert (table[[-1, -3]] - want).abs().max() <= 2.0**-21
+    keep = table[-2].clone()
+    many = ids.repeat(200)
+    ops.embedding_grad(many, up.repeat(200, 1), vocab, out=table)
+    assert keep.any() and not table[-2].any() and not table[:5].any()
+    assert (table[5] - 200 * up[2]).abs().max() <= 200 * 2.0**-13
+    del table
+    rows = torch.zeros(vocab, dim, device='cuda')
+    rows[-2:] = torch.randn(2, dim, device='cuda')
+    ids = torch.arange(vocab, device='cuda') % 7
+    got = ops.embedding_grad(ids, rows, 7)
+    want = torch.zeros(7, dim, device='cuda')
+    want[ids[-2:]] = rows[-2:]
+    assert torch.equal(got, want)
+    out = torch.full((vocab, dim), 5.0, device='cuda')
+    assert ops.embedding_lookup(got, ids, out=out) is out
+    assert torch.equal(out[-7:], got[ids[-7:]])
 
 
 # -- streams and graphs ------------------------------------------------------------
