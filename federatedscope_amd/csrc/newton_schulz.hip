@@ -1466,24 +1466,30 @@ int size_mat(Mat &M, int64_t rows, int64_t cols, int64_t batch,
 
 bool empty(const Mat &M) { return M.m == 0 || M.batch == 0; }
 
-// Stages of the last product of an entry in big tiles.
-int64_t big_stages(const Mat &M) {
-  return M.batch * (round_to(M.m, kBigSide) / kBigSide) *
-         (round_to(M.n, kBigSide) / kBigSide) *
-         (round_to(M.m, kBigSide) / kBK);
+// What big tiles gain over 64 x 64 ones, in multiplications of an m x m by an
+// m x n matrix: 7 of the entry's own to 4 of its padded one, less what the
+// shorter pipelines of small tiles save (kBigGain, for all of the group).
+// Fitted to both sides of 25 shapes; big against small tiles, us: 512 x 16384
+// 580 / 556, 512 x 32768 911 / 1011, 640 x 10000 667 / 599, 1024 x 2048
+// 505 / 355, 1024 x 8192 772 / 911, 1100 x 4000 727 / 639, 1280 x 5120
+// 798 / 1113, 16 x (512 x 1024) 430 / 512; a short side of 384 loses at any
+// length (384 x 32768 862 / 676).
+constexpr int kBigShort = 512;
+constexpr int64_t kBigGain = 12500000000;
+int64_t big_gain(const Mat &M) {
+  if (empty(M) || M.m < kBigShort) return 0;
+  const int64_t m = M.m, n = M.n, mp = round_to(m, kBigSide),
+                np = round_to(n, kBigSide);
+  const int64_t gain = 7 * (m * m * n) - 4 * (mp * mp * np);
+  return gain > 0 ? gain * M.batch : 0;
 }
 
-// Big tiles pay from about 8 stages for each of the 256 workgroups on.
-constexpr int64_t kBigStages = 2048;
-constexpr int kBigShort = 512;
-
-Way way_of(const Mat &M, const int64_t (&work)[2]) {
+Way way_of(const Mat &M, const int64_t (&gain)[2]) {
+  // narrow against 64 x 64 tiles, us: 50 x 1024 53 / 87, 50 x 16384 150 / 199
   if (M.m <= kNarrow && M.n <= kNarrowLong)
     return M.n <= 64 * kMaxWhole ? kWhole : kNarrowSlabs;
-  if (M.m >= kBigShort) {
-    const int one = M.odt == FSAGG_BF16;
-    if (work[one] >= kBigStages) return one ? kBigOne : kBig;
-  }
+  const int one = M.odt == FSAGG_BF16;
+  if (big_gain(M) > 0 && gain[one] >= kBigGain) return one ? kBigOne : kBig;
   return kMid;
 }
 
@@ -1752,13 +1758,12 @@ void run_group(Group &G, Way way, float *partial, const Step &st) {
 // and pointers.
 template <typename Fill, typename F>
 int each_group(int nmat, Fill fill, Group &G, F f) {
-  int64_t work[2] = {0, 0};
+  int64_t gain[2] = {0, 0};
   for (int i = 0; i < nmat; ++i) {
     Mat M;
     const int rc = fill(i, M);
     if (rc != FSAGG_OK) return rc;
-    if (!empty(M) && M.m >= kBigShort)
-      work[M.odt == FSAGG_BF16] += big_stages(M);
+    gain[M.odt == FSAGG_BF16] += big_gain(M);
   }
   for (int way = 0; way < kWays; ++way) {
     G.nmat = 0;
@@ -1766,7 +1771,7 @@ int each_group(int nmat, Fill fill, Group &G, F f) {
     for (int i = 0; i < nmat; ++i) {
       Mat &M = G.mat[G.nmat];
       fill(i, M);
-      if (empty(M) || way_of(M, work) != way) continue;
+      if (empty(M) || way_of(M, gain) != way) continue;
       plan_mat(M, Way(way));
       bytes += size_t(M.wstride) * M.batch;
       if (++G.nmat == kMaxGroup) {

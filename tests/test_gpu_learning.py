@@ -94,7 +94,7 @@ def _check_ns(got, g, steps=5, coef=(A, B, C), eps=1e-7, one=False,
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 200), (62, 2048), (2048, 62),
           (63, 65), (64, 64), (128, 128), (129, 127), (130, 700),
-          (300, 1000), (1000, 300), (257, 513)]
+          (300, 1000), (1000, 300), (257, 513), (515, 4100), (2603, 1101)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
@@ -193,8 +193,8 @@ def test_newton_schulz_list_of_many():
 
 # the large tiles: whole 256 x 256 ones, shared ones with their joins, 128 x
 # 128 ones; sizes that end inside a tile
-LARGE = [(17, 1200, 1300), (1, 1200, 13000), (2, 515, 4100), (2, 4100, 515),
-         (1, 1100, 2600), (1, 2603, 1101)]
+LARGE = [(17, 1200, 1300), (1, 1200, 13000), (2, 760, 8100), (2, 8100, 760),
+         (1, 1270, 7100), (1, 7103, 1269)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
@@ -334,8 +334,8 @@ def test_muon_step(nesterov, maximize, mu, wd, adjust):
 
 
 @pytest.mark.parametrize('shapes', [
-    [(1200, 1300)] * 17, [(515, 4100), (4100, 515)], [(1100, 2600)],
-    [(2603, 1101)]])
+    [(1200, 1300)] * 17, [(760, 8100), (8100, 760)], [(1270, 7100)],
+    [(7103, 1269)]])
 def test_muon_step_large(shapes):
     """The large tiles (matrices 2 and on repeat the first two)."""
     from federatedscope_amd import ops
