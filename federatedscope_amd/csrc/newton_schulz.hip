@@ -15,11 +15,25 @@
 // error 1e-6 .. 8e-6 against 64 bits by spectrum, both) at 3/16 of the cost
 // per product: 16-bit limbs run at 16 times the fp32 matrix rate.
 //
+// A bf16 result of matrices large enough for big tiles takes the high limbs'
+// product alone (aX keeps both limbs): its error against 64 bits is 1.9e-3 ..
+// 2.2e-3 for decaying spectra, where rounding the exact result to bf16 leaves
+// 1.66e-3 (2.6e-3 .. 4e-3 where all singular values are nearly equal), for a
+// third of the matrix work.  fp16 results, 8 times finer, keep both.
+//
 // A = X X^T and A^2 are products C = P R^T with both operands contiguous along
 // k; A and Q are symmetric: the tiles on and above the diagonal are computed
 // and stored twice.  QX is computed as (QX)^T = X^T Q with X's fragments read
 // transposed from LDS, so that X is kept in one orientation and a lane's
-// results lie side by side in it.
+// results lie side by side in it (against X kept both ways: 4096 x 8192
+// 7.36 -> 7.18 ms, 12 matrices' Muon step 2.23 -> 2.09).
+//
+// What bounds it: large matrices the matrix cores (4096 x 8192, QX 0.69 ms =
+// 1.2 PFLOP/s of limb products, a library fp16 product of 8192^3 reaches
+// 1.24) and, where the short side is 1024, the tiles' ends, which move 8 B a
+// value through the caches with no product to hide them; middle ones the
+// reads from L2 and three to five launches a step; narrow ones the latency
+// of a chain of one launch a step.
 #include "common.h"
 
 #include <hip/hip_fp16.h>
@@ -1410,11 +1424,12 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
 }
 
 // -- host --------------------------------------------------------------------
-// Tiles: 256 x 256 keeps a CU's matrix cores at about 80 % of what a large
+// Tiles: 256 x 256 keeps a CU's matrix cores at up to 95 % of what a large
 // library product reaches, where there is work for all of them; 128 x 128,
-// two workgroups to a CU, takes products that leave the last round of those
-// too empty (below); 64 x 64 is for matrices too small for that, where a
-// tile's latency counts.  One limb suffices for a bf16 result (below).
+// two workgroups to a CU, is bound by its reads (of LDS, and twice the L2
+// traffic), but takes products that leave the last round of large ones too
+// empty (below); 64 x 64 is for matrices too small for that, where a tile's
+// latency counts.  One limb suffices for a bf16 result (above).
 using BigTile = Tile<256, 256, 128, 64, 2, 2>;
 using BigTile1 = Tile<256, 256, 128, 64, 4, 1>;
 using HalfTile = Tile<128, 128, 64, 64, 2, 2>;
@@ -1636,7 +1651,11 @@ void launch_whole(Group &G, int src, const Step &st) {
 // kMinStages of them.  Sharing saves the stages that the last round of whole
 // tiles (or the longest tile, where there are fewer tiles than workgroups)
 // leaves idle, and costs a join: parts written and read again, about
-// kJoinStages stages' time with either tile.
+// kJoinStages stages' time with either tile (256 x 256: line and join 79 us
+// where A of 2048 x 3136 has 36 tiles of 98 stages, 290 us whole at 2.9 us a
+// stage; 128 x 128 shared: 70 + 15 us there, so those are only taken whole,
+// as for QX there, 125 us shared -> 105, or for A^2 of 12 matrices of 1024,
+// 94 us shared -> 64).
 constexpr int kMinStages = 8, kJoinStages = 16, kTileEnd = 9;
 template <class T, int MODE, class H = void>
 void launch_product(Group &G, int workers, float *partial, int src,

@@ -194,7 +194,7 @@ def test_newton_schulz_list_of_many():
 # the large tiles: whole 256 x 256 ones, shared ones with their joins, 128 x
 # 128 ones; sizes that end inside a tile
 LARGE = [(17, 1200, 1300), (1, 1200, 13000), (2, 760, 8100), (2, 8100, 760),
-         (1, 1270, 7100), (1, 7103, 1269)]
+         (1, 1270, 7100), (1, 7103, 1269), (8, 1000, 1010)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
