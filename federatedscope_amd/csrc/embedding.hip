@@ -20,7 +20,7 @@
 // row once and write each result row once (65536 x 2048 bf16 into 128000
 // rows, 0.79 GB, 183 us = 4.3 TB/s, the sum alone 142 us; 100 clients' 400
 // rows of 1024 fp32 added into 50000, 0.26 GB, 88 us, of which the sum is
-// 52 and the sort 27; a lookup of 65536 x 1024 bf16 34 us).  Small calls are
+// 52 and the sort 27; a lookup of 16384 x 4096 bf16 34 us).  Small calls are
 // bound by their launches (9 .. 30 us).
 #include "common.h"
 
@@ -110,7 +110,7 @@ __device__ __forceinline__ void load_vec(const void *p, float (&v)[VEC]) {
 }
 // (zero rows and token rows go by once: non-temporal, 65536 x 2048 bf16 into
 // 128000 rows 218 -> 182 us, 100 x 400 fp32 rows of 1024 108 -> 92 us; a
-// lookup of 65536 x 1024 bf16 45 -> 35 us.  The few rows with a sum lost by it:
+// lookup of 16384 x 4096 bf16 45 -> 35 us.  The few rows with a sum lost by it:
 // 183 -> 196 us)
 template <int DT, int VEC>
 __device__ __forceinline__ void store_zero(void *p) {
