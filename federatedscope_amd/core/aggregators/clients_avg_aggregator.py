@@ -9,6 +9,7 @@ from collections import OrderedDict
 
 import torch
 
+from ... import _lib as L
 from ... import ops
 from ..auxiliaries.utils import param2tensor
 from ._engine import DeviceEngine, _first_device, fedavg_weights
@@ -137,7 +138,8 @@ class ClientsAvgAggregator(DeviceEngine, _ModelIO, Aggregator):
 
 def sparse_keys(model):
     """The keys of a client's dict that are sparse COO tensors."""
-    if not isinstance(model, dict):      # a StagedUpdate holds dense rows
+    # (a StagedUpdate is no dict: it holds dense rows)
+    if not isinstance(model, dict) or not L.host().has_sparse(model):
         return ()
     return [k for k, v in model.items()
             if getattr(v, 'is_sparse', False)]
@@ -193,7 +195,6 @@ class OnlineClientsAvgAggregator(ClientsAvgAggregator):
 
     def _typed_inc(self, k, m, x, sample_size):
         """One key through fsagg_online_inc_typed; returns the new value."""
-        from ... import _lib as L
         if m.dtype not in _DT_CODE or x.dtype not in _DT_CODE:
             raise TypeError('online aggregation of %s/%s key %r' %
                             (m.dtype, x.dtype, k))

@@ -135,7 +135,8 @@ class AggregationServer:
         on the compute device — what a client that trains a few rows of a
         large table is sent instead of the whole of it (the reference
         broadcasts whole state dicts, server.py:636-714); it answers with a
-        row-sparse update (ClientsAvgAggregator)."""
+        row-sparse update (ClientsAvgAggregator).  A model that lies on the
+        host has the whole table copied to the device by each call."""
         dev = compute_device(self.device)
         table = self.models[model_idx].state_dict()[key].to(dev)
         return ops.embedding_lookup(table, ids.to(dev).contiguous(),

@@ -14,6 +14,9 @@
 // None is not an error: some pair is not of the plain form (contiguous int64
 // or int32 tokens; strided float32, float16 or bfloat16 rows of one type and
 // width on the tokens' GPU), and the caller's own checks say why.
+//
+// has_sparse(dict) -> bool: whether a value is a sparse COO tensor (asked of
+// every upload, most of which have none: 161 keys 2 us, 19 us in Python).
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
 #include <Python.h>
@@ -122,4 +125,15 @@ PyObject *embed_parts(PyObject *, PyObject *args) {
   } catch (...) {
     Py_RETURN_NONE;
   }
+}
+
+PyObject *has_sparse(PyObject *, PyObject *dict) {
+  if (!PyDict_Check(dict)) Py_RETURN_FALSE;
+  PyObject *key, *value;
+  Py_ssize_t pos = 0;
+  while (PyDict_Next(dict, &pos, &key, &value)) {
+    const c10::TensorImpl *t = tensor_of(value);
+    if (t && t->is_sparse()) Py_RETURN_TRUE;
+  }
+  Py_RETURN_FALSE;
 }

@@ -45,7 +45,9 @@ PyObject *b64_frame(PyObject *, PyObject *args);
 PyObject *b64_frame_many(PyObject *, PyObject *args);
 // host/krumcert.cpp: the Krum selection certificate
 PyObject *gram_select(PyObject *, PyObject *args);
+// host/embedparts.cpp: row-sparse uploads
 PyObject *embed_parts(PyObject *, PyObject *args);
+PyObject *has_sparse(PyObject *, PyObject *dict);
 
 namespace {
 
@@ -710,6 +712,8 @@ PyMethodDef kMethods[] = {
     {"embed_parts", embed_parts, METH_VARARGS,
      "embed_parts(ids, grads, coefs, out_lo, out_hi) -> (table, tokens, dim, "
      "dtype_code) or None"},
+    {"has_sparse", has_sparse, METH_O,
+     "has_sparse(dict) -> whether a value is a sparse COO tensor"},
     {"key_table", key_table, METH_VARARGS,
      "key_table(dicts, keys, shapes, device_index[, offs4]) -> (bytes, "
      "missing, aligned16) or None"},

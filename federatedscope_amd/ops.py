@@ -1775,7 +1775,9 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7,
     float32, float16 or bfloat16, any strides.  Returns a new contiguous
     tensor (list) of g's dtype, or ``out`` (contiguous, of any of the three
     dtypes, not overlapping any input).  The arithmetic is as exact as
-    float32 products.  NaN or infinity anywhere in a matrix makes all of it
+    float32 products; for a bfloat16 result of large matrices its error is
+    about that of rounding to that type (which matrices share a call decides
+    what is large, so it may change the result by as much).  NaN or infinity anywhere in a matrix makes all of it
     NaN; a zero matrix stays zero.  Not differentiable."""
     many = isinstance(g, (list, tuple))
     gs = list(g) if many else [g]
