@@ -531,7 +531,7 @@ __device__ __forceinline__ int line_at(const Line &L, int q) {
 // the workspace; only the last step checks its stores against the matrix.
 template <int BM, int BN, int WM, int WN, int NBUF, int LIMBS>
 struct Tile {
-  static constexpr int kBM = BM, kBN = BN;
+  static constexpr int kBM = BM, kBN = BN, kLimbs = LIMBS;
   static constexpr int kWaves = (BM / WM) * (BN / WN);
   static constexpr int kThreads = kWaves * 64;
   static constexpr int MI = WM / 32, NJ = WN / 32;
@@ -1435,8 +1435,9 @@ using BigTile1 = Tile<256, 256, 128, 64, 4, 1>;
 using HalfTile = Tile<128, 128, 64, 64, 2, 2>;
 using HalfTile1 = Tile<128, 128, 64, 64, 4, 1>;
 using MidTile = Tile<64, 64, 32, 32, 4, 2>;
-constexpr int kBigWorkers = 256;   // one workgroup of a big tile per CU
-constexpr int kMidWorkers = 512;
+// workgroups that the GPU holds: one of a 256 x 256 tile per CU, two of the
+// others
+constexpr int kBigPlaces = 256, kMidPlaces = 512;
 constexpr int kBigSide = 256, kMidSide = 64;
 
 // How an entry is computed: in one launch, by slabs, or by tiled products.
@@ -1483,14 +1484,16 @@ bool empty(const Mat &M) { return M.m == 0 || M.batch == 0; }
 
 // What big tiles gain over 64 x 64 ones, in multiplications of an m x m by an
 // m x n matrix: 7 of the entry's own to 4 of its padded one, less what the
-// shorter pipelines of small tiles save (kBigGain, for all of the group).
-// Fitted to both sides of 25 shapes; big against small tiles, us: 512 x 16384
-// 580 / 556, 512 x 32768 911 / 1011, 640 x 10000 667 / 599, 1024 x 2048
-// 505 / 355, 1024 x 8192 772 / 911, 1100 x 4000 727 / 639, 1280 x 5120
-// 798 / 1113, 16 x (512 x 1024) 430 / 512; a short side of 384 loses at any
-// length (384 x 32768 862 / 676).
+// shorter pipelines of small tiles save (kBigGain, for all of the group; of
+// one limb less of them is enough).  Fitted to both sides of 35 shapes; big
+// against small tiles, us: 512 x 16384 594 / 559, 512 x 32768 941 / 1022,
+// 1024 x 4096 573 / 488, 1024 x 8192 807 / 875, 1280 x 2560 677 / 518,
+// 1280 x 5120 860 / 907, 2048 x 2048 917 / 942, 2 x (1500 x 1500) 807 / 909,
+// 12 x (1024 x 1024) 1018 / 1335; a short side of 384 loses at any length
+// (384 x 32768 879 / 682).  bf16: 1024 x 2048 325 / 289, 768 x 4096 331 / 375,
+// 1536 x 1536 403 / 628.
 constexpr int kBigShort = 512;
-constexpr int64_t kBigGain = 12500000000;
+constexpr int64_t kBigGain[2] = {17500000000, 6500000000};
 int64_t big_gain(const Mat &M) {
   if (empty(M) || M.m < kBigShort) return 0;
   const int64_t m = M.m, n = M.n, mp = round_to(m, kBigSide),
@@ -1504,7 +1507,7 @@ Way way_of(const Mat &M, const int64_t (&gain)[2]) {
   if (M.m <= kNarrow && M.n <= kNarrowLong)
     return M.n <= 64 * kMaxWhole ? kWhole : kNarrowSlabs;
   const int one = M.odt == FSAGG_BF16;
-  if (big_gain(M) > 0 && gain[one] >= kBigGain) return one ? kBigOne : kBig;
+  if (big_gain(M) > 0 && gain[one] >= kBigGain[one]) return one ? kBigOne : kBig;
   return kMid;
 }
 
@@ -1527,8 +1530,9 @@ void plan_mat(Mat &M, Way way) {
     const int chunks = M.np / 64;
     // a launch reads 16 KiB of Gram shares per slab into every workgroup,
     // and works its chunks one after the other: 8 slabs' shares cost about
-    // what a chunk does
-    M.each = way == kWhole ? 1 : chunks <= 32 ? 1 : chunks <= 96 ? 2 : 4;
+    // what a chunk does (1 / 2 / 4 chunks a slab, us: 50 x 1500 62 / 64 / -,
+    // 50 x 1984 70 / 67 / -, 50 x 4096 106 / 85 / 95, 50 x 8192 178 / - / 113)
+    M.each = way == kWhole ? 1 : chunks <= 28 ? 1 : chunks <= 96 ? 2 : 4;
     M.slabs = (chunks + M.each - 1) / M.each;
     bytes = way == kWhole ? 0
                           : 8 * kMaxNorm +
@@ -1549,9 +1553,9 @@ int64_t partial_bytes(Way way) {
   switch (way) {
     case kBig:
     case kBigOne:
-      return int64_t(2) * kBigWorkers * kBigSide * kBigSide * 4;
+      return int64_t(2) * kBigPlaces * kBigSide * kBigSide * 4;
     case kMid:
-      return int64_t(2) * kMidWorkers * kMidSide * kMidSide * 4;
+      return int64_t(2) * kMidPlaces * kMidSide * kMidSide * 4;
     default:
       return 0;
   }
@@ -1604,12 +1608,6 @@ struct Step {
 struct Count {
   int64_t tiles = 0, stages = 0;
   int longest = 0;
-  // stages that the busiest of `workers` places works, a tile to a workgroup
-  int64_t whole(int workers) const {
-    const int64_t rounds = (tiles + workers - 1) / workers;
-    const int64_t s = rounds * (stages / tiles);
-    return s > longest ? s : longest;
-  }
 };
 template <class T, int MODE>
 Count count_tiles(const Group &G) {
@@ -1646,38 +1644,74 @@ void launch_whole(Group &G, int src, const Step &st) {
                      st.c, st.S);
 }
 
-// One product of the whole group: one workgroup per tile, or the line of
-// stages shared by as many workgroups as the GPU holds, each with at least
-// kMinStages of them.  Sharing saves the stages that the last round of whole
-// tiles (or the longest tile, where there are fewer tiles than workgroups)
-// leaves idle, and costs a join: parts written and read again, about
-// kJoinStages stages' time with either tile (256 x 256: line and join 79 us
-// where A of 2048 x 3136 has 36 tiles of 98 stages, 290 us whole at 2.9 us a
-// stage; 128 x 128 shared: 70 + 15 us there, so those are only taken whole,
-// as for QX there, 125 us shared -> 105, or for A^2 of 12 matrices of 1024,
-// 94 us shared -> 64).
-constexpr int kMinStages = 8, kJoinStages = 16, kTileEnd = 9;
+// One product of the whole group: one workgroup per tile, of either size, or
+// the line of stages shared by as many workgroups as the GPU holds (`places`),
+// each with at least kMinStages of them.  Whole tiles leave places idle in
+// the last round; sharing fills them, but its workgroups walk the operands
+// at different stages, so less of what they read is in the caches, and a join
+// writes parts and reads them again.  What is expected to take least is
+// taken, by times fitted to some 30 shapes with either way measured
+// (us: A of 4096 x 4096 whole 251, shared 276, halved 284; A of 2048 x 3136
+// 175 / 70 / 87; QX there 136 / 112 / 91; A^2 of 12 matrices of 1024 79 / 89 /
+// 54; 64 x 64 tiles, A of 1000 x 1000 12 / 20, of 512 x 3136 31 / 21):
+//   s0, s1  a stage, with none of the places taken and what all add (clocks
+//           and caches are shared; half of it grows with the square),
+//   e0, e1  a tile's end, as much,
+//   l0, l1  a stage of the line,  j0, j1  the join;  kPart each part of a tile.
+struct Cost {
+  double s0, s1, e0, e1, l0, l1, j0, j1;
+};
+template <class T>
+constexpr Cost cost_of() {
+  if (T::kBM == 256)
+    return T::kLimbs == 2 ? Cost{1.5, 0.9, 7, 20, 1.8, 1.6, 8, 22}
+                          : Cost{0.5, 0.6, 7, 20, 0.65, 0.6, 8, 22};
+  if (T::kBM == 128)
+    return T::kLimbs == 2 ? Cost{0.65, 0.75, 4, 9, 0, 0, 0, 0}
+                          : Cost{0.2, 0.53, 4, 9, 0, 0, 0, 0};
+  return Cost{0.25, 0.31, 4, 4, 0.3, 0.4, 8, 8};
+}
+constexpr int kMinStages = 8;
+constexpr double kPart = 0.3;
+
+double whole_time(const Count &n, int places, const Cost &c) {
+  const auto round = [&](double f, double stages) {
+    return stages * (c.s0 + c.s1 * (f + f * f) / 2) + c.e0 + c.e1 * f;
+  };
+  const double each = double(n.stages) / double(n.tiles);
+  const int64_t left = n.tiles % places;
+  const double t = double(n.tiles / places) * round(1.0, each) +
+                   (left ? round(double(left) / places, each) : 0.0);
+  const double most =
+      round(n.tiles < places ? double(n.tiles) / places : 1.0, n.longest);
+  return t > most ? t : most;
+}
+double line_time(const Count &n, int64_t workers, int places, const Cost &c) {
+  const double f = double(workers) / places,
+               each = double(n.stages) / double(workers);
+  return each * (c.l0 + c.l1 * f) + c.j0 + c.j1 * f +
+         double(n.tiles / workers) * (c.e0 + c.e1) +
+         kPart * double(n.longest) / each;
+}
+
 template <class T, int MODE, class H = void>
-void launch_product(Group &G, int workers, float *partial, int src,
+void launch_product(Group &G, int places, float *partial, int src,
                     const Step &st) {
   const Count n = count_tiles<T, MODE>(G);
   int64_t w = n.stages / kMinStages;
-  if (w > workers) w = workers;
-  if (w < 1) w = 1;
-  const bool share = n.whole(workers) - n.stages / w > kJoinStages;
+  if (w > places) w = places;
+  const double whole = whole_time(n, places, cost_of<T>());
+  const double line =
+      w > 1 ? line_time(n, w, places, cost_of<T>()) : whole;
   if constexpr (!std::is_void<H>::value) {
-    // A stage of half the tile, two workgroups to a CU, takes 1/1.8 of the
-    // time of one (2.9 -> 1.6 us, two limbs), a tile's end about 9 stages
-    // with either.
-    const int64_t mine = share ? n.stages / w + kJoinStages
-                               : n.whole(workers) + kTileEnd;
-    const Count m = count_tiles<H, MODE>(G);
-    if (m.whole(2 * workers) + kTileEnd < mine * 9 / 5) {
+    const double half =
+        whole_time(count_tiles<H, MODE>(G), 2 * places, cost_of<H>());
+    if (half < whole && half < line) {
       launch_whole<H, MODE>(G, src, st);
       return;
     }
   }
-  if (!share) {
+  if (whole <= line) {
     launch_whole<T, MODE>(G, src, st);
     return;
   }
@@ -1696,7 +1730,7 @@ void launch_product(Group &G, int workers, float *partial, int src,
 }
 
 template <class T, bool MUON, class H = void>
-void run_products(Group &G, int workers, float *partial, const Step &st) {
+void run_products(Group &G, int places, float *partial, const Step &st) {
   int total = 0;
   for (int i = 0; i < G.nmat; ++i) {
     G.start[i] = total;
@@ -1715,12 +1749,12 @@ void run_products(Group &G, int workers, float *partial, const Step &st) {
                      G, st.eps);
   int src = 0;
   for (int k = 0; k < st.steps; ++k, src ^= 1) {
-    launch_product<T, kGram, H>(G, workers, partial, src, st);
-    launch_product<T, kSquare, H>(G, workers, partial, src, st);
+    launch_product<T, kGram, H>(G, places, partial, src, st);
+    launch_product<T, kSquare, H>(G, places, partial, src, st);
     if (k + 1 < st.steps)
-      launch_product<T, kApply, H>(G, workers, partial, src, st);
+      launch_product<T, kApply, H>(G, places, partial, src, st);
     else
-      launch_product<T, MUON ? kLastMuon : kLast, H>(G, workers, partial, src,
+      launch_product<T, MUON ? kLastMuon : kLast, H>(G, places, partial, src,
                                                      st);
   }
 }
@@ -1765,11 +1799,11 @@ void run_group(Group &G, Way way, float *partial, const Step &st) {
   if (way == kWhole) run_whole<MUON>(G, st);
   else if (way == kNarrowSlabs) run_narrow<MUON>(G, st);
   else if (way == kMid)
-    run_products<MidTile, MUON>(G, kMidWorkers, partial, st);
+    run_products<MidTile, MUON>(G, kMidPlaces, partial, st);
   else if (way == kBig)
-    run_products<BigTile, MUON, HalfTile>(G, kBigWorkers, partial, st);
+    run_products<BigTile, MUON, HalfTile>(G, kBigPlaces, partial, st);
   else if constexpr (!MUON)  // (a parameter is fp32)
-    run_products<BigTile1, MUON, HalfTile1>(G, kBigWorkers, partial, st);
+    run_products<BigTile1, MUON, HalfTile1>(G, kBigPlaces, partial, st);
 }
 
 // f(group, way, bytes of its entries) for every group of entries, in turn;
