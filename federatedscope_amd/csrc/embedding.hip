@@ -108,15 +108,9 @@ template <int DT, int VEC>
 __device__ __forceinline__ void load_vec(const void *p, float (&v)[VEC]) {
   widen<DT, VEC>(load_raw<DT, VEC>(p), v);
 }
-// (zero rows and token rows go by once: non-temporal, 65536 x 2048 bf16 into
-// 128000 rows 218 -> 182 us, 100 x 400 fp32 rows of 1024 108 -> 92 us; a
-// lookup of 16384 x 4096 bf16 45 -> 35 us.  The few rows with a sum lost by it:
-// 183 -> 196 us)
-template <int DT, int VEC>
-__device__ __forceinline__ void store_zero(void *p) {
-  __builtin_nontemporal_store(typename Raw<DT, VEC>::type{},
-                              static_cast<typename Raw<DT, VEC>::type *>(p));
-}
+// (rows that go by once bypass the caches, NT here and gld_nt: a lookup of
+// 16384 x 4096 bf16 45 -> 35 us, the rows of 100 x 400 tokens of 1024 fp32
+// 108 -> 92; the sums' own rows lost by it, 65536 x 2048 bf16 183 -> 196)
 template <int DT, int VEC, bool NT = false>
 __device__ __forceinline__ void store_vec(void *p, const float (&v)[VEC]) {
   typename Raw<DT, VEC>::type x;
@@ -617,7 +611,7 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
 struct Out {
   char *out;
   int64_t row_bytes, dim, vocab, tokens;
-  int chunk, slices, accumulate;
+  int chunk, slices, accumulate, zero_nt;
   int64_t chunks;
   const uint32_t *key;
 };
@@ -663,6 +657,44 @@ __device__ __forceinline__ void wave_bounds(const uint32_t *key, int64_t n,
 }
 
 constexpr int kZeroRows = kBlock;  // most rows of a zero workgroup
+
+// Zeros into the rows [r0, r1) that are not named, by the whole workgroup:
+// `g` lanes a row, 16 bytes a lane whatever the row's alignment, single
+// elements before and behind.
+template <int OT>
+__device__ __forceinline__ void zero_rows_of(const Out &O, int64_t r0,
+                                             int64_t r1,
+                                             const uint8_t *named) {
+  using T = typename Elem<OT>::type;
+  constexpr int kOE = sizeof(T);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave =
+      __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int64_t bytes = O.dim * kOE;
+  int g = kWave;
+  while (g > 1 && bytes <= int64_t(g / 2) * 16) g /= 2;
+  const int l = lane & (g - 1), sub = lane / g, rows = kWave / g;
+  for (int64_t r = r0 + wave * rows + sub; r < r1; r += kWaves * rows) {
+    if (named[r - r0]) continue;
+    char *p = O.out + r * O.row_bytes;
+    const int64_t head =
+        int64_t(-reinterpret_cast<uint64_t>(p) & 15) < bytes
+            ? int64_t(-reinterpret_cast<uint64_t>(p) & 15)
+            : bytes;
+    const int64_t body = head + ((bytes - head) & ~int64_t(15));
+    if (O.zero_nt)
+      for (int64_t c = head + l * 16; c < body; c += g * 16)
+        __builtin_nontemporal_store(u32x4{0, 0, 0, 0},
+                                    reinterpret_cast<u32x4 *>(p + c));
+    else
+      for (int64_t c = head + l * 16; c < body; c += g * 16)
+        *reinterpret_cast<u32x4 *>(p + c) = u32x4{0, 0, 0, 0};
+    for (int64_t c = l * kOE; c < head; c += g * kOE)
+      *reinterpret_cast<T *>(p + c) = T(0);
+    for (int64_t c = body + l * kOE; c < bytes; c += g * kOE)
+      *reinterpret_cast<T *>(p + c) = T(0);
+  }
+}
 // (keys of a stretch that are looked at one by one: 15003 of 4 stretches save
 // 0.5 us against the search, 65536 of 2 would lose 7)
 constexpr int64_t kScanKeys = 32 * kBlock;
@@ -710,12 +742,7 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
       named[threadIdx.x] = lo < b && O.key[lo] == r;
     }
     __syncthreads();
-    for (int64_t r = r0 + wave; r < r1; r += kWaves) {
-      if (named[r - r0]) continue;
-      char *dst = O.out + r * O.row_bytes;
-      for (int64_t c = int64_t(lane) * VEC; c < O.dim; c += kWave * VEC)
-        store_zero<OT, VEC>(dst + c * kOE);
-    }
+    zero_rows_of<OT>(O, r0, r1, named);
     return;
   }
   const int64_t unit = int64_t(blockIdx.x) * kWaves + wave;
@@ -852,12 +879,7 @@ __global__ __launch_bounds__(kBlock) void embed_few_kernel(Parts P, Out O,
     const int64_t r1 = r0 + zero_rows < O.vocab ? r0 + zero_rows : O.vocab;
     if (t < tokens && int64_t(k) >= r0 && int64_t(k) < r1) named[k - r0] = 1;
     __syncthreads();
-    for (int64_t r = r0 + wave; r < r1; r += kWaves) {
-      if (named[r - r0]) continue;
-      char *dst = O.out + r * O.row_bytes;
-      for (int64_t c = int64_t(lane) * VEC; c < O.dim; c += kWave * VEC)
-        store_zero<OT, VEC>(dst + c * kOE);
-    }
+    zero_rows_of<OT>(O, r0, r1, named);
     return;
   }
   if (t < tokens) {
@@ -1187,13 +1209,21 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   O.chunk = int(Z.chunk);
   O.chunks = Z.chunks;
   O.accumulate = accumulate;
+  // zeros go past the caches where they would fill the last one (256 MiB) and
+  // many rows are read meanwhile (past / through, us: 128000 rows of 1024
+  // fp32, 65536 tokens 180 / 196; of 2048, 32768 tokens 271 / 282, 8192 238 /
+  // 235, 48 184 / 180; of 300, 32768 tokens 80 / 74)
+  O.zero_nt = vocab * dim * oe >= int64_t(1) << 28 && tokens >= vocab / 8;
   const int v = vec ? vec_elems : 1;
   O.slices = int((dim + int64_t(kWave) * v - 1) / (int64_t(kWave) * v));
   const bool few = tokens <= kFew && one_launch;
   const int64_t sum_units = few ? tokens : Z.chunks;
   const int64_t sum_blocks = (sum_units * O.slices + kWaves - 1) / kWaves;
-  // rows per zero workgroup: about 64 KiB
-  int64_t zero_rows = 65536 / (dim * oe);
+  // rows per zero workgroup: about 64 KiB, or 256 KiB where that leaves
+  // enough of them (128000 rows of 2048 fp32, 48 tokens: 191 / 180 us; 4000
+  // rows of 300 10.8 / 16)
+  int64_t zero_rows =
+      (vocab * dim * oe >> 29 ? 262144 : 65536) / (dim * oe);
   if (zero_rows < kWaves) zero_rows = kWaves;
   if (zero_rows > kZeroRows) zero_rows = kZeroRows;
   const int64_t zero_blocks =

@@ -580,6 +580,32 @@ def test_embedding_grad_does_not_read_padding():
     assert int(got.isfinite().logical_not().sum()) == 2
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [1, 2, 3, 5, 7, 8, 9, 17, 31, 64, 129, 1031])
+def test_embedding_grad_zero_rows(dim, dtype):
+    """Every byte of the rows that no token names, and no byte beside them:
+    odd widths, rows apart, a start at any element; few and many tokens."""
+    from federatedscope_amd import ops
+    for tokens, vocab in ((3, 50), (900, 1500)):
+        for off in (0, 1, 3):
+            buf = torch.full((vocab, dim + 5), 7.0, dtype=dtype,
+                             device='cuda')
+            flat = torch.full((vocab * dim + 8, ), 7.0, dtype=dtype,
+                              device='cuda')
+            ids = _ids(tokens, vocab, dim + off)
+            grad = torch.randn(tokens, dim, device='cuda').to(dtype)
+            out = buf[:, off:off + dim]
+            ops.embedding_grad(ids, grad, vocab, out=out)
+            _check_grad(out, [ids], [grad], vocab)
+            assert bool((buf[:, :off] == 7).all())
+            assert bool((buf[:, off + dim:] == 7).all())
+            out = flat[off:off + vocab * dim].view(vocab, dim)
+            ops.embedding_grad(ids, grad, vocab, out=out)
+            _check_grad(out, [ids], [grad], vocab)
+            assert bool((flat[:off] == 7).all())
+            assert bool((flat[off + vocab * dim:] == 7).all())
+
+
 def test_embedding_grad_views():
     from federatedscope_amd import ops
     ids = _ids(80, 30, 1)
