@@ -382,6 +382,51 @@ __device__ __forceinline__ void digit_starts(int digits, F v, uint32_t *at,
   __syncthreads();
 }
 
+// The result, and how it is cut.
+struct Out {
+  char *out;
+  int64_t row_bytes, dim, vocab, tokens;
+  int chunk, slices, accumulate, elem;
+  int zero_nt, zero_rows;  // rows per zero workgroup
+  int64_t chunks;
+  const uint32_t *key;
+};
+
+// Zeros into the rows [r0, r1) that are not named (null: into all), by the
+// whole workgroup: `g` lanes a row, 16 bytes a lane whatever the row's
+// alignment, 2 bytes at a time before and behind.
+template <int TH>
+__device__ __forceinline__ void zero_rows_of(const Out &O, int64_t r0,
+                                             int64_t r1,
+                                             const uint8_t *named) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave =
+      __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int64_t bytes = O.dim * O.elem;
+  int g = kWave;
+  while (g > 1 && bytes <= int64_t(g / 2) * 16) g /= 2;
+  const int l = lane & (g - 1), sub = lane / g, rows = kWave / g;
+  for (int64_t r = r0 + wave * rows + sub; r < r1;
+       r += TH / kWave * rows) {
+    if (named && named[r - r0]) continue;
+    char *p = O.out + r * O.row_bytes;
+    const int64_t before = -reinterpret_cast<uint64_t>(p) & 15;
+    const int64_t head = before < bytes ? before : bytes;
+    const int64_t body = head + ((bytes - head) & ~int64_t(15));
+    if (O.zero_nt)
+      for (int64_t c = head + l * 16; c < body; c += g * 16)
+        __builtin_nontemporal_store(u32x4{0, 0, 0, 0},
+                                    reinterpret_cast<u32x4 *>(p + c));
+    else
+      for (int64_t c = head + l * 16; c < body; c += g * 16)
+        *reinterpret_cast<u32x4 *>(p + c) = u32x4{0, 0, 0, 0};
+    for (int64_t c = l * 2; c < head; c += g * 2)
+      *reinterpret_cast<uint16_t *>(p + c) = 0;
+    for (int64_t c = body + l * 2; c < bytes; c += g * 2)
+      *reinterpret_cast<uint16_t *>(p + c) = 0;
+  }
+}
+
 // hist[digit][block], of the keys as they are (P.n = 0) or as they are made
 // here.
 __global__ __launch_bounds__(kTileThreads) void embed_hist_kernel(
@@ -529,10 +574,18 @@ __global__ __launch_bounds__(kTileThreads) void embed_scatter_kernel(
   }
 }
 
-// Keys and sort of one workgroup's tokens in one launch, through LDS.
+// Keys and sort of one workgroup's tokens in one launch, through LDS; the
+// other workgroups, if any, zero all rows.
 __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
     Parts P, Sort W, int src, int64_t tokens, uint32_t vocab, int passes,
-    int bits) {
+    int bits, Out O) {
+  if (blockIdx.x > 0) {
+    const int64_t r0 = int64_t(blockIdx.x - 1) * O.zero_rows;
+    const int64_t r1 =
+        r0 + O.zero_rows < O.vocab ? r0 + O.zero_rows : O.vocab;
+    zero_rows_of<kOneThreads>(O, r0, r1, nullptr);
+    return;
+  }
   constexpr int kW = kOneThreads / kWave;
   __shared__ __attribute__((aligned(16))) uint16_t cnt[kW << kMaxDigit];
   __shared__ uint32_t at[1 << kMaxDigit];
@@ -608,14 +661,6 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
 }
 
 // -- gradient: sums ------------------------------------------------------------
-struct Out {
-  char *out;
-  int64_t row_bytes, dim, vocab, tokens;
-  int chunk, slices, accumulate, zero_nt;
-  int64_t chunks;
-  const uint32_t *key;
-};
-
 // lanes from the first on that say yes
 __device__ __forceinline__ int run_length(bool yes) {
   const uint64_t m = __ballot(yes);
@@ -658,43 +703,6 @@ __device__ __forceinline__ void wave_bounds(const uint32_t *key, int64_t n,
 
 constexpr int kZeroRows = kBlock;  // most rows of a zero workgroup
 
-// Zeros into the rows [r0, r1) that are not named, by the whole workgroup:
-// `g` lanes a row, 16 bytes a lane whatever the row's alignment, single
-// elements before and behind.
-template <int OT>
-__device__ __forceinline__ void zero_rows_of(const Out &O, int64_t r0,
-                                             int64_t r1,
-                                             const uint8_t *named) {
-  using T = typename Elem<OT>::type;
-  constexpr int kOE = sizeof(T);
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave =
-      __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
-  const int64_t bytes = O.dim * kOE;
-  int g = kWave;
-  while (g > 1 && bytes <= int64_t(g / 2) * 16) g /= 2;
-  const int l = lane & (g - 1), sub = lane / g, rows = kWave / g;
-  for (int64_t r = r0 + wave * rows + sub; r < r1; r += kWaves * rows) {
-    if (named[r - r0]) continue;
-    char *p = O.out + r * O.row_bytes;
-    const int64_t head =
-        int64_t(-reinterpret_cast<uint64_t>(p) & 15) < bytes
-            ? int64_t(-reinterpret_cast<uint64_t>(p) & 15)
-            : bytes;
-    const int64_t body = head + ((bytes - head) & ~int64_t(15));
-    if (O.zero_nt)
-      for (int64_t c = head + l * 16; c < body; c += g * 16)
-        __builtin_nontemporal_store(u32x4{0, 0, 0, 0},
-                                    reinterpret_cast<u32x4 *>(p + c));
-    else
-      for (int64_t c = head + l * 16; c < body; c += g * 16)
-        *reinterpret_cast<u32x4 *>(p + c) = u32x4{0, 0, 0, 0};
-    for (int64_t c = l * kOE; c < head; c += g * kOE)
-      *reinterpret_cast<T *>(p + c) = T(0);
-    for (int64_t c = body + l * kOE; c < bytes; c += g * kOE)
-      *reinterpret_cast<T *>(p + c) = T(0);
-  }
-}
 // (keys of a stretch that are looked at one by one: 15003 of 4 stretches save
 // 0.5 us against the search, 65536 of 2 would lose 7)
 constexpr int64_t kScanKeys = 32 * kBlock;
@@ -703,8 +711,7 @@ constexpr int64_t kScanKeys = 32 * kBlock;
 // workgroups past those write the zero rows that no token names.
 template <int GT, int OT, int VEC>
 __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
-                                                           int sum_blocks,
-                                                           int zero_rows) {
+                                                           int sum_blocks) {
   constexpr int kGE = sizeof(typename Elem<GT>::type);
   constexpr int kOE = sizeof(typename Elem<OT>::type);
   const int lane = threadIdx.x & (kWave - 1);
@@ -714,8 +721,9 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
     // the rows of this stretch that a token names, from the stretch's own
     // tokens: all of them where they are few, else one search per thread
     __shared__ uint8_t named[kZeroRows];
-    const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * zero_rows;
-    const int64_t r1 = r0 + zero_rows < O.vocab ? r0 + zero_rows : O.vocab;
+    const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * O.zero_rows;
+    const int64_t r1 =
+        r0 + O.zero_rows < O.vocab ? r0 + O.zero_rows : O.vocab;
     int64_t a, b;
     wave_bounds(O.key, O.tokens, uint32_t(r0), uint32_t(r1), a, b);
     named[threadIdx.x] = 0;
@@ -742,7 +750,7 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
       named[threadIdx.x] = lo < b && O.key[lo] == r;
     }
     __syncthreads();
-    zero_rows_of<OT>(O, r0, r1, named);
+    zero_rows_of<kBlock>(O, r0, r1, named);
     return;
   }
   const int64_t unit = int64_t(blockIdx.x) * kWaves + wave;
@@ -846,8 +854,7 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
 // 13.9 / 17.2; it grows with the tokens' square.
 template <int GT, int OT, int VEC>
 __global__ __launch_bounds__(kBlock) void embed_few_kernel(Parts P, Out O,
-                                                           int sum_blocks,
-                                                           int zero_rows) {
+                                                           int sum_blocks) {
   constexpr int kGE = sizeof(typename Elem<GT>::type);
   constexpr int kOE = sizeof(typename Elem<OT>::type);
   __shared__ uint32_t starts[kMaxParts];
@@ -875,11 +882,12 @@ __global__ __launch_bounds__(kBlock) void embed_few_kernel(Parts P, Out O,
   key[t] = k;
   __syncthreads();
   if (int(blockIdx.x) >= sum_blocks) {
-    const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * zero_rows;
-    const int64_t r1 = r0 + zero_rows < O.vocab ? r0 + zero_rows : O.vocab;
+    const int64_t r0 = int64_t(blockIdx.x - sum_blocks) * O.zero_rows;
+    const int64_t r1 =
+        r0 + O.zero_rows < O.vocab ? r0 + O.zero_rows : O.vocab;
     if (t < tokens && int64_t(k) >= r0 && int64_t(k) < r1) named[k - r0] = 1;
     __syncthreads();
-    zero_rows_of<OT>(O, r0, r1, named);
+    zero_rows_of<kBlock>(O, r0, r1, named);
     return;
   }
   if (t < tokens) {
@@ -1206,6 +1214,7 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   O.dim = dim;
   O.vocab = vocab;
   O.tokens = tokens;
+  O.elem = oe;
   O.chunk = int(Z.chunk);
   O.chunks = Z.chunks;
   O.accumulate = accumulate;
@@ -1222,12 +1231,21 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   // rows per zero workgroup: about 64 KiB, or 256 KiB where that leaves
   // enough of them (128000 rows of 2048 fp32, 48 tokens: 191 / 180 us; 4000
   // rows of 300 10.8 / 16)
-  int64_t zero_rows =
+  const int64_t most =
       (vocab * dim * oe >> 29 ? 262144 : 65536) / (dim * oe);
-  if (zero_rows < kWaves) zero_rows = kWaves;
-  if (zero_rows > kZeroRows) zero_rows = kZeroRows;
+  O.zero_rows = int(most < kWaves      ? kWaves
+                    : most > kZeroRows ? kZeroRows
+                                       : most);
   const int64_t zero_blocks =
-      accumulate ? 0 : (vocab + zero_rows - 1) / zero_rows;
+      accumulate ? 0 : (vocab + O.zero_rows - 1) / O.zero_rows;
+  // Where few rows are named, all of them are zeroed while one workgroup
+  // sorts, and the named ones written again (zeros after / before, us: 700
+  // tokens of 128000 rows of 2048 fp32 201 / 186, of 100000 of 1025 97 / 86;
+  // a sort in tiles hides no more than it costs, 5000 tokens there 117 / 119).
+  const bool zero_first =
+      !few && tokens <= kOneTile && tokens < vocab / 8 &&
+      zero_blocks < kMaxGrid / (kOneThreads / kBlock);
+  const unsigned first = unsigned(zero_first ? zero_blocks : 0);
   const int64_t join_blocks =
       Z.chunks > 1 && !few
           ? ((Z.chunks - 1) * O.slices + kWaves - 1) / kWaves
@@ -1244,11 +1262,10 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
         const dim3 grid(unsigned(sum_blocks + zero_blocks)), block(kBlock);
         if (vec)
           hipLaunchKernelGGL((embed_few_kernel<D, Q, Elem<D>::kVec>), grid,
-                             block, 0, s, P, O, int(sum_blocks),
-                             int(zero_rows));
+                             block, 0, s, P, O, int(sum_blocks));
         else
           hipLaunchKernelGGL((embed_few_kernel<D, Q, 1>), grid, block, 0, s,
-                             P, O, int(sum_blocks), int(zero_rows));
+                             P, O, int(sum_blocks));
       });
     });
     return check_launch(what);
@@ -1256,8 +1273,9 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   int src = 0;
   if (tokens <= kOneTile) {
     src = 1;
-    hipLaunchKernelGGL(embed_sort_kernel, dim3(1), dim3(kOneThreads), 0, s, P,
-                       W, src, tokens, uint32_t(vocab), Z.passes, Z.digit);
+    hipLaunchKernelGGL(embed_sort_kernel, dim3(1 + first), dim3(kOneThreads),
+                       0, s, P, W, src, tokens, uint32_t(vocab), Z.passes,
+                       Z.digit, O);
   } else {
     const int scanned = Z.blocks > kSumBlocks;
     for (int p = 0; p < Z.passes; ++p, src ^= 1) {
@@ -1280,13 +1298,15 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
     with_dtype(out_dtype, [&](auto ot) {
       constexpr int D = decltype(gt)::value, Q = decltype(ot)::value;
       constexpr int V = Elem<D>::kVec;
-      const dim3 grid(unsigned(sum_blocks + zero_blocks)), block(kBlock);
+      const dim3 grid(unsigned(sum_blocks) +
+                      unsigned(zero_first ? 0 : zero_blocks)),
+          block(kBlock);
       if (vec)
         hipLaunchKernelGGL((embed_sum_kernel<D, Q, V>), grid, block, 0, s, O,
-                           W, int(sum_blocks), int(zero_rows));
+                           W, int(sum_blocks));
       else
         hipLaunchKernelGGL((embed_sum_kernel<D, Q, 1>), grid, block, 0, s, O,
-                           W, int(sum_blocks), int(zero_rows));
+                           W, int(sum_blocks));
       if (join_blocks == 0) return;
       const dim3 jg{unsigned(join_blocks)};
       if (vec)

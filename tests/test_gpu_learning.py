@@ -586,7 +586,7 @@ def test_embedding_grad_zero_rows(dim, dtype):
     """Every byte of the rows that no token names, and no byte beside them:
     odd widths, rows apart, a start at any element; few and many tokens."""
     from federatedscope_amd import ops
-    for tokens, vocab in ((3, 50), (900, 1500)):
+    for tokens, vocab in ((3, 50), (900, 1500), (300, 2600), (5000, 4000)):
         for off in (0, 1, 3):
             buf = torch.full((vocab, dim + 5), 7.0, dtype=dtype,
                              device='cuda')
