@@ -95,7 +95,8 @@ def _check_ns(got, g, steps=5, coef=(A, B, C), eps=1e-7, one=False,
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 200), (62, 2048), (2048, 62),
           (63, 65), (64, 64), (128, 128), (129, 127), (130, 700),
-          (300, 1000), (1000, 300), (257, 513), (515, 4100), (2603, 1101)]
+          (300, 1000), (1000, 300), (257, 513), (515, 4100), (2603, 1101),
+          (33, 16390), (20001, 2), (64, 16384), (1, 40000)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
@@ -770,3 +771,42 @@ def test_operators_in_captured_graphs():
             torch.cuda.synchronize()
             for b, x in zip(bufs, states[k]):
                 assert torch.equal(b, x)
+
+
+def test_large_operators_in_a_captured_graph():
+    """The ways of large and narrow calls: shared tiles and joins, slabs, one
+    limb, a sort in tiles, zeros beside a sort; every replay equals the eager
+    run, on inputs that change between replays."""
+    from federatedscope_amd import ops
+    g = [_matrix(1270, 7100, 1).cuda(), _matrix(50, 3000, 2).cuda(),
+         _matrix(1536, 1536, 3).bfloat16().cuda()]
+    outs = [torch.empty_like(x) for x in g]
+    ids = [_ids(6000, 900, 4), _ids(700, 900, 5)]
+    rows = [torch.randn(len(i), 40, device='cuda') for i in ids]
+    sums = [torch.empty(900, 40, device='cuda'),
+            torch.empty(9000, 40, device='cuda')]
+
+    def run():
+        ops.newton_schulz(g, out=outs)
+        ops.embedding_grad(ids, rows, 900, out=sums[0])
+        ops.embedding_grad(ids[1], rows[1], 9000, out=sums[1])
+    run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run()
+    for k in range(3):
+        for x in g:
+            x.mul_(-1.5)
+            x[0, 0] = 0.01 * k
+        rows[0].add_(0.5)
+        ids[1].copy_(ids[1].flip(0))
+        run()
+        want = [t.clone() for t in outs + sums]
+        for t in outs + sums:
+            t.fill_(float('nan'))
+        graph.replay()
+        torch.cuda.synchronize()
+        for t, w in zip(outs + sums, want):
+            assert torch.equal(t, w)
