@@ -12,8 +12,9 @@ HBM across rounds.  Muon (momentum, nesterov, weight_decay, ns_steps,
 ns_coefficients, eps, adjust_lr_fn as torch.optim.Muon) steps all matrix
 parameters in one ops.muon_step; like torch.optim's it takes matrices only,
 unless ``aux`` = {type, lr, **kwargs} names another of these optimizers for
-the other parameters (biases, convolutions).  The updated parameters are written back into ``self.model`` and
-``self.model.state_dict()`` is returned, as the reference does.
+the other parameters (biases, convolutions).  The updated parameters are
+written back into ``self.model`` and ``self.model.state_dict()`` is returned,
+as the reference does.
 
 Optimizer config: ``config.fedopt.optimizer`` = {type, lr, **kwargs} as in
 get_optimizer (core/auxiliaries/optimizer_builder.py:19-60); annealing:

@@ -19,6 +19,8 @@ wait for the remaining clients instead of sitting inside aggregate().
 """
 from collections import deque
 
+import torch
+
 from ... import ops
 from ..aggregators._engine import compute_device
 from ..aggregators.clients_avg_aggregator import sparse_keys
@@ -135,11 +137,17 @@ class AggregationServer:
         on the compute device — what a client that trains a few rows of a
         large table is sent instead of the whole of it (the reference
         broadcasts whole state dicts, server.py:636-714); it answers with a
-        row-sparse update (ClientsAvgAggregator).  A model that lies on the
-        host has the whole table copied to the device by each call."""
+        row-sparse update (ClientsAvgAggregator)."""
         dev = compute_device(self.device)
-        table = self.models[model_idx].state_dict()[key].to(dev)
-        return ops.embedding_lookup(table, ids.to(dev).contiguous(),
+        table = self.models[model_idx].state_dict()[key]
+        if table.device != dev and 0 < ids.numel() < len(table):
+            # of a table that lies elsewhere the named rows travel, not all
+            at = ids.to(table.device).reshape(-1).long()
+            named = (at >= 0) & (at < len(table))
+            table = table[at.where(named, at.new_zeros(()))]
+            ids = torch.arange(len(at), device=at.device).where(
+                named, at.new_full((), -1)).reshape(ids.shape)
+        return ops.embedding_lookup(table.to(dev), ids.to(dev).contiguous(),
                                     scale=scale)
 
     # -- server.py:315-383 (count-based) ---------------------------------------

@@ -277,6 +277,27 @@ def test_fedopt_takes_row_sparse_uploads(model_dev):
                      tol).all())
 
 
+@pytest.mark.parametrize('idt', [torch.int64, torch.int32])
+def test_select_rows_of_a_host_model(idt):
+    """Few tokens (their rows travel) and more than the table has rows (all of
+    it does), padding among them: as from a model on the device."""
+    from federatedscope_amd.core.workers.server import AggregationServer
+    host = _Net(False)
+    dev = _Net(False).cuda()
+    dev.load_state_dict(host.state_dict())
+    a, b = (AggregationServer(m, None, sample_client_num=1, device='cuda:0')
+            for m in (host, dev))
+    for tok in (torch.tensor([[3, -1, 39], [40, 3, 0]]),
+                torch.arange(-5, 95).reshape(2, 50),
+                torch.empty(0, 4), torch.tensor([-1, 77])):
+        tok = tok.to(idt)
+        for where in ('cpu', 'cuda'):
+            got = a.select_rows('emb.weight', tok.to(where), scale=1.5)
+            want = b.select_rows('emb.weight', tok.to(where), scale=1.5)
+            assert got.is_cuda and torch.equal(got, want)
+            assert got.shape == tuple(tok.shape) + (24, )
+
+
 def test_server_round_with_rows_and_muon():
     """A whole round: each client gets the rows of its tokens, answers with a
     row-sparse update of the table and dense matrices; the server steps the
