@@ -45,8 +45,9 @@ PyObject *b64_frame(PyObject *, PyObject *args);
 PyObject *b64_frame_many(PyObject *, PyObject *args);
 // host/krumcert.cpp: the Krum selection certificate
 PyObject *gram_select(PyObject *, PyObject *args);
-// host/embedparts.cpp: row-sparse uploads
-PyObject *embed_parts(PyObject *, PyObject *args);
+// host/embedcall.cpp: embedding calls, row-sparse uploads
+PyObject *embed_lookup(PyObject *, PyObject *args);
+PyObject *embed_grad(PyObject *, PyObject *args);
 PyObject *has_sparse(PyObject *, PyObject *dict);
 
 namespace {
@@ -709,9 +710,11 @@ PyMethodDef kMethods[] = {
     {"gram_select", gram_select, METH_VARARGS,
      "gram_select(buf, nseg, f, m, ordered) -> None or (scores, order, "
      "ambiguous)"},
-    {"embed_parts", embed_parts, METH_VARARGS,
-     "embed_parts(ids, grads, coefs, out_lo, out_hi) -> (table, tokens, dim, "
-     "dtype_code) or None"},
+    {"embed_lookup", embed_lookup, METH_VARARGS,
+     "embed_lookup(table, ids, scale, device, stream, fn) -> tensor or None"},
+    {"embed_grad", embed_grad, METH_VARARGS,
+     "embed_grad(ids, grads, coefs, num_rows, out, accumulate, device, "
+     "stream, size_fn, fn) -> tensor or None"},
     {"has_sparse", has_sparse, METH_O,
      "has_sparse(dict) -> whether a value is a sparse COO tensor"},
     {"key_table", key_table, METH_VARARGS,

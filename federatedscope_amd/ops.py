@@ -1917,6 +1917,22 @@ def _check_rows(t, what):
         raise ValueError('%s must be 2-D with contiguous rows' % what)
 
 
+_embed_fns = None
+
+
+def _embed_addresses():
+    """Addresses of (fsagg_embed_lookup, fsagg_embed_grad_workspace_bytes,
+    fsagg_embed_grad) for the native calls."""
+    global _embed_fns
+    if _embed_fns is None:
+        lib = L.load()
+        _embed_fns = tuple(
+            ctypes.cast(f, ctypes.c_void_p).value for f in
+            (lib.fsagg_embed_lookup, lib.fsagg_embed_grad_workspace_bytes,
+             lib.fsagg_embed_grad))
+    return _embed_fns
+
+
 def embedding_lookup(table, ids, scale=1.0, out=None):
     """out[..., :] = scale * table[ids[...], :], the product in float32 and
     rounded once to the table's dtype (float32, float16, bfloat16).  A token
@@ -1925,6 +1941,14 @@ def embedding_lookup(table, ids, scale=1.0, out=None):
     on the same GPU; ``out`` (contiguous, not overlapping either) or a new
     tensor [*ids.shape, dim] is returned.  Its gradient with respect to the
     table is :func:`embedding_grad`."""
+    if out is None and torch.cuda.is_initialized():
+        # the plain form natively; None: the checks below say why not
+        cur = torch.cuda.current_device()
+        got = L.host().embed_lookup(table, ids, scale, cur,
+                                    torch._C._cuda_getCurrentRawStream(cur),
+                                    _embed_addresses()[0])
+        if got is not None:
+            return got
     _check_float_cuda(table, 'table')
     _check_rows(table, 'table')
     dev = table.device
@@ -1983,12 +2007,17 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, weights=None, out=None,
         raise ValueError('num_rows must not be negative')
     if accumulate and out is None:
         raise ValueError('accumulate needs out')
-    lo, hi = (0, 0) if out is None or not isinstance(out, torch.Tensor) or \
-        not out.numel() else _extent(out)
-    got = L.host().embed_parts(ids, grad, coefs, lo, hi)
-    if got is None:
-        got = _embed_parts(ids, grad, coefs, out)
-    parts, tokens, dim, code = got
+    if torch.cuda.is_initialized():
+        # the plain form natively; None: the checks below say why not
+        cur = torch.cuda.current_device()
+        fns = _embed_addresses()
+        got = L.host().embed_grad(ids, grad, coefs, num_rows, out, accumulate,
+                                  cur,
+                                  torch._C._cuda_getCurrentRawStream(cur),
+                                  fns[1], fns[2])
+        if got is not None:
+            return got
+    parts, tokens, dim, code = _embed_parts(ids, grad, coefs, out)
     dev = grad[0].device
     if out is None:
         out = torch.empty((num_rows, dim), dtype=grad[0].dtype, device=dev)
@@ -2012,9 +2041,8 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, weights=None, out=None,
 
 
 def _embed_parts(ids, grad, coefs, out):
-    """The parts table of fsagg_embed_grad, with a message for what is wrong
-    (_fsagg_host.embed_parts takes the plain form and gives up on the
-    rest)."""
+    """The parts table of fsagg_embed_grad (tensors of another device than
+    the current one), with a message for what is wrong."""
     dev = dt = dim = None
     parts = (L.EmbedPart * len(ids))()
     tokens = 0

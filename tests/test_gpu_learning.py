@@ -607,6 +607,32 @@ def test_embedding_grad_zero_rows(dim, dtype):
             assert bool((flat[off + vocab * dim:] == 7).all())
 
 
+def test_embedding_calls_without_the_native_walk(monkeypatch):
+    """The Python way (tensors of another device than the current one take
+    it) gives the same bits."""
+    from federatedscope_amd import _lib, ops
+    table = torch.randn(60, 33, device='cuda')
+    ids = [_ids(40, 60, 1), _ids(900, 60, 2, dtype=torch.int32)]
+    grad = [torch.randn(len(i), 33, device='cuda') for i in ids]
+    out = [torch.randn(60, 33, device='cuda') for _ in range(2)]
+    out[1].copy_(out[0])
+
+    def run(o):
+        return [ops.embedding_lookup(table, ids[0].view(8, 5), scale=3),
+                ops.embedding_grad(ids, grad, 60, weights=[0.5, 2]),
+                ops.embedding_grad(ids[1], grad[1], 70, scale=0.1),
+                ops.embedding_grad(ids, grad, 60, out=o, accumulate=True)]
+    native = run(out[0])
+
+    class Host:
+        def embed_lookup(*_):
+            return None
+        embed_grad = embed_lookup
+    monkeypatch.setattr(_lib, 'host', Host)
+    for a, b in zip(native, run(out[1])):
+        assert torch.equal(a, b)
+
+
 def test_embedding_grad_views():
     from federatedscope_amd import ops
     ids = _ids(80, 30, 1)

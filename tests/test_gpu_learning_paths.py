@@ -256,6 +256,35 @@ def test_row_sparse_refusals():
         run([dense, sp])
 
 
+@pytest.mark.parametrize('dev', ['cpu', 'cuda'])
+@pytest.mark.parametrize('name', [
+    'KrumAggregator', 'MedianAggregator', 'TrimmedmeanAggregator',
+    'NormboundingAggregator', 'AsynClientsAvgAggregator',
+    'ServerClientsInterpolateAggregator', 'OnlineClientsAvgAggregator'])
+def test_other_rules_refuse_row_sparse_uploads(name, dev):
+    """They read dense tensors: an upload of rows is an error, not a value."""
+    from federatedscope_amd.core import aggregators
+    cfg = _cfg(dict(type='SGD', lr=1.0))
+    cfg.federate.restore_from = ''
+    cfg.aggregator = SimpleNamespace(
+        byzantine_node_num=1, inside_weight=0.5,
+        BFT_args=SimpleNamespace(krum_agg_num=2, normbounding_norm_bound=1.0,
+                                 trimmedmean_excluded_ratio=0.2))
+    cfg.asyn = SimpleNamespace(staleness_discount_factor=1.0)
+    model = _Net(False).cuda()
+    ups = _uploads(model, 8, 0, dev, skip=('emb.weight', ))
+    for i, (_, d) in enumerate(ups):
+        d['emb.weight'] = _sparse((40, 24), 5, i, dev)
+    agg = getattr(aggregators, name)(model=model, device='cuda:0', config=cfg)
+    with pytest.raises(RuntimeError, match='sparse'):
+        if name == 'OnlineClientsAvgAggregator':
+            agg.reset()
+            agg.inc(ups[0])
+        else:
+            agg.aggregate({'client_feedback': ups, 'recover_fun': None,
+                           'staleness': [(0, 0)] * 8})
+
+
 @pytest.mark.parametrize('model_dev', ['cpu', 'cuda'])
 def test_fedopt_takes_row_sparse_uploads(model_dev):
     """The pseudo-gradient of a sparse key is the clients' negated sum."""
