@@ -444,6 +444,18 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Group G,
   }
 }
 
+// A transposing read of LDS: of the 16 lanes of a group, lane i is given 4
+// values of row i / 4, columns 4 (i % 4) on, and gets those of column i.
+__device__ __forceinline__ half4 read_tr(const _Float16 *p) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(
+      half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                 (__attribute__((address_space(3))) s4 *)(uintptr_t)p));
+}
+__device__ __forceinline__ half8 join4(half4 x, half4 y) {
+  return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 enum Mode { kGram, kSquare, kApply, kLast, kLastMuon };
 
 constexpr bool symmetric(int mode) { return mode == kGram || mode == kSquare; }
@@ -644,9 +656,8 @@ struct Tile {
               r * BM + (((col / 8) ^ (piece(r) << 2)) * 8) + col % 8;
 #pragma unroll
           for (int l = 0; l < LIMBS; ++l) {
-            const half4 x = read_tr(st + l * BM * kBK + o);
-            const half4 y = read_tr(st + l * BM * kBK + o + 4 * BM);
-            f.a[l][i] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            const _Float16 *p = st + l * BM * kBK + o;
+            f.a[l][i] = join4(read_tr(p), read_tr(p + 4 * BM));
           }
           continue;
         }
@@ -730,13 +741,6 @@ struct Tile {
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, kMfma, 0);
-  }
-
-  static __device__ __forceinline__ half4 read_tr(const _Float16 *p) {
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    return __builtin_bit_cast(
-        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                   (__attribute__((address_space(3))) s4 *)(uintptr_t)p));
   }
 
   // all but the last N of this wave's direct loads have landed, and every
@@ -1080,28 +1084,55 @@ struct Slab {
   }
   __device__ __forceinline__ int col() const { return bj + fr; }
 
-  // x += P R^T over 64 of k; planes [64][64], limbs l at + 4096.  The small
-  // limb products go to an accumulator of their own (a chain of dependent
-  // matrix instructions is what a product this small waits for).
-  __device__ __forceinline__ void multiply(const _Float16 *p,
-                                           const _Float16 *r,
-                                           f32x16 &x) const {
+  // x += the products of 64 of k, of the fragments that left(kk, limb) and
+  // right(kk, limb) read.  The small limb products go to an accumulator of
+  // their own (a chain of dependent matrix instructions is what a product this
+  // small waits for).
+  template <typename P, typename R>
+  static __device__ __forceinline__ void chain(P left, R right, f32x16 &x) {
     f32x16 s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      const int op = swz(bi + fr, kk * 2 + fk), oq = swz(bj + fr, kk * 2 + fk);
-      const half8 ph = *reinterpret_cast<const half8 *>(p + op);
-      const half8 pl = *reinterpret_cast<const half8 *>(p + 4096 + op);
-      const half8 rh = *reinterpret_cast<const half8 *>(r + oq);
-      const half8 rl = *reinterpret_cast<const half8 *>(r + 4096 + oq);
+      const half8 ph = left(kk, 0), pl = left(kk, 4096);
+      const half8 rh = right(kk, 0), rl = right(kk, 4096);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, rh, s, 0, 0, 0);
       x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rh, x, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, rl, s, 0, 0, 0);
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = __fadd_rn(x[e], s[e]);
+  }
+
+  // x += P R^T; planes [64][64], limbs l at + 4096
+  __device__ __forceinline__ void multiply(const _Float16 *p,
+                                           const _Float16 *r,
+                                           f32x16 &x) const {
+    const auto rows = [&](const _Float16 *q, int b) {
+      return [=](int kk, int limb) {
+        return *reinterpret_cast<const half8 *>(
+            q + limb + swz(b + fr, kk * 2 + fk));
+      };
+    };
+    chain(rows(p, bi), rows(r, bj), x);
+  }
+  // x += X X^T, of the plane as put_columns leaves it (row j: column j of X):
+  // fragments by transposing reads of rows j .. j + 3 and j + 4 .. j + 7
+  __device__ __forceinline__ void gram_of(const _Float16 *p,
+                                          f32x16 &x) const {
+    const int l = lane & 15, j = fk * 8 + (l >> 2);
+    const auto rows = [&](int b) {
+      const int i = b + (fr & 16) + 4 * (l & 3);
+      const _Float16 *lo = p + swz(j, i >> 3) + (i & 7);
+      const _Float16 *hi = p + swz(j + 4, i >> 3) + (i & 7);
+      // (16 rows on, the slots are permuted alike)
+      return [=](int kk, int limb) {
+        return join4(read_tr(lo + limb + kk * 16 * 64),
+                     read_tr(hi + limb + kk * 16 * 64));
+      };
+    };
+    chain(rows(bi), rows(bj), x);
   }
   // limbs of the block's values (times kS), transposed: row col(), the rows
   // of a quad side by side
@@ -1115,22 +1146,6 @@ struct Slab {
       const int o = swz(col(), row(q) >> 3) + (row(q) & 7);
       *reinterpret_cast<half4 *>(p + o) = h;
       *reinterpret_cast<half4 *>(p + 4096 + o) = l;
-    }
-  }
-  // the same by rows
-  __device__ __forceinline__ void put_rows(_Float16 *p,
-                                           const f32x16 &x) const {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float v[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-      half4 h, l;
-      split_n<4>(v, h, l);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int o = swz(row(q) + e, col() >> 3) + (col() & 7);
-        p[o] = h[e];
-        p[4096 + o] = l[e];
-      }
     }
   }
 };
@@ -1223,14 +1238,14 @@ template <bool MUON>
 __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
     Group G, int steps, float a, float b, float c, double eps,
     MuonScalars S) {
-  // Q, and per group the columns' limbs by columns and by rows
+  // Q, and per group the columns' limbs and its Gram share
   __shared__ __attribute__((aligned(1024)))
   _Float16 lds[8192 * (1 + 2 * kMaxWhole)];
   __shared__ double part[256 * kMaxWhole];
   int z;
   const Mat &M = G.mat[find_mat(G, blockIdx.x, z)];
   const Narrow N = {};
-  const Slab W;
+  Slab W;
   const int g = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 8);
   const int t256 = threadIdx.x & 255;
   const int chunks = M.np / 64;
@@ -1244,11 +1259,12 @@ __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
   scale_update(M, W, g,
                limb_scale(block_sum<256 * kMaxWhole>(sq, part), eps), x);
   for (int step = 1; step <= steps; ++step) {
+    // (addresses are worked out anew: there are no registers to keep them)
+    asm volatile("" : "+v"(W.lane), "+v"(W.fr));
     clear16(gram);
-    if (g < chunks) W.put_rows(lx, x);
+    if (g < chunks) W.put_columns(lt, x);
     __syncthreads();
-    if (g < chunks) W.multiply(lx, lx, gram);
-    __syncthreads();
+    if (g < chunks) W.gram_of(lt, gram);
     // the groups' shares, in order
     if (chunks > 1) {
       f32x4 *mine = reinterpret_cast<f32x4 *>(lx);
@@ -1278,8 +1294,6 @@ __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
 #pragma unroll
       for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
       W.put_columns(lq, gram);
-    } else if (g < chunks) {
-      W.put_columns(lt, x);
     }
     __syncthreads();
     if (g == 0) {
@@ -1287,7 +1301,6 @@ __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
       W.multiply(lq, lq, t);
 #pragma unroll
       for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
-      W.put_columns(lt, x);
     }
     __syncthreads();
     if (g == 0) W.put_columns(lq, t);
@@ -1298,6 +1311,7 @@ __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = a * x[r] + t[r] * kInvS;
     }
+    __syncthreads();  // lt and lq have been read
   }
   if (g < chunks) store_chunk<MUON>(M, W, S, z, g, x);
 }
@@ -1332,9 +1346,9 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
     for (int ch = 0; ch < kMaxEach; ++ch) {
       if (ch >= have) break;
       scale_update(M, W, chunk0 + ch, scale, x[ch]);
-      W.put_rows(lx, x[ch]);
+      W.put_columns(lx, x[ch]);
       __syncthreads();
-      W.multiply(lx, lx, gram);
+      W.gram_of(lx, gram);
       __syncthreads();
     }
   } else {
@@ -1391,9 +1405,9 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[ch][r] = a * x[ch][r] + t[r] * kInvS;
       if (k < steps) {
-        W.put_rows(lx, x[ch]);
+        W.put_columns(lx, x[ch]);
         __syncthreads();
-        W.multiply(lx, lx, gram);
+        W.gram_of(lx, gram);
       } else {
         __syncthreads();
       }
