@@ -1084,17 +1084,17 @@ struct Slab {
   }
   __device__ __forceinline__ int col() const { return bj + fr; }
 
-  // x += the products of 64 of k, of the fragments that left(kk, limb) and
-  // right(kk, limb) read.  The small limb products go to an accumulator of
+  // x += the products of K times 16 of k, of the fragments that left(kk, limb)
+  // and right(kk, limb) read.  The small limb products go to an accumulator of
   // their own (a chain of dependent matrix instructions is what a product this
   // small waits for).
-  template <typename P, typename R>
+  template <int K, typename P, typename R>
   static __device__ __forceinline__ void chain(P left, R right, f32x16 &x) {
     f32x16 s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
+    for (int kk = 0; kk < K; ++kk) {
       const half8 ph = left(kk, 0), pl = left(kk, 4096);
       const half8 rh = right(kk, 0), rl = right(kk, 4096);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, rh, s, 0, 0, 0);
@@ -1105,7 +1105,9 @@ struct Slab {
     for (int e = 0; e < 16; ++e) x[e] = __fadd_rn(x[e], s[e]);
   }
 
-  // x += P R^T; planes [64][64], limbs l at + 4096
+  // x += P R^T over the first 16 K of k (the rest is zero); planes [64][64],
+  // limbs l at + 4096
+  template <int K>
   __device__ __forceinline__ void multiply(const _Float16 *p,
                                            const _Float16 *r,
                                            f32x16 &x) const {
@@ -1115,10 +1117,12 @@ struct Slab {
             q + limb + swz(b + fr, kk * 2 + fk));
       };
     };
-    chain(rows(p, bi), rows(r, bj), x);
+    chain<K>(rows(p, bi), rows(r, bj), x);
   }
-  // x += X X^T, of the plane as put_columns leaves it (row j: column j of X):
-  // fragments by transposing reads of rows j .. j + 3 and j + 4 .. j + 7
+  // x += X X^T over the first 16 K columns, of the plane as put_columns leaves
+  // it (row j: column j of X): fragments by transposing reads of rows j .. j + 3
+  // and j + 4 .. j + 7
+  template <int K>
   __device__ __forceinline__ void gram_of(const _Float16 *p,
                                           f32x16 &x) const {
     const int l = lane & 15, j = fk * 8 + (l >> 2);
@@ -1132,7 +1136,7 @@ struct Slab {
                      read_tr(hi + limb + kk * 16 * 64));
       };
     };
-    chain(rows(bi), rows(bj), x);
+    chain<K>(rows(bi), rows(bj), x);
   }
   // limbs of the block's values (times kS), transposed: row col(), the rows
   // of a quad side by side
@@ -1258,61 +1262,70 @@ __global__ __launch_bounds__(256 * kMaxWhole) void ns_whole_kernel(
   for (int r = 0; r < 16; ++r) sq += double(x[r]) * double(x[r]);
   scale_update(M, W, g,
                limb_scale(block_sum<256 * kMaxWhole>(sq, part), eps), x);
-  for (int step = 1; step <= steps; ++step) {
-    // (addresses are worked out anew: there are no registers to keep them)
-    asm volatile("" : "+v"(W.lane), "+v"(W.fr));
-    clear16(gram);
-    if (g < chunks) W.put_columns(lt, x);
-    __syncthreads();
-    if (g < chunks) W.gram_of(lt, gram);
-    // the groups' shares, in order
-    if (chunks > 1) {
-      f32x4 *mine = reinterpret_cast<f32x4 *>(lx);
-      if (g < chunks) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          mine[q * 256 + t256] = f32x4{gram[4 * q], gram[4 * q + 1],
-                                       gram[4 * q + 2], gram[4 * q + 3]};
-      }
+  // (16 M16 rows and, of a chunk, 16 N16 columns are all there are)
+  const auto run = [&](auto m16, auto n16) {
+    constexpr int M16 = decltype(m16)::value, N16 = decltype(n16)::value;
+    for (int step = 1; step <= steps; ++step) {
+      // (addresses are worked out anew: there are no registers to keep them)
+      asm volatile("" : "+v"(W.lane), "+v"(W.fr));
+      clear16(gram);
+      if (g < chunks) W.put_columns(lt, x);
       __syncthreads();
-      if (g == 0) clear16(gram);
-      for (int k = 0; g == 0 && k < chunks; ++k) {
-        const f32x4 *other = reinterpret_cast<const f32x4 *>(
-            lds + 8192 * (2 + 2 * k));
+      if (g < chunks) W.gram_of<N16>(lt, gram);
+      // the groups' shares, in order
+      if (chunks > 1) {
+        f32x4 *mine = reinterpret_cast<f32x4 *>(lx);
+        if (g < chunks) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 v = other[q * 256 + t256];
+          for (int q = 0; q < 4; ++q)
+            mine[q * 256 + t256] = f32x4{gram[4 * q], gram[4 * q + 1],
+                                         gram[4 * q + 2], gram[4 * q + 3]};
+        }
+        __syncthreads();
+        if (g == 0) clear16(gram);
+        for (int k = 0; g == 0 && k < chunks; ++k) {
+          const f32x4 *other = reinterpret_cast<const f32x4 *>(
+              lds + 8192 * (2 + 2 * k));
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            gram[4 * q + e] = __fadd_rn(gram[4 * q + e], v[e]);
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 v = other[q * 256 + t256];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              gram[4 * q + e] = __fadd_rn(gram[4 * q + e], v[e]);
+          }
         }
       }
-    }
-    // Q by the first group, which others wait for: all of them at it would
-    // share the one CU's vector units
-    if (g == 0) {
+      // Q by the first group, which others wait for: all of them at it would
+      // share the one CU's vector units
+      if (g == 0) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
-      W.put_columns(lq, gram);
-    }
-    __syncthreads();
-    if (g == 0) {
-      clear16(t);
-      W.multiply(lq, lq, t);
+        for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
+        W.put_columns(lq, gram);
+      }
+      __syncthreads();
+      if (g == 0) {
+        clear16(t);
+        W.multiply<M16>(lq, lq, t);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
-    }
-    __syncthreads();
-    if (g == 0) W.put_columns(lq, t);
-    __syncthreads();
-    if (g < chunks) {
-      clear16(t);
-      W.multiply(lq, lt, t);
+        for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
+      }
+      __syncthreads();
+      if (g == 0) W.put_columns(lq, t);
+      __syncthreads();
+      if (g < chunks) {
+        clear16(t);
+        W.multiply<M16>(lq, lt, t);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = a * x[r] + t[r] * kInvS;
+        for (int r = 0; r < 16; ++r) x[r] = a * x[r] + t[r] * kInvS;
+      }
+      __syncthreads();  // lt and lq have been read
     }
-    __syncthreads();  // lt and lq have been read
-  }
+  };
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  if (M.n <= 16) run(One(), One());
+  else if (M.m <= 16) run(One(), Four());
+  else run(Four(), Four());
   if (g < chunks) store_chunk<MUON>(M, W, S, z, g, x);
 }
 
@@ -1348,7 +1361,7 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
       scale_update(M, W, chunk0 + ch, scale, x[ch]);
       W.put_columns(lx, x[ch]);
       __syncthreads();
-      W.gram_of(lx, gram);
+      W.gram_of<4>(lx, gram);
       __syncthreads();
     }
   } else {
@@ -1383,35 +1396,41 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
             gram[r] = __fadd_rn(gram[r], v[u][r / 4][r % 4]);
         }
     }
-    // kS Q = b kS A + c kS A^2 from kS^2 A
+    // (16 M16 rows are all there are)
+    const auto run = [&](auto m16) {
+      constexpr int M16 = decltype(m16)::value;
+      // kS Q = b kS A + c kS A^2 from kS^2 A
 #pragma unroll
-    for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
-    W.put_columns(lt, gram);
-    __syncthreads();
-    clear16(t);
-    W.multiply(lt, lt, t);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
-    W.put_columns(lq, t);
-    clear16(gram);
-    __syncthreads();
-#pragma unroll
-    for (int ch = 0; ch < kMaxEach; ++ch) {
-      if (ch >= have) break;
-      W.put_columns(lt, x[ch]);
+      for (int r = 0; r < 16; ++r) gram[r] *= kInvS;
+      W.put_columns(lt, gram);
       __syncthreads();
       clear16(t);
-      W.multiply(lq, lt, t);
+      W.multiply<M16>(lt, lt, t);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[ch][r] = a * x[ch][r] + t[r] * kInvS;
-      if (k < steps) {
-        W.put_columns(lx, x[ch]);
+      for (int r = 0; r < 16; ++r) t[r] = b * gram[r] + c * (t[r] * kInvS);
+      W.put_columns(lq, t);
+      clear16(gram);
+      __syncthreads();
+#pragma unroll
+      for (int ch = 0; ch < kMaxEach; ++ch) {
+        if (ch >= have) break;
+        W.put_columns(lt, x[ch]);
         __syncthreads();
-        W.gram_of(lx, gram);
-      } else {
-        __syncthreads();
+        clear16(t);
+        W.multiply<M16>(lq, lt, t);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[ch][r] = a * x[ch][r] + t[r] * kInvS;
+        if (k < steps) {
+          W.put_columns(lx, x[ch]);
+          __syncthreads();
+          W.gram_of<4>(lx, gram);
+        } else {
+          __syncthreads();
+        }
       }
-    }
+    };
+    if (M.m <= 16) run(std::integral_constant<int, 1>());
+    else run(std::integral_constant<int, 4>());
   }
   if (k < steps) {
 #pragma unroll

@@ -96,7 +96,8 @@ def _check_ns(got, g, steps=5, coef=(A, B, C), eps=1e-7, one=False,
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 200), (62, 2048), (2048, 62),
           (63, 65), (64, 64), (128, 128), (129, 127), (130, 700),
           (300, 1000), (1000, 300), (257, 513), (515, 4100), (2603, 1101),
-          (33, 16390), (20001, 2), (64, 16384), (1, 40000)]
+          (33, 16390), (20001, 2), (64, 16384), (1, 40000), (16, 16),
+          (15, 13), (17, 16), (16, 250), (12, 3001), (16, 6000), (17, 900)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
