@@ -1222,17 +1222,19 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
   // many rows are read meanwhile (past / through, us: 128000 rows of 1024
   // fp32, 65536 tokens 180 / 196; of 2048, 32768 tokens 271 / 282, 8192 238 /
   // 235, 48 184 / 180; of 300, 32768 tokens 80 / 74)
-  O.zero_nt = vocab * dim * oe >= int64_t(1) << 28 && tokens >= vocab / 8;
+  O.zero_nt = vocab * dim * oe >> 28 && tokens >= vocab / 8;
   const int v = vec ? vec_elems : 1;
   O.slices = int((dim + int64_t(kWave) * v - 1) / (int64_t(kWave) * v));
   const bool few = tokens <= kFew && one_launch;
   const int64_t sum_units = few ? tokens : Z.chunks;
   const int64_t sum_blocks = (sum_units * O.slices + kWaves - 1) / kWaves;
   // rows per zero workgroup: about 64 KiB, or 256 KiB where that leaves
-  // enough of them (128000 rows of 2048 fp32, 48 tokens: 191 / 180 us; 4000
-  // rows of 300 10.8 / 16)
+  // enough of them (128000 rows of 2048 fp32, 48 tokens: 191 / 180 us), or
+  // 16 KiB where they would be few (4000 rows of 300, 48 tokens 7.6 / 5.9,
+  // 700 tokens 22.7 / 20.6)
+  const int64_t total = vocab * dim * oe;
   const int64_t most =
-      (vocab * dim * oe >> 29 ? 262144 : 65536) / (dim * oe);
+      (total >> 29 ? 262144 : total >> 24 ? 65536 : 16384) / (dim * oe);
   O.zero_rows = int(most < kWaves      ? kWaves
                     : most > kZeroRows ? kZeroRows
                                        : most);

@@ -1063,7 +1063,9 @@ __global__ __launch_bounds__(T::kThreads) void ns_join_kernel(
 // LDS).  Beyond that a workgroup is one group: a launch sums the slabs' Gram
 // shares of the step before (every workgroup the same, in order), forms Q,
 // applies it and leaves its share of the next one, so a step is one launch
-// where the tiled products take three.
+// where the tiled products take three (us: 62 x 2048 66, of which a launch
+// 11; tiled 109; one launch of all steps: 5 x 9 14.5, 50 x 60 18.4, 60 x 250
+// 31).
 __device__ __forceinline__ int swz(int r, int chunk) {
   return r * 64 + ((chunk ^ ((r >> 1) & 7)) * 8);
 }
