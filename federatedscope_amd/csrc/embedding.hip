@@ -1080,7 +1080,8 @@ extern "C" int fsagg_embed_lookup(const void *table, int64_t vocab,
   const int64_t per = int64_t(kWave) * kLookVecs * v;
   const int64_t stretches = (dim + per - 1) / per;
   const int64_t grid = (tokens * stretches + kWaves - 1) / kWaves;
-  if (stretches > INT32_MAX || grid > kMaxGrid) {
+  if (stretches > INT32_MAX || tokens > kMaxGrid * kWaves ||
+      grid > kMaxGrid) {
     set_error("%s: %lld tokens of %lld columns are too many for one call",
               what, (long long)tokens, (long long)dim);
     return FSAGG_EINVAL;
@@ -1106,7 +1107,10 @@ extern "C" int fsagg_embed_lookup(const void *table, int64_t vocab,
 extern "C" size_t fsagg_embed_grad_workspace_bytes(int64_t tokens,
                                                    int64_t dim,
                                                    int64_t vocab) {
-  if (tokens <= 0 || dim <= 0 || vocab < 0) return 0;
+  if (tokens <= 0 || tokens > FSAGG_EMBED_MAX_TOKENS || dim <= 0 ||
+      dim > FSAGG_EMBED_MAX_COLS || vocab < 0 ||
+      vocab > FSAGG_EMBED_MAX_ROWS)
+    return 0;
   return sizes_of(tokens, dim, vocab).total;
 }
 
@@ -1123,9 +1127,10 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
     set_error("%s: invalid argument", what);
     return FSAGG_EINVAL;
   }
-  if (vocab > FSAGG_EMBED_MAX_ROWS) {
-    set_error("%s: %lld rows, at most %d", what, (long long)vocab,
-              FSAGG_EMBED_MAX_ROWS);
+  if (vocab > FSAGG_EMBED_MAX_ROWS || dim > FSAGG_EMBED_MAX_COLS) {
+    set_error("%s: %lld rows of %lld columns, at most %d of %d", what,
+              (long long)vocab, (long long)dim, FSAGG_EMBED_MAX_ROWS,
+              FSAGG_EMBED_MAX_COLS);
     return FSAGG_EINVAL;
   }
   const int e = elem_bytes(dtype), oe = elem_bytes(out_dtype);

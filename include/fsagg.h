@@ -338,6 +338,7 @@ int fsagg_embed_lookup(const void *table, int64_t vocab, int64_t dim,
  *     16-byte aligned; nothing is kept in it.
  */
 #define FSAGG_EMBED_MAX_ROWS 2147483646
+#define FSAGG_EMBED_MAX_COLS 1073741824
 #define FSAGG_EMBED_MAX_TOKENS 268435456
 typedef struct fsagg_embed_part {
   const void *ids;  /* (device) */

@@ -107,7 +107,9 @@ def test_embed_abi_refusals():
     assert look(4096, 4, 8, 8, 3, 4096, 1, 1, 1.0, 4096, None) == -1
     assert look(4096, 4, 8, 8, 0, None, 1, 1, 1.0, 4096, None) == -1
     assert look(None, 4, 8, 8, 0, 4096, 1, 1, 1.0, 4096, None) == -1
-    assert look(4096, 4, 8, 8, 0, 4096, 1, 1 << 40, 1.0, 4096, None) == -1
+    for many in (1 << 40, (1 << 62) + 1):
+        assert look(4096, 4, 8, 8, 0, 4096, 1, many, 1.0, 4096, None) == -1
+    assert look(4096, 4, 1 << 50, 8, 0, 4096, 1, 1, 1.0, 4096, None) == -1
     assert look(None, 4, 8, 8, 0, None, 1, 0, 1.0, None, None) == 0
     part = (L.EmbedPart * 1)(L.EmbedPart(4096, 8192, 5, 8, 1.0, 1))
 
@@ -121,6 +123,10 @@ def test_embed_abi_refusals():
     assert grad(odt=3) == -1
     assert grad(out=None) == -1
     assert grad(vocab=1 << 31) == -1
+    for dim in (1 << 31, 1 << 40, (1 << 62) + 8):
+        assert grad(dim=dim, ld=dim) == -1
+        assert lib.fsagg_embed_grad_workspace_bytes(5, dim, 10) == 0
+    assert lib.fsagg_embed_grad_workspace_bytes(1 << 40, 8, 10) == 0
     assert grad(ws=None) == -3
     assert grad(ws_bytes=64) == -3
     assert grad(ws=4100) == -1
