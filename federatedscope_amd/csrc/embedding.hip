@@ -286,11 +286,12 @@ __global__ __launch_bounds__(kBlock) void embed_key_kernel(Parts P, Sort W,
   }
 }
 
-// token k of this thread's rounds in the tile at `base`: wave w owns tokens
-// [256 w, 256 w + 256) in rounds of 64
-__device__ __forceinline__ int64_t tile_token(int64_t base, int k) {
+// token k of this thread's `rounds` in the tile at `base`: a wave owns
+// neighbouring tokens, in rounds of 64
+__device__ __forceinline__ int64_t tile_token(int64_t base, int k,
+                                              int rounds = kRounds) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  return base + wave * (kRounds * kWave) + k * kWave + lane;
+  return base + wave * (rounds * kWave) + k * kWave + lane;
 }
 
 // Rank of every token of a workgroup's tile among the tile's tokens of the
@@ -299,7 +300,7 @@ __device__ __forceinline__ int64_t tile_token(int64_t base, int k) {
 template <int TH>
 __device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
                                            const bool (&in)[kRounds],
-                                           int shift, int bits,
+                                           int rounds, int shift, int bits,
                                            uint16_t *cnt,
                                            uint32_t (&rank)[kRounds]) {
   constexpr int kW = TH / kWave;
@@ -311,6 +312,7 @@ __device__ __forceinline__ void tile_ranks(const uint32_t (&key)[kRounds],
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
+    if (k >= rounds) break;
     const uint32_t d = (key[k] >> shift) & mask;
     uint64_t same = __ballot(in[k]);
     for (int b = 0; b < bits; ++b) {
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(kTileThreads) void embed_scatter_kernel(
         return total;
       },
       at, scratch);
-  tile_ranks<kTileThreads>(key, in, shift, bits, cnt, rank);
+  tile_ranks<kTileThreads>(key, in, kRounds, shift, bits, cnt, rank);
   for (int d = threadIdx.x; d < digits; d += kTileThreads) {
     at[d] += mine[d];
     wave_prefix<kTileThreads>(cnt, d);
@@ -600,10 +602,12 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
   uint32_t key[kRounds], tok[kRounds], rank[kRounds];
   bool in[kRounds];
   const int wave = threadIdx.x / kWave;
+  // (as few rounds as hold the tokens: all waves are at it)
+  const int rounds = int((tokens + kOneThreads - 1) / kOneThreads);
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const int t = int(tile_token(0, k));
-    in[k] = t < tokens;
+    const int t = int(tile_token(0, k, rounds));
+    in[k] = k < rounds && t < tokens;
     tok[k] = uint32_t(in[k] ? t : int(tokens) - 1);
   }
   const char *row[kRounds];
@@ -627,7 +631,7 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
   const int digits = 1 << bits;
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
-    tile_ranks<kOneThreads>(key, in, shift, bits, cnt, rank);
+    tile_ranks<kOneThreads>(key, in, rounds, shift, bits, cnt, rank);
     digit_starts<kOneThreads>(
         digits, [&](int d) { return wave_prefix<kOneThreads>(cnt, d); }, at,
         scratch);
@@ -642,7 +646,7 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {
-      const int t = int(tile_token(0, k));
+      const int t = int(tile_token(0, k, rounds));
       if (in[k]) {
         key[k] = skey[t];
         tok[k] = stok[t];
@@ -651,7 +655,7 @@ __global__ __launch_bounds__(kOneThreads) void embed_sort_kernel(
   }
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const int64_t t = tile_token(0, k);
+    const int64_t t = tile_token(0, k, rounds);
     if (in[k]) {
       W.key[src][t] = key[k];
       W.srow[t] = srow[tok[k]];
