@@ -34,7 +34,7 @@ constexpr int kWaves = kBlock / kWave;
 constexpr int kMaxParts = 112;    // parts per key launch (kernel arguments)
 // Sorting: a thread holds kRounds tokens.  Up to kOneTile tokens are one
 // workgroup's (4096 tokens of 4000 rows of 300, the whole call 25 us, in
-// tiles 30); else tiles of 1024 tokens, small enough that many sort at once.
+// tiles 30; 1000 tokens 16, 25); else tiles of 1024 tokens, small enough that many sort at once.
 constexpr int kRounds = 4;
 constexpr int kOneThreads = 1024, kOneTile = kOneThreads * kRounds;
 constexpr int kTileThreads = 256, kTile = kTileThreads * kRounds;
@@ -854,8 +854,9 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
 // token's place is the number of tokens that come before it), then a wave
 // adds up one row's tokens in one slice of columns; workgroups past those
 // write the zero rows.  Against the sort's launches, us: 64 tokens of 4000
-// rows of 300 6.7 / 19.3, 256 tokens 12.1 / 20.4, 256 of 100 rows of 64
-// 13.9 / 17.2; it grows with the tokens' square.
+// rows of 300 6.6 / 14.4, 256 tokens 11.4 / 17.2, 256 of 100 rows of 64
+// 13.7 / 15.2 (of 10 rows, which are long, 19.5 / 14.6); it grows with the
+// tokens' square.
 template <int GT, int OT, int VEC>
 __global__ __launch_bounds__(kBlock) void embed_few_kernel(Parts P, Out O,
                                                            int sum_blocks) {
