@@ -34,7 +34,8 @@ constexpr int kWaves = kBlock / kWave;
 constexpr int kMaxParts = 112;    // parts per key launch (kernel arguments)
 // Sorting: a thread holds kRounds tokens.  Up to kOneTile tokens are one
 // workgroup's (4096 tokens of 4000 rows of 300, the whole call 25 us, in
-// tiles 30; 1000 tokens 16, 25); else tiles of 1024 tokens, small enough that many sort at once.
+// tiles 30; 1000 tokens 16, 25); else tiles of 1024 tokens, small enough that
+// many sort at once.
 constexpr int kRounds = 4;
 constexpr int kOneThreads = 1024, kOneTile = kOneThreads * kRounds;
 constexpr int kTileThreads = 256, kTile = kTileThreads * kRounds;
