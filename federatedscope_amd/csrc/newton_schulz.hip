@@ -14,12 +14,8 @@
 // the error.  So the result is as exact as a chain of fp32 products (relative
 // error 1e-6 .. 8e-6 against 64 bits by spectrum, both) at 3/16 of the cost
 // per product: 16-bit limbs run at 16 times the fp32 matrix rate.
-//
-// A bf16 result of matrices large enough for big tiles takes the high limbs'
-// product alone (aX keeps both limbs): its error against 64 bits is 1.9e-3 ..
-// 2.2e-3 for decaying spectra, where rounding the exact result to bf16 leaves
-// 1.66e-3 (2.6e-3 .. 4e-3 where all singular values are nearly equal), for a
-// third of the matrix work.  fp16 results, 8 times finer, keep both.
+// The result's type does not matter to this: a 16-bit result is the fp32 one,
+// rounded once.
 //
 // A = X X^T and A^2 are products C = P R^T with both operands contiguous along
 // k; A and Q are symmetric: the tiles on and above the diagonal are computed
@@ -541,15 +537,15 @@ __device__ __forceinline__ int line_at(const Line &L, int q) {
 // Rows and columns of the padding are zero in every plane (the prepare pass
 // writes them, products of zero rows are zero), so no tile is ragged inside
 // the workspace; only the last step checks its stores against the matrix.
-template <int BM, int BN, int WM, int WN, int NBUF, int LIMBS>
+template <int BM, int BN, int WM, int WN, int NBUF>
 struct Tile {
-  static constexpr int kBM = BM, kBN = BN, kLimbs = LIMBS;
+  static constexpr int kBM = BM, kBN = BN;
   static constexpr int kWaves = (BM / WM) * (BN / WN);
   static constexpr int kThreads = kWaves * 64;
   static constexpr int MI = WM / 32, NJ = WN / 32;
-  static constexpr int kLoads = (BM + BN) * LIMBS * kBK * 2 / 1024;  // 1 KiB
+  static constexpr int kLoads = (BM + BN) * 2 * kBK * 2 / 1024;  // 1 KiB
   static constexpr int kPer = kLoads / kWaves;
-  static constexpr int kStage = (BM + BN) * LIMBS * kBK;  // halfs
+  static constexpr int kStage = (BM + BN) * 2 * kBK;  // halfs
   static constexpr int kLds = NBUF * kStage;
   static_assert(kPer * kWaves == kLoads, "loads divide over the waves");
   static_assert(BM % (kPer * 16) == 0 && BN % (kPer * 16) == 0,
@@ -590,8 +586,8 @@ struct Tile {
     // this wave's loads of a stage: LDS order is [P.h][P.l][R.h][R.l] rows
     // of 64 bytes, 16 rows per instruction, one plane per wave
     const int row0 = wave * (kPer * 16);
-    const bool right = row0 >= LIMBS * BM;
-    const int in = right ? row0 - LIMBS * BM : row0;
+    const bool right = row0 >= 2 * BM;
+    const int in = right ? row0 - 2 * BM : row0;
     const int side = right ? BN : BM;
     const _Float16 *base = in < side ? (right ? rh : ph) : (right ? rl : pl);
     const int g0 = (right ? j0 : i0) + (in < side ? in : in - side);
@@ -643,7 +639,7 @@ struct Tile {
     };
     const int fr = lane & 31, fk = lane >> 5;
     struct Frags {
-      half8 a[LIMBS][MI], b[LIMBS][NJ];
+      half8 a[2][MI], b[2][NJ];
     };
     auto read = [&](Frags &f, int k, int kk) {
       const _Float16 *st = lds + (k % NBUF) * kStage;
@@ -655,7 +651,7 @@ struct Tile {
           const int o =
               r * BM + (((col / 8) ^ (piece(r) << 2)) * 8) + col % 8;
 #pragma unroll
-          for (int l = 0; l < LIMBS; ++l) {
+          for (int l = 0; l < 2; ++l) {
             const _Float16 *p = st + l * BM * kBK + o;
             f.a[l][i] = join4(read_tr(p), read_tr(p + 4 * BM));
           }
@@ -664,7 +660,7 @@ struct Tile {
         const int r = wm + i * 32 + fr;
         const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
 #pragma unroll
-        for (int l = 0; l < LIMBS; ++l)
+        for (int l = 0; l < 2; ++l)
           f.a[l][i] = *reinterpret_cast<const half8 *>(st + l * BM * kBK + o);
       }
 #pragma unroll
@@ -672,22 +668,22 @@ struct Tile {
         const int r = wn + j * 32 + fr;
         const int o = r * kBK + (((kk * 2 + fk) ^ ((r >> 2) & 3)) * 8);
 #pragma unroll
-        for (int l = 0; l < LIMBS; ++l)
+        for (int l = 0; l < 2; ++l)
           f.b[l][j] = *reinterpret_cast<const half8 *>(
-              st + (LIMBS * BM + l * BN) * kBK + o);
+              st + (2 * BM + l * BN) * kBK + o);
       }
     };
     // l h, h l, h h (the small terms first)
     auto mul = [&](const Frags &f) {
 #pragma unroll
-      for (int t = LIMBS == 2 ? 0 : 2; t < 3; ++t)
+      for (int t = 0; t < 3; ++t)
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
           for (int j = 0; j < NJ; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                f.a[t == 0 ? LIMBS - 1 : 0][i],
-                f.b[t == 1 ? LIMBS - 1 : 0][j], acc[i][j], 0, 0, 0);
+                f.a[t == 0 ? 1 : 0][i], f.b[t == 1 ? 1 : 0][j], acc[i][j], 0, 0,
+                0);
     };
     clear();
     // nothing of the previous tile is on its way, and every wave has read its
@@ -726,8 +722,8 @@ struct Tile {
   // for the LDS and the memory pipe while the matrix cores wait.
   template <int LOADS, bool TR>
   static __device__ __forceinline__ void spread() {
-    constexpr int kMfma = MI * NJ * (LIMBS == 2 ? 3 : 1);
-    constexpr int kReads = LIMBS * ((TR ? 2 : 1) * MI + NJ);
+    constexpr int kMfma = MI * NJ * 3;
+    constexpr int kReads = 2 * ((TR ? 2 : 1) * MI + NJ);
     constexpr int kEach = kMfma > kReads + LOADS ? kMfma / (kReads + LOADS)
                                                  : 1;
 #pragma unroll
@@ -776,13 +772,10 @@ struct Tile {
           p)[(block * 4 + q) * kThreads + threadIdx.x];
   }
 
-  // f(integral constant): the result's type as a template argument (one limb
-  // goes with bf16 results only)
+  // f(integral constant): the result's type as a template argument
   template <int MODE, typename F>
   static __device__ __forceinline__ void with_result_type(const Mat &M, F f) {
-    if constexpr (MODE == kLast && LIMBS == 1) {
-      f(std::integral_constant<int, FSAGG_BF16>());
-    } else if constexpr (MODE == kLast) {
+    if constexpr (MODE == kLast) {
       if (M.odt == FSAGG_BF16) f(std::integral_constant<int, FSAGG_BF16>());
       else if (M.odt == FSAGG_F16)
         f(std::integral_constant<int, FSAGG_F16>());
@@ -903,21 +896,18 @@ struct Tile {
         split_n<8>(v, h, l);
         _Float16 *ch = kX ? P.xh(src ^ 1) : MODE == kGram ? P.ah : P.qh;
         _Float16 *cl = kX ? P.xl(src ^ 1) : MODE == kGram ? P.al : P.ql;
-        // (of one limb's products, Q has none to multiply; A and X are added,
-        // too)
-        constexpr bool kLow = LIMBS == 2 || MODE != kSquare;
         // C's other half, unless the tile is its own transpose
         if (!kX && ti != tj) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int64_t o = int64_t(gi + e) * ld + gj;
             ch[o] = h[e];
-            if (kLow) cl[o] = l[e];
+            cl[o] = l[e];
           }
         }
         const int64_t o = int64_t(gj) * ld + gi;
         *reinterpret_cast<half8 *>(ch + o) = h;
-        if (kLow) *reinterpret_cast<half8 *>(cl + o) = l;
+        *reinterpret_cast<half8 *>(cl + o) = l;
       }
     }
   }
@@ -1464,19 +1454,17 @@ __global__ __launch_bounds__(256) void ns_narrow_kernel(
 // two workgroups to a CU, is bound by its reads (of LDS, and twice the L2
 // traffic), but takes products that leave the last round of large ones too
 // empty (below); 64 x 64 is for matrices too small for that, where a tile's
-// latency counts.  One limb suffices for a bf16 result (above).
-using BigTile = Tile<256, 256, 128, 64, 2, 2>;
-using BigTile1 = Tile<256, 256, 128, 64, 4, 1>;
-using HalfTile = Tile<128, 128, 64, 64, 2, 2>;
-using HalfTile1 = Tile<128, 128, 64, 64, 4, 1>;
-using MidTile = Tile<64, 64, 32, 32, 4, 2>;
+// latency counts.
+using BigTile = Tile<256, 256, 128, 64, 2>;
+using HalfTile = Tile<128, 128, 64, 64, 2>;
+using MidTile = Tile<64, 64, 32, 32, 4>;
 // workgroups that the GPU holds: one of a 256 x 256 tile per CU, two of the
 // others
 constexpr int kBigPlaces = 256, kMidPlaces = 512;
 constexpr int kBigSide = 256, kMidSide = 64;
 
 // How an entry is computed: in one launch, by slabs, or by tiled products.
-enum Way { kWhole, kNarrowSlabs, kMid, kBig, kBigOne, kWays };
+enum Way { kWhole, kNarrowSlabs, kMid, kBig, kWays };
 
 int64_t round_to(int64_t v, int64_t p) { return (v + p - 1) / p * p; }
 
@@ -1519,16 +1507,15 @@ bool empty(const Mat &M) { return M.m == 0 || M.batch == 0; }
 
 // What big tiles gain over 64 x 64 ones, in multiplications of an m x m by an
 // m x n matrix: 7 of the entry's own to 4 of its padded one, less what the
-// shorter pipelines of small tiles save (kBigGain, for all of the group; of
-// one limb less of them is enough).  Fitted to both sides of 35 shapes; big
-// against small tiles, us: 512 x 16384 594 / 559, 512 x 32768 941 / 1022,
-// 1024 x 4096 573 / 488, 1024 x 8192 807 / 875, 1280 x 2560 677 / 518,
-// 1280 x 5120 860 / 907, 2048 x 2048 917 / 942, 2 x (1500 x 1500) 807 / 909,
-// 12 x (1024 x 1024) 1018 / 1335; a short side of 384 loses at any length
-// (384 x 32768 879 / 682).  bf16: 1024 x 2048 325 / 289, 768 x 4096 331 / 375,
-// 1536 x 1536 403 / 628.
+// shorter pipelines of small tiles save (kBigGain, for all of the group).
+// Fitted to both sides of 35 shapes; big against small tiles, us:
+// 512 x 16384 594 / 559, 512 x 32768 941 / 1022, 1024 x 4096 573 / 488,
+// 1024 x 8192 807 / 875, 1280 x 2560 677 / 518, 1280 x 5120 860 / 907,
+// 2048 x 2048 917 / 942, 2 x (1500 x 1500) 807 / 909, 12 x (1024 x 1024)
+// 1018 / 1335; a short side of 384 loses at any length (384 x 32768 879 /
+// 682).
 constexpr int kBigShort = 512;
-constexpr int64_t kBigGain[2] = {17500000000, 6500000000};
+constexpr int64_t kBigGain = 17500000000;
 int64_t big_gain(const Mat &M) {
   if (empty(M) || M.m < kBigShort) return 0;
   const int64_t m = M.m, n = M.n, mp = round_to(m, kBigSide),
@@ -1537,13 +1524,11 @@ int64_t big_gain(const Mat &M) {
   return gain > 0 ? gain * M.batch : 0;
 }
 
-Way way_of(const Mat &M, const int64_t (&gain)[2]) {
+Way way_of(const Mat &M, int64_t gain) {
   // narrow against 64 x 64 tiles, us: 50 x 1024 53 / 87, 50 x 16384 150 / 199
   if (M.m <= kNarrow && M.n <= kNarrowLong)
     return M.n <= 64 * kMaxWhole ? kWhole : kNarrowSlabs;
-  const int one = M.odt == FSAGG_BF16;
-  if (big_gain(M) > 0 && gain[one] >= kBigGain[one]) return one ? kBigOne : kBig;
-  return kMid;
+  return big_gain(M) > 0 && gain >= kBigGain ? kBig : kMid;
 }
 
 // The derived fields of an entry computed that way.
@@ -1587,7 +1572,6 @@ void plan_mat(Mat &M, Way way) {
 int64_t partial_bytes(Way way) {
   switch (way) {
     case kBig:
-    case kBigOne:
       return int64_t(2) * kBigPlaces * kBigSide * kBigSide * 4;
     case kMid:
       return int64_t(2) * kMidPlaces * kMidSide * kMidSide * 4;
@@ -1699,11 +1683,8 @@ struct Cost {
 template <class T>
 constexpr Cost cost_of() {
   if (T::kBM == 256)
-    return T::kLimbs == 2 ? Cost{1.5, 0.9, 7, 20, 1.8, 1.6, 8, 22}
-                          : Cost{0.5, 0.6, 7, 20, 0.65, 0.6, 8, 22};
-  if (T::kBM == 128)
-    return T::kLimbs == 2 ? Cost{0.65, 0.75, 4, 9, 0, 0, 0, 0}
-                          : Cost{0.2, 0.53, 4, 9, 0, 0, 0, 0};
+    return Cost{1.5, 0.9, 7, 20, 1.8, 1.6, 8, 22};
+  if (T::kBM == 128) return Cost{0.65, 0.75, 4, 9, 0, 0, 0, 0};
   return Cost{0.25, 0.31, 4, 4, 0.3, 0.4, 8, 8};
 }
 constexpr int kMinStages = 8;
@@ -1835,10 +1816,8 @@ void run_group(Group &G, Way way, float *partial, const Step &st) {
   else if (way == kNarrowSlabs) run_narrow<MUON>(G, st);
   else if (way == kMid)
     run_products<MidTile, MUON>(G, kMidPlaces, partial, st);
-  else if (way == kBig)
+  else
     run_products<BigTile, MUON, HalfTile>(G, kBigPlaces, partial, st);
-  else if constexpr (!MUON)  // (a parameter is fp32)
-    run_products<BigTile1, MUON, HalfTile1>(G, kBigPlaces, partial, st);
 }
 
 // f(group, way, bytes of its entries) for every group of entries, in turn;
@@ -1846,12 +1825,12 @@ void run_group(Group &G, Way way, float *partial, const Step &st) {
 // and pointers.
 template <typename Fill, typename F>
 int each_group(int nmat, Fill fill, Group &G, F f) {
-  int64_t gain[2] = {0, 0};
+  int64_t gain = 0;
   for (int i = 0; i < nmat; ++i) {
     Mat M;
     const int rc = fill(i, M);
     if (rc != FSAGG_OK) return rc;
-    gain[M.odt == FSAGG_BF16] += big_gain(M);
+    gain += big_gain(M);
   }
   for (int way = 0; way < kWays; ++way) {
     G.nmat = 0;

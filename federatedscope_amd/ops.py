@@ -1775,10 +1775,10 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7,
     float32, float16 or bfloat16, any strides.  Returns a new contiguous
     tensor (list) of g's dtype, or ``out`` (contiguous, of any of the three
     dtypes, not overlapping any input).  The arithmetic is as exact as
-    float32 products; for a bfloat16 result of large matrices its error is
-    about that of rounding to that type (which matrices share a call decides
-    what is large, so it may change the result by as much).  NaN or infinity anywhere in a matrix makes all of it
-    NaN; a zero matrix stays zero.  Not differentiable."""
+    float32 products whatever the types, rounded once at the end; which
+    matrices share a call may change a result within that error, as sums are
+    split by the work of all.  NaN or infinity anywhere in a matrix makes
+    all of it NaN; a zero matrix stays zero.  Not differentiable."""
     many = isinstance(g, (list, tuple))
     gs = list(g) if many else [g]
     if not gs:

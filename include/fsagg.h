@@ -239,9 +239,8 @@ int fsagg_server_opt_step_f64(double *param, const double *avg,
  * n = max of its sides, X = the m x n orientation of G / max(|G|_F, eps):
  *     A = X X^T,  X <- a X + (b A + c A^2) X      `steps` times,
  * stored back in G's own orientation.  The arithmetic is as exact as fp32
- * products (two fp16 limbs per value, fp32 sums, the norm in fp64; for bf16
- * results of large entries the high limbs' products alone, an error about
- * that of the type's rounding); the result is rounded once to out_dtype.
+ * products (two fp16 limbs per value, fp32 sums, the norm in fp64); the
+ * result is rounded once to out_dtype.
  * Which entries share a call may change a result within these errors, as the
  * products are split by the work of all.  A NaN or an infinity in a matrix
  * makes the whole of that matrix NaN; a zero matrix gives zeros.
