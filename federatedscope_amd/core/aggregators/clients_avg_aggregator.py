@@ -52,24 +52,41 @@ class ClientsAvgAggregator(DeviceEngine, _ModelIO, Aggregator):
     _row_keys = ()
 
     def _avg_with_rows(self, models, weights):
-        """_weighted_avg_device, with the keys that client 0 sends as sparse
+        """_weighted_avg_device, with the keys that a client sends as sparse
         COO tensors (one sparse dimension: the gradient layout of
         nn.Embedding(sparse=True)) taken as row-sparse *updates* of the
         server model's value: model + sum of w_i * update_i, through
         ops.embedding_grad.  Rows no client touched keep the model's value;
-        a client that lacks the key adds nothing.  The reference's loop has
-        no sparse form (clients_avg_aggregator.py:69-98 reduces dense
-        tensors)."""
-        self._row_keys = sparse_keys(models[0][1])
+        a client that lacks the key, the first one too, adds nothing.  The
+        reference's loop has no sparse form (clients_avg_aggregator.py:69-98
+        reduces dense tensors)."""
+        first = models[0][1]
+        self._row_keys = sparse_keys(first)
+        dense = models
+        if self._row_keys:
+            self._row_keys = sparse_keys_of_all(models)
+            dense = [(s, OrderedDict((k, v) for k, v in m.items()
+                                     if k not in self._row_keys))
+                     for s, m in models]
+        layout, flat, extra, keys = self._weighted_avg_device(dense, weights)
         if not self._row_keys:
-            return self._weighted_avg_device(models, weights)
-        sums = OrderedDict((k, self._row_sum(k, models, weights))
-                           for k in self._row_keys)
-        dense = [(s, OrderedDict((k, v) for k, v in m.items()
-                                 if k not in sums)) for s, m in models]
-        layout, flat, extra, _ = self._weighted_avg_device(dense, weights)
-        extra.update(sums)
-        return layout, flat, extra, list(models[0][1].keys())
+            # (100 dicts of 161 keys take 60 us, beside the sum that has
+            # been launched)
+            self._row_keys = sparse_keys_of_all(models)
+        if self._row_keys:
+            for k in self._row_keys:
+                extra[k] = self._row_sum(k, models, weights)
+            keys = self._with_row_keys(list(first))
+        return layout, flat, extra, keys
+
+    def _with_row_keys(self, keys):
+        """``keys`` and the row-sparse ones; in the server model's order
+        where the first client has not all of them."""
+        more = [k for k in self._row_keys if k not in keys]
+        if not more:
+            return keys
+        at = {k: i for i, k in enumerate(self.model.state_dict())}
+        return sorted(keys + more, key=lambda k: at.get(k, len(at)))
 
     def _row_sum(self, key, models, weights):
         dev = self.compute_device
@@ -87,8 +104,8 @@ class ClientsAvgAggregator(DeviceEngine, _ModelIO, Aggregator):
                     x.sparse_dim() == 1 and x.shape == base.shape):
                 raise ValueError(
                     'client %d: key %r must be a sparse COO update of shape '
-                    '%s with one sparse dimension, as the first client '
-                    'sends it' % (i, key, tuple(base.shape)))
+                    '%s with one sparse dimension, as another client sends '
+                    'it as one' % (i, key, tuple(base.shape)))
             # (_indices / _values: uncoalesced tensors, too)
             ids.append(x._indices()[0].to(dev).contiguous())
             vals.append(x._values().to(dev).reshape(ids[-1].numel(),
@@ -143,6 +160,15 @@ def sparse_keys(model):
         return ()
     return [k for k, v in model.items()
             if getattr(v, 'is_sparse', False)]
+
+
+def sparse_keys_of_all(models):
+    """The keys that any client of the (sample_size, dict) list sends as
+    sparse COO tensors, in the order in which they come."""
+    found = OrderedDict()
+    for i in L.host().sparse_dicts([m for _, m in models]):
+        found.update((k, None) for k in sparse_keys(models[i][1]))
+    return list(found)
 
 
 def _share_to_device(x, dev):

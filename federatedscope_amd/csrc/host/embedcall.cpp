@@ -24,6 +24,8 @@
 //
 // has_sparse(dict) -> bool: whether a value is a sparse COO tensor (asked of
 // every upload, most of which have none: 161 keys 2 us, 19 us in Python).
+// sparse_dicts(list) -> list of int: the places of the dicts for which it is
+// (100 dicts of 161 keys 60 us).
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
 #include <Python.h>
@@ -250,13 +252,48 @@ PyObject *embed_grad(PyObject *, PyObject *args) {
   }
 }
 
-PyObject *has_sparse(PyObject *, PyObject *dict) {
-  if (!PyDict_Check(dict)) Py_RETURN_FALSE;
+namespace {
+
+bool any_sparse(PyObject *dict) {
   PyObject *key, *value;
   Py_ssize_t pos = 0;
+  // (nearly all values are of one type, which is asked about once)
+  PyTypeObject *last = nullptr;
+  bool tensor = false;
   while (PyDict_Next(dict, &pos, &key, &value)) {
-    const c10::TensorImpl *t = tensor_of(value);
-    if (t && t->is_sparse()) Py_RETURN_TRUE;
+    if (Py_TYPE(value) != last) {
+      last = Py_TYPE(value);
+      tensor = THPVariable_Check(value);
+    }
+    if (tensor && THPVariable_Unpack(value).unsafeGetTensorImpl()->is_sparse())
+      return true;
   }
-  Py_RETURN_FALSE;
+  return false;
+}
+
+}  // namespace
+
+PyObject *has_sparse(PyObject *, PyObject *dict) {
+  return PyBool_FromLong(PyDict_Check(dict) && any_sparse(dict));
+}
+
+PyObject *sparse_dicts(PyObject *, PyObject *dicts) {
+  if (!PyList_Check(dicts)) {
+    PyErr_SetString(PyExc_TypeError, "a list of dicts is expected");
+    return nullptr;
+  }
+  PyObject *found = PyList_New(0);
+  if (!found) return nullptr;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(dicts); ++i) {
+    PyObject *d = PyList_GET_ITEM(dicts, i);
+    if (!PyDict_Check(d) || !any_sparse(d)) continue;
+    PyObject *at = PyLong_FromSsize_t(i);
+    if (!at || PyList_Append(found, at) != 0) {
+      Py_XDECREF(at);
+      Py_DECREF(found);
+      return nullptr;
+    }
+    Py_DECREF(at);
+  }
+  return found;
 }

@@ -49,6 +49,7 @@ PyObject *gram_select(PyObject *, PyObject *args);
 PyObject *embed_lookup(PyObject *, PyObject *args);
 PyObject *embed_grad(PyObject *, PyObject *args);
 PyObject *has_sparse(PyObject *, PyObject *dict);
+PyObject *sparse_dicts(PyObject *, PyObject *dicts);
 
 namespace {
 
@@ -717,6 +718,8 @@ PyMethodDef kMethods[] = {
      "stream, size_fn, fn) -> tensor or None"},
     {"has_sparse", has_sparse, METH_O,
      "has_sparse(dict) -> whether a value is a sparse COO tensor"},
+    {"sparse_dicts", sparse_dicts, METH_O,
+     "sparse_dicts(list) -> the places of the dicts that hold one"},
     {"key_table", key_table, METH_VARARGS,
      "key_table(dicts, keys, shapes, device_index[, offs4]) -> (bytes, "
      "missing, aligned16) or None"},

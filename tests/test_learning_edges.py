@@ -31,3 +31,16 @@ def test_damaged_results_are_told_from_right_ones(dtype):
     for x in bad + [_without_last_columns(g).to(dtype)]:
         with pytest.raises(AssertionError):
             _check_ns(x, g)
+
+
+def test_sparse_keys_of_every_client_are_seen():
+    from federatedscope_amd.core.aggregators.clients_avg_aggregator import \
+        sparse_keys_of_all
+    sp = torch.sparse_coo_tensor(torch.tensor([[1, 3]]), torch.ones(2, 4),
+                                 (5, 4))
+    plain = torch.zeros(2)
+    assert sparse_keys_of_all([(1, {'a': plain}), (2, 'no dict'),
+                               (3, {'b': sp, 'a': plain}), (4, {}),
+                               (5, {'c': torch.nn.Parameter(plain), 'd': sp,
+                                    'b': sp})]) == ['b', 'd']
+    assert sparse_keys_of_all([(1, {'a': plain, 'b': 'text'})]) == []
