@@ -65,9 +65,10 @@ class ClientsAvgAggregator(DeviceEngine, _ModelIO, Aggregator):
         dense = models
         if self._row_keys:
             self._row_keys = sparse_keys_of_all(models)
+            # (a StagedUpdate stays one: its slot is waited for by that)
             dense = [(s, OrderedDict((k, v) for k, v in m.items()
-                                     if k not in self._row_keys))
-                     for s, m in models]
+                                     if k not in self._row_keys)
+                      if isinstance(m, dict) else m) for s, m in models]
         layout, flat, extra, keys = self._weighted_avg_device(dense, weights)
         if not self._row_keys:
             # (100 dicts of 161 keys take 60 us, beside the sum that has

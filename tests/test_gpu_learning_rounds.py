@@ -103,3 +103,33 @@ def test_server_takes_rows_whoever_comes_first(rule, dev):
             tol = tol + 3 * 2.0**-24 * (want.abs() + (before[k] - avg).abs())
             assert bool(((v.cpu().double() - want).abs() <= tol).all())
             assert not torch.equal(v.cpu().double(), before[k])
+
+
+@pytest.mark.parametrize('dev', ['cpu', 'cuda'])
+def test_staged_uploads_beside_row_sparse_ones_have_landed(dev):
+    """Host uploads on their way to their slots (held up on the side stream)
+    when a list whose first client sent rows is reduced."""
+    from federatedscope_amd.core.aggregators import ClientsAvgAggregator
+    from federatedscope_amd.core.workers.ingress import DeviceIngress
+    from federatedscope_amd.layout import HostStager
+    model = _Net(False).cuda()
+    agg = ClientsAvgAggregator(model=model, device='cuda:0', config=_cfg())
+    # (two, as many as there are pinned buffers: a third would wait for one)
+    ups = _uploads(model, 3, 2, 'cpu', skip=('emb.weight', ))
+    rows = _sparse((40, 24), 6, 1, dev)
+    first = (ups[0][0], OrderedDict(
+        [(k, v.to(dev)) for k, v in ups[0][1].items()] +
+        [('emb.weight', rows)]))
+    want = agg.aggregate({'client_feedback': [first] + ups[1:],
+                          'recover_fun': None})
+    ing = DeviceIngress(ups[1][1], 2, device='cuda:0')
+    ing._stager = HostStager(ing.device)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(ing._stager.stream):
+        torch.cuda._sleep(100000000)
+    staged = [ing.receive(n, d) for n, d in ups[1:]]
+    got = agg.aggregate({'client_feedback': [first] + staged,
+                         'recover_fun': None})
+    assert list(got) == list(want)
+    for k in want:
+        assert torch.equal(got[k], want[k])
