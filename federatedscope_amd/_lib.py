@@ -240,6 +240,7 @@ SIGNATURES['fsagg_newton_schulz_workspace_bytes'] = (_c_sz, [_c_p, _c_i])
 SIGNATURES['fsagg_muon_workspace_bytes'] = (_c_sz, [_c_p, _c_i])
 SIGNATURES['fsagg_newton_schulz'] = (
     _c_i, [_c_p, _c_i, _c_i, _c_p, _c_d, _c_p, _c_sz, _c_p])
+SIGNATURES['fsagg_muon_check'] = (_c_i, [_c_p, _c_i, _c_p])
 SIGNATURES['fsagg_muon_step_f32'] = (
     _c_i, [_c_p, _c_i, _c_p, _c_p, _c_sz, _c_p])
 SIGNATURES['fsagg_embed_lookup'] = (

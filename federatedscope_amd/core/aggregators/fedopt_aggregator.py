@@ -168,6 +168,10 @@ class FedOptAggregator(ClientsAvgAggregator):
             need(self.ns_steps >= 1, 'ns_steps should be >= 1 but is: %s',
                  self.ns_steps)
             need(self.eps > 0.0, 'eps should be > 0 but is: %s', self.eps)
+            ops.muon_check(
+                [p.shape for p in self.model.parameters() if p.dim() == 2]
+                if self.model is not None else [], steps=self.ns_steps,
+                coefficients=self.ns_coefficients, eps=self.eps)
             if self._aux is None and self.model is not None:
                 for p in self.model.parameters():
                     need(p.dim() == 2, 'Muon only supports 2D parameters '
@@ -253,28 +257,31 @@ class FedOptAggregator(ClientsAvgAggregator):
         average), both flat.  Muon takes the matrices in one call, its aux
         optimizer the rest."""
         fn = L.load().fsagg_server_opt_step_f32
-        mats = []
+        mats, rest = [], []
         for k in keys:
             shape, param, avg = views(k)
             _check_f32_cuda(param, 'FedOpt parameter', align=4)
             _check_f32_cuda(avg, 'FedOpt bucket')
-            opt = self
-            if self.opt_type == 'Muon':
-                if len(shape) == 2:
-                    st = self._states(k, avg)
-                    mats.append((param.view(shape), avg, st[0]))
-                    st[3] += 1
-                    continue
-                opt = self._aux
-            opt._step(fn, param, avg, opt._states(k, avg))
+            if self.opt_type == 'Muon' and len(shape) == 2:
+                mats.append((param.view(shape), avg, self._states(k, avg)))
+            else:
+                opt = self._aux if self.opt_type == 'Muon' else self
+                rest.append((opt, param, avg, opt._states(k, avg)))
+        # the one call that may be refused comes before any other step: a
+        # round that raises has changed nothing
         if mats:
-            ops.muon_step(*map(list, zip(*mats)), lr=self._lr(),
+            ps, avgs, sts = map(list, zip(*mats))
+            ops.muon_step(ps, avgs, [st[0] for st in sts], lr=self._lr(),
                           momentum=self.momentum, nesterov=self.nesterov,
                           weight_decay=self.weight_decay,
                           steps=self.ns_steps,
                           coefficients=self.ns_coefficients, eps=self.eps,
                           adjust_lr=self.adjust_lr_fn,
                           maximize=self.maximize)
+            for st in sts:
+                st[3] += 1
+        for opt, param, avg, st in rest:
+            opt._step(fn, param, avg, st)
 
     def _step(self, fn, param, avg, st):
         """One optimizer step of a contiguous device parameter range."""

@@ -1873,10 +1873,9 @@ bool nothing(int nmat, Fill fill) {
   return true;
 }
 
-template <bool MUON, typename Fill>
-int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
-            const MuonScalars &S, void *ws, size_t ws_bytes,
-            hipStream_t stream, const char *what) {
+// What a call may be refused for, its sizes, pointers and workspace apart.
+int check_settings(int steps, const double *coef, double eps,
+                   const char *what) {
   if (steps < 1 || steps > 99) {
     set_error("%s: steps must be in [1, 99], got %d", what, steps);
     return FSAGG_EINVAL;
@@ -1890,9 +1889,18 @@ int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
               "limbs hold", what);
     return FSAGG_EINVAL;
   }
+  return FSAGG_OK;
+}
+
+template <bool MUON, typename Fill>
+int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
+            const MuonScalars &S, void *ws, size_t ws_bytes,
+            hipStream_t stream, const char *what) {
+  int rc = check_settings(steps, coef, eps, what);
+  if (rc != FSAGG_OK) return rc;
   // everything is checked before anything is launched
   size_t need = 0;
-  int rc = workspace_of(nmat, fill, need);
+  rc = workspace_of(nmat, fill, need);
   if (rc != FSAGG_OK) return rc;
   if (need > 0 && (!ws || ws_bytes < need)) {
     set_error("%s: workspace of %zu bytes, %zu needed", what,
@@ -2009,11 +2017,10 @@ extern "C" size_t fsagg_muon_workspace_bytes(const fsagg_muon_mat *mats,
   return need;
 }
 
-extern "C" int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
-                                   const fsagg_muon_params *hp,
-                                   void *workspace, size_t workspace_bytes,
-                                   fsagg_stream_t stream) {
-  const char *what = "fsagg_muon_step_f32";
+namespace {
+// the arguments that both calls below take
+int muon_arguments(const fsagg_muon_mat *mats, int nmat,
+                   const fsagg_muon_params *hp, const char *what) {
   if (nmat < 0 || (nmat > 0 && !mats) || !hp) {
     set_error("%s: invalid argument", what);
     return FSAGG_EINVAL;
@@ -2023,6 +2030,29 @@ extern "C" int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
     set_error("%s: unknown learning-rate adjustment %d", what, hp->adjust);
     return FSAGG_EINVAL;
   }
+  return FSAGG_OK;
+}
+}  // namespace
+
+extern "C" int fsagg_muon_check(const fsagg_muon_mat *mats, int nmat,
+                                const fsagg_muon_params *hp) {
+  const char *what = "fsagg_muon_check";
+  int rc = muon_arguments(mats, nmat, hp, what);
+  if (rc != FSAGG_OK) return rc;
+  const double coef[3] = {hp->a, hp->b, hp->c};
+  rc = check_settings(hp->steps, coef, hp->eps, what);
+  if (rc != FSAGG_OK) return rc;
+  size_t need = 0;
+  return workspace_of(nmat, muon_fill(mats, false, what), need);
+}
+
+extern "C" int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
+                                   const fsagg_muon_params *hp,
+                                   void *workspace, size_t workspace_bytes,
+                                   fsagg_stream_t stream) {
+  const char *what = "fsagg_muon_step_f32";
+  const int rc = muon_arguments(mats, nmat, hp, what);
+  if (rc != FSAGG_OK) return rc;
   MuonScalars S;
   S.keep = float(1.0 - hp->momentum);
   S.mu = float(hp->momentum);

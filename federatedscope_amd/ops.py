@@ -1886,6 +1886,22 @@ def muon_step(params, avgs, bufs, lr, momentum=0.95, nesterov=True,
                                         _stream(dev)), 'fsagg_muon_step_f32')
 
 
+def muon_check(shapes, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """ValueError if :func:`muon_step` would refuse matrices of these shapes
+    or these settings, for what its products hold; needs no GPU."""
+    coef = [float(x) for x in coefficients]
+    if len(coef) != 3:
+        raise ValueError('coefficients must be exactly 3 values')
+    table = (L.MuonMat * max(1, len(shapes)))()
+    for m, (rows, cols) in zip(table, shapes):
+        m.rows, m.cols = rows, cols
+    hp = L.MuonParams(a=coef[0], b=coef[1], c=coef[2], eps=float(eps),
+                      steps=int(steps))
+    lib = L.load()
+    if lib.fsagg_muon_check(table, len(shapes), ctypes.byref(hp)) != 0:
+        raise ValueError(lib.fsagg_last_error().decode())
+
+
 def _check_disjoint(written, read):
     """No written tensor overlaps any other (the read ones may coincide)."""
     spans = sorted([_extent(t) + (1, ) for t in written if t.numel()] +

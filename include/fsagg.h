@@ -299,6 +299,10 @@ typedef struct fsagg_muon_params {
   int32_t steps, nesterov, maximize, adjust;
 } fsagg_muon_params;
 size_t fsagg_muon_workspace_bytes(const fsagg_muon_mat *mats, int nmat);
+/* What the step would refuse of these sizes and settings (the entries'
+ * pointers and the workspace apart): FSAGG_OK, or its error.  Needs no GPU. */
+int fsagg_muon_check(const fsagg_muon_mat *mats, int nmat,
+                     const fsagg_muon_params *hp);
 int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
                         const fsagg_muon_params *hp, void *workspace,
                         size_t workspace_bytes, fsagg_stream_t stream);

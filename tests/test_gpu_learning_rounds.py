@@ -1,5 +1,6 @@
 """Rounds of the framework's paths through the learning operators that come
-in another order: a first client without a row-sparse key.
+in another order: a first client without a row-sparse key; and of such that
+end early: a refused Muon step.
 
 Tolerances are those of test_gpu_learning_paths."""
 from collections import OrderedDict
@@ -133,3 +134,58 @@ def test_staged_uploads_beside_row_sparse_ones_have_landed(dev):
     assert list(got) == list(want)
     for k in want:
         assert torch.equal(got[k], want[k])
+
+
+def _all_states(agg):
+    return [(k, st[3], [None if t is None else t.clone() for t in st[:3]])
+            for a in (agg, agg._aux) for k, st in a._state.items()]
+
+
+@pytest.mark.parametrize('model_dev', ['cpu', 'cuda'])
+@pytest.mark.parametrize('first', [True, False])
+def test_a_refused_muon_step_changes_nothing(first, model_dev, monkeypatch):
+    """Neither the parameters nor the states nor their counts, Muon's and the
+    aux optimizer's; and the step that follows is as if it had not been."""
+    from federatedscope_amd import ops
+    from federatedscope_amd.core.aggregators import FedOptAggregator
+    opt = dict(type='Muon', lr=0.05, aux=dict(type='Adam', lr=0.01))
+    models = [_Net(True).to(model_dev) for _ in range(2)]
+    aggs = [FedOptAggregator(config=_cfg(opt), model=m) for m in models]
+    if not first:
+        ups = _uploads(models[0], 3, 8, model_dev)
+        for a in aggs:
+            a.aggregate({'client_feedback': ups, 'recover_fun': None})
+    ups = _uploads(models[0], 3, 9, model_dev)
+    info = {'client_feedback': ups, 'recover_fun': None}
+    before = {k: v.clone() for k, v in models[0].state_dict().items()}
+    states, rounds = _all_states(aggs[0]), aggs[0]._rounds
+
+    def unchanged():
+        for k, v in models[0].state_dict().items():
+            assert torch.equal(v, before[k])
+        now = _all_states(aggs[0])
+        had = {k: (n, t) for k, n, t in states}
+        for k, n, t in now:
+            assert n == (had[k][0] if k in had else 0)
+            for x, y in zip(t, had[k][1] if k in had else [None] * 3):
+                assert x is None or (torch.equal(x, y) if y is not None else
+                                     not x.any())
+        assert (aggs[0]._rounds, aggs[0]._aux._rounds) == (rounds, rounds)
+    keep = aggs[0].ns_coefficients
+    aggs[0].ns_coefficients = (9.0, 9.0, 9.0)
+    with pytest.raises(Exception, match='coefficients'):
+        aggs[0].aggregate(info)
+    unchanged()
+    aggs[0].ns_coefficients = keep
+
+    def no_memory(*_, **__):
+        raise torch.cuda.OutOfMemoryError('no workspace')
+    with monkeypatch.context() as m:
+        m.setattr(ops, 'muon_step', no_memory)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            aggs[0].aggregate(info)
+    unchanged()
+    for a in aggs:
+        a.aggregate(info)
+    for k, v in models[0].state_dict().items():
+        assert torch.equal(v, models[1].state_dict()[k])

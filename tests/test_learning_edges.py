@@ -1,8 +1,14 @@
 """What the learning operators' checks catch, and the host's refusals at
 their edges; without a GPU."""
+import ctypes
+from types import SimpleNamespace
+
 import pytest
 import torch
 
+from federatedscope_amd import _lib as L
+from federatedscope_amd import ops
+from federatedscope_amd.core.aggregators import FedOptAggregator
 from test_gpu_learning import A, B, C, _chain, _check_ns, _matrix
 
 
@@ -44,3 +50,50 @@ def test_sparse_keys_of_every_client_are_seen():
                                (5, {'c': torch.nn.Parameter(plain), 'd': sp,
                                     'b': sp})]) == ['b', 'd']
     assert sparse_keys_of_all([(1, {'a': plain, 'b': 'text'})]) == []
+
+
+def _fedopt(model, **kw):
+    cfg = SimpleNamespace(
+        federate=SimpleNamespace(ignore_weight=False, use_ss=False),
+        fedopt=SimpleNamespace(optimizer=dict(type='Muon', lr=0.1, **kw),
+                               annealing=False))
+    return FedOptAggregator(config=cfg, model=model)
+
+
+def test_fedopt_muon_refuses_at_once_what_its_step_would():
+    """Coefficients, eps and matrices that the step does not take are refused
+    with the configuration, not in the first round."""
+    model = torch.nn.Linear(3, 2, bias=False)
+    for kw, word in ((dict(ns_coefficients=(9.0, 9.0, 9.0)), 'coefficients'),
+                     (dict(ns_coefficients=(float('nan'), 0.0, 0.0)),
+                      'coefficients'), (dict(eps=float('inf')), 'eps')):
+        with pytest.raises(ValueError, match=word):
+            _fedopt(model, **kw)
+    with pytest.raises(ValueError, match='20000 x 30000'):
+        _fedopt(torch.nn.Linear(30000, 20000, bias=False, device='meta'))
+    with pytest.raises(ValueError, match='1073741824 elements'):
+        _fedopt(torch.nn.Linear(256000, 5376, bias=False, device='meta'))
+    _fedopt(torch.nn.Linear(128000, 4096, bias=False, device='meta'))
+    _fedopt(None)
+
+
+def test_muon_check():
+    ops.muon_check([])
+    ops.muon_check([(3, 4), (0, 7), (16384, 65536), (1048576, 1024)])
+    for shapes, kw in (([(3, 4), (16385, 16385)], {}),
+                       ([(1, 1048577)], {}), ([(2048, 1048576)], {}),
+                       ([(-1, 4)], {}), ([], dict(steps=0)),
+                       ([(3, 4)], dict(steps=100)), ([], dict(eps=0.0)),
+                       ([], dict(coefficients=(9.0, 9.0, 9.0))),
+                       ([], dict(coefficients=(1.0, 2.0)))):
+        with pytest.raises(ValueError):
+            ops.muon_check(shapes, **kw)
+    lib = L.load()
+    hp = L.MuonParams(0.1, 0.9, 0.1, A, B, C, 1e-7, 5, 1, 0, 0)
+    t = (L.MuonMat * 1)(L.MuonMat(None, None, None, 4, 600))
+    assert lib.fsagg_muon_check(t, 1, ctypes.byref(hp)) == 0
+    assert lib.fsagg_muon_check(t, 1, None) == -1
+    assert lib.fsagg_muon_check(None, 1, ctypes.byref(hp)) == -1
+    assert lib.fsagg_muon_check(t, -1, ctypes.byref(hp)) == -1
+    hp.adjust = 2
+    assert lib.fsagg_muon_check(t, 1, ctypes.byref(hp)) == -1
