@@ -52,8 +52,11 @@ const c10::TensorImpl *tensor_of(PyObject *o) {
 }
 
 // the first element's address; false for a tensor that is not plain memory
+// (nor for a view whose memory holds the negative of its values)
 bool address(const c10::TensorImpl *t, uintptr_t &p) {
-  if (t->layout() != c10::kStrided || !t->has_storage()) return false;
+  if (t->layout() != c10::kStrided || !t->has_storage() ||
+      t->key_set().has(c10::DispatchKey::Negative))
+    return false;
   const void *d = t->storage().data();
   p = d ? reinterpret_cast<uintptr_t>(d) +
               uintptr_t(t->storage_offset()) * t->dtype().itemsize()

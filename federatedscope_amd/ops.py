@@ -224,8 +224,17 @@ def _check_f32_cuda(t, what, align=ALIGN_BYTES):
         raise ValueError('%s must be float32 (got %s)' % (what, t.dtype))
     if not t.is_contiguous():
         raise ValueError('%s must be contiguous' % what)
+    _check_plain(t, what)
     if t.data_ptr() % align:
         raise ValueError('%s must be %d-byte aligned' % (what, align))
+
+
+def _check_plain(t, what):
+    """Not a view whose memory holds the negative of its values (the
+    imaginary part of a conjugate)."""
+    if t.is_neg():
+        raise ValueError('%s is a lazily negated view: resolve_neg() first' %
+                         what)
 
 
 class RowTable:
@@ -1754,6 +1763,7 @@ def _check_float_cuda(t, what, device=None):
     if t.dtype not in _FLOAT_CODE:
         raise ValueError('%s must be float32, float16 or bfloat16 (got %s)' %
                          (what, t.dtype))
+    _check_plain(t, what)
 
 
 def _scratch(device, nbytes):
@@ -1925,6 +1935,7 @@ def _check_ids(ids, what, device):
                          (what, ids.dtype))
     if not ids.is_contiguous():
         raise ValueError('%s must be contiguous' % what)
+    _check_plain(ids, what)
 
 
 def _check_rows(t, what):

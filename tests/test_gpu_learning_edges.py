@@ -1,5 +1,5 @@
 """Calls of the learning operators at the edges of what they take: results of
-16-bit types, neighbours in a list.
+16-bit types, neighbours in a list, lazily negated views.
 
 Tolerances are those of test_gpu_learning, where they are not bits."""
 import pytest
@@ -46,3 +46,48 @@ def test_newton_schulz_is_as_exact_beside_others():
                 ops.newton_schulz([big] * 4 + [g])[4]):
         assert float((got.cpu().double() - want).norm()) <= tol
         _check_ns(got, g, where='cuda')
+
+
+def _negated(*shape):
+    """A view whose memory holds the negative of its values."""
+    return torch.randn(*shape, dtype=torch.complex64, device='cuda').conj() \
+        .imag
+
+
+def test_lazily_negated_views_are_refused():
+    """Their memory is not what they hold: resolved first, they are taken."""
+    from federatedscope_amd import ops
+    g = _negated(40, 60)
+    assert g.is_neg()
+    with pytest.raises(ValueError, match='resolve_neg'):
+        ops.newton_schulz(g)
+    _check_ns(ops.newton_schulz(g.resolve_neg()), g.resolve_neg())
+    x = torch.randn(40, 60, device='cuda')
+    with pytest.raises(ValueError, match='resolve_neg'):
+        ops.newton_schulz(x, out=torch._neg_view(torch.empty_like(x)))
+    for k in range(3):
+        t = [x.clone(), x.clone(), x.clone()]
+        t[k] = torch._neg_view(t[k])
+        with pytest.raises(ValueError, match='resolve_neg'):
+            ops.muon_step(t[:1], t[1:2], t[2:], lr=0.1)
+    ids = torch.arange(40, device='cuda')
+    one = _negated(40, 1)
+    for table in (one, torch._neg_view(x)):
+        with pytest.raises(ValueError, match='resolve_neg'):
+            ops.embedding_lookup(table, ids)
+        with pytest.raises(ValueError, match='resolve_neg'):
+            ops.embedding_grad(ids, table, 40)
+        assert torch.equal(
+            ops.embedding_lookup(table.resolve_neg(), ids), table)
+        assert torch.equal(
+            ops.embedding_grad(ids, table.resolve_neg(), 40), table)
+    with pytest.raises(ValueError, match='resolve_neg'):
+        ops.embedding_lookup(x, torch._neg_view(ids))
+    with pytest.raises(ValueError, match='resolve_neg'):
+        ops.embedding_grad(torch._neg_view(ids), x, 40)
+    with pytest.raises(ValueError, match='resolve_neg'):
+        ops.embedding_lookup(x, ids, out=torch._neg_view(x.clone()))
+    for acc in (False, True):
+        with pytest.raises(ValueError, match='resolve_neg'):
+            ops.embedding_grad(ids, x, 40, out=torch._neg_view(x.clone()),
+                               accumulate=acc)
