@@ -1912,7 +1912,10 @@ int run_all(int nmat, Fill fill, int steps, const double *coef, double eps,
     return FSAGG_EINVAL;
   }
   if (need == 0 && nothing(nmat, fill)) return FSAGG_OK;
-  const Step st = {float(coef[0]), float(coef[1]), float(coef[2]), eps,
+  // (the norm of an fp32 matrix is zero or over 1e-45, so a divisor below
+  // 1e-300 meets zeros only; kS / eps has to stay finite for them)
+  const double least = eps > 1e-300 ? eps : 1e-300;
+  const Step st = {float(coef[0]), float(coef[1]), float(coef[2]), least,
                    steps,          S,              stream};
   Group G;
   each_group(nmat, fill, G, [&](Group &g, Way way, size_t bytes) {

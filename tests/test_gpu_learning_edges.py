@@ -1,5 +1,5 @@
 """Calls of the learning operators at the edges of what they take: results of
-16-bit types, neighbours in a list, lazily negated views.
+16-bit types, neighbours in a list, lazily negated views, the least divisor.
 
 Tolerances are those of test_gpu_learning, where they are not bits."""
 import pytest
@@ -46,6 +46,19 @@ def test_newton_schulz_is_as_exact_beside_others():
                 ops.newton_schulz([big] * 4 + [g])[4]):
         assert float((got.cpu().double() - want).norm()) <= tol
         _check_ns(got, g, where='cuda')
+
+
+@pytest.mark.parametrize('shape', [(9, 14), (60, 2000), (90, 150),
+                                   (1200, 1300)])
+def test_newton_schulz_of_zeros_at_any_eps(shape):
+    """A zero matrix stays zero however small its divisor."""
+    from federatedscope_amd import ops
+    z = torch.zeros(*shape, device='cuda')
+    for eps in (1e-7, 1e-200, 1e-306, 5e-324):
+        assert torch.equal(ops.newton_schulz(z, eps=eps), z)
+    g = _matrix(*shape, seed=3).cuda()
+    assert torch.equal(ops.newton_schulz(g, eps=5e-324),
+                       ops.newton_schulz(g, eps=1e-200))
 
 
 def _negated(*shape):
