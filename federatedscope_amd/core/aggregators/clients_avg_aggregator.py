@@ -12,7 +12,8 @@ import torch
 from ... import _lib as L
 from ... import ops
 from ..auxiliaries.utils import param2tensor
-from ._engine import DeviceEngine, _first_device, fedavg_weights
+from ._engine import (DeviceEngine, _first_device, _host_ext,
+                      fedavg_weights)
 from .aggregator import Aggregator, _ModelIO
 
 
@@ -157,7 +158,9 @@ class ClientsAvgAggregator(DeviceEngine, _ModelIO, Aggregator):
 def sparse_keys(model):
     """The keys of a client's dict that are sparse COO tensors."""
     # (a StagedUpdate is no dict: it holds dense rows)
-    if not isinstance(model, dict) or not L.host().has_sparse(model):
+    host = _host_ext()
+    if not isinstance(model, dict) or (host is not None and
+                                       not host.has_sparse(model)):
         return ()
     return [k for k, v in model.items()
             if getattr(v, 'is_sparse', False)]
@@ -166,8 +169,10 @@ def sparse_keys(model):
 def sparse_keys_of_all(models):
     """The keys that any client of the (sample_size, dict) list sends as
     sparse COO tensors, in the order in which they come."""
+    host = _host_ext()
     found = OrderedDict()
-    for i in L.host().sparse_dicts([m for _, m in models]):
+    for i in (range(len(models)) if host is None else
+              host.sparse_dicts([m for _, m in models])):
         found.update((k, None) for k in sparse_keys(models[i][1]))
     return list(found)
 

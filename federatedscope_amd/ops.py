@@ -1944,6 +1944,15 @@ def _check_rows(t, what):
         raise ValueError('%s must be 2-D with contiguous rows' % what)
 
 
+def _host_ext():
+    """The _fsagg_host extension, or None where it was not built: the calls
+    are then made from here."""
+    try:
+        return L.host()
+    except (L.FsaggError, ImportError, OSError):
+        return None
+
+
 _embed_fns = None
 
 
@@ -1968,12 +1977,13 @@ def embedding_lookup(table, ids, scale=1.0, out=None):
     on the same GPU; ``out`` (contiguous, not overlapping either) or a new
     tensor [*ids.shape, dim] is returned.  Its gradient with respect to the
     table is :func:`embedding_grad`."""
-    if out is None and torch.cuda.is_initialized():
+    host = _host_ext()
+    if host is not None and out is None and torch.cuda.is_initialized():
         # the plain form natively; None: the checks below say why not
         cur = torch.cuda.current_device()
-        got = L.host().embed_lookup(table, ids, scale, cur,
-                                    torch._C._cuda_getCurrentRawStream(cur),
-                                    _embed_addresses()[0])
+        got = host.embed_lookup(table, ids, scale, cur,
+                                torch._C._cuda_getCurrentRawStream(cur),
+                                _embed_addresses()[0])
         if got is not None:
             return got
     _check_float_cuda(table, 'table')
@@ -2034,14 +2044,14 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, weights=None, out=None,
         raise ValueError('num_rows must not be negative')
     if accumulate and out is None:
         raise ValueError('accumulate needs out')
-    if torch.cuda.is_initialized():
+    host = _host_ext()
+    if host is not None and torch.cuda.is_initialized():
         # the plain form natively; None: the checks below say why not
         cur = torch.cuda.current_device()
         fns = _embed_addresses()
-        got = L.host().embed_grad(ids, grad, coefs, num_rows, out, accumulate,
-                                  cur,
-                                  torch._C._cuda_getCurrentRawStream(cur),
-                                  fns[1], fns[2])
+        got = host.embed_grad(ids, grad, coefs, num_rows, out, accumulate,
+                              cur, torch._C._cuda_getCurrentRawStream(cur),
+                              fns[1], fns[2])
         if got is not None:
             return got
     parts, tokens, dim, code = _embed_parts(ids, grad, coefs, out)

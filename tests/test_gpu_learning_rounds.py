@@ -1,6 +1,6 @@
 """Rounds of the framework's paths through the learning operators that come
 in another order: a first client without a row-sparse key; and of such that
-end early: a refused Muon step.
+end early: a refused Muon step; and without the host extension.
 
 Tolerances are those of test_gpu_learning_paths."""
 from collections import OrderedDict
@@ -189,3 +189,44 @@ def test_a_refused_muon_step_changes_nothing(first, model_dev, monkeypatch):
         a.aggregate(info)
     for k, v in models[0].state_dict().items():
         assert torch.equal(v, models[1].state_dict()[k])
+
+
+def _no_host():
+    from federatedscope_amd import _lib
+    raise _lib.FsaggError('_fsagg_host.so not found')
+
+
+def test_paths_without_the_host_extension(monkeypatch):
+    """The operators and FedAvg need libfsagg alone: where the host extension
+    was not built, the Python ways give the same bits."""
+    from federatedscope_amd import _lib, ops
+    from federatedscope_amd.core.aggregators import (ClientsAvgAggregator,
+                                                     _engine)
+    from federatedscope_amd.core.workers.server import AggregationServer
+    model = _Net(False).cuda()
+    ids = torch.tensor([3, -1, 39, 3], device='cuda')
+    table = model.state_dict()['emb.weight']
+    ups = _round(model, 3, 'cuda', without=(1, ))
+
+    def run():
+        agg = ClientsAvgAggregator(model=model, device='cuda:0',
+                                   config=_cfg())
+        a = agg.aggregate({'client_feedback': ups, 'recover_fun': None})
+        b = agg.aggregate({'client_feedback': [
+            (s, {k: v for k, v in d.items() if not v.is_sparse})
+            for s, d in ups], 'recover_fun': None})
+        other = _Net(False).cuda()
+        srv = AggregationServer(other, ClientsAvgAggregator(
+            model=other, device='cuda:0', config=_cfg()),
+            sample_client_num=4, device='cuda:0')
+        for c, u in enumerate(ups):
+            srv.callback_funcs_model_para(0, c, u)
+        return list(a.values()) + list(b.values()) + list(
+            other.state_dict().values()) + [
+                ops.embedding_lookup(table, ids, scale=2.0),
+                ops.embedding_grad(ids, table[:4], 50)]
+    want = run()
+    monkeypatch.setattr(_lib, 'host', _no_host)
+    monkeypatch.setattr(_engine, '_HOST', [None])
+    for x, y in zip(run(), want):
+        assert torch.equal(x, y)

@@ -97,3 +97,16 @@ def test_muon_check():
     assert lib.fsagg_muon_check(t, -1, ctypes.byref(hp)) == -1
     hp.adjust = 2
     assert lib.fsagg_muon_check(t, 1, ctypes.byref(hp)) == -1
+
+
+def test_sparse_keys_without_the_host_extension(monkeypatch):
+    from federatedscope_amd.core.aggregators import _engine
+    from federatedscope_amd.core.aggregators.clients_avg_aggregator import (
+        sparse_keys, sparse_keys_of_all)
+    monkeypatch.setattr(_engine, '_HOST', [None])
+    sp = torch.sparse_coo_tensor(torch.tensor([[1, 3]]), torch.ones(2, 4),
+                                 (5, 4))
+    models = [(1, {'a': torch.zeros(2)}), (2, 'no dict'), (3, {'b': sp})]
+    assert list(sparse_keys(models[0][1])) == []
+    assert sparse_keys(models[2][1]) == ['b']
+    assert sparse_keys_of_all(models) == ['b']
