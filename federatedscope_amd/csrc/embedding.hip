@@ -1073,7 +1073,8 @@ extern "C" int fsagg_embed_lookup(const void *table, int64_t vocab,
                                   float scale, void *out,
                                   fsagg_stream_t stream) {
   const char *what = "fsagg_embed_lookup";
-  if (vocab < 0 || dim < 0 || tokens < 0 || !float_dtype(dtype) ||
+  if (vocab < 0 || dim < 0 || tokens < 0 || row_stride < 0 ||
+      !float_dtype(dtype) ||
       (tokens > 0 && dim > 0 && (!ids || !out || (vocab > 0 && !table)))) {
     set_error("%s: invalid argument", what);
     return FSAGG_EINVAL;
@@ -1137,6 +1138,11 @@ extern "C" int fsagg_embed_grad(const fsagg_embed_part *parts, int nparts,
     set_error("%s: %lld rows of %lld columns, at most %d of %d", what,
               (long long)vocab, (long long)dim, FSAGG_EMBED_MAX_ROWS,
               FSAGG_EMBED_MAX_COLS);
+    return FSAGG_EINVAL;
+  }
+  if (out_stride < 0 || (vocab > 1 && out_stride < dim)) {
+    set_error("%s: result rows of %lld columns, %lld apart, overlap", what,
+              (long long)dim, (long long)out_stride);
     return FSAGG_EINVAL;
   }
   const int e = elem_bytes(dtype), oe = elem_bytes(out_dtype);

@@ -313,7 +313,7 @@ int fsagg_muon_step_f32(const fsagg_muon_mat *mats, int nmat,
  * What a server sends a client that needs only its tokens' rows (the
  * reference sends whole state dicts, core/workers/server.py:636-714).
  *   table (device) vocab rows of dim elements of `dtype` (FSAGG_F32, _F16,
- *     _BF16), row_stride elements apart; ids (device) int64 (ids64 != 0) or
+ *     _BF16), row_stride >= 0 elements apart; ids (device) int64 (ids64 != 0) or
  *     int32; out (device) contiguous [tokens][dim] of the table's dtype,
  *     not overlapping it.  Any alignment; 16-byte aligned rows are read 16
  *     bytes at a time.
@@ -335,8 +335,9 @@ int fsagg_embed_lookup(const void *table, int64_t vocab, int64_t dim,
  * by the sizes alone).  Stands in for the dense per-key average of
  * clients_avg_aggregator.py:60-100 where a client changed few rows.
  *   parts (host): nparts entries (one per client); ids (device) int64 or
- *     int32, rows (device) of `dtype`, row_stride elements apart; out
- *     (device) vocab rows, out_stride elements apart, overlapping no part.
+ *     int32, rows (device) of `dtype`, row_stride >= 0 elements apart; out
+ *     (device) vocab rows, out_stride >= dim elements apart (any for one
+ *     row), overlapping no part.
  *   Workspace: fsagg_embed_grad_workspace_bytes(all tokens, dim, vocab),
  *     16-byte aligned; nothing is kept in it.
  */

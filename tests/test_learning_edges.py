@@ -110,3 +110,21 @@ def test_sparse_keys_without_the_host_extension(monkeypatch):
     assert list(sparse_keys(models[0][1])) == []
     assert sparse_keys(models[2][1]) == ['b']
     assert sparse_keys_of_all(models) == ['b']
+
+
+def test_embed_abi_refuses_strides():
+    """Result rows that overlap (two workgroups would write one place), and
+    rows that lie backwards."""
+    lib = L.load()
+    look = lib.fsagg_embed_lookup
+    assert look(4096, 4, 8, -8, 0, 4096, 1, 1, 1.0, 4096, None) == -1
+    part = (L.EmbedPart * 1)(L.EmbedPart(4096, 8192, 5, 8, 1.0, 1))
+
+    def grad(vocab, stride, acc=0):
+        # (a call that is taken this far lacks its workspace)
+        return lib.fsagg_embed_grad(part, 1, 0, vocab, 8, 1 << 20, 0, stride,
+                                    acc, None, 0, None)
+    for vocab, stride in ((10, 7), (10, 0), (10, -8), (2, 7), (1, -1)):
+        assert grad(vocab, stride) == grad(vocab, stride, 1) == -1
+    for vocab, stride in ((10, 8), (10, 9), (1, 0), (1, 3)):
+        assert grad(vocab, stride) == grad(vocab, stride, 1) == -3
