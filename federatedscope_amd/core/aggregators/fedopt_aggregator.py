@@ -12,9 +12,10 @@ HBM across rounds.  Muon (momentum, nesterov, weight_decay, ns_steps,
 ns_coefficients, eps, adjust_lr_fn as torch.optim.Muon) steps all matrix
 parameters in one ops.muon_step; like torch.optim's it takes matrices only,
 unless ``aux`` = {type, lr, **kwargs} names another of these optimizers for
-the other parameters (biases, convolutions).  The updated parameters are
-written back into ``self.model`` and ``self.model.state_dict()`` is returned,
-as the reference does.
+the other parameters (biases, convolutions) and for the matrices whose names
+``aux`` lists as ``keys`` (embedding tables, output heads).  The updated
+parameters are written back into ``self.model`` and
+``self.model.state_dict()`` is returned, as the reference does.
 
 Optimizer config: ``config.fedopt.optimizer`` = {type, lr, **kwargs} as in
 get_optimizer (core/auxiliaries/optimizer_builder.py:19-60); annealing:
@@ -84,7 +85,7 @@ class FedOptAggregator(ClientsAvgAggregator):
         # torch.optim defaults per class
         self.weight_decay = float(opt.pop(
             'weight_decay', {'AdamW': 1e-2, 'Muon': 0.1}.get(t, 0.0)))
-        self._aux = None
+        self._aux, self._aux_keys = None, frozenset()
         self.amsgrad = False
         if t == 'SGD':
             self.momentum = float(opt.pop('momentum', 0.0))
@@ -116,6 +117,11 @@ class FedOptAggregator(ClientsAvgAggregator):
                 if aux.get('type') == 'Muon':
                     raise ValueError('the aux optimizer takes what Muon '
                                      'does not: it cannot be Muon')
+                keys = aux.pop('keys', None) or ()
+                if not isinstance(keys, (list, tuple)):
+                    raise TypeError('aux keys must be a list of parameter '
+                                    'names (got %r)' % (keys, ))
+                self._aux_keys = frozenset(keys)
                 # a second optimizer over the same model, stepping the
                 # parameters Muon does not take
                 self._aux = FedOptAggregator(
@@ -168,10 +174,16 @@ class FedOptAggregator(ClientsAvgAggregator):
             need(self.ns_steps >= 1, 'ns_steps should be >= 1 but is: %s',
                  self.ns_steps)
             need(self.eps > 0.0, 'eps should be > 0 but is: %s', self.eps)
+            named = dict(self.model.named_parameters()) \
+                if self.model is not None else {}
+            if self.model is not None:
+                need(self._aux_keys <= set(named),
+                     'aux keys that are no parameters: %s',
+                     sorted(self._aux_keys - set(named)))
             ops.muon_check(
-                [p.shape for p in self.model.parameters() if p.dim() == 2]
-                if self.model is not None else [], steps=self.ns_steps,
-                coefficients=self.ns_coefficients, eps=self.eps)
+                [p.shape for k, p in named.items() if self._takes(k, p.shape)],
+                steps=self.ns_steps, coefficients=self.ns_coefficients,
+                eps=self.eps)
             if self._aux is None and self.model is not None:
                 for p in self.model.parameters():
                     need(p.dim() == 2, 'Muon only supports 2D parameters '
@@ -204,6 +216,10 @@ class FedOptAggregator(ClientsAvgAggregator):
             need(0.0 <= self.momentum, 'Invalid momentum value: %s',
                  self.momentum)
             need(0.0 <= self.alpha, 'Invalid alpha value: %s', self.alpha)
+
+    def _takes(self, key, shape):
+        """Whether Muon itself steps this parameter."""
+        return len(shape) == 2 and key not in self._aux_keys
 
     def _lr(self):
         if not self._annealing:
@@ -254,7 +270,7 @@ class FedOptAggregator(ClientsAvgAggregator):
     def _step_keys(self, keys, views):
         """One optimizer step of the fp32 parameters ``keys``;
         ``views(k)`` gives a parameter's (shape, contiguous device values,
-        average), both flat.  Muon takes the matrices in one call, its aux
+        average), both flat.  Muon takes its matrices in one call, its aux
         optimizer the rest."""
         fn = L.load().fsagg_server_opt_step_f32
         mats, rest = [], []
@@ -262,7 +278,7 @@ class FedOptAggregator(ClientsAvgAggregator):
             shape, param, avg = views(k)
             _check_f32_cuda(param, 'FedOpt parameter', align=4)
             _check_f32_cuda(avg, 'FedOpt bucket')
-            if self.opt_type == 'Muon' and len(shape) == 2:
+            if self.opt_type == 'Muon' and self._takes(k, shape):
                 mats.append((param.view(shape), avg, self._states(k, avg)))
             else:
                 opt = self._aux if self.opt_type == 'Muon' else self
@@ -308,7 +324,7 @@ class FedOptAggregator(ClientsAvgAggregator):
                 raise NotImplementedError(
                     'FedOpt on %s parameter %r' % (named[k].dtype, k))
             if k in extra and self.opt_type == 'Muon' and \
-                    (self._aux is None or named[k].dim() == 2):
+                    (self._aux is None or self._takes(k, named[k].shape)):
                 raise NotImplementedError('Muon on %s parameter %r' %
                                           (extra[k].dtype, k))
         dev = self.compute_device

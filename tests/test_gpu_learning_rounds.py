@@ -1,6 +1,7 @@
 """Rounds of the framework's paths through the learning operators that come
 in another order: a first client without a row-sparse key; and of such that
-end early: a refused Muon step; and without the host extension.
+end early: a refused Muon step; without the host extension; with matrices that
+Muon is not to step.
 
 Tolerances are those of test_gpu_learning_paths."""
 from collections import OrderedDict
@@ -230,3 +231,42 @@ def test_paths_without_the_host_extension(monkeypatch):
     monkeypatch.setattr(_engine, '_HOST', [None])
     for x, y in zip(run(), want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize('model_dev', ['cpu', 'cuda'])
+@pytest.mark.parametrize('rows', [False, True])
+def test_fedopt_muon_leaves_the_keys_of_aux_alone(rows, model_dev):
+    """A table and a head that aux names take its step exactly as without
+    Muon (rows that no client touched stay as they are under SGD), the other
+    matrix Muon's."""
+    from federatedscope_amd.core.aggregators import FedOptAggregator
+    aux = dict(type='SGD', lr=0.5) if rows else dict(type='AdamW', lr=0.01)
+    both, alone = _Net(True).to(model_dev), _Net(True).to(model_dev)
+    a1 = FedOptAggregator(config=_cfg(dict(type='Muon', lr=0.05, aux=dict(
+        aux, keys=['emb.weight', 'b.weight']))), model=both)
+    a2 = FedOptAggregator(config=_cfg(aux), model=alone)
+    for r in range(2):
+        before = {k: v.detach().cpu().double() for k, v in
+                  both.named_parameters()}
+        mom = a1._state['a.weight'][0].view(70, 24).cpu().double() if r \
+            else torch.zeros(70, 24, dtype=torch.float64)
+        ups = _uploads(both, 3, r, model_dev)
+        if rows:
+            for i, (_, d) in enumerate(ups):
+                d['emb.weight'] = _sparse((40, 24), 4, 10 * r + i, model_dev)
+        info = {'client_feedback': ups, 'recover_fun': None}
+        got, want = a1.aggregate(info), a2.aggregate(info)
+        for k in got:
+            if k != 'a.weight':
+                assert torch.equal(got[k], want[k])
+        w, _, tol = _muon_ref(before['a.weight'], _avg(ups, 'a.weight'), mom,
+                              0.05)
+        assert float((got['a.weight'].cpu().double() - w).abs().max()) <= \
+            tol + 3 * 2.0**-24 * float(w.abs().max())
+        if rows:
+            named = set(torch.cat([d['emb.weight']._indices()[0].cpu()
+                                   for _, d in ups]).tolist())
+            rest = [i for i in range(40) if i not in named]
+            assert torch.equal(got['emb.weight'].cpu().double()[rest],
+                               before['emb.weight'][rest])
+    assert sorted(a1._state) == ['a.weight']

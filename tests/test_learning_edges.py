@@ -128,3 +128,21 @@ def test_embed_abi_refuses_strides():
         assert grad(vocab, stride) == grad(vocab, stride, 1) == -1
     for vocab, stride in ((10, 8), (10, 9), (1, 0), (1, 3)):
         assert grad(vocab, stride) == grad(vocab, stride, 1) == -3
+
+
+def test_fedopt_muon_aux_keys_config():
+    """Matrices that aux names are not Muon's: neither stepped by it nor
+    measured against its limits."""
+    aux = dict(type='Adam', lr=0.2, keys=['weight'])
+    agg = _fedopt(torch.nn.Linear(30000, 20000, bias=False, device='meta'),
+                  aux=aux)
+    assert agg._aux.opt_type == 'Adam' and 'keys' in aux
+    assert not agg._takes('weight', (20000, 30000))
+    assert agg._takes('other', (3, 4)) and not agg._takes('other', (3, ))
+    with pytest.raises(ValueError, match='nothing.weight'):
+        _fedopt(torch.nn.Linear(3, 2), aux=dict(type='SGD', lr=0.1, keys=[
+            'weight', 'nothing.weight']))
+    with pytest.raises(TypeError, match='list'):
+        _fedopt(torch.nn.Linear(3, 2), aux=dict(type='SGD', lr=0.1,
+                                                keys='weight'))
+    _fedopt(None, aux=dict(type='SGD', lr=0.1, keys=['weight']))
