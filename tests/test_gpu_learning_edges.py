@@ -104,3 +104,62 @@ def test_lazily_negated_views_are_refused():
         with pytest.raises(ValueError, match='resolve_neg'):
             ops.embedding_grad(ids, x, 40, out=torch._neg_view(x.clone()),
                                accumulate=acc)
+
+
+@pytest.mark.parametrize('rows,cols', [(8, 1048576), (130, 1048576),
+                                       (1025, 4090 * 256)])
+def test_newton_schulz_of_the_longest_is_as_exact(rows, cols):
+    """The longest rows that are taken, and planes past 2 GB: within four
+    times the float32 chain's error and the limbs' own, over all and for
+    every 256 columns of a row (a missing limb is off by a thousandth)."""
+    from federatedscope_amd import ops
+    t = torch.Generator(device='cuda').manual_seed(rows)
+    g = torch.randn(rows, cols, generator=t, device='cuda')
+
+    def chain(x):
+        for _ in range(5):
+            gram = x @ x.T
+            x = A * x + (B * gram + C * (gram @ gram)) @ x
+        return x
+    x = g.double()
+    x /= x.norm()
+    y = chain(x.float())
+    want = chain(x)
+    del x
+    got = ops.newton_schulz(g)
+    limb = _limb_error(g, 5, (A, B, C), 1e-7, where='cuda')
+    del g
+    errors = []
+    for z in (got, y):
+        off = torch.empty(rows, cols // 256, device='cuda',
+                          dtype=torch.float64)
+        for i in range(0, rows, 64):
+            d = z[i:i + 64].double() - want[i:i + 64]
+            off[i:i + 64] = d.view(len(d), -1, 256).square().sum(-1).sqrt()
+        errors.append(off)
+    own, plain = errors
+    assert float(own.norm()) <= 4 * float(plain.norm()) + limb
+    # a block's share of the limbs' error is at most all of it
+    assert bool((own <= 4 * float(plain.max()) + limb).all())
+
+
+@pytest.mark.parametrize('rows,cols', [(9, 14), (60, 2000), (90, 150)])
+def test_newton_schulz_of_negative_strides(rows, cols):
+    """A matrix that lies backwards, through the C entry point (torch has no
+    such views): the same as its copy the right way round."""
+    import ctypes
+
+    from federatedscope_amd import _lib as L
+    from federatedscope_amd import ops
+    g = _matrix(rows, cols, 4).cuda()
+    last = g.data_ptr() + 4 * (rows * cols - 1)
+    out = torch.empty_like(g)
+    table = (L.NsMat * 1)(L.NsMat(last, out.data_ptr(), rows, cols, 1, 0,
+                                  -cols, -1, 0, 0))
+    lib = L.load()
+    ws = torch.empty(max(16, lib.fsagg_newton_schulz_workspace_bytes(
+        table, 1)), dtype=torch.uint8, device='cuda')
+    assert lib.fsagg_newton_schulz(
+        table, 1, 5, (ctypes.c_double * 3)(A, B, C), 1e-7, ws.data_ptr(),
+        ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, ops.newton_schulz(g.flip(0, 1)))
