@@ -21,7 +21,7 @@
 // rows, 0.79 GB, 183 us = 4.3 TB/s, the sum alone 142 us; 100 clients' 400
 // rows of 1024 fp32 added into 50000, 0.26 GB, 88 us, of which the sum is
 // 52 and the sort 27; a lookup of 16384 x 4096 bf16 34 us).  Small calls are
-// bound by their launches (9 .. 30 us).
+// bound by the host and their launches (7 rows 5 us, 48 tokens 7, 5001 22).
 #include "common.h"
 
 #include <hip/hip_fp16.h>
@@ -717,7 +717,6 @@ constexpr int64_t kScanKeys = 32 * kBlock;
 template <int GT, int OT, int VEC>
 __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Out O, Sort W,
                                                            int sum_blocks) {
-  constexpr int kGE = sizeof(typename Elem<GT>::type);
   constexpr int kOE = sizeof(typename Elem<OT>::type);
   const int lane = threadIdx.x & (kWave - 1);
   const int wave =
@@ -1081,6 +1080,8 @@ extern "C" int fsagg_embed_lookup(const void *table, int64_t vocab,
   }
   if (tokens == 0 || dim == 0) return FSAGG_OK;
   const int e = elem_bytes(dtype);
+  // 16 bytes a lane, else an element (65536 tokens of 1024 / 1025, us: bf16
+  // 38 / 69, fp32 75 / 94; the gradient 87 / 133, 116 / 143)
   const bool vec = (dim * e) % 16 == 0 && (row_stride * e) % 16 == 0 &&
                    aligned16(table) && aligned16(out);
   const int v = vec ? 16 / e : 1;

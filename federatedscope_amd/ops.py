@@ -1788,7 +1788,8 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7,
     float32 products whatever the types, rounded once at the end; which
     matrices share a call may change a result within that error, as sums are
     split by the work of all.  NaN or infinity anywhere in a matrix makes
-    all of it NaN; a zero matrix stays zero.  Not differentiable."""
+    all of it NaN; a zero matrix stays zero.  Not differentiable: the result
+    of a tensor that requires grad carries no graph."""
     many = isinstance(g, (list, tuple))
     gs = list(g) if many else [g]
     if not gs:
@@ -1975,8 +1976,8 @@ def embedding_lookup(table, ids, scale=1.0, out=None):
     outside [0, len(table)) is padding: a zero row.  ``table`` is 2-D with
     contiguous rows, ``ids`` a contiguous int64 or int32 tensor of any shape
     on the same GPU; ``out`` (contiguous, not overlapping either) or a new
-    tensor [*ids.shape, dim] is returned.  Its gradient with respect to the
-    table is :func:`embedding_grad`."""
+    tensor [*ids.shape, dim] is returned.  It carries no autograd graph: its
+    gradient with respect to the table is :func:`embedding_grad`."""
     host = _host_ext()
     if host is not None and out is None and torch.cuda.is_initialized():
         # the plain form natively; None: the checks below say why not
