@@ -257,6 +257,13 @@ PyObject *embed_grad(PyObject *, PyObject *args) {
 
 namespace {
 
+// after an exception of torch's: its Python error, or one of ours
+PyObject *failed() {
+  if (!PyErr_Occurred())
+    PyErr_SetString(PyExc_RuntimeError, "a value could not be looked at");
+  return nullptr;
+}
+
 bool any_sparse(PyObject *dict) {
   PyObject *key, *value;
   Py_ssize_t pos = 0;
@@ -277,7 +284,11 @@ bool any_sparse(PyObject *dict) {
 }  // namespace
 
 PyObject *has_sparse(PyObject *, PyObject *dict) {
-  return PyBool_FromLong(PyDict_Check(dict) && any_sparse(dict));
+  try {
+    return PyBool_FromLong(PyDict_Check(dict) && any_sparse(dict));
+  } catch (...) {
+    return failed();
+  }
 }
 
 PyObject *sparse_dicts(PyObject *, PyObject *dicts) {
@@ -287,16 +298,21 @@ PyObject *sparse_dicts(PyObject *, PyObject *dicts) {
   }
   PyObject *found = PyList_New(0);
   if (!found) return nullptr;
-  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(dicts); ++i) {
-    PyObject *d = PyList_GET_ITEM(dicts, i);
-    if (!PyDict_Check(d) || !any_sparse(d)) continue;
-    PyObject *at = PyLong_FromSsize_t(i);
-    if (!at || PyList_Append(found, at) != 0) {
-      Py_XDECREF(at);
-      Py_DECREF(found);
-      return nullptr;
+  try {
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(dicts); ++i) {
+      PyObject *d = PyList_GET_ITEM(dicts, i);
+      if (!PyDict_Check(d) || !any_sparse(d)) continue;
+      PyObject *at = PyLong_FromSsize_t(i);
+      if (!at || PyList_Append(found, at) != 0) {
+        Py_XDECREF(at);
+        Py_DECREF(found);
+        return nullptr;
+      }
+      Py_DECREF(at);
     }
-    Py_DECREF(at);
+  } catch (...) {
+    Py_DECREF(found);
+    return failed();
   }
   return found;
 }

@@ -146,3 +146,19 @@ def test_fedopt_muon_aux_keys_config():
         _fedopt(torch.nn.Linear(3, 2), aux=dict(type='SGD', lr=0.1,
                                                 keys='weight'))
     _fedopt(None, aux=dict(type='SGD', lr=0.1, keys=['weight']))
+
+
+def test_sparse_search_passes_on_what_a_value_raises():
+    """A value whose class cannot be asked for is an error, not an abort."""
+    class Odd:
+        @property
+        def __class__(self):
+            raise ZeroDivisionError
+    host = L.host()
+    with pytest.raises(ZeroDivisionError):
+        host.has_sparse({'a': Odd()})
+    with pytest.raises(ZeroDivisionError):
+        host.sparse_dicts([{'a': torch.zeros(2)}, {'b': Odd()}])
+    assert host.has_sparse('no dict') is False
+    with pytest.raises(TypeError):
+        host.sparse_dicts(({}, ))
