@@ -139,6 +139,9 @@ class AggregationServer:
         broadcasts whole state dicts, server.py:636-714); it answers with a
         row-sparse update (ClientsAvgAggregator)."""
         dev = compute_device(self.device)
+        if ids.dtype not in (torch.int64, torch.int32):
+            raise ValueError('ids must be int64 or int32 (got %s)' %
+                             ids.dtype)
         table = self.models[model_idx].state_dict()[key]
         if table.device != dev and 0 < ids.numel() < len(table):
             # of a table that lies elsewhere the named rows travel, not all

@@ -270,3 +270,14 @@ def test_fedopt_muon_leaves_the_keys_of_aux_alone(rows, model_dev):
             assert torch.equal(got['emb.weight'].cpu().double()[rest],
                                before['emb.weight'][rest])
     assert sorted(a1._state) == ['a.weight']
+
+
+@pytest.mark.parametrize('model_dev', ['cpu', 'cuda'])
+def test_select_rows_refuses_other_tokens_wherever_the_model_lies(model_dev):
+    from federatedscope_amd.core.workers.server import AggregationServer
+    srv = AggregationServer(_Net(False).to(model_dev), None,
+                            sample_client_num=1, device='cuda:0')
+    for dt in (torch.float32, torch.bool, torch.uint8, torch.int16):
+        for n in (3, 60):
+            with pytest.raises(ValueError, match='int64 or int32'):
+                srv.select_rows('emb.weight', torch.ones(n, dtype=dt))
