@@ -224,7 +224,6 @@ def _check_f32_cuda(t, what, align=ALIGN_BYTES):
         raise ValueError('%s must be float32 (got %s)' % (what, t.dtype))
     if not t.is_contiguous():
         raise ValueError('%s must be contiguous' % what)
-    _check_plain(t, what)
     if t.data_ptr() % align:
         raise ValueError('%s must be %d-byte aligned' % (what, align))
 
@@ -1872,6 +1871,7 @@ def muon_step(params, avgs, bufs, lr, momentum=0.95, nesterov=True,
     for i, (p, a, b) in enumerate(zip(params, avgs, bufs)):
         for t, what in ((p, 'param'), (a, 'average'), (b, 'momentum')):
             _check_f32_cuda(t, '%s %d' % (what, i), align=4)
+            _check_plain(t, '%s %d' % (what, i))
             if dev is not None and t.device != dev:
                 raise ValueError('%s %d on %s, expected %s' %
                                  (what, i, t.device, dev))
